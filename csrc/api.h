@@ -53,6 +53,7 @@ int rb_projection_inputs(const void* qkv, int ld, const void* q_w, const void* k
 #include <pybind11/pybind11.h>
 void register_more(pybind11::module_& m);
 void register_serving(pybind11::module_& m);
+void register_rows(pybind11::module_& m);
 #endif
 
 // ---- attention / decode / sampling / fused LM head (declared again for C callers)
@@ -214,6 +215,26 @@ int rb_moe_simt(const void* A, const void* B, void* C, const int* tiles, const i
                 K, int act, float limit, int fp32, cudaStream_t st);
 int rb_moe_gemm(const void* X, const void* W, void* out, const int* tiles, const int* n_tiles, const int* row_token, int x_rows, int capacity, int
                 cap, int E, int N, int K, int act, float limit, int bn, int full, int* err, cudaStream_t st);
+// ---- rows by key (rows_sm100.cu) and distillation (distill_sm100.cu); dtype 0 = bf16, 1 = fp16, 2 = fp32; ids int64 (wide) or int32
+int rb_sort_counters(long long n, int bins);
+int rb_expert_layout(const void* ids, int wide, int n, int experts, int align, int cap, int* dest, int* source, int* tile_expert, int* bounds, int* hist,
+                     cudaStream_t st);
+int rb_expert_dispatch(const void* x, long long ld, const int* source, void* out, int cap, int k, int cols, int dtype, cudaStream_t st);
+int rb_expert_combine(const void* y, long long ld, const int* dest, const float* weight, void* out, int n, int k, int cols, int dtype, int out_fp32,
+                      cudaStream_t st);
+int rb_expert_combine_bwd(const void* d_out, long long ld, const void* y, long long ldy, const int* source, const int* dest, const float* weight, void* d_y,
+                          float* d_w, int cap, int n, int k, int cols, int dtype, cudaStream_t st);
+int rb_embedding(const void* ids, int wide, long long start, const void* table, long long ld, int rows, void* out, int n, int cols, float scale, int dtype,
+                 cudaStream_t st);
+int rb_embedding_bwd_bins(int rows);
+int rb_embedding_bwd(const void* ids, int wide, long long start, const void* dy, long long ld, void* out, int add, int2* pairs, int* hist, float* part, int
+                     n, int rows, int cols, float scale, int dtype, cudaStream_t st);
+int rb_topk_distill_parts(long long rows, int vocab);
+int rb_topk_distill(const void* z, long long ld, const long long* ids, const float* teacher, float* loss, float* coef, float* stats, float* log_probs,
+                    float2* sums, long long rows, int vocab, int k, int kl, int norm, double alpha, double clamp, float inv_temp, int dtype, cudaStream_t
+                    st);
+int rb_topk_distill_bwd(const void* z, long long ld, const long long* ids, const float* coef, const float* stats, const float* g, void* dz, long long rows,
+                        int vocab, int k, float inv_temp, int dtype, int out_dtype, cudaStream_t st);
 #ifdef __cplusplus
 }
 #endif

@@ -159,4 +159,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("fp8_block_dequant", &fp8_block_dequant);
   register_serving(m);
   register_more(m);
+  register_rows(m);
 }

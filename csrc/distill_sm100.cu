@@ -1,0 +1,639 @@
+// Divergence of a student from a teacher known on K token ids per row, and the gradient of the student's logits.
+//
+//   s_i = z_i / T - log sum_v exp(z_v / T) on the K ids (the student), t_i given (the teacher), P = exp(s), Q = exp(t)
+//   reverse  sum P (s - t),  forward  sum Q (t - s),  mixed  (1 - a) sum P (s - m) + a sum Q (t - m)  with exp(m) = (1 - a) P + a Q,
+//   low variance  sum exp(t - s) - 1 + s - t;   over the K ids as they are, over the K ids renormalised, or over the K ids and one
+//   bin with all other mass (no less than 1 - exp(-1e-7) of it).
+//   d z_v = g / T (sum_i c_i [v = id_i] - P_v sum_i c_i)  with  c_i = dD / ds_i
+//
+// Both directions are bound by memory: the forward kernel reads the logits once (maximum and sum together, the sum rescaled when
+// the maximum grows), the backward kernel reads them once more and writes the gradient; everything about the K ids is a few
+// values per row.  The mass outside the ids is summed by itself - the ids are marked in a bitmap and left out - because 1 - sum P
+// loses all digits where the ids hold nearly everything.  The forward pass is two kernels: one that streams the rows (several blocks
+// per row where there are few of them) and a small one with the 64-bit arithmetic, which would cost the first its occupancy.
+// Arithmetic: 32-bit exponentials and sums over the vocabulary, 64 bits for the K ids (a few hundred values per row).
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <type_traits>
+
+#include "api.h"
+#include "host_utils.h"
+
+namespace rb {
+namespace distill {
+
+constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr int kMaxIds = 1024;      // eight per thread of id_kernel
+constexpr int kMaxVocab = 1 << 24;
+constexpr int kStats = 4;      // per row: log2 reference, 1 / sum, sum of the slopes, (unused)
+constexpr double kLn2 = 0.6931471805599453;
+constexpr double kLeastRest = 9.9999995e-08;      // 1 - exp(-1e-7)
+
+enum Kl { kReverse = 0, kForward = 1, kMixed = 2, kLowVar = 3 };
+enum Norm { kTail = 0, kNorm = 1, kTrunc = 2 };
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// two 32-bit operations at a time
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  unsigned long long r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(r)
+      : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)), "l"(*reinterpret_cast<unsigned long long*>(&c)));
+  return *reinterpret_cast<float2*>(&r);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  unsigned long long r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)));
+  return *reinterpret_cast<float2*>(&r);
+}
+
+// eight consecutive elements, aligned to their size
+template <typename T> struct Eight;
+template <> struct Eight<float> {
+  float4 a, b;
+  __device__ __forceinline__ void load(const float* p) {
+    a = reinterpret_cast<const float4*>(p)[0];
+    b = reinterpret_cast<const float4*>(p)[1];
+  }
+  __device__ __forceinline__ float max() const { return fmaxf(fmaxf(fmaxf(a.x, a.y), fmaxf(a.z, a.w)), fmaxf(fmaxf(b.x, b.y), fmaxf(b.z, b.w))); }
+  __device__ __forceinline__ void get(float* f) const {
+    f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
+  }
+  __device__ __forceinline__ static void store(float* p, const float* f) {
+    reinterpret_cast<float4*>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
+    reinterpret_cast<float4*>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
+  }
+};
+template <> struct Eight<__nv_bfloat16> {
+  __nv_bfloat162 h[4];
+  __device__ __forceinline__ void load(const __nv_bfloat16* p) { *reinterpret_cast<uint4*>(h) = *reinterpret_cast<const uint4*>(p); }
+  __device__ __forceinline__ float max() const {
+    const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+    return fmaxf(__low2float(m), __high2float(m));
+  }
+  __device__ __forceinline__ void get(float* f) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 v = __bfloat1622float2(h[i]);
+      f[2 * i] = v.x, f[2 * i + 1] = v.y;
+    }
+  }
+  __device__ __forceinline__ static void store(__nv_bfloat16* p, const float* f) {
+    uint4 u;
+    __nv_bfloat162* o = reinterpret_cast<__nv_bfloat162*>(&u);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+    *reinterpret_cast<uint4*>(p) = u;
+  }
+};
+template <> struct Eight<__half> {
+  __half2 h[4];
+  __device__ __forceinline__ void load(const __half* p) { *reinterpret_cast<uint4*>(h) = *reinterpret_cast<const uint4*>(p); }
+  __device__ __forceinline__ float max() const {
+    const __half2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+    return fmaxf(__low2float(m), __high2float(m));
+  }
+  __device__ __forceinline__ void get(float* f) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 v = __half22float2(h[i]);
+      f[2 * i] = v.x, f[2 * i + 1] = v.y;
+    }
+  }
+  __device__ __forceinline__ static void store(__half* p, const float* f) {
+    uint4 u;
+    __half2* o = reinterpret_cast<__half2*>(&u);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+    *reinterpret_cast<uint4*>(p) = u;
+  }
+};
+__device__ __forceinline__ float up(float v) { return v; }
+__device__ __forceinline__ float up(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float up(__half v) { return __half2float(v); }
+__device__ __forceinline__ void put(float* p, float v) { *p = v; }
+__device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16(v); }
+__device__ __forceinline__ void put(__half* p, float v) { *p = __float2half(v); }
+
+struct Params {
+  const void* z;               // [rows, vocab] logits, pitch ld
+  long long ld;
+  const long long* ids;        // [rows, k]; outside 0 .. vocab - 1: no id
+  const float* teacher;        // [rows, k] log-probs
+  float* loss;                 // [rows]
+  float* coef;                 // [rows, k] dD / ds, added up over equal ids
+  float* stats;                // [rows, kStats]
+  float* log_probs;            // [rows, k] or null
+  float2* sums;                // [rows, parts] (reference, sum) of the parts of a row
+  int vocab, k, kl, norm, parts;
+  float c2;                    // log2(e) / T
+  double alpha, clamp;         // weight of the teacher; least log-prob
+};
+
+// (reference, sum): the sum of 2^(z c2) is sum 2^reference
+struct Sum {
+  float ref, sum;
+  __device__ __forceinline__ void add(float r, float s) {      // nothing yet: ref -inf, sum 0
+    const float m = fmaxf(ref, r), at = m == -INFINITY ? 0.f : m;
+    sum = sum * ex2(ref - at) + s * ex2(r - at);
+    ref = m;
+  }
+};
+
+constexpr int kIdThreads = 128, kIdWarps = kIdThreads / 32;      // most of the kernel that looks at a row's ids
+template <int N>
+__device__ __forceinline__ void block_sums(double (&v)[N], double (*sm)[kIdWarps]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+  const int warps = blockDim.x >> 5;
+  if (warps == 1) return;
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) sm[i][threadIdx.x >> 5] = v[i];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    v[i] = 0.0;
+    for (int w = 0; w < warps; ++w) v[i] += sm[i][w];
+  }
+}
+
+__device__ __forceinline__ double least(double x, double c) { return x < c ? c : x; }      // (NaN stays)
+// 0 log 0 = 0: a term whose weight is nothing counts nothing
+__device__ __forceinline__ double weighted(double w, double x) { return w == 0.0 ? 0.0 : w * x; }
+// masses in 32 bits: off by 2^-22 like the exponentials of the sum, against which they are weighed
+__device__ __forceinline__ double mass_of(double log_prob) { return static_cast<double>(ex2(static_cast<float>(log_prob * 1.4426950408889634))); }
+
+struct Term {
+  double d, slope;      // D's term and its derivative by P
+};
+// p, q the masses and l = log(p / q).  The mixture's logs come from l: log(p / m) = -log(1 + a (q / p - 1)) keeps its digits where p
+// and q are near each other, and the like from the side of q where q is the larger.
+__device__ __forceinline__ Term term_of(int kl, double a, double p, double q, double l) {
+  Term r;
+  if (kl == kReverse) {
+    r.d = weighted(p, l);
+    r.slope = l + 1.0;
+  } else if (kl == kForward) {
+    r.d = weighted(q, -l);
+    r.slope = -q / p;
+  } else {
+    double pm, qm;      // log(p / m), log(q / m)
+    if (l >= 0.0) {
+      pm = -static_cast<double>(log1pf(static_cast<float>(a) * expm1f(static_cast<float>(-l))));
+      qm = pm - l;
+    } else {
+      qm = -static_cast<double>(log1pf(static_cast<float>(1.0 - a) * expm1f(static_cast<float>(l))));
+      pm = l + qm;
+    }
+    r.d = (1.0 - a) * weighted(p, pm) + a * weighted(q, qm);
+    r.slope = (1.0 - a) * pm;
+  }
+  return r;
+}
+
+// Sums over the vocabulary, `parts` blocks per row.  The row counts from the last address in front of it that is a multiple of eight
+// elements, so that all but its first and last group of eight are whole; groups are shared out to the blocks in runs.
+template <typename T, bool kMarks>
+__global__ void __launch_bounds__(kThreads, 4) sum_kernel(Params p) {
+  const long long row = blockIdx.x / p.parts;
+  const int part = static_cast<int>(blockIdx.x - row * p.parts), t = threadIdx.x;
+  extern __shared__ unsigned marks[];      // a bit per element of this block's groups
+  __shared__ Sum warp_sum[kWarps];
+  const T* z = static_cast<const T*>(p.z) + row * p.ld;
+  const int skip = static_cast<int>((reinterpret_cast<uintptr_t>(z) / sizeof(T)) & 7);      // elements in front of the row in its first group
+  const T* origin = z - skip;
+  const int groups = (skip + p.vocab + 7) >> 3, each = (groups + p.parts - 1) / p.parts;
+  const int g0 = min(groups, part * each), g1 = min(groups, g0 + each);
+  const int w0 = g0 == 0 && skip ? 1 : g0, w1 = (g1 == groups && ((skip + p.vocab) & 7)) ? g1 - 1 : g1;      // whole groups
+
+  if constexpr (kMarks) {
+    for (int i = t; i < (each + 3) / 4; i += kThreads) marks[i] = 0;
+    __syncthreads();
+  }
+  // logits of this part's ids, for the kernel behind this one: fetched here, where other blocks keep the memory busy meanwhile (K
+  // scattered reads per row by themselves took 116 us for 4096 rows of 128), and put down at the end
+  constexpr int kMine = kMaxIds / kThreads;
+  float at_id[kMine];
+  unsigned here = 0;
+#pragma unroll
+  for (int j = 0; j < kMine; ++j) {
+    const int i = t + j * kThreads;
+    if (i >= p.k) break;
+    const long long v = p.ids[row * p.k + i], b = v + skip - 8ll * g0;
+    if (v >= 0 && v < p.vocab && b >= 0 && b < 8ll * (g1 - g0)) {
+      here |= 1u << j;
+      at_id[j] = up(z[v]);
+      if constexpr (kMarks) atomicOr(&marks[b >> 5], 1u << (b & 31));
+    }
+  }
+  if constexpr (kMarks) __syncthreads();
+  const unsigned char* mark = reinterpret_cast<const unsigned char*>(marks);
+
+  Sum s{-INFINITY, 0.f};
+  constexpr int U = sizeof(T) == 4 ? 2 : 4;      // groups of a thread in one step
+  // U groups from g on, in strides of the block; the last step (kAll false) holds what is left
+  auto step = [&](int g, auto all) {
+    constexpr bool kAll = decltype(all)::value;
+    Eight<T> e[U];
+    unsigned m[U];
+    float big = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (kAll || g + u * kThreads < w1) e[u].load(origin + 8ll * (g + u * kThreads));
+    if constexpr (kMarks) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) m[u] = kAll || g + u * kThreads < w1 ? mark[g + u * kThreads - g0] : 0;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (kAll || g + u * kThreads < w1) big = fmaxf(big, e[u].max());
+    big *= p.c2;
+    if (big > s.ref) {
+      s.sum *= ex2(s.ref - big);
+      s.ref = big;
+    }
+    const float at = s.ref == -INFINITY ? 0.f : s.ref;
+    const float2 c = make_float2(p.c2, p.c2), o = make_float2(-at, -at);
+    float2 add = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (kAll || g + u * kThreads < w1) {
+        float f[8];
+        e[u].get(f);
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+          const float2 x = fma2(make_float2(f[i], f[i + 1]), c, o);
+          f[i] = ex2(x.x), f[i + 1] = ex2(x.y);
+        }
+        if constexpr (kMarks) {
+          if (m[u]) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] = (m[u] >> i) & 1 ? 0.f : f[i];
+          }
+        }
+        add = add2(add, add2(add2(make_float2(f[0], f[1]), make_float2(f[2], f[3])), add2(make_float2(f[4], f[5]), make_float2(f[6], f[7]))));
+      }
+    s.sum += add.x + add.y;
+  };
+  int g = w0 + t;
+  for (; g + (U - 1) * kThreads < w1; g += U * kThreads) step(g, std::true_type{});
+  if (g < w1) step(g, std::false_type{});
+  // the row's first and last group, where they are not whole: one element per thread
+  if (t < 16) {
+    const int g = t < 8 ? 0 : groups - 1, i = t & 7;
+    const long long v = 8ll * g + i - skip;
+    const bool mine = t < 8 ? (g0 == 0 && skip) : (g1 == groups && ((skip + p.vocab) & 7) && !(groups == 1 && skip));
+    if (mine && g0 < g1 && v >= 0 && v < p.vocab) {
+      bool counts = true;
+      if constexpr (kMarks) counts = !((mark[g - g0] >> i) & 1);
+      const float x = up(z[v]) * p.c2;
+      s.add(x, counts ? (x == -INFINITY ? 0.f : (x == x ? 1.f : x)) : 0.f);
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s.add(__shfl_xor_sync(0xffffffffu, s.ref, o), __shfl_xor_sync(0xffffffffu, s.sum, o));
+  if ((t & 31) == 0) warp_sum[t >> 5] = s;
+  __syncthreads();
+  if (t == 0) {
+    Sum b = warp_sum[0];
+#pragma unroll
+    for (int w = 1; w < kWarps; ++w) b.add(warp_sum[w].ref, warp_sum[w].sum);
+    p.sums[blockIdx.x] = make_float2(b.ref, b.sum);
+  }
+#pragma unroll
+  for (int j = 0; j < kMine; ++j)
+    if ((here >> j) & 1) p.coef[row * p.k + t + j * kThreads] = at_id[j];
+}
+
+// every bit of an id in every bit of its slot: ids at even distances would fill one stretch of the table otherwise
+__device__ __forceinline__ unsigned mixed(unsigned x) {
+  x = (x ^ (x >> 16)) * 0x9e3779b1u;
+  x = (x ^ (x >> 15)) * 0x9e3779b1u;
+  return x ^ (x >> 16);
+}
+
+// The K ids of a row: the divergence, its slopes, the row's statistics.  Log-probs, their differences and the sums over the ids are in
+// 64 bits, exponentials in 32.  Equal ids are found with a hash table that keeps the first place of every id.
+__global__ void __launch_bounds__(kIdThreads) id_kernel(Params p, int slots) {
+  const long long row = blockIdx.x;
+  const int t = threadIdx.x, threads = blockDim.x;
+  extern __shared__ __align__(16) unsigned char dyn[];
+  double* lp = reinterpret_cast<double*>(dyn);                // [k] log-probs of the student, then slopes
+  int* id = reinterpret_cast<int*>(lp + p.k);                 // [k] the row's ids, -1: none
+  float* pm = reinterpret_cast<float*>(id + p.k);             // [k] masses of the student (before clamping)
+  float* tl = pm + p.k;                                       // [k] log-probs of the teacher
+  int* key = reinterpret_cast<int*>(tl + p.k);                // [slots] ids (a power of two, at least 2 k)
+  int* place = key + slots;                                   // [slots] where they stand first
+  __shared__ double red[4][kIdWarps];
+  const bool tail = p.norm == kTail && p.kl != kLowVar, renorm = p.norm == kNorm && p.kl != kLowVar;
+  for (int i = t; i < slots; i += threads) key[i] = -1, place[i] = p.k;
+  Sum all{-INFINITY, 0.f};
+  for (int r = 0; r < p.parts; ++r) {
+    const float2 s = p.sums[row * p.parts + r];
+    all.add(s.x, s.y);
+  }
+  const double ref = all.ref == -INFINITY ? 0.0 : static_cast<double>(all.ref), c2 = p.c2, counted = all.sum;
+  __syncthreads();
+  for (int i0 = t; i0 < p.k; i0 += 4 * threads) {      // four ids at a time: they wait for memory
+    int v[4];
+    float z[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int i = i0 + u * threads;
+      const long long w = i < p.k ? p.ids[row * p.k + i] : -1;
+      v[u] = w >= 0 && w < p.vocab ? static_cast<int>(w) : -1;
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int i = i0 + u * threads;
+      if (i < p.k) tl[i] = p.teacher[row * p.k + i];
+      z[u] = v[u] >= 0 ? p.coef[row * p.k + i] : 0.f;      // (its logit, for now)
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int i = i0 + u * threads;
+      if (i >= p.k) break;
+      id[i] = v[u];
+      if (v[u] < 0) continue;
+      lp[i] = (static_cast<double>(z[u]) * c2 - ref) * kLn2;      // z - reference in units of ln
+      unsigned h = mixed(v[u]);
+      for (;; ++h) {      // (ends: no more than half the slots are taken)
+        const int was = atomicCAS(&key[h & (slots - 1)], -1, v[u]);
+        if (was == -1 || was == v[u]) break;
+      }
+      atomicMin(&place[h & (slots - 1)], i);
+      pm[i] = __int_as_float(static_cast<int>(h & (slots - 1)));
+    }
+  }
+  __syncthreads();
+  double one[1] = {0.0};
+  unsigned firsts = 0;      // a bit for each of this thread's ids
+  for (int i = t, n = 0; i < p.k; i += threads, ++n) {
+    if (id[i] < 0) continue;
+    const bool first = place[__float_as_int(pm[i])] == i;
+    firsts |= static_cast<unsigned>(first) << n;
+    const double e = mass_of(lp[i]);
+    pm[i] = static_cast<float>(e);
+    if (first && tail) one[0] += e;
+  }
+  if (tail) block_sums(one, red);      // the sum over the vocabulary left the ids out
+  const double total = counted + one[0], log_total = log(total), inv_total = 1.0 / total;
+
+  // masses of the ids (renormalised: of all of them), and what the rest lacks: equal ids and clamped ones count as written
+  double mass[3] = {0.0, 0.0, 0.0};
+  bool twice = false;
+  for (int i = t, n = 0; i < p.k; i += threads, ++n) {
+    if (id[i] < 0) continue;
+    const bool first = (firsts >> n) & 1;
+    twice |= !first;
+    lp[i] -= log_total;
+    if (p.log_probs) p.log_probs[row * p.k + i] = static_cast<float>(lp[i]);
+    if (!tail && !renorm) continue;
+    const double used = least(lp[i], p.clamp), pi = pm[i] * inv_total, pu = used == lp[i] ? pi : used == used ? exp(used) : used;
+    mass[0] += pu;
+    mass[1] += exp(least(static_cast<double>(tl[i]), p.clamp));      // (64 bits: the rest is one minus their sum)
+    mass[2] += pu - (first ? pi : 0.0);
+  }
+  if (tail || renorm) block_sums(mass, red);
+  double rest_slope = 0.0, rest = 0.0;
+  if (tail) {
+    const double free = counted / total - mass[2];      // (exactly one where there are no ids)
+    const double pr = least(free, kLeastRest), qr = least(1.0 - mass[1], kLeastRest);
+    const Term r = term_of(p.kl, p.alpha, pr, qr, log(pr / qr));
+    rest = r.d;
+    rest_slope = free >= kLeastRest ? r.slope : 0.0;
+  }
+  const double ls = renorm ? log(mass[0] / mass[1]) : 0.0, np = renorm ? 1.0 / mass[0] : 1.0, nq = renorm ? 1.0 / mass[1] : 1.0;
+  double sums[4] = {0.0, 0.0, 0.0, 0.0};      // the divergence; slopes of all ids; slopes and masses of those that move
+  for (int i = t; i < p.k; i += threads) {
+    if (id[i] < 0) {
+      if (p.log_probs) p.log_probs[row * p.k + i] = -INFINITY;
+      continue;
+    }
+    const double s_i = lp[i], t_i = least(static_cast<double>(tl[i]), p.clamp), used = least(s_i, p.clamp);
+    const bool moves = !(s_i < p.clamp);      // clamped ids do not
+    double c, pp = 0.0;
+    if (p.kl == kLowVar) {
+      const double r = used - t_i, x = exp(-r);
+      sums[0] += x - 1.0 + r;
+      c = 1.0 - x;
+    } else {
+      const double qq = mass_of(t_i) * nq;
+      pp = (moves ? pm[i] * inv_total : exp(used)) * np;
+      const Term r = term_of(p.kl, p.alpha, pp, qq, used - t_i - ls);
+      sums[0] += r.d;
+      c = (p.kl == kForward ? -qq : weighted(pp, r.slope)) - weighted(pp, rest_slope);
+    }
+    sums[1] += c;
+    if (moves) {
+      sums[2] += c;
+      sums[3] += pp;
+    }
+    lp[i] = moves ? c : 0.0;
+    pm[i] = moves ? static_cast<float>(pp) : 0.f;
+  }
+  block_sums(sums, red);
+  double move = sums[2];
+  if (renorm) {      // c_i - P_i sum c
+    move -= sums[1] * sums[3];
+    for (int i = t; i < p.k; i += threads)
+      if (id[i] >= 0) lp[i] -= pm[i] * sums[1];
+  }
+  const bool sum_equals = __syncthreads_or(twice);      // equal ids move together
+  for (int i = t; i < p.k; i += threads) {
+    double c = id[i] < 0 ? 0.0 : lp[i];
+    if (sum_equals && id[i] >= 0) {
+      c = 0.0;
+      for (int j = 0; j < p.k; ++j) c += id[j] == id[i] ? lp[j] : 0.0;
+    }
+    p.coef[row * p.k + i] = static_cast<float>(c);
+  }
+  if (t == 0) {
+    p.loss[row] = static_cast<float>(sums[0] + rest);
+    *reinterpret_cast<float4*>(p.stats + row * kStats) =
+        make_float4(static_cast<float>(ref), static_cast<float>(inv_total), static_cast<float>(move), 0.f);
+  }
+}
+
+struct BwdParams {
+  const void* z;
+  long long ld;
+  const long long* ids;
+  const float* coef;
+  const float* stats;
+  const float* g;          // [rows] gradient of the divergence
+  void* dz;                // [rows, vocab] dense (may be z itself where types agree)
+  int vocab, k, parts;
+  float c2, inv_t;
+};
+
+// A block per part of a row: -g / T (sum c) P over its elements, then the K ids of that part in place of what stands there.
+template <typename T, typename O, bool kWhole>
+__global__ void __launch_bounds__(kThreads) bwd_kernel(BwdParams p) {
+  const long long row = blockIdx.x / p.parts;
+  const int part = static_cast<int>(blockIdx.x - row * p.parts), t = threadIdx.x;
+  const T* z = static_cast<const T*>(p.z) + row * p.ld;
+  O* d = static_cast<O*>(p.dz) + row * p.vocab;
+  const float g = p.g[row] * p.inv_t;
+  const float ref = p.stats[row * kStats], inv = p.stats[row * kStats + 1], csum = p.stats[row * kStats + 2];
+  const float f = g == 0.f ? 0.f : -g * csum * inv;
+  const int skip = kWhole ? static_cast<int>((reinterpret_cast<uintptr_t>(z) / sizeof(T)) & 7) : 0;
+  const int groups = (skip + p.vocab + 7) >> 3, each = (groups + p.parts - 1) / p.parts;
+  const int g0 = min(groups, part * each), g1 = min(groups, g0 + each);
+  const long long lo = max(0ll, 8ll * g0 - skip), hi = min(static_cast<long long>(p.vocab), 8ll * g1 - skip);
+  if (lo >= hi) return;
+  // probabilities of this part's ids are read before they are overwritten (dz may be z)
+  extern __shared__ float at_id[];
+  if (g != 0.f) {
+    for (int i = t; i < p.k; i += kThreads) {
+      const long long v = p.ids[row * p.k + i];
+      if (v >= lo && v < hi) at_id[i] = g * p.coef[row * p.k + i] + f * ex2(fmaf(up(z[v]), p.c2, -ref));
+    }
+    __syncthreads();
+  }
+  auto one = [&](long long v) { put(d + v, g == 0.f ? 0.f : f * ex2(fmaf(up(z[v]), p.c2, -ref))); };
+  if constexpr (!kWhole) {
+    for (long long v = lo + t; v < hi; v += kThreads) one(v);
+  } else {
+    const int w0 = g0 == 0 && skip ? 1 : g0, w1 = (g1 == groups && ((skip + p.vocab) & 7)) ? g1 - 1 : g1;
+    constexpr int U = sizeof(T) == 4 ? 2 : 4;
+    for (int q = w0 + t; q < w1; q += kThreads * U) {
+      Eight<T> e[U];
+      if (g != 0.f) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (q + u * kThreads < w1) e[u].load(z + (8ll * (q + u * kThreads) - skip));
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (q + u * kThreads < w1) {
+          float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+          if (g != 0.f) {
+            e[u].get(x);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = f * ex2(fmaf(x[i], p.c2, -ref));
+          }
+          Eight<O>::store(d + (8ll * (q + u * kThreads) - skip), x);
+        }
+    }
+    if (t < 16) {
+      const int q = t < 8 ? 0 : groups - 1;
+      const long long v = 8ll * q + (t & 7) - skip;
+      const bool mine = t < 8 ? (g0 == 0 && skip) : (g1 == groups && ((skip + p.vocab) & 7) && !(groups == 1 && skip));
+      if (mine && v >= 0 && v < p.vocab) one(v);
+    }
+  }
+  if (g == 0.f) return;
+  __syncthreads();
+  for (int i = t; i < p.k; i += kThreads) {
+    const long long v = p.ids[row * p.k + i];
+    if (v >= lo && v < hi) put(d + v, at_id[i]);
+  }
+}
+
+// Blocks of a row: one where rows alone fill the machine, else as many as it takes, each with at least 4096 elements (parts of a row
+// cost: finer ones, for a fuller last wave, made the sums slower)
+inline int parts_of(long long rows, int vocab, int most) {
+  int parts = 1;
+  while (parts < most && rows * parts < 8ll * num_sms() && vocab / (2 * parts) >= 4096) parts *= 2;
+  return parts;
+}
+constexpr int kSumParts = 32;
+
+template <typename T, bool kMarks>
+int sums_t(const Params& p, long long rows, cudaStream_t st) {
+  const int each = ((p.vocab + 14) / 8 + p.parts - 1) / p.parts + 1;
+  const size_t smem = kMarks ? (each + 3) / 4 * 4 + 16 : 0;
+  if (smem > 200 * 1024) return -4;      // (a vocabulary of more than a million ids, in one part)
+  auto kernel = sum_kernel<T, kMarks>;
+  if (smem > 40 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    if (e != cudaSuccess) return static_cast<int>(e);
+  }
+  kernel<<<static_cast<unsigned>(rows * p.parts), kThreads, smem, st>>>(p);
+  rb_note_launch(1);
+  return static_cast<int>(cudaGetLastError());
+}
+template <typename T>
+int sums_any(const Params& p, long long rows, cudaStream_t st) {
+  return p.norm == kTail && p.kl != kLowVar ? sums_t<T, true>(p, rows, st) : sums_t<T, false>(p, rows, st);
+}
+
+template <typename T, typename O>
+int bwd_t(BwdParams p, long long rows, cudaStream_t st) {
+  p.parts = parts_of(rows, p.vocab, 32);
+  if (rows * p.parts > 2147483647ll) return -3;
+  // groups of eight line up in both where rows keep their distance and begin alike
+  const uintptr_t a = reinterpret_cast<uintptr_t>(p.z) / sizeof(T), b = reinterpret_cast<uintptr_t>(p.dz) / sizeof(O);
+  const bool whole = (a - b) % 8 == 0 && (rows == 1 || (p.ld - p.vocab) % 8 == 0);
+  const int grid = static_cast<int>(rows * p.parts);
+  const size_t smem = static_cast<size_t>(p.k) * 4 + 4;
+  if (whole) bwd_kernel<T, O, true><<<grid, kThreads, smem, st>>>(p);
+  else bwd_kernel<T, O, false><<<grid, kThreads, smem, st>>>(p);
+  rb_note_launch(1);
+  return static_cast<int>(cudaGetLastError());
+}
+
+}  // namespace distill
+}  // namespace rb
+
+using namespace rb;
+using namespace rb::distill;
+
+// Blocks per row, and so pairs of floats per row that rb_topk_distill takes as workspace.
+extern "C" int rb_topk_distill_parts(long long rows, int vocab) {
+  int parts = parts_of(rows, vocab, kSumParts);
+  while (parts < kSumParts && vocab / parts > (1 << 20)) parts *= 2;      // the bitmap of a part fits shared memory
+  return parts;
+}
+
+// dtype: 0 bf16, 1 fp16, 2 fp32.  kl: reverse, forward, mixed, low variance; norm: tail bin, renormalised, as they are.
+extern "C" int rb_topk_distill(const void* z, long long ld, const long long* ids, const float* teacher, float* loss, float* coef, float* stats,
+                               float* log_probs, float2* sums, long long rows, int vocab, int k, int kl, int norm, double alpha, double clamp,
+                               float inv_temp, int dtype, cudaStream_t st) {
+  if (rows < 0 || vocab < 1 || vocab > kMaxVocab || k < 0 || k > kMaxIds || kl < 0 || kl > 3 || norm < 0 || norm > 2 || !(inv_temp > 0.f)) return -1;
+  if (rows == 0) return 0;
+  const int parts = rb_topk_distill_parts(rows, vocab);
+  if (rows * parts > 2147483647ll) return -3;
+  const Params p{z, ld, ids, teacher, loss, coef, stats, log_probs, sums, vocab, k, kl, norm, parts, inv_temp * 1.4426950408889634f, alpha, clamp};
+  int rc = -1;
+  switch (dtype) {
+    case 0: rc = sums_any<__nv_bfloat16>(p, rows, st); break;
+    case 1: rc = sums_any<__half>(p, rows, st); break;
+    case 2: rc = sums_any<float>(p, rows, st); break;
+  }
+  if (rc) return rc;
+  // many rows: a warp each, which spends the fewest instructions; few: a thread per id, for the shortest way
+  int threads = rows >= 8ll * num_sms() ? 32 : (k + 31) / 32 * 32, slots = 32;
+  threads = threads < 32 ? 32 : threads > kIdThreads ? kIdThreads : threads;
+  while (slots < 2 * k) slots *= 2;
+  id_kernel<<<static_cast<unsigned>(rows), threads, static_cast<size_t>(k) * 20 + slots * 8, st>>>(p, slots);
+  rb_note_launch(1);
+  return static_cast<int>(cudaGetLastError());
+}
+
+// out_dtype: that of the logits, or 0 (bf16) for logits in fp32
+extern "C" int rb_topk_distill_bwd(const void* z, long long ld, const long long* ids, const float* coef, const float* stats, const float* g, void* dz,
+                                   long long rows, int vocab, int k, float inv_temp, int dtype, int out_dtype, cudaStream_t st) {
+  if (rows < 0 || vocab < 1 || vocab > kMaxVocab || k < 0 || k > kMaxIds || !(inv_temp > 0.f)) return -1;
+  if (rows == 0) return 0;
+  const BwdParams p{z, ld, ids, coef, stats, g, dz, vocab, k, 1, inv_temp * 1.4426950408889634f, inv_temp};
+  if (dtype == 0 && out_dtype == 0) return bwd_t<__nv_bfloat16, __nv_bfloat16>(p, rows, st);
+  if (dtype == 1 && out_dtype == 1) return bwd_t<__half, __half>(p, rows, st);
+  if (dtype == 2 && out_dtype == 2) return bwd_t<float, float>(p, rows, st);
+  if (dtype == 2 && out_dtype == 0) return bwd_t<float, __nv_bfloat16>(p, rows, st);
+  return -1;
+}

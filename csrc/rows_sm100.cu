@@ -1,0 +1,802 @@
+// Rows moved by key: the layout of routed rows sorted by expert, their way there and back (with weights), the rows of an
+// embedding table and the table's gradient by sorted tokens.
+//
+// All of it is bound by memory: every kernel touches each row it needs once, in 16-byte vectors where rows allow it, one warp
+// per row or part of a row, sums in 32 bits in a fixed order (no floating-point atomics, so reruns give the same bits).
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <type_traits>
+
+#include "api.h"
+#include "host_utils.h"
+
+namespace rb {
+namespace rows {
+
+constexpr int kWarps = 16, kThreads = 32 * kWarps;      // of the sorting kernels
+constexpr int kMaxBins = 2048;                          // 16 warps x 2048 counters: 128 KB of shared memory
+
+// ----------------------------------------------------------------------------- elements
+__device__ __forceinline__ float up(float v) { return v; }
+__device__ __forceinline__ float up(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float up(__half v) { return __half2float(v); }
+template <typename T> __device__ __forceinline__ T down(float v);
+template <> __device__ __forceinline__ float down<float>(float v) { return v; }
+template <> __device__ __forceinline__ __nv_bfloat16 down<__nv_bfloat16>(float v) { return __float2bfloat16(v); }
+template <> __device__ __forceinline__ __half down<__half>(float v) { return __float2half(v); }
+
+// N consecutive elements: 16 bytes, or one element for rows of odd size or alignment (and eight floats: the sums of 16 bytes).
+// 16-bit elements stay packed until they are used: unpacked, a vector takes twice the registers.
+template <typename T, int N> struct alignas(N * sizeof(T)) Pack {
+  T v[N];
+  __device__ __forceinline__ void get(float* f) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) f[i] = up(v[i]);
+  }
+  __device__ __forceinline__ void set(const float* f) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = down<T>(f[i]);
+  }
+};
+template <> struct alignas(16) Pack<__nv_bfloat16, 8> {
+  uint32_t v[4];
+  __device__ __forceinline__ void get(float* f) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[2 * i] = __uint_as_float(v[i] << 16), f[2 * i + 1] = __uint_as_float(v[i] & 0xffff0000u);
+  }
+  __device__ __forceinline__ void set(const float* f) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+      v[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+  }
+};
+template <> struct alignas(16) Pack<__half, 8> {
+  uint32_t v[4];
+  __device__ __forceinline__ void get(float* f) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&v[i]));
+      f[2 * i] = h.x, f[2 * i + 1] = h.y;
+    }
+  }
+  __device__ __forceinline__ void set(const float* f) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __half2 h = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+      v[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+  }
+};
+template <typename T, int N>
+__device__ __forceinline__ Pack<T, N> zeros() {
+  Pack<T, N> p;
+  const float z[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  p.set(z);
+  return p;
+}
+
+// ----------------------------------------------------------------------------- stable counting sort
+// One pass puts rows in the order of a key with few values ("bins"), rows of a bin in their old order.  A block counts its rows
+// (count_kernel); with every block's counts known, each block derives where its rows of every bin go and writes them
+// (place_kernel).  Ranks inside a block: every warp owns a run of rows and a counter per bin; 32 rows at a time find their
+// equals with one match instruction.  Up to kOneBlock rows take place_kernel alone.
+
+struct ExpertKeys {      // expert ids; others than 0 .. bins - 1 live elsewhere and take no part
+  const void* ids;
+  int wide, bins;
+  __device__ __forceinline__ int digit(int i) const {
+    const long long e = wide ? static_cast<const long long*>(ids)[i] : static_cast<const int*>(ids)[i];
+    return e >= 0 && e < bins ? static_cast<int>(e) : -1;
+  }
+};
+struct TokenKeys {      // first pass over token ids: a row's key is its table row, or `rows` (behind all) for tokens of other shards
+  const void* ids;
+  int wide, rows, shift, mask;
+  long long start;
+  __device__ __forceinline__ int key(int i) const {
+    const long long a = (wide ? static_cast<const long long*>(ids)[i] : static_cast<const int*>(ids)[i]) - start;
+    return a >= 0 && a < rows ? static_cast<int>(a) : rows;
+  }
+  __device__ __forceinline__ int pos(int i) const { return i; }
+  __device__ __forceinline__ int digit(int i) const { return (key(i) >> shift) & mask; }
+};
+struct PairKeys {      // later passes over the sorted pairs of the pass in front
+  const int2* pairs;
+  int shift, mask;
+  __device__ __forceinline__ int key(int i) const { return pairs[i].x; }
+  __device__ __forceinline__ int pos(int i) const { return pairs[i].y; }
+  __device__ __forceinline__ int digit(int i) const { return (key(i) >> shift) & mask; }
+};
+
+struct ExpertOut {
+  int* dest;          // [n] buffer row of every routed row, -1: elsewhere
+  int* source;        // [cap] routed row of every buffer row, -1: padding
+  int* tile_expert;   // [cap / align] expert of every tile, -1: unused; null when align == 1
+  int* bounds;        // [bins + 1] first buffer row of every expert
+  int cap, tiles;
+};
+struct PairOut {
+  int2* pairs;      // (key, row) in order
+};
+
+// What a launch fills beside the sort: `near` with -1 (entries that the sort fills in part: by the blocks that sort, before they do),
+// and a share of `far` with zeros (a gradient that waits for the sorted rows: by blocks of its own on SMs that would be idle)
+struct Fill {
+  int* near;
+  long long n_near;
+  uint4* far;
+  long long lo, hi;
+  unsigned char* rest;      // the bytes behind the last whole vector
+  int n_rest;
+};
+__device__ __forceinline__ void fill_near(const Fill& f, int blocks) {
+  const long long t = blockIdx.x * static_cast<long long>(kThreads) + threadIdx.x, all = static_cast<long long>(blocks) * kThreads;
+  for (long long i = t; i < f.n_near; i += all) f.near[i] = -1;
+}
+constexpr int kFillRun = 16;      // vectors of a thread: a block fills 128 KB in one piece (measured against a stride of the whole grid: 5.1 TB/s)
+__device__ __forceinline__ void fill_far(const Fill& f, int blocks) {
+  const long long b = blockIdx.x - blocks, v0 = f.lo + b * (kThreads * kFillRun) + threadIdx.x;
+  const uint4 z = make_uint4(0, 0, 0, 0);
+#pragma unroll
+  for (int u = 0; u < kFillRun; ++u)
+    if (v0 + u * kThreads < f.hi) f.far[v0 + u * kThreads] = z;
+  if (b == 0 && static_cast<int>(threadIdx.x) < f.n_rest) f.rest[threadIdx.x] = 0;
+}
+
+template <typename Src>
+__global__ void __launch_bounds__(kThreads) count_kernel(Src src, int n, int chunk, int bins, int blocks, int* __restrict__ hist, Fill fill) {
+  extern __shared__ int cnt[];
+  if (static_cast<int>(blockIdx.x) >= blocks) return fill_far(fill, blocks);
+  for (int b = threadIdx.x; b < bins; b += kThreads) cnt[b] = 0;
+  fill_near(fill, blocks);
+  __syncthreads();
+  const int lo = blockIdx.x * chunk, hi = min(n, lo + chunk);
+  for (int i = lo + threadIdx.x; i < hi; i += kThreads) {
+    const int d = src.digit(i);
+    if (d >= 0) atomicAdd(&cnt[d], 1);
+  }
+  __syncthreads();
+  for (int b = threadIdx.x; b < bins; b += kThreads) hist[static_cast<size_t>(blockIdx.x) * bins + b] = cnt[b];
+}
+
+template <typename Src, typename Out>
+__global__ void __launch_bounds__(kThreads) place_kernel(Src src, Out out, int n, int chunk, int bins, int align, int blocks, const int* __restrict__ hist,
+                                                         Fill fill) {
+  constexpr bool kExperts = std::is_same<Out, ExpertOut>::value;
+  extern __shared__ int sm[];
+  __shared__ int part[kWarps];
+  if (static_cast<int>(blockIdx.x) >= blocks) return fill_far(fill, blocks);
+  const int t = threadIdx.x, w = t >> 5, lane = t & 31;
+  const int per = chunk / kWarps;      // rows of a warp (a multiple of 32)
+  const int first = blockIdx.x * chunk, warps = min(kWarps, (min(n - first, chunk) + per - 1) / per);      // that have rows
+  int* start = sm;                     // [bins] first output row of the bin
+  int* total = sm + bins;              // [bins] rows of the bin
+  int* cnt = total + bins;             // [warps][bins]
+  for (int b = t; b < warps * bins; b += kThreads) cnt[b] = 0;
+  if (blocks == 1) fill_near(fill, 1);
+  __syncthreads();
+  const int lo = min(n, first + w * per), hi = min(n, lo + per);
+  int* mine = cnt + w * bins;
+  for (int i = lo + lane; i < hi; i += 32) {
+    const int d = src.digit(i);
+    if (d >= 0) atomicAdd(&mine[d], 1);
+  }
+  __syncthreads();
+  // counters become the rows of the same bin in warps in front, and those of blocks in front; `total`: of all blocks.  First output
+  // row of every bin: running sum of the (padded) counts; a thread looks after a run of bins
+  const int each = (bins + kThreads - 1) / kThreads, b0 = min(bins, t * each), b1 = min(bins, b0 + each);
+  int sum = 0;
+  for (int b = b0; b < b1; ++b) {
+    int before = 0, all = 0;
+    if (blocks > 1) {
+#pragma unroll 16
+      for (int k = 0; k < blocks; ++k) {
+        const int h = hist[static_cast<size_t>(k) * bins + b];
+        all += h;
+        before += k < static_cast<int>(blockIdx.x) ? h : 0;
+      }
+    }
+    int run = before, mine_of[kWarps];
+#pragma unroll
+    for (int k = 0; k < kWarps; ++k) mine_of[k] = k < warps ? cnt[k * bins + b] : 0;
+#pragma unroll
+    for (int k = 0; k < kWarps; ++k) {
+      if (k < warps) cnt[k * bins + b] = run;
+      run += mine_of[k];
+    }
+    total[b] = blocks > 1 ? all : run;
+    sum += (total[b] + align - 1) / align * align;
+  }
+  int scan = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, scan, o);
+    if (lane >= o) scan += v;
+  }
+  if (lane == 31) part[w] = scan;
+  __syncthreads();
+  int base = scan - sum;
+#pragma unroll
+  for (int k = 0; k < kWarps; ++k) base += k < w ? part[k] : 0;
+  for (int b = b0; b < b1; ++b) {
+    start[b] = base;
+    const int rows = (total[b] + align - 1) / align * align;
+    if constexpr (kExperts) {
+      // (every block knows all bounds: bins are shared out to the blocks)
+      if (b % blocks == static_cast<int>(blockIdx.x)) {
+        out.bounds[b] = base;
+        if (b == bins - 1) out.bounds[bins] = base + rows;
+      }
+    }
+    base += rows;
+  }
+  __syncthreads();
+  if constexpr (kExperts) {
+    for (int q = blockIdx.x * kThreads + t; q < out.tiles; q += blocks * kThreads) {      // the last expert that begins at or in front of the tile
+      int b = 0;
+      for (int step = 1 << (31 - __clz(bins)); step > 0; step >>= 1)
+        if (b + step < bins && start[b + step] <= q * align) b += step;
+      out.tile_expert[q] = q * align < start[b] + (total[b] + align - 1) / align * align ? b : -1;
+    }
+  }
+  for (int i0 = lo; i0 < hi; i0 += 32) {
+    const int i = i0 + lane;
+    const int d = i < hi ? src.digit(i) : -1;
+    const unsigned same = __match_any_sync(0xffffffffu, d);
+    int at = -1;
+    if (d >= 0) at = start[d] + mine[d] + __popc(same & ((1u << lane) - 1));
+    __syncwarp();
+    if (d >= 0 && lane == __ffs(same) - 1) mine[d] += __popc(same);
+    __syncwarp();
+    if (i < hi) {
+      if constexpr (kExperts) {
+        out.dest[i] = at;
+        if (at >= 0) out.source[at] = i;
+      } else {
+        out.pairs[at] = make_int2(src.key(i), src.pos(i));
+      }
+    }
+  }
+}
+
+constexpr int kMaxSort = 1 << 30;      // rows and keys of a sort (places are 32-bit)
+constexpr int kOneBlock = 4096;        // rows that one block sorts by itself
+inline int sort_chunk(long long n) {      // rows of a block: enough blocks to spread the work, few enough that reading all their counts is cheap
+  if (n <= kOneBlock) return n <= 0 ? kThreads : static_cast<int>((n + kThreads - 1) / kThreads) * kThreads;
+  long long c = (n + 63) / 64;
+  c = (c + kThreads - 1) / kThreads * kThreads;
+  return static_cast<int>(c < 1024 ? 1024 : c);
+}
+inline int sort_blocks(long long n) {
+  const int c = sort_chunk(n);
+  return n <= 0 ? 1 : static_cast<int>((n + c - 1) / c);
+}
+
+// `launches` of the whole sort share the far fill evenly; `at` counts them
+template <typename Src, typename Out>
+int sort_pass(const Src& src, const Out& out, int n, int bins, int align, int* hist, Fill fill, int launches, int* at, cudaStream_t st) {
+  const int chunk = sort_chunk(n), nb = sort_blocks(n);
+  const size_t smem = static_cast<size_t>(kWarps + 2) * bins * sizeof(int);
+  if (smem > 48 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(place_kernel<Src, Out>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    if (e != cudaSuccess) return static_cast<int>(e);
+  }
+  const long long vectors = fill.hi;
+  auto share = [&](Fill f) {
+    f.lo = vectors * *at / launches;
+    f.hi = vectors * (*at + 1) / launches;
+    if (*at > 0) f.n_rest = 0;
+    ++*at;
+    return f;
+  };
+  const int more = fill.far == nullptr ? 0 : static_cast<int>(vectors / launches / (kThreads * kFillRun)) + 2;      // (covers a share of vectors / launches + 1)
+  if (nb > 1) {
+    count_kernel<Src><<<nb + more, kThreads, bins * sizeof(int), st>>>(src, n, chunk, bins, nb, hist, share(fill));
+    rb_note_launch(1);
+  }
+  place_kernel<Src, Out><<<nb + more, kThreads, smem, st>>>(src, out, n, chunk, bins, align, nb, hist, share(fill));
+  rb_note_launch(1);
+  return static_cast<int>(cudaGetLastError());
+}
+
+// ----------------------------------------------------------------------------- copies of rows
+struct SourceRow {      // buffer row r <- row source[r] / k of the input
+  const int* source;
+  int k;
+  __device__ __forceinline__ long long row(long long r) const {
+    const int s = source[r];
+    return s < 0 ? -1 : s / k;
+  }
+};
+struct TokenRow {      // row r <- table row of its token
+  const void* ids;
+  int wide, rows;
+  long long start;
+  __device__ __forceinline__ long long row(long long r) const {
+    const long long a = (wide ? static_cast<const long long*>(ids)[r] : static_cast<const int*>(ids)[r]) - start;
+    return a >= 0 && a < rows ? a : -1;
+  }
+};
+
+constexpr int kMove = 4;      // vectors of a lane in flight
+// out[r] = scale * in[row(r)], zeros where there is no such row; a warp takes 32 x kMove vectors of a row
+template <typename T, int N, bool kScale, typename Row>
+__global__ void __launch_bounds__(256) move_kernel(const T* __restrict__ in, long long ld, Row src, T* __restrict__ out, long long n, int cols, int parts,
+                                                   float scale) {
+  const long long unit = blockIdx.x * 8ll + (threadIdx.x >> 5);
+  const long long r = unit / parts;
+  if (r >= n) return;
+  const int lane = threadIdx.x & 31, vecs = cols / N;
+  const int v0 = static_cast<int>(unit - r * parts) * (32 * kMove) + lane;
+  const long long s = src.row(r);
+  const Pack<T, N>* a = reinterpret_cast<const Pack<T, N>*>(in + (s < 0 ? 0 : s) * ld);
+  Pack<T, N>* o = reinterpret_cast<Pack<T, N>*>(out + r * cols);
+  Pack<T, N> p[kMove];
+#pragma unroll
+  for (int u = 0; u < kMove; ++u) {
+    const int v = v0 + u * 32;
+    p[u] = zeros<T, N>();
+    if (s >= 0 && v < vecs) p[u] = a[v];
+  }
+#pragma unroll
+  for (int u = 0; u < kMove; ++u) {
+    const int v = v0 + u * 32;
+    if (v >= vecs) break;
+    if constexpr (kScale) {
+      float f[N];
+      p[u].get(f);
+#pragma unroll
+      for (int i = 0; i < N; ++i) f[i] *= scale;
+      p[u].set(f);
+    }
+    o[v] = p[u];
+  }
+}
+
+// out[t] = sum_j w[t, j] in[dest[t, j]] in 32 bits, j ascending.  A block per token: its places are read once, and the rows that follow
+// from them in vectors of all threads, eight rows in flight (a warp per part of a row waited for its places as long as for the rows:
+// 61 us against 47 us for 65536 rows of 4 KB).
+template <typename T, int N, bool kWeight, typename OutT>
+__global__ void __launch_bounds__(256) sum_kernel(const T* __restrict__ in, long long ld, const int* __restrict__ dest, const float* __restrict__ weight,
+                                                  OutT* __restrict__ out, int k, int cols) {
+  const long long row = blockIdx.x;
+  const int vecs = cols / N;
+  constexpr int J = 8;
+  for (int v = threadIdx.x; v < vecs; v += blockDim.x) {
+    float acc[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) acc[i] = 0.f;
+    for (int j0 = 0; j0 < k; j0 += J) {
+      int d[J];
+      float w[J];
+      Pack<T, N> p[J];
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        d[j] = j0 + j < k ? dest[row * k + j0 + j] : -1;
+        w[j] = kWeight && d[j] >= 0 ? weight[row * k + j0 + j] : 1.f;
+      }
+#pragma unroll
+      for (int j = 0; j < J; ++j)
+        if (d[j] >= 0) p[j] = reinterpret_cast<const Pack<T, N>*>(in + d[j] * ld)[v];
+#pragma unroll
+      for (int j = 0; j < J; ++j)
+        if (d[j] >= 0) {
+          float f[N];
+          p[j].get(f);
+#pragma unroll
+          for (int i = 0; i < N; ++i) acc[i] = kWeight ? fmaf(w[j], f[i], acc[i]) : acc[i] + f[i];
+        }
+    }
+    Pack<OutT, N> o;
+    o.set(acc);
+    reinterpret_cast<Pack<OutT, N>*>(out + row * cols)[v] = o;
+  }
+}
+
+// Backward of the weighted sum: d_y[dest] = w d_out[t] and d_w = <d_out[t], y[dest]>.  A block per token holds its row of d_out while
+// it walks over the token's rows of y, so that all of them pass once; blocks behind the tokens write the zeros of padding rows.
+template <typename T, int N>
+__global__ void __launch_bounds__(256) sum_bwd_kernel(const T* __restrict__ d_out, long long ld, const T* __restrict__ y, long long ldy,
+                                                      const int* __restrict__ source, const int* __restrict__ dest, const float* __restrict__ weight,
+                                                      T* __restrict__ d_y, float* __restrict__ d_w, long long cap, long long n, int k, int cols) {
+  const int t = threadIdx.x, lane = t & 31, w = t >> 5, warps = blockDim.x >> 5, vecs = cols / N;
+  const long long row = blockIdx.x;
+  if (row >= n) {
+    const long long r = (row - n) * warps + w;
+    if (r >= cap || source[r] >= 0) return;
+    const Pack<T, N> z = zeros<T, N>();
+    for (int v = lane; v < vecs; v += 32) reinterpret_cast<Pack<T, N>*>(d_y + r * cols)[v] = z;
+    return;
+  }
+  __shared__ float red[8][8];
+  constexpr int J = 8;      // rows of y at a time, four of them in flight
+  const Pack<T, N>* a = reinterpret_cast<const Pack<T, N>*>(d_out + row * ld);
+  for (int j0 = 0; j0 < k; j0 += J) {
+    int d[J];
+    float wj[J], dot[J];
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      d[j] = j0 + j < k ? dest[row * k + j0 + j] : -1;
+      wj[j] = d[j] >= 0 ? weight[row * k + j0 + j] : 0.f;
+      dot[j] = 0.f;
+    }
+    for (int v = t; v < vecs; v += blockDim.x) {
+      float f[N];
+      a[v].get(f);
+#pragma unroll
+      for (int h = 0; h < J; h += 4) {
+        Pack<T, N> q[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (d[h + j] >= 0) q[j] = reinterpret_cast<const Pack<T, N>*>(y + d[h + j] * ldy)[v];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (d[h + j] >= 0) {
+            float b[N];
+            q[j].get(b);
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+              dot[h + j] = fmaf(f[i], b[i], dot[h + j]);
+              b[i] = f[i] * wj[h + j];
+            }
+            Pack<T, N> o;
+            o.set(b);
+            reinterpret_cast<Pack<T, N>*>(d_y + static_cast<long long>(d[h + j]) * cols)[v] = o;
+          }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+#pragma unroll
+      for (int m = 16; m > 0; m >>= 1) dot[j] += __shfl_xor_sync(0xffffffffu, dot[j], m);
+    }
+    if (j0 > 0) __syncthreads();
+    if (lane == 0) {
+#pragma unroll
+      for (int j = 0; j < J; ++j) red[w][j] = dot[j];
+    }
+    __syncthreads();
+    if (t < J && j0 + t < k) {
+      float s = red[0][t];
+      for (int i = 1; i < warps; ++i) s += red[i][t];
+      d_w[row * k + j0 + t] = s;
+    }
+  }
+}
+
+// ----------------------------------------------------------------------------- gradient of a table by sorted rows
+// `pairs` holds (table row, input row) in order.  A warp walks 32 of them for 32 vectors of columns and keeps one running sum; a run
+// of equal keys that ends inside goes out at once, one that goes on in the next 32 (or came from those in front) leaves a partial
+// sum, and merge_kernel adds those of a run from left to right.  The longest run does not hold up one warp this way.
+constexpr int kRun = 32;
+
+template <typename OutT, int N, bool kAdd>
+__device__ __forceinline__ void put_sum(OutT* out, long long row, int cols, int v, const float* acc, float scale) {
+  if constexpr (kAdd && N % 4 == 0) {      // (rows of 16-byte vectors)
+    float4* o = reinterpret_cast<float4*>(out + row * cols + v * N);
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {
+      float4 f = o[i];
+      f.x += acc[4 * i] * scale;
+      f.y += acc[4 * i + 1] * scale;
+      f.z += acc[4 * i + 2] * scale;
+      f.w += acc[4 * i + 3] * scale;
+      o[i] = f;
+    }
+  } else if constexpr (kAdd) {
+    out[row * cols + v] += acc[0] * scale;
+  } else {
+    float f[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) f[i] = acc[i] * scale;
+    Pack<OutT, N> p;
+    p.set(f);
+    reinterpret_cast<Pack<OutT, N>*>(out + row * cols)[v] = p;
+  }
+}
+
+template <typename T, int N, typename OutT, bool kAdd>
+__global__ void __launch_bounds__(256) run_kernel(const T* __restrict__ dy, long long ld, const int2* __restrict__ pairs, OutT* __restrict__ out,
+                                                  float* __restrict__ part, int n, int rows, int cols, int parts, float scale) {
+  const long long unit = blockIdx.x * 8ll + (threadIdx.x >> 5);
+  const int c = static_cast<int>(unit / parts);
+  if (static_cast<long long>(c) * kRun >= n) return;
+  const int lane = threadIdx.x & 31;
+  const int v = static_cast<int>(unit - static_cast<long long>(c) * parts) * 32 + lane;
+  const bool there = v < cols / N;
+  const int i0 = c * kRun;
+  const int2 pr = i0 + lane < n ? pairs[i0 + lane] : make_int2(rows, 0);
+  const int prev = i0 > 0 ? pairs[i0 - 1].x : -1, next = i0 + kRun < n ? pairs[i0 + kRun].x : rows;
+  int after = __shfl_down_sync(0xffffffffu, pr.x, 1);
+  if (lane == 31) after = next;
+  const int m = __popc(__ballot_sync(0xffffffffu, pr.x < rows));                          // keys behind the table's rows stand last
+  const unsigned ends = __ballot_sync(0xffffffffu, pr.x != after) | 1u << 31;             // a run ends here, or at least its part in this chunk
+  const bool from_front = __shfl_sync(0xffffffffu, pr.x, 0) == prev, goes_on = __shfl_sync(0xffffffffu, pr.x, 31) == next;
+  const bool copies = std::is_same<T, OutT>::value && !kAdd && scale == 1.f;              // runs of one row go out as they are
+  float acc[N];
+  bool fresh = true, head = true;      // nothing in `acc`; no run has ended in here yet
+  constexpr int U = 8;
+  for (int j0 = 0; j0 < m; j0 += U) {
+    Pack<T, N> p[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const long long pos = __shfl_sync(0xffffffffu, pr.y, j0 + u);
+      if (j0 + u < m && there) p[u] = reinterpret_cast<const Pack<T, N>*>(dy + pos * ld)[v];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int j = j0 + u;
+      if (j >= m) break;
+      const bool end = (ends >> j) & 1, before = head && from_front, behind = j == kRun - 1 && goes_on;
+      const bool whole = end && !before && !behind;
+      const long long key = __shfl_sync(0xffffffffu, pr.x, j);
+      if (copies && whole && fresh) {
+        if constexpr (std::is_same<T, OutT>::value) {
+          if (there) reinterpret_cast<Pack<T, N>*>(out + key * cols)[v] = p[u];
+        }
+        head = false;
+        continue;
+      }
+      float f[N];
+      p[u].get(f);
+#pragma unroll
+      for (int i = 0; i < N; ++i) acc[i] = fresh ? f[i] : acc[i] + f[i];
+      fresh = end;
+      if (!end) continue;
+      head = false;
+      if (!there) continue;
+      if (whole) put_sum<OutT, N, kAdd>(out, key, cols, v, acc, scale);
+      else {
+        Pack<float, N> q;
+        q.set(acc);
+        *reinterpret_cast<Pack<float, N>*>(part + (static_cast<long long>(c) * 2 + (before ? 0 : 1)) * cols + v * N) = q;
+      }
+    }
+  }
+}
+
+template <int N, typename OutT, bool kAdd>
+__global__ void __launch_bounds__(256) merge_kernel(const int2* __restrict__ pairs, const float* __restrict__ part, OutT* __restrict__ out, int n, int rows,
+                                                    int cols, int parts, float scale) {
+  const long long unit = blockIdx.x * 8ll + (threadIdx.x >> 5);
+  const long long c = unit / parts;
+  if ((c + 1) * kRun >= n) return;      // nothing behind this chunk
+  const int key = pairs[c * kRun + kRun - 1].x;
+  if (key >= rows || pairs[(c + 1) * kRun].x != key) return;                         // no run goes on
+  if (c > 0 && pairs[c * kRun].x == key && pairs[c * kRun - 1].x == key) return;      // it came from in front: another warp's
+  const int lane = threadIdx.x & 31;
+  const int v = static_cast<int>(unit % parts) * 32 + lane;
+  const bool there = v < cols / N;
+  float acc[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) acc[i] = 0.f;
+  const float* base = part + v * N;
+  if (there) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) acc[i] = base[(c * 2 + 1) * cols + i];
+  }
+  for (long long d = c + 1;; d += 32) {      // 32 chunks at a time: how many of them begin with this key
+    const long long i = (d + lane) * kRun;
+    const unsigned in = __ballot_sync(0xffffffffu, i < n && pairs[i < n ? i : 0].x == key);
+    const int m = in == 0xffffffffu ? 32 : __ffs(~in) - 1;
+    if (there) {
+      for (int j = 0; j < m; j += 8) {
+        Pack<float, N> p[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+          if (j + u < m) p[u] = *reinterpret_cast<const Pack<float, N>*>(base + (d + j + u) * 2 * cols);
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+          if (j + u < m) {
+#pragma unroll
+            for (int i2 = 0; i2 < N; ++i2) acc[i2] += p[u].v[i2];
+          }
+      }
+    }
+    if (m < 32) break;
+  }
+  if (there) put_sum<OutT, N, kAdd>(out, key, cols, v, acc, scale);
+}
+
+// ----------------------------------------------------------------------------- host
+inline bool wide_rows(const void* p, long long ld, int cols, int size) {      // rows that split into aligned 16-byte vectors
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (ld * size) % 16 == 0 && (static_cast<long long>(cols) * size) % 16 == 0;
+}
+inline long long grid_of(long long units) { return (units + 7) / 8; }
+constexpr long long kMaxGrid = 2147483647ll;
+
+template <typename T, typename Row>
+int move_t(const void* in, long long ld, const Row& src, void* out, long long n, int cols, float scale, cudaStream_t st) {
+  constexpr int NV = 16 / sizeof(T);
+  const bool wide = wide_rows(in, ld, cols, sizeof(T)) && wide_rows(out, cols, cols, sizeof(T));
+  const int per = 32 * kMove * (wide ? NV : 1), parts = (cols + per - 1) / per;
+  const long long grid = grid_of(n * parts);
+  if (grid > kMaxGrid) return -3;
+  const T* a = static_cast<const T*>(in);
+  T* o = static_cast<T*>(out);
+  const int g = static_cast<int>(grid);
+  if (wide && scale == 1.f) move_kernel<T, NV, false><<<g, 256, 0, st>>>(a, ld, src, o, n, cols, parts, scale);
+  else if (wide) move_kernel<T, NV, true><<<g, 256, 0, st>>>(a, ld, src, o, n, cols, parts, scale);
+  else if (scale == 1.f) move_kernel<T, 1, false><<<g, 256, 0, st>>>(a, ld, src, o, n, cols, parts, scale);
+  else move_kernel<T, 1, true><<<g, 256, 0, st>>>(a, ld, src, o, n, cols, parts, scale);
+  rb_note_launch(1);
+  return static_cast<int>(cudaGetLastError());
+}
+
+template <typename Row>
+int move_any(const void* in, long long ld, const Row& src, void* out, long long n, int cols, float scale, int dtype, cudaStream_t st) {
+  if (n == 0 || cols == 0) return 0;
+  switch (dtype) {
+    case 0: return move_t<__nv_bfloat16>(in, ld, src, out, n, cols, scale, st);
+    case 1: return move_t<__half>(in, ld, src, out, n, cols, scale, st);
+    case 2: return move_t<float>(in, ld, src, out, n, cols, scale, st);
+  }
+  return -1;
+}
+
+inline int row_threads(int vecs) { return vecs <= 32 ? 32 : vecs <= 64 ? 64 : vecs <= 256 ? 128 : 256; }
+
+template <typename T, int N, typename OutT>
+int sum_t(const void* in, long long ld, const int* dest, const float* weight, void* out, int n, int k, int cols, cudaStream_t st) {
+  const T* a = static_cast<const T*>(in);
+  OutT* o = static_cast<OutT*>(out);
+  const int threads = row_threads(cols / N);
+  if (weight) sum_kernel<T, N, true, OutT><<<n, threads, 0, st>>>(a, ld, dest, weight, o, k, cols);
+  else sum_kernel<T, N, false, OutT><<<n, threads, 0, st>>>(a, ld, dest, weight, o, k, cols);
+  rb_note_launch(1);
+  return static_cast<int>(cudaGetLastError());
+}
+template <typename T, typename OutT>
+int sum_any(const void* in, long long ld, const int* dest, const float* weight, void* out, int n, int k, int cols, cudaStream_t st) {
+  return wide_rows(in, ld, cols, sizeof(T)) && reinterpret_cast<uintptr_t>(out) % 32 == 0
+             ? sum_t<T, 16 / sizeof(T), OutT>(in, ld, dest, weight, out, n, k, cols, st)
+             : sum_t<T, 1, OutT>(in, ld, dest, weight, out, n, k, cols, st);
+}
+
+template <typename T>
+int sum_bwd_t(const void* d_out, long long ld, const void* y, long long ldy, const int* source, const int* dest, const float* weight, void* d_y, float* d_w,
+              long long cap, long long n, int k, int cols, cudaStream_t st) {
+  const bool wide = wide_rows(d_out, ld, cols, sizeof(T)) && wide_rows(y, ldy, cols, sizeof(T)) && wide_rows(d_y, cols, cols, sizeof(T));
+  const int threads = row_threads(cols / (wide ? 16 / static_cast<int>(sizeof(T)) : 1));
+  const long long warps = threads / 32, grid = n + (cap + warps - 1) / warps;
+  if (grid > kMaxGrid) return -3;
+  const T *a = static_cast<const T*>(d_out), *b = static_cast<const T*>(y);
+  T* o = static_cast<T*>(d_y);
+  const int g = static_cast<int>(grid);
+  if (wide) sum_bwd_kernel<T, 16 / sizeof(T)><<<g, threads, 0, st>>>(a, ld, b, ldy, source, dest, weight, o, d_w, cap, n, k, cols);
+  else sum_bwd_kernel<T, 1><<<g, threads, 0, st>>>(a, ld, b, ldy, source, dest, weight, o, d_w, cap, n, k, cols);
+  rb_note_launch(1);
+  return static_cast<int>(cudaGetLastError());
+}
+
+template <typename T, int N, typename OutT, bool kAdd>
+int runs_t(const void* dy, long long ld, const int2* pairs, void* out, float* part, int n, int rows, int cols, float scale, cudaStream_t st) {
+  const int per = 32 * N, parts = (cols + per - 1) / per;
+  const long long chunks = (n + kRun - 1) / kRun, grid = grid_of(chunks * parts);
+  if (grid > kMaxGrid) return -3;
+  run_kernel<T, N, OutT, kAdd><<<static_cast<int>(grid), 256, 0, st>>>(static_cast<const T*>(dy), ld, pairs, static_cast<OutT*>(out), part, n, rows, cols,
+                                                                       parts, scale);
+  rb_note_launch(1);
+  if (chunks > 1) {
+    merge_kernel<N, OutT, kAdd><<<static_cast<int>(grid), 256, 0, st>>>(pairs, part, static_cast<OutT*>(out), n, rows, cols, parts, scale);
+    rb_note_launch(1);
+  }
+  return static_cast<int>(cudaGetLastError());
+}
+template <typename T>
+int runs_any(const void* dy, long long ld, const int2* pairs, void* out, float* part, int n, int rows, int cols, float scale, int add, cudaStream_t st) {
+  constexpr int NV = 16 / sizeof(T);
+  const bool wide = wide_rows(dy, ld, cols, sizeof(T)) && wide_rows(out, cols, cols, add ? 4 : sizeof(T)) && wide_rows(part, cols, cols, 4);
+  if (add) return wide ? runs_t<T, NV, float, true>(dy, ld, pairs, out, part, n, rows, cols, scale, st)
+                       : runs_t<T, 1, float, true>(dy, ld, pairs, out, part, n, rows, cols, scale, st);
+  return wide ? runs_t<T, NV, T, false>(dy, ld, pairs, out, part, n, rows, cols, scale, st)
+              : runs_t<T, 1, T, false>(dy, ld, pairs, out, part, n, rows, cols, scale, st);
+}
+
+inline int key_bits(int rows) {      // of the keys 0 .. rows
+  int b = 1;
+  while (b < 31 && (rows >> b) != 0) ++b;
+  return b;
+}
+constexpr int kPassBits = 10;
+
+}  // namespace rows
+}  // namespace rb
+
+using namespace rb;
+using namespace rb::rows;
+
+extern "C" int rb_sort_counters(long long n, int bins) { return n > 0 && sort_blocks(n) > 1 ? sort_blocks(n) * bins : 1; }
+
+extern "C" int rb_expert_layout(const void* ids, int wide, int n, int experts, int align, int cap, int* dest, int* source, int* tile_expert, int* bounds,
+                                int* hist, cudaStream_t st) {
+  if (n < 0 || n > kMaxSort || experts < 1 || experts > kMaxBins || align < 1 || cap < 0 || cap % align) return -1;
+  const int tiles = align > 1 ? cap / align : 0;
+  int at = 0;
+  return sort_pass(ExpertKeys{ids, wide, experts}, ExpertOut{dest, source, align > 1 ? tile_expert : nullptr, bounds, cap, tiles}, n, experts, align, hist,
+                   Fill{source, cap, nullptr, 0, 0, nullptr, 0}, 1, &at, st);
+}
+
+extern "C" int rb_expert_dispatch(const void* x, long long ld, const int* source, void* out, int cap, int k, int cols, int dtype, cudaStream_t st) {
+  if (k < 1 || cap < 0 || cols < 0) return -1;
+  return move_any(x, ld, SourceRow{source, k}, out, cap, cols, 1.f, dtype, st);
+}
+
+extern "C" int rb_expert_combine(const void* y, long long ld, const int* dest, const float* weight, void* out, int n, int k, int cols, int dtype,
+                                 int out_fp32, cudaStream_t st) {
+  if (k < 1 || n < 0 || cols < 0) return -1;
+  if (n == 0 || cols == 0) return 0;
+  switch (dtype) {
+    case 0:
+      return out_fp32 ? sum_any<__nv_bfloat16, float>(y, ld, dest, weight, out, n, k, cols, st)
+                      : sum_any<__nv_bfloat16, __nv_bfloat16>(y, ld, dest, weight, out, n, k, cols, st);
+    case 1: return out_fp32 ? sum_any<__half, float>(y, ld, dest, weight, out, n, k, cols, st) : sum_any<__half, __half>(y, ld, dest, weight, out, n, k, cols, st);
+    case 2: return sum_any<float, float>(y, ld, dest, weight, out, n, k, cols, st);
+  }
+  return -1;
+}
+
+extern "C" int rb_expert_combine_bwd(const void* d_out, long long ld, const void* y, long long ldy, const int* source, const int* dest, const float* weight,
+                                     void* d_y, float* d_w, int cap, int n, int k, int cols, int dtype, cudaStream_t st) {
+  if (k < 1 || n < 0 || cap < 0 || cols < 0) return -1;
+  if (cap == 0 && n == 0) return 0;
+  switch (dtype) {
+    case 0: return sum_bwd_t<__nv_bfloat16>(d_out, ld, y, ldy, source, dest, weight, d_y, d_w, cap, n, k, cols, st);
+    case 1: return sum_bwd_t<__half>(d_out, ld, y, ldy, source, dest, weight, d_y, d_w, cap, n, k, cols, st);
+    case 2: return sum_bwd_t<float>(d_out, ld, y, ldy, source, dest, weight, d_y, d_w, cap, n, k, cols, st);
+  }
+  return -1;
+}
+
+extern "C" int rb_embedding(const void* ids, int wide, long long start, const void* table, long long ld, int rows, void* out, int n, int cols, float scale,
+                            int dtype, cudaStream_t st) {
+  if (n < 0 || cols < 0 || rows < 0) return -1;
+  return move_any(table, ld, TokenRow{ids, wide, rows, start}, out, n, cols, scale, dtype, st);
+}
+
+extern "C" int rb_embedding_bwd_bins(int rows) {      // counters of one block in every pass
+  const int bits = key_bits(rows), passes = (bits + kPassBits - 1) / kPassBits;
+  return 1 << ((bits + passes - 1) / passes);
+}
+
+extern "C" int rb_embedding_bwd(const void* ids, int wide, long long start, const void* dy, long long ld, void* out, int add, int2* pairs, int* hist,
+                                float* part, int n, int rows, int cols, float scale, int dtype, cudaStream_t st) {
+  if (n < 0 || n > kMaxSort || rows < 0 || rows > kMaxSort || cols < 0) return -1;
+  if (rows == 0 || cols == 0) return 0;
+  const size_t bytes = static_cast<size_t>(rows) * cols * (dtype == 2 ? 4 : 2);
+  if (n == 0) return add ? 0 : static_cast<int>(cudaMemsetAsync(out, 0, bytes, st));
+  const int bits = key_bits(rows), passes = (bits + kPassBits - 1) / kPassBits, each = (bits + passes - 1) / passes;
+  const int bins = 1 << each, mask = bins - 1;
+  Fill fill{};
+  if (!add) {
+    if (reinterpret_cast<uintptr_t>(out) % 16) return -4;
+    fill.far = static_cast<uint4*>(out);
+    fill.hi = static_cast<long long>(bytes / 16);
+    fill.rest = static_cast<unsigned char*>(out) + bytes / 16 * 16;
+    fill.n_rest = static_cast<int>(bytes % 16);
+  }
+  const int launches = passes * (sort_blocks(n) > 1 ? 2 : 1);
+  int at = 0;
+  int2* to = pairs;
+  int2* from = pairs + n;
+  for (int p = 0; p < passes; ++p) {
+    int rc;
+    if (p == 0) rc = sort_pass(TokenKeys{ids, wide, rows, 0, mask, start}, PairOut{to}, n, bins, 1, hist, fill, launches, &at, st);
+    else rc = sort_pass(PairKeys{from, p * each, mask}, PairOut{to}, n, bins, 1, hist, fill, launches, &at, st);
+    if (rc) return rc;
+    int2* s = to;
+    to = from;
+    from = s;
+  }
+  switch (dtype) {
+    case 0: return runs_any<__nv_bfloat16>(dy, ld, from, out, part, n, rows, cols, scale, add, st);
+    case 1: return runs_any<__half>(dy, ld, from, out, part, n, rows, cols, scale, add, st);
+    case 2: return runs_any<float>(dy, ld, from, out, part, n, rows, cols, scale, add, st);
+  }
+  return -1;
+}

@@ -140,26 +140,24 @@ def padded_expert_layout(expert_of_row: torch.Tensor, num_experts: int, align: i
     return order, dest, cap, tile_expert, expert_rows
 
 
+def experts_mlp(x, expert, weights, w1, w2, dtype=None):
+    """SwiGLU expert MLPs of ``x [T, H]`` for routed rows with (local) expert ids ``expert [T, k]``: rows are copied into a buffer sorted by
+    expert, the two grouped GEMMs (one launch each for all experts) and the activation run on it, and every token's rows come back as
+    their sum with ``weights [T, k]`` (None: ones) in ``dtype`` (that of ``x``).  ``w1 [E, 2F, H]``, ``w2 [E, H, F]``.  Ids outside ``[0, E)`` (experts that live on
+    another rank) cost nothing and count nothing."""
+    if not x.shape[0]:      # no rows: one that belongs to nobody, so that the graph still reaches the weights
+        pad = torch.nn.functional.pad
+        return experts_mlp(pad(x, (0, 0, 0, 1)), expert.new_full((1, expert.shape[1]), -1), None if weights is None else pad(weights, (0, 0, 0, 1)),
+                           w1, w2, dtype)[:0]
+    rows = ops.expert_layout(expert, w1.shape[0], EXPERT_ROW_ALIGN)
+    a = ops.swiglu(ops.grouped_linear(ops.expert_dispatch(x, rows), w1, rows.tile_expert, rows.expert_rows))
+    return ops.expert_combine(ops.grouped_linear(a, w2, rows.tile_expert, rows.expert_rows), weights, rows, dtype)
+
+
 def grouped_swiglu_mlp(x, expert_of_row, w1, w2, skip_foreign: bool = False):
-    """SwiGLU expert MLPs for rows ``x [R, H]`` with (local) expert ids ``expert_of_row [R]``, in the ORIGINAL row
-    order: rows are scattered into the padded expert-sorted buffer, the two grouped GEMMs (one launch each for all
-    experts) and the activation run on it, and the rows are gathered back.  ``w1 [E, 2F, H]``, ``w2 [E, H, F]``.
-    With ``skip_foreign`` rows whose id is outside ``[0, E)`` (experts that live on another rank) are parked in an
-    extra bucket whose tiles are marked unused: they cost no math and come back as zeros."""
-    E = w1.shape[0]
-    if skip_foreign:
-        eo = torch.where((expert_of_row >= 0) & (expert_of_row < E), expert_of_row, torch.full_like(expert_of_row, E))
-        order, dest, cap, tile_expert, expert_rows = padded_expert_layout(eo, E + 1)
-        tile_expert = torch.where(tile_expert == E, torch.full_like(tile_expert, -1), tile_expert)
-        expert_rows = expert_rows[:E + 1].contiguous()
-    else:
-        order, dest, cap, tile_expert, expert_rows = padded_expert_layout(expert_of_row, E)
-    xp = x.new_zeros(cap, x.shape[1]).index_copy(0, dest, x.index_select(0, order))
-    a = ops.swiglu(ops.grouped_linear(xp, w1, tile_expert, expert_rows))
-    yp = ops.grouped_linear(a, w2, tile_expert, expert_rows)
-    inv = torch.empty_like(order)
-    inv[order] = dest                       # buffer row of every original row
-    return yp.index_select(0, inv)
+    """:func:`experts_mlp` of rows ``x [R, H]`` with one expert each, in the ORIGINAL row order.  With ``skip_foreign`` rows whose id is
+    outside ``[0, E)`` come back as zeros."""
+    return experts_mlp(x, expert_of_row[:, None], None, w1, w2)
 
 
 def route_tokens(logits, cfg, bias=None):
@@ -256,51 +254,45 @@ class MoEMLP(nn.Module):
             f = torch.zeros(E, device=x.device).index_add_(0, idx.reshape(-1), torch.ones(T * k, device=x.device))
             self.last_aux = cfg.moe_aux_loss_coef * E * ((f / (T * k)) * probs.mean(0)).sum()
 
-        flat_e = idx.reshape(-1)                      # [T*k]
-        order = torch.argsort(flat_e, stable=True)    # permutation: sorted by expert
-        src_tok = order // k
-        xp = x[src_tok]                               # permuted copies [T*k, H]
-        counts = torch.bincount(flat_e, minlength=E)  # tokens per (global) expert
         if cfg.moe_router_bias and self.training:
+            counts = torch.bincount(idx.reshape(-1), minlength=E)
             self.last_counts = counts.detach() if self.last_counts is None else self.last_counts + counts.detach()
+        if ps.ep.size > 1:
+            # copies of the tokens in the order of their experts, so that every rank's rows lie together
+            rows = ops.expert_layout(idx, E, 1)
+            xp = ops.expert_dispatch(x, rows)
+            out = ops.expert_combine(self._on_owners(xp, rows.expert_rows.diff().long()), w, rows)
+        else:
+            out = experts_mlp(x, idx, w, self.experts.linear_fc1.weight, self.experts.linear_fc2.weight)
+        if cfg.moe_shared_expert_ffn > 0:
+            out = out + self._shared(x).to(out.dtype)
+        return out.to(x.dtype)
 
-        comm = getattr(self, "ep_comm", None) if x.is_cuda else None
-        if ps.ep.size > 1 and comm is not None:
+    def _on_owners(self, xp, counts):
+        """Rows ``xp`` (sorted by expert, ``counts`` per expert) through the experts, each on the rank that holds it, and back."""
+        ps = self.ps
+        ep, w1, w2 = ps.ep.size, self.experts.linear_fc1.weight, self.experts.linear_fc2.weight
+        comm = getattr(self, "ep_comm", None) if xp.is_cuda else None
+        if comm is not None:
             # dispatch / combine by peer stores into the expert owners' buffers (parallel/ep_peer.py)
             from ..parallel.ep_peer import peer_all_to_all
 
-            ep = ps.ep.size
             allc = comm.exchange_counts(counts).view(ep, ep, self.e_local)          # [src][dst][local expert]
             matrix = allc.sum(-1).tolist()
             recv_counts = allc[:, ps.ep.rank, :]
             xr = peer_all_to_all(xp, matrix, comm)
             rc = recv_counts.reshape(-1)
-            seg_expert = torch.arange(self.e_local, device=x.device).repeat(ep)
-            ye = grouped_swiglu_mlp(xr, torch.repeat_interleave(seg_expert, rc), self.experts.linear_fc1.weight,
-                                    self.experts.linear_fc2.weight)
-            yp = peer_all_to_all(ye, [[matrix[d][s_] for d in range(ep)] for s_ in range(ep)], comm)
-        elif ps.ep.size > 1:
-            ep = ps.ep.size
-            send_counts = counts.view(ep, self.e_local)
-            recv_counts = torch.empty_like(send_counts)
-            dist.all_to_all_single(recv_counts, send_counts.contiguous(), group=ps.ep.group)
-            in_splits = send_counts.sum(1).tolist()
-            out_splits = recv_counts.sum(1).tolist()
-            xr = _AllToAll.apply(xp, out_splits, in_splits, ps.ep.group)
-            # received rows are ordered (src rank, local expert); regroup by local expert
-            rc = recv_counts.reshape(-1)
-            seg_expert = torch.arange(self.e_local, device=x.device).repeat(ep)
-            row_expert = torch.repeat_interleave(seg_expert, rc)
-            yr = grouped_swiglu_mlp(xr, row_expert, self.experts.linear_fc1.weight, self.experts.linear_fc2.weight)
-            yp = _AllToAll.apply(yr, in_splits, out_splits, ps.ep.group)
-        else:
-            # rows of ``xp`` are already sorted by expert; the grouped path re-derives the (padded) layout on the
-            # device, so no count leaves the GPU
-            yp = grouped_swiglu_mlp(xp, flat_e[order], self.experts.linear_fc1.weight, self.experts.linear_fc2.weight)
-
-        wf = w.reshape(-1)[order].to(yp.dtype)
-        out = torch.zeros(T, H, dtype=yp.dtype, device=x.device)
-        out = out.index_add(0, src_tok, yp * wf[:, None])
-        if cfg.moe_shared_expert_ffn > 0:
-            out = out + self._shared(x).to(out.dtype)
-        return out.to(x.dtype)
+            seg_expert = torch.arange(self.e_local, device=xp.device).repeat(ep)
+            ye = grouped_swiglu_mlp(xr, torch.repeat_interleave(seg_expert, rc), w1, w2)
+            return peer_all_to_all(ye, [[matrix[d][s_] for d in range(ep)] for s_ in range(ep)], comm)
+        send_counts = counts.view(ep, self.e_local)
+        recv_counts = torch.empty_like(send_counts)
+        dist.all_to_all_single(recv_counts, send_counts.contiguous(), group=ps.ep.group)
+        in_splits = send_counts.sum(1).tolist()
+        out_splits = recv_counts.sum(1).tolist()
+        xr = _AllToAll.apply(xp, out_splits, in_splits, ps.ep.group)
+        # received rows are ordered (src rank, local expert); regroup by local expert
+        rc = recv_counts.reshape(-1)
+        seg_expert = torch.arange(self.e_local, device=xp.device).repeat(ep)
+        yr = grouped_swiglu_mlp(xr, torch.repeat_interleave(seg_expert, rc), w1, w2)
+        return _AllToAll.apply(yr, in_splits, out_splits, ps.ep.group)

@@ -208,39 +208,10 @@ def _vocab_shard(gen, name, cfg, v_pad, start, v_local, dtype):
     return full[start:start + v_local].to(dtype).contiguous()
 
 
-class _EmbeddingLookup(torch.autograd.Function):
-    """``weight[idx]`` (rows with ``keep`` false give zeros) whose backward adds the incoming rows straight into the
-    optimizer's fp32 gradient buffer of the weight (``weight.main_grad``) instead of materialising a dense
-    [vocab, hidden] gradient and adding that: per micro-batch only the rows that were looked up are touched."""
-
-    @staticmethod
-    def forward(ctx, weight, idx, keep):
-        ctx.weight = weight
-        ctx.save_for_backward(idx, keep if keep is not None else idx.new_empty(0))
-        ctx.has_keep = keep is not None
-        out = weight.detach()[idx]
-        return out * keep[:, None].to(out.dtype) if keep is not None else out
-
-    @staticmethod
-    def backward(ctx, dy):
-        idx, keep = ctx.saved_tensors
-        w = ctx.weight
-        if ctx.has_keep:
-            dy = dy * keep[:, None].to(dy.dtype)
-        mg = getattr(w, "main_grad", None)
-        if mg is not None and mg.dtype == torch.float32 and w.grad is not mg:
-            # sort-based accumulation: repeated tokens are summed in a fixed order (bit-identical reruns)
-            mg.index_put_((idx,), dy.float(), accumulate=True)
-            return None, None, None
-        g = torch.zeros_like(w)
-        g.index_put_((idx,), dy.to(g.dtype), accumulate=True)
-        return g, None, None
-
-
 class VocabParallelEmbedding(nn.Module):
     def __init__(self, cfg, ps, dtype, device, gen):
         super().__init__()
-        self.ps = ps
+        self.ps, self.scale = ps, cfg.embed_scale
         tp = ps.tp.size
         self.v_pad = (cfg.vocab_size + tp - 1) // tp * tp
         self.v_local = self.v_pad // tp
@@ -248,16 +219,12 @@ class VocabParallelEmbedding(nn.Module):
         self.weight = nn.Parameter(_vocab_shard(gen, "embedding", cfg, self.v_pad, self.start, self.v_local, dtype))
 
     def forward(self, tokens, sequence_parallel: bool):
+        # tokens of other shards give zeros; the gradient goes straight into the optimizer's fp32 buffer of the weight, where it touches
+        # only the rows that were looked up
         g = self.ps.tp
+        e = ops.embedding(tokens, self.weight, self.scale, self.start)
         if g.size == 1:
-            return _EmbeddingLookup.apply(self.weight, tokens, None) if self.weight.requires_grad else self.weight[tokens]
-        loc = tokens - self.start
-        ok = (loc >= 0) & (loc < self.v_local)
-        loc = torch.where(ok, loc, torch.zeros_like(loc))
-        if self.weight.requires_grad:
-            e = _EmbeddingLookup.apply(self.weight, loc, ok)
-        else:
-            e = self.weight[loc] * ok[:, None].to(self.weight.dtype)
+            return e
         if sequence_parallel:
             return TP.reduce_scatter_seq(e, g)
         return TP.reduce_from_tp(e, g)

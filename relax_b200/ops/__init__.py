@@ -307,6 +307,95 @@ def grouped_linear(x, w, tile_expert, expert_rows):
     return ref.grouped_linear(x, w, tile_expert, expert_rows)
 
 
+def expert_layout(expert_of_row, num_experts: int, align: int = 128):
+    """Layout of routed rows sorted by expert: ``expert_of_row`` (``[T, k]`` or ``[R]``, int64 or int32) names the expert of every routed row;
+    ids outside ``0 .. num_experts - 1`` live elsewhere and get no place.  Rows of an expert keep their order, and every expert begins at a
+    multiple of ``align`` (128: the tiles of :func:`grouped_linear`; 1: no padding).  Nothing is read back: the buffer has room for any routing,
+    ``min(R, E) + (R - min(R, E)) // align`` tiles.  Returns :class:`relax_b200.ops.reference.ExpertRows`."""
+    if expert_of_row.dim() not in (1, 2) or expert_of_row.dtype not in (torch.int64, torch.int32):
+        raise ValueError(f"expert_layout: int64 or int32 ids of shape [T, k] or [R], got {expert_of_row.dtype} {tuple(expert_of_row.shape)}")
+    if not 1 <= num_experts <= 2048 or not 1 <= align <= 65536:
+        raise ValueError(f"expert_layout: 1 to 2048 experts and 1 <= align <= 65536, got {num_experts} and {align}")
+    ids = expert_of_row if expert_of_row.dim() == 2 else expert_of_row[:, None]
+    if ids.shape[1] < 1:
+        raise ValueError("expert_layout: at least one expert per row")
+    return (_cuda() if _use_cuda(ids) else ref).expert_layout(ids, int(num_experts), int(align))
+
+
+def _rows_match(what, t, n):
+    if t.dim() != 2 or t.shape[0] != n:
+        raise ValueError(f"{what}: expected [{n}, columns], got {tuple(t.shape)}")
+
+
+def expert_dispatch(x, rows):
+    """``x [T, H]`` copied to the places that :func:`expert_layout` gives its routed rows, zeros in between: ``[cap, H]``.  The gradient
+    of a row is the sum over its copies, in 32 bits and in the order of the choices."""
+    _rows_match("expert_dispatch", x, rows.dest.shape[0])
+    return (_cuda() if _use_cuda(x) else ref).expert_dispatch(x, rows)
+
+
+def expert_combine(y, weights, rows, dtype=None):
+    """``out[t] = sum_j weights[t, j] y[dest[t, j]]`` (32-bit sums in the order of the choices; rows that live elsewhere count nothing; ``weights``
+    None: ones), the way back from :func:`expert_dispatch`.  ``dtype``: of the result, that of ``y`` or fp32 (the sum as it is).
+    Differentiable in ``y`` (padding rows get zeros) and in ``weights``."""
+    _rows_match("expert_combine", y, rows.source.shape[0])
+    if weights is not None and weights.shape != rows.dest.shape:
+        raise ValueError(f"expert_combine: weights of shape {tuple(rows.dest.shape)}, got {tuple(weights.shape)}")
+    if dtype not in (None, y.dtype, torch.float32):
+        raise ValueError(f"expert_combine: a result in {y.dtype} or float32, got {dtype}")
+    return (_cuda() if _use_cuda(y) else ref).expert_combine(y, weights, rows, dtype)
+
+
+def embedding(tokens, weight, scale: float = 1.0, vocab_start: int = 0):
+    """``scale * weight[tokens - vocab_start]``, zeros for tokens outside the table's rows (those of other shards).  The gradient sorts the
+    tokens and sums every table row's incoming rows in 32 bits in the order of the tokens, so reruns give the same bits; it is added to
+    the weight's fp32 ``main_grad`` where there is one, which touches only rows that were looked up."""
+    if tokens.dtype not in (torch.int64, torch.int32) or weight.dim() != 2:
+        raise ValueError(f"embedding: int64 or int32 tokens and a matrix, got {tokens.dtype} and {weight.dim()} dimensions")
+    return (_cuda() if _use_cuda(weight) else ref).embedding(tokens, weight, float(scale), int(vocab_start))
+
+
+def _distill_args(what, rows, ids, teacher_log_probs, kl_type, alpha, norm_mode, temperature):
+    if ids.dim() != 2 or ids.dtype != torch.int64 or ids.shape[0] != rows or teacher_log_probs.shape != ids.shape:
+        raise ValueError(f"{what}: int64 ids [{rows}, K] and teacher log-probs of their shape, got {ids.dtype} {tuple(ids.shape)} and "
+                         f"{tuple(teacher_log_probs.shape)}")
+    if ids.shape[1] > 1024:
+        raise ValueError(f"{what}: up to 1024 ids per row, got {ids.shape[1]}")
+    if kl_type not in ("reverse_kl", "forward_kl", "jsd", "low_var_kl"):
+        raise ValueError(f"{what}: unknown divergence {kl_type!r}")
+    if norm_mode not in ("tail", "norm", "trunc"):
+        raise ValueError(f"{what}: norm_mode is tail, norm or trunc, got {norm_mode!r}")
+    if not 0.0 <= alpha <= 1.0:
+        raise ValueError(f"{what}: alpha must lie in [0, 1], got {alpha}")
+    if not 0.0 < temperature < float("inf"):
+        raise ValueError(f"{what}: temperature must be positive, got {temperature}")
+
+
+def topk_distill(logits, ids, teacher_log_probs, kl_type: str = "reverse_kl", alpha: float = 0.5, norm_mode: str = "tail", temperature: float = 1.0,
+                 log_prob_min_clamp=None, return_log_probs: bool = False):
+    """Divergence ``[R]`` of a student, given by whole rows of ``logits [R, V]``, from a teacher known on ``K`` ids per row (``ids [R, K]``, entries
+    outside ``0 .. V - 1`` are absent; fp32 ``teacher_log_probs [R, K]``): :func:`relax_b200.algo.opd.token_kl` on the student's log-probs of the
+    ids, differentiable in the logits.  The forward pass reads the logits once, the backward pass once more; rows whose incoming gradient is
+    zero get zeros.  With ``return_log_probs`` also the student's log-probs of the ids (-inf where absent; no gradient)."""
+    if logits.dim() != 2 or logits.shape[1] < 1:
+        raise ValueError(f"topk_distill: logits [rows, vocabulary], got {tuple(logits.shape)}")
+    _distill_args("topk_distill", logits.shape[0], ids, teacher_log_probs, kl_type, alpha, norm_mode, temperature)
+    return (_cuda() if _use_cuda(logits) else ref).topk_distill(logits, ids, teacher_log_probs, kl_type, float(alpha), norm_mode, float(temperature),
+                                                                log_prob_min_clamp, return_log_probs)
+
+
+def fused_lm_head_topk_distill(hidden, weight, ids, teacher_log_probs, kl_type: str = "reverse_kl", alpha: float = 0.5, norm_mode: str = "tail",
+                               temperature: float = 1.0, log_prob_min_clamp=None, chunk_size: int = 2048):
+    """:func:`topk_distill` of ``hidden @ weight.T`` in fp32, ``chunk_size`` rows of logits at a time; the backward pass computes them again."""
+    _distill_args("fused_lm_head_topk_distill", hidden.shape[0], ids, teacher_log_probs, kl_type, alpha, norm_mode, temperature)
+    if _use_cuda(hidden):
+        return _cuda().fused_lm_head_topk_distill(hidden, weight, ids, teacher_log_probs, kl_type, float(alpha), norm_mode, float(temperature),
+                                                  log_prob_min_clamp, chunk_size)
+    out = [ref.topk_distill(hidden[s:s + chunk_size] @ weight.t(), ids[s:s + chunk_size], teacher_log_probs[s:s + chunk_size], kl_type, alpha, norm_mode,
+                            temperature, log_prob_min_clamp, False) for s in range(0, max(1, hidden.shape[0]), chunk_size)]
+    return torch.cat(out)
+
+
 def decode_advance(tok_new, lp_new, state, block_size):
     """In-place advance of the rollout engine's device-resident batch state after one decode step."""
     if _use_cuda(tok_new):

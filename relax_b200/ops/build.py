@@ -25,7 +25,7 @@ SERVING_SOURCES = ["attention_fwd_sm100.cu", "decode_attn_tc_sm100.cu", "decode_
                    "moe_stack_sm100.cu", "paged_flash_sm100.cu", "stack_sm100.cu", "stream_sm100.cu", "talk_decode_sm100.cu", "talk_flash_sm100.cu",
                    "bindings_serving.cpp", "launch_count.cpp", "module_serving.cpp"]
 # fp32 results of these kernels are compared at fp32 rounding: IEEE division, square root and library exponentials
-PRECISE_SOURCES = {"stack_sm100.cu", "gqa_stack_sm100.cu", "mingru_sm100.cu", "moe_stack_sm100.cu", "stream_sm100.cu"}
+PRECISE_SOURCES = {"stack_sm100.cu", "gqa_stack_sm100.cu", "mingru_sm100.cu", "moe_stack_sm100.cu", "stream_sm100.cu", "rows_sm100.cu", "distill_sm100.cu"}
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "--use_fast_math",

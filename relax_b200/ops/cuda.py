@@ -11,6 +11,9 @@ import os
 from typing import Optional
 
 import torch
+from torch.autograd.function import once_differentiable
+
+from .reference import ExpertRows, main_grad_of
 
 _SO = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "_C.so")
 _SO_SERVING = _SO.replace("_C.so", "_C_serving.so")      # serving subset (ops/build.py)
@@ -1220,6 +1223,90 @@ def grouped_linear(x, w, tile_expert, expert_rows):
     if x.dtype != torch.bfloat16 or x.shape[0] % 128 or w.shape[1] % 64 or w.shape[2] % 64:
         raise ValueError("grouped GEMM: bf16, token rows padded to 128 per expert, expert dims multiples of 64")
     return _GroupedLinear.apply(x, w, tile_expert, expert_rows)
+
+
+# --------------------------------------------------------------------------- rows by key
+
+
+def expert_layout(ids, num_experts, align):
+    return ExpertRows(*_load().expert_layout(ids, num_experts, align), num_experts, align)
+
+
+def expert_dispatch(x, rows):
+    return _load().expert_dispatch(x, rows.dest, rows.source)
+
+
+def expert_combine(y, weights, rows, dtype=None):
+    return _load().expert_combine(y, weights, rows.dest, rows.source, dtype == torch.float32)
+
+
+def embedding(tokens, weight, scale, vocab_start):
+    mg = main_grad_of(weight)
+    return _load().embedding(weight, tokens, scale, vocab_start, mg if mg is not None and mg.is_contiguous() else None)
+
+
+# --------------------------------------------------------------------------- distillation from top ids
+
+_DISTILL_KL = {"reverse_kl": 0, "forward_kl": 1, "jsd": 2, "low_var_kl": 3}
+_DISTILL_NORM = {"tail": 0, "norm": 1, "trunc": 2}
+
+
+def _distill_codes(kl_type, alpha, norm_mode, temperature, clamp):
+    kl = _DISTILL_KL[kl_type]
+    if kl == 2 and alpha in (0.0, 1.0):      # the mixture is one of the two
+        kl = int(alpha)
+    return kl, _DISTILL_NORM[norm_mode], alpha, -math.inf if clamp is None else float(clamp), 1.0 / temperature
+
+
+def topk_distill(logits, ids, teacher, kl_type, alpha, norm_mode, temperature, clamp, want):
+    return _load().topk_distill(logits, ids, teacher.detach(), *_distill_codes(kl_type, alpha, norm_mode, temperature, clamp), bool(want))
+
+
+class _FusedHeadDistill(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, hidden, weight, ids, teacher, codes, chunk):
+        L = _load()
+        h, w = hidden.contiguous(), weight.contiguous()
+        R, K = ids.shape
+        f32 = lambda *s: torch.empty(*s, dtype=torch.float32, device=h.device)      # noqa: E731
+        loss, coef, stats = f32(R), f32(R, K), f32(R, 4)
+        for s in range(0, R, chunk):
+            e = min(R, s + chunk)
+            z = matmul_nt(h[s:e], w, out_dtype=torch.float32)
+            loss[s:e], coef[s:e], stats[s:e] = L.topk_distill_rows(z, ids[s:e], teacher[s:e], *codes)
+        ctx.save_for_backward(h, w, ids, coef, stats)
+        ctx.meta = (codes[-1], chunk, weight)
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        h, w, ids, coef, stats = ctx.saved_tensors
+        inv_temp, chunk, weight = ctx.meta
+        L = _load()
+        g = g.float().contiguous()
+        R, V = h.shape[0], w.shape[0]
+        dh = torch.empty_like(h)
+        mg = main_grad_of(weight)
+        direct = mg is not None and mg.stride(-1) == 1
+        dw = mg if direct else torch.zeros(w.shape, dtype=torch.float32, device=h.device)
+        for s in range(0, R, chunk):
+            e = min(R, s + chunk)
+            z = matmul_nt(h[s:e], w, out_dtype=torch.float32)
+            d = torch.empty(e - s, V, dtype=h.dtype, device=h.device)
+            L.topk_distill_rows_bwd(z, ids[s:e], coef[s:e], stats[s:e], g[s:e], inv_temp, d)
+            matmul_nn(d, w, out=dh[s:e])
+            matmul_tn(d, h[s:e], out=dw, accumulate=True)
+        return dh, None if direct else dw.to(weight.dtype), None, None, None, None
+
+
+def fused_lm_head_topk_distill(hidden, weight, ids, teacher, kl_type, alpha, norm_mode, temperature, clamp, chunk):
+    if hidden.dtype != torch.bfloat16 or weight.dtype != torch.bfloat16:
+        raise TypeError("fused LM head expects bf16 hidden states")
+    if weight.shape[0] % 8 or weight.shape[1] % 8:
+        raise ValueError(f"fused LM head: vocabulary and width are multiples of 8, got {tuple(weight.shape)}")
+    return _FusedHeadDistill.apply(hidden, weight, ids.contiguous(), teacher.detach().float().contiguous(),
+                                   _distill_codes(kl_type, alpha, norm_mode, temperature, clamp), int(chunk))
 
 
 def launch_count() -> int:

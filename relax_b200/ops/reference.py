@@ -715,3 +715,139 @@ def blockwise_dequant_fp8(q, scale_inv, block: int = 128, dtype=torch.bfloat16):
     M, N = q.shape
     s = scale_inv.repeat_interleave(block, 0)[:M].repeat_interleave(block, 1)[:, :N]
     return (q.float() * s).to(dtype)
+
+
+# --------------------------------------------------------------------------- rows by key
+
+
+class ExpertRows:
+    """Where routed rows go in a buffer sorted by expert (:func:`relax_b200.ops.expert_layout`): ``dest [T, k]`` the buffer row of every
+    routed row (-1: its expert is elsewhere), ``source [cap]`` the routed row of every buffer row (-1: padding), ``tile_expert`` the expert of
+    every ``align`` buffer rows (-1: unused; None where ``align`` is 1), ``expert_rows [E + 1]`` the experts' first buffer rows."""
+    __slots__ = ("dest", "source", "tile_expert", "expert_rows", "experts", "align")
+
+    def __init__(self, dest, source, tile_expert, expert_rows, experts, align):
+        self.dest, self.source, self.tile_expert, self.expert_rows, self.experts, self.align = dest, source, tile_expert, expert_rows, experts, align
+
+
+def expert_layout(expert_of_row, num_experts: int, align: int = 128) -> ExpertRows:
+    e = expert_of_row.reshape(-1).long()
+    n, dev = e.numel(), e.device
+    some = min(n, num_experts)
+    cap = n if align == 1 else (some + (n - some) // align) * align
+    key = torch.where((e >= 0) & (e < num_experts), e, num_experts)
+    count = torch.zeros(num_experts + 1, dtype=torch.int64, device=dev).index_add_(0, key, torch.ones_like(key))[:num_experts]
+    ends = ((count + align - 1) // align * align).cumsum(0)
+    first = torch.cat([ends.new_zeros(1), ends])
+    order = torch.argsort(key, stable=True)
+    rank = torch.empty_like(key)
+    rank[order] = torch.arange(n, device=dev)
+    rank -= torch.cat([count.new_zeros(1), count.cumsum(0)])[key]       # among the rows of the same expert
+    dest = torch.where(key < num_experts, first[key] + rank, -1)
+    source = torch.full((cap + 1,), -1, dtype=torch.int64, device=dev)
+    source[torch.where(dest < 0, cap, dest)] = torch.arange(n, device=dev)
+    tiles = None
+    if align > 1:
+        start = torch.arange(cap // align, device=dev) * align
+        tiles = torch.searchsorted(ends, start, right=True)
+        tiles = torch.where(tiles < num_experts, tiles, -1).int()
+    return ExpertRows(dest.view(expert_of_row.shape).int(), source[:cap].int(), tiles, first.int(), num_experts, align)
+
+
+def _with_zero_row(t):
+    return torch.cat([t, t.new_zeros(1, t.shape[1])])
+
+
+def expert_dispatch(x, rows: ExpertRows):
+    s, k = rows.source.long(), rows.dest.shape[1]
+    return _with_zero_row(x)[torch.where(s < 0, x.shape[0], torch.div(s, k, rounding_mode="floor"))]
+
+
+def expert_combine(y, weights, rows: ExpertRows, dtype=None):
+    d = rows.dest.long()
+    here = d >= 0
+    yz = _with_zero_row(y)
+    acc = torch.zeros(d.shape[0], y.shape[1], dtype=torch.float32, device=y.device)
+    for j in range(d.shape[1]):
+        v = yz[torch.where(here[:, j], d[:, j], y.shape[0])].float()
+        acc = acc + (v if weights is None else v * torch.where(here[:, j], weights[:, j].float(), 0.0)[:, None])
+    return acc.to(dtype or y.dtype)
+
+
+def main_grad_of(w):
+    """The optimizer's fp32 gradient buffer of a weight, where a gradient can be added to it."""
+    mg = getattr(w, "main_grad", None)
+    return mg if mg is not None and mg.dtype == torch.float32 and mg.shape == w.shape and w.grad is not mg else None
+
+
+class _Embedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, weight, tokens, scale, start):
+        at = tokens - start
+        here = (at >= 0) & (at < weight.shape[0])
+        at = torch.where(here, at, torch.zeros_like(at))
+        ctx.weight, ctx.scale = weight, scale
+        ctx.save_for_backward(at, here)
+        if not weight.shape[0]:
+            return weight.new_zeros(*tokens.shape, weight.shape[1])
+        out = weight.detach()[at]
+        if scale != 1.0:
+            out = (out.float() * scale).to(weight.dtype)
+        return torch.where(here[..., None], out, torch.zeros((), dtype=out.dtype, device=out.device))
+
+    @staticmethod
+    def backward(ctx, dy):
+        at, here = ctx.saved_tensors
+        w, mg = ctx.weight, main_grad_of(ctx.weight)
+        g = torch.zeros(w.shape, dtype=torch.float32, device=w.device) if mg is None else mg
+        if w.shape[0]:
+            # repeated tokens are summed in a fixed order (bit-identical reruns)
+            d = dy[here].float()
+            g.index_put_((at[here],), d * ctx.scale if ctx.scale != 1.0 else d, accumulate=True)
+        return (g.to(w.dtype) if mg is None else None), None, None, None
+
+
+def embedding(tokens, weight, scale: float = 1.0, vocab_start: int = 0):
+    return _Embedding.apply(weight, tokens, float(scale), int(vocab_start))
+
+
+# --------------------------------------------------------------------------- distillation from top ids
+
+
+def topk_distill(logits, ids, teacher_log_probs, kl_type, alpha, norm_mode, temperature, log_prob_min_clamp, return_log_probs):
+    z = logits.double() / temperature
+    away = (ids < 0) | (ids >= z.shape[1])
+    lp = (z - torch.logsumexp(z, -1, keepdim=True)).gather(1, torch.where(away, 0, ids))
+    found = lp.masked_fill(away, float("-inf")).float()
+    t = teacher_log_probs.double()
+    if log_prob_min_clamp is not None:
+        lp, t = lp.clamp_min(log_prob_min_clamp), t.clamp_min(log_prob_min_clamp)
+    none = torch.zeros((), dtype=torch.float64, device=z.device)
+    if kl_type == "low_var_kl":
+        r = torch.where(away, none, lp - t)
+        loss = (torch.exp(-r) - 1.0 + r).sum(-1)
+    else:
+        a = {"reverse_kl": 0.0, "forward_kl": 1.0}.get(kl_type, alpha)
+        gone = -1e30                                             # (finite: gradients of absent ids are zeros)
+        s, t = lp.masked_fill(away, gone), t.masked_fill(away, gone)
+        keep = ~away
+        if norm_mode == "norm":
+            s, t = torch.log_softmax(s, -1), torch.log_softmax(t, -1)
+        elif norm_mode == "tail":
+            rest = lambda l: torch.log(-torch.expm1(torch.logsumexp(l, -1, keepdim=True).clamp(max=-1e-7)))      # noqa: E731
+            s, t = torch.cat([s, rest(s)], -1), torch.cat([t, rest(t)], -1)
+            keep = torch.cat([keep, torch.ones_like(keep[:, :1])], -1)
+
+        def kl(p, q):      # sum exp(p) (p - q); an outcome without mass counts nothing
+            keep_p = keep & (p > float("-inf"))
+            d = torch.where(keep_p, p, none) - torch.where(keep_p, q, none)
+            return torch.where(keep_p, torch.where(keep_p, p, none).exp() * d, none).sum(-1)
+
+        if a == 0.0:
+            loss = kl(s, t)
+        elif a == 1.0:
+            loss = kl(t, s)
+        else:
+            m = torch.logaddexp(s + math.log(1.0 - a), t + math.log(a))
+            loss = (1.0 - a) * kl(s, m) + a * kl(t, m)
+    return (loss.float(), found.detach()) if return_log_probs else loss.float()

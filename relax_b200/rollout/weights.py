@@ -216,12 +216,9 @@ class RolloutWeights(ComposedForward):
 
     # ------------------------------------------------------------------ model pieces
     def _embed(self, tokens, tp: GroupInfo):
-        w = self.p["embed"]
         if tp.size == 1:
-            return w[tokens]
-        loc = tokens - self.vocab_start
-        ok = (loc >= 0) & (loc < self.v_local)
-        e = w[torch.where(ok, loc, torch.zeros_like(loc))] * ok[:, None].to(w.dtype)
+            return ops.embedding(tokens, self.p["embed"], self.cfg.embed_scale)
+        e = ops.embedding(tokens, self.p["embed"], self.cfg.embed_scale, self.vocab_start)
         dist.all_reduce(e, group=tp.group)
         return e
 
@@ -252,22 +249,17 @@ class RolloutWeights(ComposedForward):
             w, idx, _ = route_tokens(logits, cfg, p.get(pre + "router_bias"))
             if self.routing_capture is not None:
                 self.routing_capture.append(idx)
-            out = torch.zeros_like(x, dtype=torch.float32)
+            # every routed (token, slot) pair through the grouped expert GEMMs in one go: rows of experts that live on another EP rank get
+            # no place, and the per-token sum over the k slots applies the gate weights in fp32
+            from ..models.moe import experts_mlp
+
+            el = p[pre + "experts_gate_up"].shape[0]
+            out = experts_mlp(x, idx - self.ep_rank * el, w, p[pre + "experts_gate_up"], p[pre + "experts_down"], torch.float32)
             if pre + "shared_gate_up" in p and self.ep_rank == 0:     # summed over the EP ranks afterwards: one rank adds it
                 sh = ops.linear(ops.swiglu(ops.linear(x, p[pre + "shared_gate_up"])), p[pre + "shared_down"]).float()
                 if pre + "shared_gate" in p:
                     sh = sh * torch.sigmoid(ops.linear(x, p[pre + "shared_gate"]).float())
-                out += sh
-            # every routed (token, slot) pair through the grouped expert GEMMs in one go: rows of experts that live on
-            # another EP rank are parked (no math), the per-token sum over the k slots applies the gate weights
-            from ..models.moe import grouped_swiglu_mlp
-
-            el = p[pre + "experts_gate_up"].shape[0]
-            T, k = idx.shape
-            rows = x.repeat_interleave(k, 0)                        # row t*k + j = token t, slot j
-            y = grouped_swiglu_mlp(rows, idx.reshape(-1) - self.ep_rank * el, p[pre + "experts_gate_up"],
-                                   p[pre + "experts_down"], skip_foreign=True)
-            out += (y.float().view(T, k, -1) * w.float().unsqueeze(-1)).sum(1)
+                out = sh + out
             return out.to(x.dtype), (self.ep_group if self.ep_size > 1 else None)
         if self.lora:       # adapter-mode serving: the factors' products join before the activation / before the reduction
             a = ops.swiglu(self._lora_add(pre + "gate_up", x, ops.linear(x, p[pre + "gate_up"])))

@@ -1,0 +1,391 @@
+"""sm_100a kernels of rows sorted by expert and back, the embedding with its gradient and the distillation divergence, against plain statements in 64
+bits.  Tolerances count roundings: half a step of the result's type (eps / 2) and 2^-24 per 32-bit operation."""
+import math
+
+import pytest
+import torch
+
+import oracle_rows as O
+from relax_b200 import ops
+
+pytestmark = pytest.mark.gpu
+
+F = 2.0 ** -24
+DT = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
+
+
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _half_step(t):
+    return torch.finfo(t).eps / 2
+
+
+def _within(got, want, tol, what=""):
+    got = got.detach().double().cpu()
+    bad = ~((got - want).abs() <= tol)
+    assert not bool(bad.any()), f"{what}: {int(bad.sum())} of {bad.numel()}, worst {float(((got - want).abs() - tol).max()):.3e} over"
+
+
+# --------------------------------------------------------------------------- experts' rows
+
+
+@pytest.mark.parametrize("wide", [True, False])
+@pytest.mark.parametrize("T,k,E,align", [(0, 2, 4, 128), (1, 1, 1, 128), (1, 8, 128, 128), (96, 8, 32, 128), (513, 3, 11, 128), (5000, 2, 300, 128), (2500, 8, 256, 1),
+                                         (1700, 3, 2048, 16), (7, 40, 60, 128), (9001, 1, 5, 1)])
+def test_layout(T, k, E, align, wide):
+    g = torch.Generator().manual_seed(T + k)
+    ids = (torch.randn(T, k, generator=g) * E * 0.6).long()              # half of them elsewhere, experts of very different load
+    rows = ops.expert_layout((ids if wide else ids.int()).cuda(), E, align)
+    dest, source, tiles, bounds = O.layout(ids, E, align)
+    assert rows.dest.shape == (T, k) and rows.dest.reshape(-1).tolist() == dest
+    assert rows.source.tolist() == source and rows.expert_rows.tolist() == bounds
+    assert rows.tile_expert is None if align == 1 else rows.tile_expert.tolist() == tiles
+
+
+@pytest.mark.parametrize("pattern", ["one expert", "all elsewhere", "descending"])
+def test_layout_of_lopsided_rows(pattern):
+    n = 6000
+    ids = {"one expert": torch.full((n, 1), 3), "all elsewhere": torch.full((n, 1), -1), "descending": torch.arange(n - 1, -1, -1)[:, None] // 60}[pattern]
+    rows = ops.expert_layout(ids.cuda(), 100, 128)
+    dest, source, tiles, bounds = O.layout(ids, 100, 128)
+    assert rows.dest.reshape(-1).tolist() == dest and rows.source.tolist() == source
+    assert rows.tile_expert.tolist() == tiles and rows.expert_rows.tolist() == bounds
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("T,k,E,H", [(1, 1, 1, 8), (1, 8, 128, 2048), (70, 2, 9, 1), (333, 3, 11, 1001), (260, 8, 16, 264), (50, 37, 40, 520)])
+def test_dispatch_and_combine(T, k, E, H, dtype):
+    dt, g = DT[dtype], _gen(T + H)
+    ids = torch.randint(-1, E + 1, (T, k), device="cuda", generator=g)
+    rows = ops.expert_layout(ids, E)
+    dest, source, _, _ = O.layout(ids.cpu(), E, 128)
+    cap = len(source)
+    x = torch.randn(T, H + 8, device="cuda", generator=g).to(dt)[:, :H].requires_grad_()               # rows apart from one another
+    y = torch.randn(cap, H, device="cuda", generator=g).to(dt)
+    pad = torch.tensor(source) < 0
+    y[pad.cuda()] = float("nan")                                                                       # padding is not looked at
+    y.requires_grad_()
+    w = torch.rand(T, k, device="cuda", generator=g)
+    w[ids < 0] = float("inf")                                                                          # nor are weights of rows elsewhere
+    w.requires_grad_()
+    srt, out = ops.expert_dispatch(x, rows), ops.expert_combine(y, w, rows)
+    assert torch.equal(srt.detach().double().cpu(), O.dispatch(x.detach().cpu(), source, k))
+    yc, wc = y.detach().cpu(), w.detach().cpu()
+    want, size = O.combine(yc, wc, dest, k)
+    half = _half_step(dt)
+    _within(out, want, half * want.abs() + (1 + half) * (k + 1) * F * size + 2.0 ** -25, "combine")
+    _within(ops.expert_combine(y, w, rows, torch.float32), want, (k + 1) * F * size, "combine in fp32")
+    plain, psize = O.combine(yc, None, dest, k)
+    _within(ops.expert_combine(y, None, rows), plain, half * plain.abs() + (1 + half) * (k + 1) * F * psize + 2.0 ** -25, "plain sum")
+
+    d_s, d_o = torch.randn(cap, H, device="cuda", generator=g).to(dt), torch.randn(T, H, device="cuda", generator=g).to(dt)
+    d_x, d_y, d_w = torch.autograd.grad([srt, out], [x, y, w], [d_s, d_o])
+    want, size = O.combine(d_s.cpu(), None, dest, k)
+    _within(d_x, want, half * want.abs() + (1 + half) * (k + 1) * F * size + 2.0 ** -25, "d x")
+    doc = d_o.cpu().double()
+    want_y, want_w, size_w = torch.zeros(cap, H, dtype=torch.float64), torch.zeros(T * k, dtype=torch.float64), torch.zeros(T * k, dtype=torch.float64)
+    for i, d in enumerate(dest):
+        if d >= 0:
+            want_y[d] = doc[i // k] * float(wc.reshape(-1)[i])
+            terms = doc[i // k] * yc[d].double()
+            want_w[i], size_w[i] = terms.sum(), terms.abs().sum()
+    _within(d_y, want_y, (half + 2 * F) * want_y.abs() + 2.0 ** -25, "d y")
+    _within(d_w.reshape(-1), want_w, (H / 32 + 8) * F * size_w, "d weights")      # a lane sums H / 32 terms, five more additions join the lanes
+
+
+def test_rows_again_give_the_same_bits_and_may_be_captured():
+    g = _gen(5)
+    ids = torch.randint(0, 16, (700, 4), device="cuda", generator=g)
+    x = torch.randn(700, 256, device="cuda", generator=g).bfloat16()
+    w = torch.rand(700, 4, device="cuda", generator=g)
+    tok = torch.randint(0, 50, (5000,), device="cuda", generator=g)
+    table = torch.randn(64, 256, device="cuda", generator=g).bfloat16()
+    dy = torch.randn(5000, 256, device="cuda", generator=g).bfloat16()
+
+    def all_of_them():
+        rows = ops.expert_layout(ids, 16)
+        y = ops.expert_dispatch(x, rows)
+        t = table.detach().requires_grad_()
+        d = torch.autograd.grad(ops.embedding(tok, t, 2.0), t, dy)[0]
+        return [rows.dest, rows.source, y, ops.expert_combine(y, w, rows), d]
+
+    first = [t.clone() for t in all_of_them()]
+    assert all(torch.equal(a, b) for a, b in zip(first, all_of_them()))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        all_of_them()
+        again = all_of_them()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(first, again))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = all_of_them()
+    ids.copy_(torch.randint(0, 16, (700, 4), device="cuda", generator=g))
+    tok.copy_(torch.randint(0, 50, (5000,), device="cuda", generator=g))
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip([t.clone() for t in held], all_of_them()))
+
+
+def test_refusals():
+    ids = torch.zeros(4, 2, dtype=torch.int64, device="cuda")
+    rows = ops.expert_layout(ids, 3)
+    with pytest.raises(TypeError, match="bf16, fp16 or fp32"):
+        ops.expert_dispatch(torch.zeros(4, 8, device="cuda", dtype=torch.float64), rows)
+    with pytest.raises(TypeError, match="bf16, fp16 or fp32"):
+        ops.embedding(ids[:, 0], torch.zeros(4, 8, device="cuda", dtype=torch.float64))
+    with pytest.raises(ValueError, match="is on"):
+        ops.embedding(ids[:, 0].cpu(), torch.zeros(4, 8, device="cuda"))
+    with pytest.raises(ValueError, match="is on"):
+        ops.expert_dispatch(torch.zeros(4, 8, device="cuda"), ops.expert_layout(ids.cpu(), 3))
+    with pytest.raises(ValueError, match="is on"):
+        ops.topk_distill(torch.zeros(4, 8, device="cuda"), ids.cpu(), torch.zeros(4, 2, device="cuda"))
+    with pytest.raises(TypeError, match="bf16, fp16 or fp32"):
+        ops.topk_distill(torch.zeros(4, 8, device="cuda", dtype=torch.float64), ids, torch.zeros(4, 2, device="cuda"))
+    with pytest.raises(ValueError, match="float32"):
+        ops.expert_combine(torch.zeros(rows.source.numel(), 8, device="cuda"), None, rows, torch.bfloat16)
+    with pytest.raises(TypeError, match="bf16"):
+        ops.fused_lm_head_topk_distill(torch.zeros(4, 8, device="cuda"), torch.zeros(16, 8, device="cuda"), ids, torch.zeros(4, 2, device="cuda"))
+    with pytest.raises(ValueError, match="multiples of 8"):
+        ops.fused_lm_head_topk_distill(torch.zeros(4, 8, device="cuda").bfloat16(), torch.zeros(15, 8, device="cuda").bfloat16(), ids,
+                                       torch.zeros(4, 2, device="cuda"))
+
+
+# --------------------------------------------------------------------------- embedding
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("n,V,H,start,scale,tokens", [
+    (0, 16, 8, 0, 1.0, "few"), (1, 1, 1, 0, 1.0, "few"), (33, 7, 3, 0, 45.0, "few"), (700, 1000, 264, 0, 1.0, "few"), (9000, 151936, 40, 0, 1.0, "zipf"),
+    (5000, 2000, 136, 4000, 2.0, "zipf"), (5000, 300, 72, 0, 1.0, "one"), (8300, 2500, 11, 0, 1.0, "runs"), (64, 1 << 20, 8, 0, 1.0, "zipf")])
+def test_embedding(n, V, H, start, scale, tokens, dtype):
+    dt, g = DT[dtype], _gen(n + H)
+    u = torch.rand(n, device="cuda", generator=g)
+    ids = {"few": (u * (V + 2)).long() - 1, "zipf": torch.exp(u * math.log(V + start)).long() - 1, "one": torch.full((n,), V - 1, device="cuda"),
+           "runs": torch.arange(n, device="cuda") // 32 % V}[tokens]
+    table = torch.randn(V, H, device="cuda", generator=g).to(dt).requires_grad_()
+    out = ops.embedding(ids, table, scale, start)
+    at = (ids - start).cpu()
+    here = (at >= 0) & (at < V)
+    want = torch.where(here[:, None], table.detach().cpu().double()[at.clamp(0, V - 1)] * scale, torch.zeros((), dtype=torch.float64))
+    half = _half_step(dt)
+    _within(out, want, 0.0 if scale == 1.0 else (half + 2 * F) * want.abs(), "rows")
+    dy = torch.randn(n, H, device="cuda", generator=g).to(dt)
+    (d,) = torch.autograd.grad(out, table, dy)
+    here_at = at[here]
+    c = torch.zeros(V, dtype=torch.float64).index_add_(0, here_at, torch.ones(here_at.numel(), dtype=torch.float64))
+    up = dy.cpu().double()[here] * scale
+    want = torch.zeros(V, H, dtype=torch.float64).index_add_(0, here_at, up)
+    size = torch.zeros(V, H, dtype=torch.float64).index_add_(0, here_at, up.abs())
+    sums = (c[:, None] + 2) * F * size
+    assert d.dtype == dt
+    _within(d, want, half * want.abs() + (1 + half) * sums + 2.0 ** -25, "gradient")
+    # into the optimizer's buffer: one more addition
+    table.main_grad = torch.randn(V, H, device="cuda", generator=g)
+    before = table.main_grad.cpu().double()
+    ops.embedding(ids, table, scale, start).backward(dy)
+    assert table.grad is None
+    _within(table.main_grad, before + want, sums + F * (before.abs() + want.abs() + sums), "main_grad")
+    untouched = c == 0
+    assert torch.equal(table.main_grad.cpu().double()[untouched], before[untouched])
+
+
+def test_embedding_of_odd_views():
+    g = _gen(1)
+    table = torch.randn(50, 24, device="cuda", generator=g).bfloat16()[:, 3:20]                 # rows that begin anywhere
+    ids = torch.randint(0, 50, (4, 9), device="cuda", generator=g, dtype=torch.int32)
+    assert torch.equal(ops.embedding(ids, table), table[ids.long()])
+    assert torch.equal(ops.embedding(ids.t(), table), table[ids.t().long()])
+    leaf = table.contiguous().requires_grad_()
+    dy = torch.randn(4, 17, device="cuda", generator=g).bfloat16()[:, None].expand(4, 9, 17)      # a broadcast gradient
+    (d,) = torch.autograd.grad(ops.embedding(ids, leaf), leaf, dy)
+    want, size = O.embedding_grad(ids.cpu(), dy.reshape(-1, 17).cpu(), 50, 0, 1.0)
+    _within(d, want, 2.0 ** -8 * want.abs() + 40 * F * size, "gradient")
+
+
+# --------------------------------------------------------------------------- distillation
+
+
+def _case(R, V, K, dtype, seed, spread=3.0):
+    g = _gen(seed)
+    z = (spread * torch.randn(R, V, device="cuda", generator=g)).to(DT[dtype])
+    ids = torch.stack([torch.randperm(V, device="cuda", generator=g)[:K] for _ in range(R)]) if R else torch.zeros(0, K, dtype=torch.int64, device="cuda")
+    t = torch.log_softmax(2.0 * torch.randn(R, K + 1, device="cuda", generator=g), 1)[:, :K].contiguous()
+    w = 0.5 + torch.rand(R, device="cuda", generator=g)
+    return z, ids, t, w
+
+
+def _check(z, ids, t, w, **kw):
+    """Loss and gradient against 64 bits.  With A the widest exponent of a row: the exponentials are off by 2^-22 (the instruction) and A 2^-23
+    (their arguments, the rounded factor log2(e) / T), their sum by (V / 2048 + 40) 2^-24 more; every mass and log-prob is off by at most a
+    small multiple of that, and the divergence and its slopes by as much times their terms (`size`)."""
+    temperature = kw.get("temperature", 1.0)
+    zl = z.detach().requires_grad_()
+    loss = ops.topk_distill(zl, ids, t, kw.get("kl", "reverse_kl"), kw.get("alpha", 0.5), kw.get("norm", "tail"), temperature, kw.get("clamp"))
+    (d,) = torch.autograd.grad(loss, zl, w)
+    want, d_want, size = O.distill(z, ids, t, w, **kw)
+    A = (z.double().cpu().amax(1) - z.double().cpu().amin(1)) / temperature * 1.5 + z.double().cpu().abs().amax(1) / temperature
+    off = 4 * (2.0 ** -22 + (2 * A + z.shape[1] / 2048 + 40) * F)
+    _within(loss, want, off * size + F * want.abs(), f"loss {kw}")
+    p = torch.softmax(z.double().cpu() / temperature, 1)
+    at = torch.zeros_like(p)
+    idc = ids.cpu()
+    ok = (idc >= 0) & (idc < z.shape[1])
+    rows = torch.arange(z.shape[0])[:, None].expand_as(idc)
+    at[rows[ok], idc[ok]] = 1.0
+    g = w.cpu().double()[:, None] / temperature
+    half = _half_step(d.dtype)
+    tol = g * (off * size)[:, None] * (p + at)
+    _within(d, d_want, half * d_want.abs() + (1 + half) * tol + (2.0 ** -25 if d.dtype == torch.float16 else 1e-37), f"gradient {kw}")
+    return loss, d
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("R,V,K", [(1, 1, 1), (1, 7, 3), (5, 1000, 8), (3, 4099, 64), (6, 33001, 17), (150, 515, 128), (2, 151936, 64), (0, 100, 4), (4, 16, 0)])
+def test_distill(R, V, K, dtype):
+    z, ids, t, w = _case(R, V, K, dtype, R + V)
+    if R > 2 and K > 2:
+        ids[0, K // 2:] = -1
+        ids[1] = V + 5                                          # nothing of this row is known
+        w[2] = 0.0                                              # nor asked of this one
+    loss, d = _check(z, ids, t, w)
+    if R > 2 and K > 2:
+        assert float(loss[1]) == 0.0 and not d[1].any() and not d[2].any()
+
+
+@pytest.mark.parametrize("kl", ["reverse_kl", "forward_kl", "jsd", "low_var_kl"])
+@pytest.mark.parametrize("norm", ["tail", "norm", "trunc"])
+@pytest.mark.parametrize("clamp,temperature", [(None, 1.0), (-6.0, 0.7), (None, 3.0)])
+def test_distill_divergences(kl, norm, clamp, temperature):
+    z, ids, t, w = _case(9, 2050, 33, "fp32", 4, 2.0)
+    z[torch.arange(9, device="cuda")[:, None], ids[:, :6]] += 9.0           # rows whose ids hold most of the mass
+    ids[3, 5:] = -1
+    ids[4] = -1
+    _check(z, ids, t, w, kl=kl, alpha=0.3, norm=norm, clamp=clamp, temperature=temperature)
+
+
+def test_distill_where_the_ids_hold_everything():
+    """1 - sum P has no digits left in 32 bits; the mass outside is summed by itself, down to its floor."""
+    for lift in (8.0, 14.0, 17.0, 30.0):
+        z, ids, t, w = _case(4, 3001, 5, "fp32", 6, 1.0)
+        z[torch.arange(4, device="cuda")[:, None], ids] += lift
+        for kl in ("reverse_kl", "forward_kl", "jsd"):
+            _check(z, ids, t, w, kl=kl)
+
+
+def test_distill_ids_twice_and_views():
+    z, ids, t, w = _case(5, 700, 12, "bf16", 8)
+    ids[:, 7] = ids[:, 2]
+    ids[1, :] = ids[1, 0]
+    t = t - 2.0                                                  # (so that equal ids together stay below one)
+    z2 = torch.zeros(5, 720, device="cuda", dtype=torch.bfloat16)
+    z2[:, 5:705] = z
+    for norm in ("tail", "norm", "trunc"):
+        a = _check(z, ids, t, w, norm=norm)
+        b = _check(z2[:, 5:705], ids, t, w, norm=norm)           # rows that begin anywhere
+        assert torch.allclose(a[0], b[0], rtol=1e-5, atol=1e-6)
+    c = ops.topk_distill(z.t().contiguous().t(), ids, t)         # columns first
+    assert torch.equal(c, ops.topk_distill(z, ids, t))
+
+
+def test_distill_infinities():
+    z, ids, t, w = _case(4, 600, 6, "fp32", 12)
+    z[:, 300:] = -math.inf                                       # tokens that the student cannot give
+    ids[0, 0] = 400
+    ids[1:] = ids[1:] % 300
+    t[1, 2] = -math.inf
+    loss = ops.topk_distill(z, ids, t)
+    ref = ops.topk_distill(z.cpu(), ids.cpu(), t.cpu())
+    assert torch.isinf(loss[1]) and torch.allclose(loss[[0, 2, 3]].cpu(), ref[[0, 2, 3]], rtol=1e-4, atol=1e-5)
+    z[3, 17] = math.nan
+    out = ops.topk_distill(z, ids, t, "forward_kl")
+    assert torch.isnan(out[3]) and torch.isinf(out[0]) and torch.isfinite(out[[1, 2]]).all()
+
+
+def test_distill_log_probs():
+    z, ids, t, _ = _case(6, 5000, 20, "bf16", 3)
+    ids[2, 4:] = -1
+    _, lp = ops.topk_distill(z, ids, t, return_log_probs=True)
+    want = torch.log_softmax(z.double(), 1).gather(1, ids.clamp_min(0))
+    assert torch.equal(torch.isinf(lp), ids < 0)
+    there = ids >= 0
+    # the sum's error (2^-22 and A 2^-23 with |A| < 60, 45 additions) and the value's own rounding
+    assert ((lp.double() - want).abs()[there] <= 2.0 ** -22 + 170 * F + F * want.abs()[there]).all()
+
+
+def test_distill_gradient_against_differences():
+    z, ids, t, w = _case(4, 777, 9, "fp32", 15)
+    v = torch.randn(z.shape, generator=torch.Generator().manual_seed(5), dtype=torch.float64)
+    for kl in ("reverse_kl", "forward_kl", "jsd", "low_var_kl"):
+        zz = z.clone().requires_grad_()
+        (d,) = torch.autograd.grad(ops.topk_distill(zz, ids, t, kl), zz, w)
+        h = 1e-5
+        up, dn = (O.distill(z.double().cpu() + e * v, ids, t, w, kl)[0] for e in (h, -h))
+        slope = float(((up - dn) / (2 * h) * w.cpu()).sum())
+        dv = d.double().cpu() * v
+        assert abs(float(dv.sum()) - slope) <= 1e-5 * float(dv.abs().sum() + 1.0), kl
+
+
+def test_fused_head_distill():
+    g = _gen(21)
+    R, V, H, K = 300, 4096, 256, 16
+    _, ids, t, w = _case(R, V, K, "fp32", 2)
+    h = torch.randn(R, H, device="cuda", generator=g).bfloat16().requires_grad_()
+    wt = (torch.randn(V, H, device="cuda", generator=g) * 0.1).bfloat16().requires_grad_()
+    loss = ops.fused_lm_head_topk_distill(h, wt, ids, t, "jsd", chunk_size=128)
+    d_h, d_w = torch.autograd.grad(loss, [h, wt], w)
+    hd, wd = h.detach().double().requires_grad_(), wt.detach().double().requires_grad_()
+    from relax_b200.ops import reference as ref
+
+    ld = ref.topk_distill(hd @ wd.t(), ids, t, "jsd", 0.5, "tail", 1.0, None, False)
+    assert torch.allclose(loss, ld, rtol=1e-4, atol=1e-5)
+    e_h, e_w = torch.autograd.grad(ld, [hd, wd], w)
+    for got, want in ((d_h, e_h), (d_w, e_w)):
+        # d logits and the product are rounded to bf16 (2^-8 each) among terms of the product's size
+        assert float((got.double() - want).norm() / want.norm()) < 2.0 ** -7
+    wt.main_grad = torch.zeros(V, H, device="cuda")
+    h2 = h.detach().requires_grad_()
+    ops.fused_lm_head_topk_distill(h2, wt, ids, t, "jsd", chunk_size=300).backward(w)
+    assert wt.grad is None and float((wt.main_grad.double() - e_w).norm() / e_w.norm()) < 2.0 ** -7
+    assert float((h2.grad.double() - e_h).norm() / e_h.norm()) < 2.0 ** -7
+
+
+# --------------------------------------------------------------------------- together
+
+
+def test_step_of_a_routed_student():
+    """Embedding, routed experts and the distillation loss of one step on the GPU in bf16 against the same layers in 64-bit plain torch."""
+    g = _gen(33)
+    T, V, H, E, k, Fh, K = 300, 2048, 256, 8, 2, 128, 12
+    tok = torch.randint(0, V, (T,), device="cuda", generator=g)
+    mk = lambda *s, m=1.0: (torch.randn(*s, device="cuda", generator=g) * m).bfloat16().requires_grad_()      # noqa: E731
+    table, w1, w2, head = mk(V, H), mk(E, 2 * Fh, H, m=0.06), mk(E, H, Fh, m=0.1), mk(V, H, m=0.08)
+    idx = torch.stack([torch.randperm(E, device="cuda", generator=g)[:k] for _ in range(T)])
+    gate = torch.rand(T, k, device="cuda", generator=g).requires_grad_()
+    _, ids, teacher, w = _case(T, V, K, "fp32", 3)
+
+    from relax_b200.models.moe import experts_mlp
+
+    x = ops.embedding(tok, table, 2.0)
+    h = x + experts_mlp(x, idx, gate, w1, w2)
+    loss = (ops.fused_lm_head_topk_distill(h, head, ids, teacher) * w).mean()
+    grads = torch.autograd.grad(loss, [table, w1, w2, head, gate])
+
+    D = [p.detach().double().requires_grad_() for p in (table, w1, w2, head, gate)]
+    xd = D[0][tok] * 2.0
+    gu = torch.einsum("th,tknh->tkn", xd, D[1][idx])
+    act = torch.nn.functional.silu(gu[..., :Fh]) * gu[..., Fh:]
+    hd = xd + (torch.einsum("tkf,tkhf->tkh", act, D[2][idx]) * D[4][..., None]).sum(1)
+    z = hd @ D[3].t()
+    lp = torch.log_softmax(z, 1).gather(1, ids)
+    p, q = lp.exp(), teacher.double().exp()
+    rp, rq = 1 - p.sum(1), 1 - q.sum(1)
+    ld = (((p * (lp - teacher.double())).sum(1) + rp * (rp.log() - rq.log())) * w).mean()
+    want = torch.autograd.grad(ld, D)
+    assert abs(float(loss) - float(ld)) < 2e-2 * abs(float(ld))      # bf16 activations: four roundings of 2^-8 in front of the logits
+    for got, ref in zip(grads, want):
+        assert float((got.double() - ref).norm() / ref.norm()) < 5e-2, got.shape

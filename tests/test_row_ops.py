@@ -1,0 +1,184 @@
+"""Rows sorted by expert and back, the embedding with its gradient and the distillation divergence on the CPU: statements against one-row-at-a-time
+oracles, refusals, and the paths of the framework that call them."""
+import math
+
+import pytest
+import torch
+
+import oracle_rows as O
+from relax_b200 import ops
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+@pytest.mark.parametrize("align", [1, 4, 128])
+@pytest.mark.parametrize("T,k,E", [(0, 2, 4), (1, 1, 1), (1, 3, 5), (40, 3, 7), (33, 2, 300)])
+def test_expert_rows_statement(T, k, E, align):
+    g = _gen(T + E)
+    ids = torch.randint(-2, E + 2, (T, k), generator=g)
+    rows = ops.expert_layout(ids, E, align)
+    dest, source, tiles, bounds = O.layout(ids, E, align)
+    assert rows.dest.reshape(-1).tolist() == dest and rows.source.tolist() == source and rows.expert_rows.tolist() == bounds
+    assert (rows.tile_expert is None) == (align == 1)
+    if align > 1:
+        assert rows.tile_expert.tolist() == tiles
+    x = torch.randn(T, 6, generator=g, dtype=torch.float32).requires_grad_()
+    y = torch.randn(len(source), 6, generator=g).requires_grad_()
+    w = torch.rand(T, k, generator=g).requires_grad_()
+    srt, out = ops.expert_dispatch(x, rows), ops.expert_combine(y, w, rows)
+    assert torch.equal(srt.double(), O.dispatch(x.detach(), source, k))
+    want, size = O.combine(y.detach(), w.detach(), dest, k)
+    assert ((out.double() - want).abs() <= (k + 1) * 2.0 ** -24 * size).all()
+    d_s, d_o = torch.randn(srt.shape, generator=g), torch.randn(T, 6, generator=g)
+    d_x, d_y, d_w = torch.autograd.grad([srt, out], [x, y, w], [d_s, d_o])
+    want, size = O.combine(d_s, None, dest, k)
+    assert ((d_x.double() - want).abs() <= (k + 1) * 2.0 ** -24 * size).all()
+    for i, d in enumerate(dest):
+        if d < 0:
+            assert float(d_w.reshape(-1)[i]) == 0.0
+        else:
+            terms = d_o[i // k].double() * y[d].detach().double()
+            assert abs(float(d_w.reshape(-1)[i]) - float(terms.sum())) <= 8 * 2.0 ** -24 * float(terms.abs().sum())
+            assert torch.allclose(d_y[d], d_o[i // k] * w.detach().reshape(-1)[i], rtol=2.0 ** -23, atol=0)
+    assert all((d_y[r] == 0).all() for r, s in enumerate(source) if s < 0)
+
+
+def test_expert_rows_refusals():
+    with pytest.raises(ValueError, match="int64 or int32"):
+        ops.expert_layout(torch.zeros(3, 2), 4)
+    with pytest.raises(ValueError, match="2048 experts"):
+        ops.expert_layout(torch.zeros(3, 2, dtype=torch.int64), 0)
+    with pytest.raises(ValueError, match="align"):
+        ops.expert_layout(torch.zeros(3, 2, dtype=torch.int64), 4, 0)
+    with pytest.raises(ValueError, match="at least one expert"):
+        ops.expert_layout(torch.zeros(3, 0, dtype=torch.int64), 4)
+    rows = ops.expert_layout(torch.zeros(3, 2, dtype=torch.int64), 4)
+    with pytest.raises(ValueError, match="expert_dispatch"):
+        ops.expert_dispatch(torch.zeros(4, 8), rows)
+    with pytest.raises(ValueError, match="expert_combine"):
+        ops.expert_combine(torch.zeros(5, 8), torch.ones(3, 2), rows)
+    with pytest.raises(ValueError, match="weights"):
+        ops.expert_combine(torch.zeros(rows.source.numel(), 8), torch.ones(2, 3), rows)
+
+
+@pytest.mark.parametrize("scale", [1.0, 45.0])
+@pytest.mark.parametrize("start", [0, 10])
+def test_embedding_statement(scale, start):
+    g = _gen(7)
+    w = torch.randn(20, 5, generator=g).requires_grad_()
+    tok = torch.randint(0, 40, (3, 11), generator=g)
+    out = ops.embedding(tok, w, scale, start)
+    dy = torch.randn(out.shape, generator=g)
+    for i, t in enumerate(tok.reshape(-1).tolist()):
+        here = 0 <= t - start < 20
+        assert torch.equal(out.reshape(-1, 5)[i], w.detach()[t - start] * scale if here else torch.zeros(5))
+    want, size = O.embedding_grad(tok, dy.reshape(-1, 5), 20, start, scale)
+    (got,) = torch.autograd.grad(out, w, dy)
+    assert ((got.double() - want).abs() <= 36 * 2.0 ** -24 * size).all()
+    # into the optimizer's buffer
+    w.main_grad = torch.full((20, 5), 0.5)
+    ops.embedding(tok, w, scale, start).backward(dy)
+    assert w.grad is None and torch.allclose(w.main_grad, got + 0.5, rtol=2.0 ** -20, atol=2.0 ** -20 * float(size.max()))
+    with pytest.raises(ValueError, match="tokens"):
+        ops.embedding(tok.float(), w)
+
+
+def test_model_embedding_takes_the_configured_scale():
+    import dataclasses
+
+    from relax_b200.models.config import get_config
+    from relax_b200.models.transformer import GPTModel
+    from relax_b200.rollout.weights import RolloutWeights
+
+    cfg = dataclasses.replace(get_config("tiny"), embed_scale=3.0)
+    m, plain = GPTModel(cfg, seed=1), GPTModel(get_config("tiny"), seed=1)
+    tok = torch.tensor([1, 5, 1023])
+    assert torch.equal(m.embedding.word_embeddings(tok, False), 3.0 * plain.embedding.word_embeddings(tok, False))
+    del RolloutWeights
+
+
+def _rows(R, V, K, seed, absent=True):
+    g = _gen(seed)
+    z = 3.0 * torch.randn(R, V, generator=g)
+    ids = torch.stack([torch.randperm(V, generator=g)[:K] for _ in range(R)]) if R else torch.zeros(0, K, dtype=torch.int64)
+    t = torch.log_softmax(2.0 * torch.randn(R, K + 1, generator=g), 1)[:, :K].contiguous()
+    if absent and K > 1 and R > 1:
+        ids[0, K // 2:] = -1
+        ids[R - 1] = -1
+    return z, ids, t, 0.5 + torch.rand(R, generator=g)
+
+
+@pytest.mark.parametrize("kl", ["reverse_kl", "forward_kl", "jsd", "low_var_kl"])
+@pytest.mark.parametrize("norm", ["tail", "norm", "trunc"])
+@pytest.mark.parametrize("clamp,temperature", [(None, 1.0), (-4.0, 0.7)])
+def test_distill_statement(kl, norm, clamp, temperature):
+    from relax_b200.algo import opd
+
+    z, ids, t, w = _rows(5, 23, 6, 3)
+    want, d_want, size = O.distill(z, ids, t, w, kl, 0.3, norm, temperature, clamp)
+    z.requires_grad_()
+    loss, lp = ops.topk_distill(z, ids, t, kl, 0.3, norm, temperature, clamp, return_log_probs=True)
+    assert not lp.requires_grad
+    # 64-bit arithmetic, one rounding to 32 bits
+    assert ((loss.detach().double() - want).abs() <= 2.0 ** -24 * want.abs() + 1e-13 * size).all()
+    (d,) = torch.autograd.grad(loss, z, w)
+    assert ((d.double() - d_want).abs() <= 2.0 ** -23 * d_want.abs() + 1e-7 * size[:, None] * w[:, None]).all()
+    away = ids < 0
+    ref = (z.detach() / temperature).log_softmax(-1).gather(1, ids.clamp_min(0))
+    assert torch.equal(torch.isinf(lp), away) and torch.allclose(lp[~away], ref[~away], atol=1e-5)
+    # the same divergence as on gathered log-probs (32-bit arithmetic there, whose bin of all other mass loses digits)
+    old = opd.token_kl(ref.masked_fill(away, 0.0), t, kl, 0.3, norm, clamp, mask=~away)
+    assert torch.allclose(loss.detach(), old, atol=1e-4, rtol=1e-4)
+
+
+def test_distill_gradient_against_differences():
+    z, ids, t, w = _rows(4, 31, 5, 11)
+    for kl in ("reverse_kl", "forward_kl", "jsd", "low_var_kl"):
+        for norm in ("tail", "norm", "trunc"):
+            zz = z.clone().requires_grad_()
+            (d,) = torch.autograd.grad(ops.topk_distill(zz, ids, t, kl, 0.3, norm), zz, w)
+            v = torch.randn(z.shape, generator=_gen(5), dtype=torch.float64)
+            h = 1e-5
+            up, dn = (O.distill(z.double() + e * v, ids, t, w, kl, 0.3, norm)[0] for e in (h, -h))
+            slope = float(((up - dn) / (2 * h) * w).sum())
+            # central differences: h^2 / 6 times the third derivative, of the order of the slope's terms
+            assert abs(float((d.double() * v).sum()) - slope) <= 1e-5 * float((d.double() * v).abs().sum() + 1.0), (kl, norm)
+
+
+def test_distill_edges_and_refusals():
+    z, ids, t, _ = _rows(3, 9, 4, 1, absent=False)
+    ids[1, 3] = ids[1, 0]                        # an id twice counts twice, as written
+    want, _, _ = O.distill(z, ids, t, torch.ones(3), "reverse_kl", norm="trunc")
+    assert torch.allclose(ops.topk_distill(z, ids, t, norm_mode="trunc").double(), want, rtol=1e-6)
+    assert torch.equal(ops.topk_distill(z, torch.full_like(ids, 9), t), torch.zeros(3))
+    assert ops.topk_distill(z, ids[:, :0], t[:, :0]).tolist() == [0.0] * 3
+    t2 = t.clone()
+    t2[0, 0] = -math.inf                         # the teacher rules a token out that the student gives mass
+    assert torch.isinf(ops.topk_distill(z, ids, t2)[0]) and torch.isfinite(ops.topk_distill(z, ids, t2, "forward_kl")).all()
+    for bad, match in ((dict(kl_type="kl"), "unknown divergence"), (dict(norm_mode="none"), "norm_mode"), (dict(alpha=1.5), "alpha"),
+                       (dict(temperature=0.0), "temperature")):
+        with pytest.raises(ValueError, match=match):
+            ops.topk_distill(z, ids, t, **bad)
+    with pytest.raises(ValueError, match="ids"):
+        ops.topk_distill(z, ids[:2], t)
+    with pytest.raises(ValueError, match="1024"):
+        ops.topk_distill(z, torch.zeros(3, 1025, dtype=torch.int64), torch.zeros(3, 1025))
+    with pytest.raises(ValueError, match="logits"):
+        ops.topk_distill(z[0], ids, t)
+
+
+def test_fused_head_distill_chunks():
+    g = _gen(2)
+    _, ids, t, w = _rows(7, 24, 4, 9)
+    h, wt = torch.randn(7, 8, generator=g), torch.randn(24, 8, generator=g)
+    outs = []
+    for chunk in (3, 100):
+        a, b = h.clone().requires_grad_(), wt.clone().requires_grad_()
+        loss = ops.fused_lm_head_topk_distill(a, b, ids, t, "jsd", chunk_size=chunk)
+        outs.append((loss.detach(), *torch.autograd.grad(loss, [a, b], w)))
+    for x, y in zip(*outs):
+        assert torch.allclose(x, y, atol=1e-5, rtol=1e-5)
+    assert torch.allclose(outs[0][0], ops.topk_distill(h @ wt.t(), ids, t, "jsd"), atol=1e-6)
+    assert ops.fused_lm_head_topk_distill(h[:0], wt, ids[:0], t[:0]).shape == (0,)
