@@ -40,7 +40,16 @@ inline int as_int(int64_t v, const char* what) {
   TORCH_CHECK_VALUE(v >= 0 && v <= (1ll << 30), what, ": ", v, " is out of range");
   return static_cast<int>(v);
 }
-inline torch::Tensor ints(at::IntArrayRef shape, const torch::Tensor& like) { return at::empty(shape, like.options().dtype(at::kInt)); }
+// Integers (or, for workspaces, whatever lies in them) in one allocation, and tensors on parts of it: an allocation costs as much as a
+// launch, and a few rows take six of these.
+inline torch::Tensor ints(int64_t n, const torch::Tensor& like) { return at::empty({n > 0 ? n : 1}, like.options().dtype(at::kInt)); }
+inline torch::Tensor part_of(const torch::Tensor& all, int64_t offset, at::IntArrayRef shape) {
+  auto t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), all.key_set(), all.dtype());
+  t.unsafeGetTensorImpl()->set_storage_offset(offset);
+  t.unsafeGetTensorImpl()->set_sizes_contiguous(shape);
+  return t;
+}
+inline bool recorded(const torch::Tensor& t) { return t.requires_grad() && at::GradMode::is_enabled(); }
 
 using torch::autograd::AutogradContext;
 using torch::autograd::Function;
@@ -74,17 +83,16 @@ py::tuple expert_layout(torch::Tensor ids, int64_t experts, int64_t align) {
   TORCH_CHECK_VALUE(align >= 1 && align <= 65536, "expert_layout: align must lie in 1 .. 65536, got ", align);
   const int n = as_int(ids.numel(), "expert_layout: rows");
   const int64_t full = std::min<int64_t>(n, experts), tiles = full + (n - full) / align, cap = align == 1 ? n : tiles * align;
-  auto dest = ints(ids.sizes(), ids), source = ints({as_int(cap, "expert_layout: buffer rows")}, ids), bounds = ints({experts + 1}, ids);
-  torch::Tensor tile;
-  if (align > 1) tile = ints({tiles}, ids);
-  torch::Tensor hist;
+  as_int(cap, "expert_layout: buffer rows");
   const int counters = rb_sort_counters(n, static_cast<int>(experts));
-  if (counters > 1) hist = ints({counters}, ids);
-  check(rb_expert_layout(ids.data_ptr(), wide, n, static_cast<int>(experts), static_cast<int>(align), static_cast<int>(cap), dest.data_ptr<int>(),
-                         source.data_ptr<int>(), align > 1 ? tile.data_ptr<int>() : nullptr, bounds.data_ptr<int>(),
-                         counters > 1 ? hist.data_ptr<int>() : nullptr, cur_stream()),
+  const auto all = ints(n + cap + (align > 1 ? tiles : 0) + experts + 1 + (counters > 1 ? counters : 0), ids);
+  int* p = all.data_ptr<int>();
+  const int64_t at_source = n, at_bounds = at_source + cap, at_tiles = at_bounds + experts + 1, at_hist = at_tiles + (align > 1 ? tiles : 0);
+  check(rb_expert_layout(ids.data_ptr(), wide, n, static_cast<int>(experts), static_cast<int>(align), static_cast<int>(cap), p, p + at_source,
+                         align > 1 ? p + at_tiles : nullptr, p + at_bounds, counters > 1 ? p + at_hist : nullptr, cur_stream()),
         "rb_expert_layout");
-  return py::make_tuple(dest, source, align > 1 ? py::cast(tile) : py::none(), bounds);
+  return py::make_tuple(part_of(all, 0, ids.sizes()), part_of(all, at_source, {cap}), align > 1 ? py::cast(part_of(all, at_tiles, {tiles})) : py::none(),
+                        part_of(all, at_bounds, {experts + 1}));
 }
 
 torch::Tensor scatter_rows(const torch::Tensor& in, const torch::Tensor& source, int64_t k, const char* what) {
@@ -120,7 +128,9 @@ struct Dispatch : Function<Dispatch> {
     return once({gather_rows(g[0], saved[0], c10::nullopt, false, "expert_dispatch"), torch::Tensor(), torch::Tensor()}, g);
   }
 };
-torch::Tensor expert_dispatch(const torch::Tensor& x, const torch::Tensor& dest, const torch::Tensor& source) { return Dispatch::apply(x, dest, source); }
+torch::Tensor expert_dispatch(const torch::Tensor& x, const torch::Tensor& dest, const torch::Tensor& source) {
+  return recorded(x) ? Dispatch::apply(x, dest, source) : scatter_rows(x, source, dest.size(1), "expert_dispatch");
+}
 
 struct Combine : Function<Combine> {
   static torch::Tensor forward(AutogradContext* ctx, const torch::Tensor& y, const Maybe& weight, const torch::Tensor& dest, const torch::Tensor& source,
@@ -149,32 +159,38 @@ struct Combine : Function<Combine> {
   }
 };
 torch::Tensor expert_combine(const torch::Tensor& y, const Maybe& weight, const torch::Tensor& dest, const torch::Tensor& source, bool fp32) {
-  return Combine::apply(y, weight, dest, source, fp32);
+  if (recorded(y) || (weight.has_value() && recorded(*weight))) return Combine::apply(y, weight, dest, source, fp32);
+  if (!weight.has_value()) return gather_rows(y, dest, weight, fp32, "expert_combine");
+  return gather_rows(y, dest, weight->to(at::kFloat).contiguous(), fp32, "expert_combine");
 }
 
 // ----------------------------------------------------------------------------- embedding
 
+torch::Tensor look_up(const torch::Tensor& weight, const torch::Tensor& ids, double scale, int64_t start) {
+  const c10::cuda::CUDAGuard guard(weight.device());
+  const auto table = dense(weight, "embedding");
+  const int wide = wide_ids(ids, "embedding");
+  same_device(ids, table, "embedding: tokens");
+  auto shape = ids.sizes().vec();
+  shape.push_back(table.size(1));
+  auto out = at::empty(shape, table.options());
+  check(rb_embedding(ids.data_ptr(), wide, start, table.data_ptr(), table.stride(0), as_int(table.size(0), "embedding: table rows"), out.data_ptr(),
+                     as_int(ids.numel(), "embedding: tokens"), as_int(table.size(1), "embedding: columns"), static_cast<float>(scale),
+                     code_of(table, "embedding"), cur_stream()),
+        "rb_embedding");
+  return out;
+}
+
 // The gradient is a new matrix in the rows' type, or is added to `main_grad` (fp32), which then stands for it.
 struct Embedding : Function<Embedding> {
-  static torch::Tensor forward(AutogradContext* ctx, const torch::Tensor& weight, const torch::Tensor& tokens, double scale, int64_t start,
+  static torch::Tensor forward(AutogradContext* ctx, const torch::Tensor& weight, const torch::Tensor& ids, double scale, int64_t start,
                                const Maybe& main_grad) {
-    const c10::cuda::CUDAGuard guard(weight.device());
-    const auto table = dense(weight, "embedding"), ids = tokens.contiguous();
-    const int wide = wide_ids(ids, "embedding");
-    same_device(ids, table, "embedding: tokens");
-    auto shape = ids.sizes().vec();
-    shape.push_back(table.size(1));
-    auto out = at::empty(shape, table.options());
-    check(rb_embedding(ids.data_ptr(), wide, start, table.data_ptr(), table.stride(0), as_int(table.size(0), "embedding: table rows"), out.data_ptr(),
-                       as_int(ids.numel(), "embedding: tokens"), as_int(table.size(1), "embedding: columns"), static_cast<float>(scale),
-                       code_of(table, "embedding"), cur_stream()),
-          "rb_embedding");
     ctx->save_for_backward({ids});
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["start"] = start;
-    ctx->saved_data["rows"] = table.size(0);
+    ctx->saved_data["rows"] = weight.size(0);
     ctx->saved_data["main_grad"] = main_grad;
-    return out;
+    return look_up(weight, ids, scale, start);
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     const auto saved = ctx->get_saved_variables();
@@ -185,12 +201,12 @@ struct Embedding : Function<Embedding> {
     const auto dy = dense(g[0].reshape({ids.numel(), g[0].size(-1)}), "embedding");
     const int n = as_int(ids.numel(), "embedding: tokens"), V = as_int(rows, "embedding: table rows"), cols = as_int(dy.size(1), "embedding: columns");
     auto out = into.has_value() ? *into : at::empty({rows, cols}, dy.options());
-    const int64_t chunks = (n + 31) / 32;
-    auto pairs = ints({std::max<int64_t>(n, 1), 4}, dy);      // two buffers of (key, row)
-    auto hist = ints({rb_sort_counters(n, rb_embedding_bwd_bins(V))}, dy);
-    auto part = at::empty({chunks > 1 ? chunks * 2 * cols : 1}, dy.options().dtype(at::kFloat));
+    // two buffers of (key, row), partial sums of runs (32-byte vectors), counters
+    const int64_t chunks = (n + 31) / 32, at_part = (4ll * n + 7) / 8 * 8, at_hist = at_part + (chunks > 1 ? chunks * 2 * cols : 0);
+    const auto work = ints(at_hist + rb_sort_counters(n, rb_embedding_bwd_bins(V)), dy);
+    int* p = work.data_ptr<int>();
     check(rb_embedding_bwd(ids.data_ptr(), ids.scalar_type() == at::kLong, ctx->saved_data["start"].toInt(), dy.data_ptr(), dy.stride(0), out.data_ptr(),
-                           into.has_value(), reinterpret_cast<int2*>(pairs.data_ptr<int>()), hist.data_ptr<int>(), part.data_ptr<float>(), n, V, cols,
+                           into.has_value(), reinterpret_cast<int2*>(p), p + at_hist, reinterpret_cast<float*>(p + at_part), n, V, cols,
                            static_cast<float>(ctx->saved_data["scale"].toDouble()), code_of(dy, "embedding"), cur_stream()),
           "rb_embedding_bwd");
     return once({into.has_value() ? torch::Tensor() : out, torch::Tensor(), torch::Tensor(), torch::Tensor(), torch::Tensor()}, g);
@@ -202,14 +218,17 @@ torch::Tensor embedding(const torch::Tensor& weight, const torch::Tensor& tokens
     TORCH_CHECK_VALUE(main_grad->scalar_type() == at::kFloat && main_grad->is_contiguous() && main_grad->sizes() == weight.sizes(),
                       "embedding: main_grad is a dense fp32 matrix of the table's shape");
   }
-  return Embedding::apply(weight, tokens, scale, start, main_grad);
+  const auto ids = tokens.contiguous();
+  return recorded(weight) ? Embedding::apply(weight, ids, scale, start, main_grad) : look_up(weight, ids, scale, start);
 }
 
 // ----------------------------------------------------------------------------- distillation from top ids
 
 struct Distilled {
-  torch::Tensor loss, coef, stats, log_probs;
+  torch::Tensor loss, kept, log_probs;      // kept: statistics [R, 4], sums of parts (a workspace), slopes [R, K]
 };
+inline int64_t slopes_at(const torch::Tensor& z) { return z.size(0) * (4 + 2 * rb_topk_distill_parts(z.size(0), static_cast<int>(z.size(1)))); }
+
 Distilled distill_rows(const torch::Tensor& z, const torch::Tensor& ids, const torch::Tensor& teacher, int64_t kl, int64_t norm, double alpha, double clamp,
                        double inv_temp, bool log_probs) {
   const c10::cuda::CUDAGuard guard(z.device());
@@ -221,41 +240,40 @@ Distilled distill_rows(const torch::Tensor& z, const torch::Tensor& ids, const t
   TORCH_CHECK_VALUE(ids.size(1) <= 1024, "topk_distill: up to 1024 ids per row, got ", ids.size(1));
   TORCH_CHECK_VALUE(z.size(1) >= 1 && z.size(1) <= (1 << 24), "topk_distill: 1 to 2^24 tokens in the vocabulary, got ", z.size(1));
   const auto f32 = z.options().dtype(at::kFloat);
-  const int64_t R = z.size(0), K = ids.size(1);
-  const int V = as_int(z.size(1), "topk_distill: vocabulary"), code = code_of(z, "topk_distill");
-  Distilled d{at::empty({R}, f32), at::empty({R, K}, f32), at::empty({R, 4}, f32), torch::Tensor()};
-  auto sums = at::empty({R, rb_topk_distill_parts(R, V), 2}, f32);
+  const int64_t R = z.size(0), K = ids.size(1), slopes = slopes_at(z);
+  const int code = code_of(z, "topk_distill");
+  Distilled d{at::empty({R}, f32), at::empty({slopes + R * K}, f32), torch::Tensor()};
+  float* kept = d.kept.data_ptr<float>();
   if (log_probs) d.log_probs = at::empty({R, K}, f32);
   check(rb_topk_distill(z.data_ptr(), z.stride(0), reinterpret_cast<const long long*>(ids.data_ptr<int64_t>()), teacher.data_ptr<float>(),
-                        d.loss.data_ptr<float>(), d.coef.data_ptr<float>(), d.stats.data_ptr<float>(), log_probs ? d.log_probs.data_ptr<float>() : nullptr,
-                        reinterpret_cast<float2*>(sums.data_ptr<float>()), R, V, static_cast<int>(K), static_cast<int>(kl), static_cast<int>(norm), alpha,
-                        clamp, static_cast<float>(inv_temp), code, cur_stream()),
+                        d.loss.data_ptr<float>(), kept + slopes, kept, log_probs ? d.log_probs.data_ptr<float>() : nullptr,
+                        reinterpret_cast<float2*>(kept + 4 * R), R, static_cast<int>(z.size(1)), static_cast<int>(K), static_cast<int>(kl),
+                        static_cast<int>(norm), alpha, clamp, static_cast<float>(inv_temp), code, cur_stream()),
         "rb_topk_distill");
   return d;
 }
 
 // d logits, into `out` (a dense matrix of the logits' type, or of bf16 for fp32 logits)
-void distill_rows_bwd(const torch::Tensor& z, const torch::Tensor& ids, const torch::Tensor& coef, const torch::Tensor& stats, const torch::Tensor& g,
-                      double inv_temp, const torch::Tensor& out) {
+void distill_rows_bwd(const torch::Tensor& z, const torch::Tensor& ids, const torch::Tensor& kept, const torch::Tensor& g, double inv_temp,
+                      const torch::Tensor& out) {
   const c10::cuda::CUDAGuard guard(z.device());
   TORCH_CHECK_VALUE(out.is_contiguous() && out.sizes() == z.sizes(), "topk_distill: a dense gradient of the logits' shape");
-  TORCH_CHECK_VALUE(g.scalar_type() == at::kFloat && g.is_contiguous() && g.numel() == z.size(0) && ids.is_contiguous() && coef.is_contiguous() &&
-                        stats.is_contiguous() && coef.sizes() == ids.sizes() && ids.size(0) == z.size(0) && stats.numel() == 4 * z.size(0),
-                    "topk_distill: gradient or saved values of another shape");
-  check(rb_topk_distill_bwd(z.data_ptr(), z.stride(0), reinterpret_cast<const long long*>(ids.data_ptr<int64_t>()), coef.data_ptr<float>(),
-                            stats.data_ptr<float>(), g.data_ptr<float>(), out.data_ptr(), z.size(0), as_int(z.size(1), "topk_distill: vocabulary"),
+  const int64_t slopes = slopes_at(z);
+  TORCH_CHECK_VALUE(g.scalar_type() == at::kFloat && g.is_contiguous() && g.numel() == z.size(0) && ids.is_contiguous() && ids.size(0) == z.size(0) &&
+                        kept.scalar_type() == at::kFloat && kept.is_contiguous() && kept.numel() == slopes + ids.numel(),
+                    "topk_distill: gradient or kept values of another shape");
+  check(rb_topk_distill_bwd(z.data_ptr(), z.stride(0), reinterpret_cast<const long long*>(ids.data_ptr<int64_t>()), kept.data_ptr<float>() + slopes,
+                            kept.data_ptr<float>(), g.data_ptr<float>(), out.data_ptr(), z.size(0), as_int(z.size(1), "topk_distill: vocabulary"),
                             static_cast<int>(ids.size(1)), static_cast<float>(inv_temp), code_of(z, "topk_distill"), code_of(out, "topk_distill"),
                             cur_stream()),
         "rb_topk_distill_bwd");
 }
 
 struct TopkDistill : Function<TopkDistill> {
-  static variable_list forward(AutogradContext* ctx, const torch::Tensor& logits, const torch::Tensor& ids, const torch::Tensor& teacher, int64_t kl,
-                               int64_t norm, double alpha, double clamp, double inv_temp, bool log_probs) {
-    const c10::cuda::CUDAGuard guard(logits.device());
-    const auto z = dense(logits, "topk_distill"), i = ids.contiguous();
-    const auto d = distill_rows(z, i, teacher.to(at::kFloat).contiguous(), kl, norm, alpha, clamp, inv_temp, log_probs);
-    ctx->save_for_backward({z, i, d.coef, d.stats});
+  static variable_list forward(AutogradContext* ctx, const torch::Tensor& z, const torch::Tensor& ids, const torch::Tensor& teacher, int64_t kl, int64_t norm,
+                               double alpha, double clamp, double inv_temp, bool log_probs) {
+    const auto d = distill_rows(z, ids, teacher, kl, norm, alpha, clamp, inv_temp, log_probs);
+    ctx->save_for_backward({z, ids, d.kept});
     ctx->saved_data["inv_temp"] = inv_temp;
     if (!log_probs) return {d.loss};
     ctx->mark_non_differentiable({d.log_probs});
@@ -263,8 +281,9 @@ struct TopkDistill : Function<TopkDistill> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     const auto saved = ctx->get_saved_variables();
+    const c10::cuda::CUDAGuard guard(saved[0].device());
     auto out = at::empty({saved[0].size(0), saved[0].size(1)}, saved[0].options());
-    distill_rows_bwd(saved[0], saved[1], saved[2], saved[3], g[0].to(at::kFloat).contiguous(), ctx->saved_data["inv_temp"].toDouble(), out);
+    distill_rows_bwd(saved[0], saved[1], saved[2], g[0].to(at::kFloat).contiguous(), ctx->saved_data["inv_temp"].toDouble(), out);
     variable_list d(9);
     d[0] = out;
     return once(d, g);
@@ -272,13 +291,18 @@ struct TopkDistill : Function<TopkDistill> {
 };
 py::object topk_distill(const torch::Tensor& logits, const torch::Tensor& ids, const torch::Tensor& teacher, int64_t kl, int64_t norm, double alpha,
                         double clamp, double inv_temp, bool log_probs) {
-  const auto out = TopkDistill::apply(logits, ids, teacher, kl, norm, alpha, clamp, inv_temp, log_probs);
-  return log_probs ? py::object(py::make_tuple(out[0], out[1])) : py::cast(out[0]);
+  const auto z = dense(logits, "topk_distill"), i = ids.contiguous(), t = teacher.detach().to(at::kFloat).contiguous();
+  if (recorded(z)) {
+    const auto out = TopkDistill::apply(z, i, t, kl, norm, alpha, clamp, inv_temp, log_probs);
+    return log_probs ? py::object(py::make_tuple(out[0], out[1])) : py::cast(out[0]);
+  }
+  const auto d = distill_rows(z, i, t, kl, norm, alpha, clamp, inv_temp, log_probs);
+  return log_probs ? py::object(py::make_tuple(d.loss, d.log_probs)) : py::cast(d.loss);
 }
 py::tuple topk_distill_rows(const torch::Tensor& z, const torch::Tensor& ids, const torch::Tensor& teacher, int64_t kl, int64_t norm, double alpha,
                             double clamp, double inv_temp) {
   const auto d = distill_rows(z, ids, teacher, kl, norm, alpha, clamp, inv_temp, false);
-  return py::make_tuple(d.loss, d.coef, d.stats);
+  return py::make_tuple(d.loss, d.kept);
 }
 }  // namespace
 

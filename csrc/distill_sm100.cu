@@ -28,6 +28,7 @@ namespace distill {
 constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kMaxIds = 1024;      // eight per thread of id_kernel
 constexpr int kMaxVocab = 1 << 24;
+constexpr int kMaxParts = 32;      // blocks of a row
 constexpr int kStats = 4;      // per row: log2 reference, 1 / sum, sum of the slopes, (unused)
 constexpr double kLn2 = 0.6931471805599453;
 constexpr double kLeastRest = 9.9999995e-08;      // 1 - exp(-1e-7)
@@ -243,7 +244,7 @@ __global__ void __launch_bounds__(kThreads, 4) sum_kernel(Params p) {
   const unsigned char* mark = reinterpret_cast<const unsigned char*>(marks);
 
   Sum s{-INFINITY, 0.f};
-  constexpr int U = sizeof(T) == 4 ? 2 : 4;      // groups of a thread in one step
+  constexpr int U = sizeof(T) == 4 ? 4 : 8;      // groups of a thread in one step: 128 bytes of it under way
   // U groups from g on, in strides of the block; the last step (kAll false) holds what is left
   auto step = [&](int g, auto all) {
     constexpr bool kAll = decltype(all)::value;
@@ -544,15 +545,19 @@ __global__ void __launch_bounds__(kThreads) bwd_kernel(BwdParams p) {
   }
 }
 
-// Blocks of a row: one where rows alone fill the machine, else as many as it takes, each with at least 4096 elements (parts of a row
-// cost: finer ones, for a fuller last wave, made the sums slower)
-inline int parts_of(long long rows, int vocab, int most) {
-  int parts = 1;
-  while (parts < most && rows * parts < 8ll * num_sms() && vocab / (2 * parts) >= 4096) parts *= 2;
-  return parts;
+// Blocks of a row for kernels of `slots` blocks at a time: the number with the shortest waves, where a block costs as much as `fixed`
+// groups of eight beside its own.  (2048 rows of 151936: two parts in 7 waves, 108 us; one part in 4 waves, the last of them less
+// than half full, 115 us; four parts 127 us.)
+inline int parts_of(long long rows, int vocab, long long slots, int fixed) {
+  const long long groups = (vocab + 7) / 8;
+  int best = 1;
+  long long cost = 0;
+  for (int p = 1; p <= kMaxParts && (p == 1 || groups / p >= 512); ++p) {
+    const long long c = (rows * p + slots - 1) / slots * (groups / p + fixed);
+    if (p == 1 || c < cost) best = p, cost = c;
+  }
+  return best;
 }
-constexpr int kSumParts = 32;
-
 template <typename T, bool kMarks>
 int sums_t(const Params& p, long long rows, cudaStream_t st) {
   const int each = ((p.vocab + 14) / 8 + p.parts - 1) / p.parts + 1;
@@ -574,7 +579,7 @@ int sums_any(const Params& p, long long rows, cudaStream_t st) {
 
 template <typename T, typename O>
 int bwd_t(BwdParams p, long long rows, cudaStream_t st) {
-  p.parts = parts_of(rows, p.vocab, 32);
+  p.parts = parts_of(rows, p.vocab, 5ll * num_sms(), 500);
   if (rows * p.parts > 2147483647ll) return -3;
   // groups of eight line up in both where rows keep their distance and begin alike
   const uintptr_t a = reinterpret_cast<uintptr_t>(p.z) / sizeof(T), b = reinterpret_cast<uintptr_t>(p.dz) / sizeof(O);
@@ -595,9 +600,8 @@ using namespace rb::distill;
 
 // Blocks per row, and so pairs of floats per row that rb_topk_distill takes as workspace.
 extern "C" int rb_topk_distill_parts(long long rows, int vocab) {
-  int parts = parts_of(rows, vocab, kSumParts);
-  while (parts < kSumParts && vocab / parts > (1 << 20)) parts *= 2;      // the bitmap of a part fits shared memory
-  return parts;
+  const int parts = parts_of(rows, vocab, 4ll * num_sms(), 1000);      // (a fixed 2 us of 4 blocks per SM)
+  return vocab / parts > (1 << 20) ? kMaxParts : parts;                 // the bitmap of a part fits shared memory
 }
 
 // dtype: 0 bf16, 1 fp16, 2 fp32.  kl: reverse, forward, mixed, low variance; norm: tail bin, renormalised, as they are.

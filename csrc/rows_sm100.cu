@@ -323,7 +323,7 @@ struct TokenRow {      // row r <- table row of its token
   }
 };
 
-constexpr int kMove = 4;      // vectors of a lane in flight
+template <int N> constexpr int kMove = N == 1 ? 8 : 4;      // vectors of a lane in flight
 // out[r] = scale * in[row(r)], zeros where there is no such row; a warp takes 32 x kMove vectors of a row
 template <typename T, int N, bool kScale, typename Row>
 __global__ void __launch_bounds__(256) move_kernel(const T* __restrict__ in, long long ld, Row src, T* __restrict__ out, long long n, int cols, int parts,
@@ -332,19 +332,19 @@ __global__ void __launch_bounds__(256) move_kernel(const T* __restrict__ in, lon
   const long long r = unit / parts;
   if (r >= n) return;
   const int lane = threadIdx.x & 31, vecs = cols / N;
-  const int v0 = static_cast<int>(unit - r * parts) * (32 * kMove) + lane;
+  const int v0 = static_cast<int>(unit - r * parts) * (32 * kMove<N>) + lane;
   const long long s = src.row(r);
   const Pack<T, N>* a = reinterpret_cast<const Pack<T, N>*>(in + (s < 0 ? 0 : s) * ld);
   Pack<T, N>* o = reinterpret_cast<Pack<T, N>*>(out + r * cols);
-  Pack<T, N> p[kMove];
+  Pack<T, N> p[kMove<N>];
 #pragma unroll
-  for (int u = 0; u < kMove; ++u) {
+  for (int u = 0; u < kMove<N>; ++u) {
     const int v = v0 + u * 32;
     p[u] = zeros<T, N>();
     if (s >= 0 && v < vecs) p[u] = a[v];
   }
 #pragma unroll
-  for (int u = 0; u < kMove; ++u) {
+  for (int u = 0; u < kMove<N>; ++u) {
     const int v = v0 + u * 32;
     if (v >= vecs) break;
     if constexpr (kScale) {
@@ -358,23 +358,27 @@ __global__ void __launch_bounds__(256) move_kernel(const T* __restrict__ in, lon
   }
 }
 
+constexpr int kSingleThreads = 128;      // of a block that works on a row of single elements
 // out[t] = sum_j w[t, j] in[dest[t, j]] in 32 bits, j ascending.  A block per token: its places are read once, and the rows that follow
-// from them in vectors of all threads, eight rows in flight (a warp per part of a row waited for its places as long as for the rows:
-// 61 us against 47 us for 65536 rows of 4 KB).
+// from them in vectors of all threads, eight rows in flight (single elements: four rows, eight elements of a thread).  Measured for
+// 65536 rows of 4 KB, 47 us of memory: 54 us; a warp per part of a row, which waits for its places as long as for the rows, 61 us; blocks
+// that fetch the places of their next token meanwhile, but wait for one another between tokens, 63 us.
 template <typename T, int N, bool kWeight, typename OutT>
-__global__ void __launch_bounds__(256) sum_kernel(const T* __restrict__ in, long long ld, const int* __restrict__ dest, const float* __restrict__ weight,
+__global__ void __launch_bounds__(N == 1 ? kSingleThreads : 256) sum_kernel(const T* __restrict__ in, long long ld, const int* __restrict__ dest, const float* __restrict__ weight,
                                                   OutT* __restrict__ out, int k, int cols) {
   const long long row = blockIdx.x;
-  const int vecs = cols / N;
-  constexpr int J = 8;
-  for (int v = threadIdx.x; v < vecs; v += blockDim.x) {
-    float acc[N];
+  constexpr int S = N == 1 ? 4 : 1, J = N == 1 ? 4 : 8;      // vectors of a thread at a time, rows in flight
+  const int vecs = cols / N, step = N == 1 ? kSingleThreads : blockDim.x;
+  for (int v = threadIdx.x; v < vecs; v += S * step) {
+    float acc[S][N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) acc[i] = 0.f;
+    for (int s = 0; s < S; ++s)
+#pragma unroll
+      for (int i = 0; i < N; ++i) acc[s][i] = 0.f;
     for (int j0 = 0; j0 < k; j0 += J) {
       int d[J];
       float w[J];
-      Pack<T, N> p[J];
+      Pack<T, N> p[J][S];
 #pragma unroll
       for (int j = 0; j < J; ++j) {
         d[j] = j0 + j < k ? dest[row * k + j0 + j] : -1;
@@ -382,26 +386,34 @@ __global__ void __launch_bounds__(256) sum_kernel(const T* __restrict__ in, long
       }
 #pragma unroll
       for (int j = 0; j < J; ++j)
-        if (d[j] >= 0) p[j] = reinterpret_cast<const Pack<T, N>*>(in + d[j] * ld)[v];
+#pragma unroll
+        for (int s = 0; s < S; ++s)
+          if (d[j] >= 0 && v + s * step < vecs) p[j][s] = reinterpret_cast<const Pack<T, N>*>(in + d[j] * ld)[v + s * step];
 #pragma unroll
       for (int j = 0; j < J; ++j)
-        if (d[j] >= 0) {
-          float f[N];
-          p[j].get(f);
 #pragma unroll
-          for (int i = 0; i < N; ++i) acc[i] = kWeight ? fmaf(w[j], f[i], acc[i]) : acc[i] + f[i];
-        }
+        for (int s = 0; s < S; ++s)
+          if (d[j] >= 0 && v + s * step < vecs) {
+            float f[N];
+            p[j][s].get(f);
+#pragma unroll
+            for (int i = 0; i < N; ++i) acc[s][i] = kWeight ? fmaf(w[j], f[i], acc[s][i]) : acc[s][i] + f[i];
+          }
     }
-    Pack<OutT, N> o;
-    o.set(acc);
-    reinterpret_cast<Pack<OutT, N>*>(out + row * cols)[v] = o;
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      if (v + s * step >= vecs) break;
+      Pack<OutT, N> o;
+      o.set(acc[s]);
+      reinterpret_cast<Pack<OutT, N>*>(out + row * cols)[v + s * step] = o;
+    }
   }
 }
 
 // Backward of the weighted sum: d_y[dest] = w d_out[t] and d_w = <d_out[t], y[dest]>.  A block per token holds its row of d_out while
 // it walks over the token's rows of y, so that all of them pass once; blocks behind the tokens write the zeros of padding rows.
 template <typename T, int N>
-__global__ void __launch_bounds__(256) sum_bwd_kernel(const T* __restrict__ d_out, long long ld, const T* __restrict__ y, long long ldy,
+__global__ void __launch_bounds__(N == 1 ? kSingleThreads : 256) sum_bwd_kernel(const T* __restrict__ d_out, long long ld, const T* __restrict__ y, long long ldy,
                                                       const int* __restrict__ source, const int* __restrict__ dest, const float* __restrict__ weight,
                                                       T* __restrict__ d_y, float* __restrict__ d_w, long long cap, long long n, int k, int cols) {
   const int t = threadIdx.x, lane = t & 31, w = t >> 5, warps = blockDim.x >> 5, vecs = cols / N;
@@ -425,29 +437,61 @@ __global__ void __launch_bounds__(256) sum_bwd_kernel(const T* __restrict__ d_ou
       wj[j] = d[j] >= 0 ? weight[row * k + j0 + j] : 0.f;
       dot[j] = 0.f;
     }
-    for (int v = t; v < vecs; v += blockDim.x) {
-      float f[N];
-      a[v].get(f);
+    if constexpr (N == 1) {      // four elements of a thread at a time, four rows in flight
+      constexpr int S = 4;
+      for (int v = t; v < vecs; v += S * kSingleThreads) {
+        float f[S];
+        const T* av = d_out + row * ld + v;
 #pragma unroll
-      for (int h = 0; h < J; h += 4) {
-        Pack<T, N> q[4];
+        for (int s = 0; s < S; ++s) f[s] = v + s * kSingleThreads < vecs ? up(av[s * kSingleThreads]) : 0.f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (d[h + j] >= 0) q[j] = reinterpret_cast<const Pack<T, N>*>(y + d[h + j] * ldy)[v];
+        for (int h = 0; h < J; h += 4) {
+          if (j0 + h >= k) continue;
+          T q[4][S];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (d[h + j] >= 0) {
-            float b[N];
-            q[j].get(b);
+          for (int j = 0; j < 4; ++j) {
+            const T* b = y + (d[h + j] < 0 ? 0 : d[h + j]) * ldy + v;
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-              dot[h + j] = fmaf(f[i], b[i], dot[h + j]);
-              b[i] = f[i] * wj[h + j];
-            }
-            Pack<T, N> o;
-            o.set(b);
-            reinterpret_cast<Pack<T, N>*>(d_y + static_cast<long long>(d[h + j]) * cols)[v] = o;
+            for (int s = 0; s < S; ++s)
+              if (d[h + j] >= 0 && v + s * kSingleThreads < vecs) q[j][s] = b[s * kSingleThreads];
           }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            T* o = d_y + static_cast<long long>(d[h + j] < 0 ? 0 : d[h + j]) * cols + v;
+#pragma unroll
+            for (int s = 0; s < S; ++s)
+              if (d[h + j] >= 0 && v + s * kSingleThreads < vecs) {
+                dot[h + j] = fmaf(f[s], up(q[j][s]), dot[h + j]);
+                o[s * kSingleThreads] = down<T>(f[s] * wj[h + j]);
+              }
+          }
+        }
+      }
+    } else {
+      for (int v = t; v < vecs; v += blockDim.x) {
+        float f[N];
+        a[v].get(f);
+#pragma unroll
+        for (int h = 0; h < J; h += 4) {
+          Pack<T, N> q[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (d[h + j] >= 0) q[j] = reinterpret_cast<const Pack<T, N>*>(y + d[h + j] * ldy)[v];
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (d[h + j] >= 0) {
+              float b[N];
+              q[j].get(b);
+#pragma unroll
+              for (int i = 0; i < N; ++i) {
+                dot[h + j] = fmaf(f[i], b[i], dot[h + j]);
+                b[i] = f[i] * wj[h + j];
+              }
+              Pack<T, N> o;
+              o.set(b);
+              reinterpret_cast<Pack<T, N>*>(d_y + static_cast<long long>(d[h + j]) * cols)[v] = o;
+            }
+        }
       }
     }
 #pragma unroll
@@ -614,7 +658,7 @@ template <typename T, typename Row>
 int move_t(const void* in, long long ld, const Row& src, void* out, long long n, int cols, float scale, cudaStream_t st) {
   constexpr int NV = 16 / sizeof(T);
   const bool wide = wide_rows(in, ld, cols, sizeof(T)) && wide_rows(out, cols, cols, sizeof(T));
-  const int per = 32 * kMove * (wide ? NV : 1), parts = (cols + per - 1) / per;
+  const int per = wide ? 32 * kMove<NV> * NV : 32 * kMove<1>, parts = (cols + per - 1) / per;
   const long long grid = grid_of(n * parts);
   if (grid > kMaxGrid) return -3;
   const T* a = static_cast<const T*>(in);
@@ -639,13 +683,17 @@ int move_any(const void* in, long long ld, const Row& src, void* out, long long 
   return -1;
 }
 
-inline int row_threads(int vecs) { return vecs <= 32 ? 32 : vecs <= 64 ? 64 : vecs <= 256 ? 128 : 256; }
+// threads of a block that works on one row: up to two vectors each
+inline int row_threads(int vecs, bool single) {
+  if (single) return kSingleThreads;
+  return vecs <= 32 ? 32 : vecs <= 64 ? 64 : vecs <= 256 ? 128 : 256;
+}
 
 template <typename T, int N, typename OutT>
 int sum_t(const void* in, long long ld, const int* dest, const float* weight, void* out, int n, int k, int cols, cudaStream_t st) {
   const T* a = static_cast<const T*>(in);
   OutT* o = static_cast<OutT*>(out);
-  const int threads = row_threads(cols / N);
+  const int threads = row_threads(cols / N, N == 1);
   if (weight) sum_kernel<T, N, true, OutT><<<n, threads, 0, st>>>(a, ld, dest, weight, o, k, cols);
   else sum_kernel<T, N, false, OutT><<<n, threads, 0, st>>>(a, ld, dest, weight, o, k, cols);
   rb_note_launch(1);
@@ -662,7 +710,7 @@ template <typename T>
 int sum_bwd_t(const void* d_out, long long ld, const void* y, long long ldy, const int* source, const int* dest, const float* weight, void* d_y, float* d_w,
               long long cap, long long n, int k, int cols, cudaStream_t st) {
   const bool wide = wide_rows(d_out, ld, cols, sizeof(T)) && wide_rows(y, ldy, cols, sizeof(T)) && wide_rows(d_y, cols, cols, sizeof(T));
-  const int threads = row_threads(cols / (wide ? 16 / static_cast<int>(sizeof(T)) : 1));
+  const int threads = row_threads(cols / (wide ? 16 / static_cast<int>(sizeof(T)) : 1), !wide);
   const long long warps = threads / 32, grid = n + (cap + warps - 1) / warps;
   if (grid > kMaxGrid) return -3;
   const T *a = static_cast<const T*>(d_out), *b = static_cast<const T*>(y);

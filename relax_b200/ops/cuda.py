@@ -1259,42 +1259,39 @@ def _distill_codes(kl_type, alpha, norm_mode, temperature, clamp):
 
 
 def topk_distill(logits, ids, teacher, kl_type, alpha, norm_mode, temperature, clamp, want):
-    return _load().topk_distill(logits, ids, teacher.detach(), *_distill_codes(kl_type, alpha, norm_mode, temperature, clamp), bool(want))
+    return _load().topk_distill(logits, ids, teacher, *_distill_codes(kl_type, alpha, norm_mode, temperature, clamp), bool(want))
 
 
 class _FusedHeadDistill(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, ids, teacher, codes, chunk):
-        L = _load()
         h, w = hidden.contiguous(), weight.contiguous()
-        R, K = ids.shape
-        f32 = lambda *s: torch.empty(*s, dtype=torch.float32, device=h.device)      # noqa: E731
-        loss, coef, stats = f32(R), f32(R, K), f32(R, 4)
+        R = ids.shape[0]
+        loss, kept = torch.empty(R, dtype=torch.float32, device=h.device), []
         for s in range(0, R, chunk):
             e = min(R, s + chunk)
-            z = matmul_nt(h[s:e], w, out_dtype=torch.float32)
-            loss[s:e], coef[s:e], stats[s:e] = L.topk_distill_rows(z, ids[s:e], teacher[s:e], *codes)
-        ctx.save_for_backward(h, w, ids, coef, stats)
+            loss[s:e], k = _load().topk_distill_rows(matmul_nt(h[s:e], w, out_dtype=torch.float32), ids[s:e], teacher[s:e], *codes)
+            kept.append(k)
+        ctx.save_for_backward(h, w, ids, *kept)
         ctx.meta = (codes[-1], chunk, weight)
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
-        h, w, ids, coef, stats = ctx.saved_tensors
+        h, w, ids, *kept = ctx.saved_tensors
         inv_temp, chunk, weight = ctx.meta
-        L = _load()
         g = g.float().contiguous()
         R, V = h.shape[0], w.shape[0]
         dh = torch.empty_like(h)
         mg = main_grad_of(weight)
-        direct = mg is not None and mg.stride(-1) == 1
+        direct = mg is not None and mg.is_contiguous()
         dw = mg if direct else torch.zeros(w.shape, dtype=torch.float32, device=h.device)
-        for s in range(0, R, chunk):
+        for k, s in zip(kept, range(0, R, chunk)):
             e = min(R, s + chunk)
             z = matmul_nt(h[s:e], w, out_dtype=torch.float32)
             d = torch.empty(e - s, V, dtype=h.dtype, device=h.device)
-            L.topk_distill_rows_bwd(z, ids[s:e], coef[s:e], stats[s:e], g[s:e], inv_temp, d)
+            _load().topk_distill_rows_bwd(z, ids[s:e], k, g[s:e], inv_temp, d)
             matmul_nn(d, w, out=dh[s:e])
             matmul_tn(d, h[s:e], out=dw, accumulate=True)
         return dh, None if direct else dw.to(weight.dtype), None, None, None, None
