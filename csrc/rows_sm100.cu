@@ -16,8 +16,8 @@
 namespace rb {
 namespace rows {
 
-constexpr int kWarps = 16, kThreads = 32 * kWarps;      // of the sorting kernels
-constexpr int kMaxBins = 2048;                          // 16 warps x 2048 counters: 128 KB of shared memory
+constexpr int kWarps = 32, kThreads = 32 * kWarps;      // of the sorting kernels
+constexpr int kMaxBins = 2048;                          // 32 warps x 2048 counters of 16 bits: 128 KB of shared memory
 
 // ----------------------------------------------------------------------------- elements
 __device__ __forceinline__ float up(float v) { return v; }
@@ -81,10 +81,10 @@ __device__ __forceinline__ Pack<T, N> zeros() {
 }
 
 // ----------------------------------------------------------------------------- stable counting sort
-// One pass puts rows in the order of a key with few values ("bins"), rows of a bin in their old order.  A block counts its rows
-// (count_kernel); with every block's counts known, each block derives where its rows of every bin go and writes them
-// (place_kernel).  Ranks inside a block: every warp owns a run of rows and a counter per bin; 32 rows at a time find their
-// equals with one match instruction.  Up to kOneBlock rows take place_kernel alone.
+// One pass puts rows in the order of a key with few values ("bins"), rows of a bin in their old order.  In place_kernel every warp of
+// a block has a run of rows and a counter per bin; 32 rows at a time find their equals with one match instruction, which gives
+// their rank in the warp and moves the counter.  Counters of warps in front, and of blocks in front (count_kernel's), are added then.
+// Up to kOneBlock rows take place_kernel alone.
 
 struct ExpertKeys {      // expert ids; others than 0 .. bins - 1 live elsewhere and take no part
   const void* ids;
@@ -138,7 +138,7 @@ __device__ __forceinline__ void fill_near(const Fill& f, int blocks) {
   const long long t = blockIdx.x * static_cast<long long>(kThreads) + threadIdx.x, all = static_cast<long long>(blocks) * kThreads;
   for (long long i = t; i < f.n_near; i += all) f.near[i] = -1;
 }
-constexpr int kFillRun = 16;      // vectors of a thread: a block fills 128 KB in one piece (measured against a stride of the whole grid: 5.1 TB/s)
+constexpr int kFillRun = 8;      // vectors of a thread: a block fills 128 KB in one piece (6.9 TB/s; a stride of the whole grid: 5.1)
 __device__ __forceinline__ void fill_far(const Fill& f, int blocks) {
   const long long b = blockIdx.x - blocks, v0 = f.lo + b * (kThreads * kFillRun) + threadIdx.x;
   const uint4 z = make_uint4(0, 0, 0, 0);
@@ -164,33 +164,89 @@ __global__ void __launch_bounds__(kThreads) count_kernel(Src src, int n, int chu
   for (int b = threadIdx.x; b < bins; b += kThreads) hist[static_cast<size_t>(blockIdx.x) * bins + b] = cnt[b];
 }
 
-template <typename Src, typename Out>
-__global__ void __launch_bounds__(kThreads) place_kernel(Src src, Out out, int n, int chunk, int bins, int align, int blocks, const int* __restrict__ hist,
-                                                         Fill fill) {
+// `sum` of all threads in front of this one, in `all` that of the block; `part`: kWarps ints of shared memory
+__device__ __forceinline__ int scan_block(int sum, int* part, int* all) {
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  int scan = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, scan, o);
+    if (lane >= o) scan += v;
+  }
+  if (lane == 31) part[w] = scan;
+  __syncthreads();
+  int mine = part[lane];
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, mine, o);
+    if (lane >= o) mine += v;
+  }
+  *all = __shfl_sync(0xffffffffu, mine, 31);
+  const int before = __shfl_sync(0xffffffffu, mine, (w + 31) & 31);
+  return scan - sum + (w > 0 ? before : 0);
+}
+// the rank of this lane's digit among those of its warp so far; the warp's counters move on (digit -1: none)
+__device__ __forceinline__ int rank_in_warp(uint16_t* mine, int d) {
+  const unsigned lane = threadIdx.x & 31, same = __match_any_sync(0xffffffffu, d);
+  const int c = d >= 0 ? mine[d] : 0;
+  __syncwarp();
+  if (d >= 0 && static_cast<int>(lane) == __ffs(same) - 1) mine[d] = static_cast<uint16_t>(c + __popc(same));
+  __syncwarp();
+  return c + __popc(same & ((1u << lane) - 1));
+}
+// a bin's counters of `warps` warps become those of the warps in front; returns their sum
+__device__ __forceinline__ int scan_warps(uint16_t* cnt, int bins, int b, int warps) {
+  int run = 0;
+#pragma unroll
+  for (int k0 = 0; k0 < kWarps; k0 += 8) {
+    if (k0 >= warps) break;
+    int c[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) c[k] = k0 + k < warps ? cnt[(k0 + k) * bins + b] : 0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      if (k0 + k < warps) cnt[(k0 + k) * bins + b] = static_cast<uint16_t>(run);
+      run += c[k];
+    }
+  }
+  return run;
+}
+
+// kSteps x 1024 rows per block
+template <typename Src, typename Out, int kSteps>
+__global__ void __launch_bounds__(kThreads) place_kernel(Src src, Out out, int n, int bins, int align, int blocks, const int* __restrict__ hist, Fill fill) {
   constexpr bool kExperts = std::is_same<Out, ExpertOut>::value;
   extern __shared__ int sm[];
   __shared__ int part[kWarps];
   if (static_cast<int>(blockIdx.x) >= blocks) return fill_far(fill, blocks);
   const int t = threadIdx.x, w = t >> 5, lane = t & 31;
-  const int per = chunk / kWarps;      // rows of a warp (a multiple of 32)
-  const int first = blockIdx.x * chunk, warps = min(kWarps, (min(n - first, chunk) + per - 1) / per);      // that have rows
-  int* start = sm;                     // [bins] first output row of the bin
-  int* total = sm + bins;              // [bins] rows of the bin
-  int* cnt = total + bins;             // [warps][bins]
-  for (int b = t; b < warps * bins; b += kThreads) cnt[b] = 0;
+  constexpr int kPer = 32 * kSteps;      // rows of a warp
+  const int first = blockIdx.x * (kSteps * kThreads), here = min(n - first, kSteps * kThreads), warps = (here + kPer - 1) / kPer;
+  int* start = sm;                       // [bins] first output row of the bin (of this block's rows of it)
+  int* total = sm + bins;                // [bins] rows of the bin
+  int* first_row = total + bins;         // [bins] first output row of the bin
+  uint16_t* cnt = reinterpret_cast<uint16_t*>(first_row + bins);      // [warps][bins]
+  for (int i = t; i < warps * bins; i += kThreads) cnt[i] = 0;
+  int at[kSteps];      // digits, then digits and ranks
+#pragma unroll
+  for (int s = 0; s < kSteps; ++s) {
+    const int i = first + w * kPer + s * 32 + lane;
+    at[s] = i < n ? src.digit(i) : -1;
+  }
   if (blocks == 1) fill_near(fill, 1);
   __syncthreads();
-  const int lo = min(n, first + w * per), hi = min(n, lo + per);
-  int* mine = cnt + w * bins;
-  for (int i = lo + lane; i < hi; i += 32) {
-    const int d = src.digit(i);
-    if (d >= 0) atomicAdd(&mine[d], 1);
+  uint16_t* mine = cnt + w * bins;
+  if (w < warps) {
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      const int rank = rank_in_warp(mine, at[s]);
+      at[s] = at[s] < 0 ? -1 : at[s] << 16 | rank;      // (ranks of a warp's 512 rows)
+    }
   }
   __syncthreads();
-  // counters become the rows of the same bin in warps in front, and those of blocks in front; `total`: of all blocks.  First output
-  // row of every bin: running sum of the (padded) counts; a thread looks after a run of bins
+  // first output row of every bin: running sum of the (padded) counts; a thread looks after a run of bins
   const int each = (bins + kThreads - 1) / kThreads, b0 = min(bins, t * each), b1 = min(bins, b0 + each);
-  int sum = 0;
+  int sum = 0, end;
   for (int b = b0; b < b1; ++b) {
     int before = 0, all = 0;
     if (blocks > 1) {
@@ -201,38 +257,20 @@ __global__ void __launch_bounds__(kThreads) place_kernel(Src src, Out out, int n
         before += k < static_cast<int>(blockIdx.x) ? h : 0;
       }
     }
-    int run = before, mine_of[kWarps];
-#pragma unroll
-    for (int k = 0; k < kWarps; ++k) mine_of[k] = k < warps ? cnt[k * bins + b] : 0;
-#pragma unroll
-    for (int k = 0; k < kWarps; ++k) {
-      if (k < warps) cnt[k * bins + b] = run;
-      run += mine_of[k];
-    }
-    total[b] = blocks > 1 ? all : run;
+    const int own = scan_warps(cnt, bins, b, warps);
+    start[b] = before;
+    total[b] = blocks > 1 ? all : own;
     sum += (total[b] + align - 1) / align * align;
   }
-  int scan = sum;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int v = __shfl_up_sync(0xffffffffu, scan, o);
-    if (lane >= o) scan += v;
-  }
-  if (lane == 31) part[w] = scan;
-  __syncthreads();
-  int base = scan - sum;
-#pragma unroll
-  for (int k = 0; k < kWarps; ++k) base += k < w ? part[k] : 0;
+  int base = scan_block(sum, part, &end);
   for (int b = b0; b < b1; ++b) {
-    start[b] = base;
     const int rows = (total[b] + align - 1) / align * align;
     if constexpr (kExperts) {
-      // (every block knows all bounds: bins are shared out to the blocks)
-      if (b % blocks == static_cast<int>(blockIdx.x)) {
-        out.bounds[b] = base;
-        if (b == bins - 1) out.bounds[bins] = base + rows;
-      }
+      if (b % blocks == static_cast<int>(blockIdx.x)) out.bounds[b] = base;      // (every block knows all bounds)
+      if (b == bins - 1 && blockIdx.x == 0) out.bounds[bins] = end;
+      first_row[b] = base;
     }
+    start[b] += base;
     base += rows;
   }
   __syncthreads();
@@ -240,68 +278,156 @@ __global__ void __launch_bounds__(kThreads) place_kernel(Src src, Out out, int n
     for (int q = blockIdx.x * kThreads + t; q < out.tiles; q += blocks * kThreads) {      // the last expert that begins at or in front of the tile
       int b = 0;
       for (int step = 1 << (31 - __clz(bins)); step > 0; step >>= 1)
-        if (b + step < bins && start[b + step] <= q * align) b += step;
-      out.tile_expert[q] = q * align < start[b] + (total[b] + align - 1) / align * align ? b : -1;
+        if (b + step < bins && first_row[b + step] <= q * align) b += step;
+      out.tile_expert[q] = q * align < end && q * align < first_row[b] + (total[b] + align - 1) / align * align ? b : -1;
     }
   }
-  for (int i0 = lo; i0 < hi; i0 += 32) {
-    const int i = i0 + lane;
-    const int d = i < hi ? src.digit(i) : -1;
-    const unsigned same = __match_any_sync(0xffffffffu, d);
-    int at = -1;
-    if (d >= 0) at = start[d] + mine[d] + __popc(same & ((1u << lane) - 1));
-    __syncwarp();
-    if (d >= 0 && lane == __ffs(same) - 1) mine[d] += __popc(same);
-    __syncwarp();
-    if (i < hi) {
-      if constexpr (kExperts) {
-        out.dest[i] = at;
-        if (at >= 0) out.source[at] = i;
-      } else {
-        out.pairs[at] = make_int2(src.key(i), src.pos(i));
-      }
+#pragma unroll
+  for (int s = 0; s < kSteps; ++s) {
+    const int i = first + w * kPer + s * 32 + lane;
+    if (i >= n) break;
+    const int d = at[s] >> 16, to = at[s] < 0 ? -1 : start[d] + mine[d] + (at[s] & 0xffff);
+    if constexpr (kExperts) {
+      out.dest[i] = to;
+      if (to >= 0) out.source[to] = i;
+    } else {
+      out.pairs[to] = make_int2(src.key(i), src.pos(i));
     }
   }
 }
 
+// Tokens sorted by table row in one launch: (key, position) in 32 bits, all passes in the shared memory of one block (two passes of
+// 16384 tokens 13 us, four launches of the kernels above 16 us).
+template <int kSteps>
+__global__ void __launch_bounds__(kThreads) pack_sort_kernel(TokenKeys src, int2* __restrict__ pairs, int n, int pos_bits, int passes, int each, Fill fill) {
+  extern __shared__ int sm[];
+  __shared__ int part[kWarps];
+  if (blockIdx.x > 0) return fill_far(fill, 1);
+  const int t = threadIdx.x, w = t >> 5, lane = t & 31, bins = 1 << each;
+  constexpr int kPer = 32 * kSteps;
+  const int warps = (n + kPer - 1) / kPer;
+  unsigned* a = reinterpret_cast<unsigned*>(sm);                       // [n] (between two barriers all of them are in registers)
+  int* start = sm + n;                                                 // [bins]
+  uint16_t* cnt = reinterpret_cast<uint16_t*>(start + bins);           // [warps][bins]
+  unsigned v[kSteps];
+#pragma unroll
+  for (int s = 0; s < kSteps; ++s) {
+    const int i = w * kPer + s * 32 + lane;
+    v[s] = i < n ? static_cast<unsigned>(src.key(i)) << pos_bits | i : 0;
+  }
+  uint16_t* mine = cnt + w * bins;
+  for (int p = 0; p < passes; ++p) {
+    const int shift = pos_bits + p * each;
+    for (int i = t; i < warps * bins; i += kThreads) cnt[i] = 0;
+    if (p > 0) {
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        const int i = w * kPer + s * 32 + lane;
+        v[s] = i < n ? a[i] : 0;
+      }
+    }
+    __syncthreads();
+    int rank[kSteps];
+    if (w < warps) {
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        const int i = w * kPer + s * 32 + lane;
+        rank[s] = rank_in_warp(mine, i < n ? static_cast<int>(v[s] >> shift) & (bins - 1) : -1);
+      }
+    }
+    __syncthreads();
+    const int own = t < bins ? scan_warps(cnt, bins, t, warps) : 0;      // (bins <= threads)
+    int end;
+    const int base = scan_block(own, part, &end);
+    if (t < bins) start[t] = base;
+    __syncthreads();
+    if (w < warps) {
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        const int i = w * kPer + s * 32 + lane;
+        if (i >= n) break;
+        const int d = static_cast<int>(v[s] >> shift) & (bins - 1);
+        a[start[d] + mine[d] + rank[s]] = v[s];
+      }
+    }
+    __syncthreads();
+  }
+  for (int i = t; i < n; i += kThreads) pairs[i] = make_int2(static_cast<int>(a[i] >> pos_bits), static_cast<int>(a[i] & ((1u << pos_bits) - 1)));
+}
+
 constexpr int kMaxSort = 1 << 30;      // rows and keys of a sort (places are 32-bit)
-constexpr int kOneBlock = 4096;        // rows that one block sorts by itself
-inline int sort_chunk(long long n) {      // rows of a block: enough blocks to spread the work, few enough that reading all their counts is cheap
-  if (n <= kOneBlock) return n <= 0 ? kThreads : static_cast<int>((n + kThreads - 1) / kThreads) * kThreads;
-  long long c = (n + 63) / 64;
-  c = (c + kThreads - 1) / kThreads * kThreads;
-  return static_cast<int>(c < 1024 ? 1024 : c);
+constexpr int kMostSteps = 16;         // counters of a warp's rows have 16 bits, and so have all of a block's
+constexpr int kOneBlock = 4096;        // rows that one block sorts by itself (9003 rows: 18 us, in nine blocks after a count 9 us)
+constexpr int kPackSort = 16384;       // ... and that pack_sort_kernel takes, where a key and a position fit 32 bits
+// 1024-row steps of a block: enough blocks to spread the work, few enough that reading all their counts is cheap
+inline int sort_steps(long long n) {
+  const long long want = n <= kOneBlock ? (n + kThreads - 1) / kThreads : (n + 64ll * kThreads - 1) / (64ll * kThreads);
+  return want <= 1 ? 1 : want <= 2 ? 2 : want <= 4 ? 4 : want <= 8 ? 8 : kMostSteps;
 }
 inline int sort_blocks(long long n) {
-  const int c = sort_chunk(n);
+  const long long c = static_cast<long long>(sort_steps(n)) * kThreads;
   return n <= 0 ? 1 : static_cast<int>((n + c - 1) / c);
+}
+inline int fill_blocks(const Fill& f, long long vectors) {
+  return f.far == nullptr ? 0 : static_cast<int>((vectors + kThreads * kFillRun - 1) / (kThreads * kFillRun)) + 1;
+}
+template <typename K>
+int allow_smem(K kernel, size_t bytes) {
+  return bytes <= 48 * 1024 ? 0 : static_cast<int>(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)));
+}
+
+template <int kSteps, typename Src, typename Out>
+int place(const Src& src, const Out& out, int n, int bins, int align, int blocks, int more, const int* hist, const Fill& fill, cudaStream_t st) {
+  const size_t smem = static_cast<size_t>(bins) * (12 + 2 * kWarps);
+  const int rc = allow_smem(place_kernel<Src, Out, kSteps>, smem);
+  if (rc) return rc;
+  place_kernel<Src, Out, kSteps><<<blocks + more, kThreads, smem, st>>>(src, out, n, bins, align, blocks, hist, fill);
+  rb_note_launch(1);
+  return static_cast<int>(cudaGetLastError());
 }
 
 // `launches` of the whole sort share the far fill evenly; `at` counts them
 template <typename Src, typename Out>
-int sort_pass(const Src& src, const Out& out, int n, int bins, int align, int* hist, Fill fill, int launches, int* at, cudaStream_t st) {
-  const int chunk = sort_chunk(n), nb = sort_blocks(n);
-  const size_t smem = static_cast<size_t>(kWarps + 2) * bins * sizeof(int);
-  if (smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(place_kernel<Src, Out>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-    if (e != cudaSuccess) return static_cast<int>(e);
-  }
+int sort_pass(const Src& src, const Out& out, int n, int bins, int align, int* hist, const Fill& fill, int launches, int* at, cudaStream_t st) {
+  const int nb = sort_blocks(n), steps = sort_steps(n);
   const long long vectors = fill.hi;
-  auto share = [&](Fill f) {
+  auto share = [&]() {
+    Fill f = fill;
     f.lo = vectors * *at / launches;
     f.hi = vectors * (*at + 1) / launches;
     if (*at > 0) f.n_rest = 0;
     ++*at;
     return f;
   };
-  const int more = fill.far == nullptr ? 0 : static_cast<int>(vectors / launches / (kThreads * kFillRun)) + 2;      // (covers a share of vectors / launches + 1)
   if (nb > 1) {
-    count_kernel<Src><<<nb + more, kThreads, bins * sizeof(int), st>>>(src, n, chunk, bins, nb, hist, share(fill));
+    const Fill f = share();
+    count_kernel<Src><<<nb + fill_blocks(f, f.hi - f.lo), kThreads, bins * sizeof(int), st>>>(src, n, steps * kThreads, bins, nb, hist, f);
     rb_note_launch(1);
   }
-  place_kernel<Src, Out><<<nb + more, kThreads, smem, st>>>(src, out, n, chunk, bins, align, nb, hist, share(fill));
+  const Fill f = share();
+  const int more = fill_blocks(f, f.hi - f.lo);
+  switch (steps) {
+    case 1: return place<1>(src, out, n, bins, align, nb, more, hist, f, st);
+    case 2: return place<2>(src, out, n, bins, align, nb, more, hist, f, st);
+    case 4: return place<4>(src, out, n, bins, align, nb, more, hist, f, st);
+    case 8: return place<8>(src, out, n, bins, align, nb, more, hist, f, st);
+    default: return place<kMostSteps>(src, out, n, bins, align, nb, more, hist, f, st);
+  }
+}
+
+template <int kSteps>
+int pack_sort_t(const TokenKeys& src, int2* pairs, int n, int pos_bits, int passes, int each, const Fill& fill, cudaStream_t st) {
+  const size_t smem = static_cast<size_t>(n) * 4 + (size_t{1} << each) * (4 + 2 * kWarps);
+  const int rc = allow_smem(pack_sort_kernel<kSteps>, smem);
+  if (rc) return rc;
+  pack_sort_kernel<kSteps><<<1 + fill_blocks(fill, fill.hi), kThreads, smem, st>>>(src, pairs, n, pos_bits, passes, each, fill);
   rb_note_launch(1);
   return static_cast<int>(cudaGetLastError());
+}
+int pack_sort(const TokenKeys& src, int2* pairs, int n, int pos_bits, int passes, int each, const Fill& fill, cudaStream_t st) {
+  if (n <= 1 * kThreads) return pack_sort_t<1>(src, pairs, n, pos_bits, passes, each, fill, st);
+  if (n <= 4 * kThreads) return pack_sort_t<4>(src, pairs, n, pos_bits, passes, each, fill, st);
+  return pack_sort_t<16>(src, pairs, n, pos_bits, passes, each, fill, st);
 }
 
 // ----------------------------------------------------------------------------- copies of rows
@@ -828,18 +954,25 @@ extern "C" int rb_embedding_bwd(const void* ids, int wide, long long start, cons
     fill.rest = static_cast<unsigned char*>(out) + bytes / 16 * 16;
     fill.n_rest = static_cast<int>(bytes % 16);
   }
-  const int launches = passes * (sort_blocks(n) > 1 ? 2 : 1);
-  int at = 0;
+  int pos_bits = 1;
+  while (pos_bits < 31 && ((n - 1) >> pos_bits) != 0) ++pos_bits;
   int2* to = pairs;
   int2* from = pairs + n;
-  for (int p = 0; p < passes; ++p) {
-    int rc;
-    if (p == 0) rc = sort_pass(TokenKeys{ids, wide, rows, 0, mask, start}, PairOut{to}, n, bins, 1, hist, fill, launches, &at, st);
-    else rc = sort_pass(PairKeys{from, p * each, mask}, PairOut{to}, n, bins, 1, hist, fill, launches, &at, st);
+  if (n <= kPackSort && pos_bits + bits <= 32) {
+    const int rc = pack_sort(TokenKeys{ids, wide, rows, 0, mask, start}, from, n, pos_bits, passes, each, fill, st);
     if (rc) return rc;
-    int2* s = to;
-    to = from;
-    from = s;
+  } else {
+    const int launches = passes * (sort_blocks(n) > 1 ? 2 : 1);
+    int at = 0;
+    for (int p = 0; p < passes; ++p) {
+      int rc;
+      if (p == 0) rc = sort_pass(TokenKeys{ids, wide, rows, 0, mask, start}, PairOut{to}, n, bins, 1, hist, fill, launches, &at, st);
+      else rc = sort_pass(PairKeys{from, p * each, mask}, PairOut{to}, n, bins, 1, hist, fill, launches, &at, st);
+      if (rc) return rc;
+      int2* s = to;
+      to = from;
+      from = s;
+    }
   }
   switch (dtype) {
     case 0: return runs_any<__nv_bfloat16>(dy, ld, from, out, part, n, rows, cols, scale, add, st);

@@ -33,7 +33,7 @@ def _within(got, want, tol, what=""):
 
 @pytest.mark.parametrize("wide", [True, False])
 @pytest.mark.parametrize("T,k,E,align", [(0, 2, 4, 128), (1, 1, 1, 128), (1, 8, 128, 128), (96, 8, 32, 128), (513, 3, 11, 128), (5000, 2, 300, 128), (2500, 8, 256, 1),
-                                         (1700, 3, 2048, 16), (7, 40, 60, 128), (9001, 1, 5, 1)])
+                                         (1700, 3, 2048, 16), (7, 40, 60, 128), (9001, 1, 5, 1), (16384, 1, 33, 128), (16385, 1, 2048, 128), (30000, 3, 64, 128)])
 def test_layout(T, k, E, align, wide):
     g = torch.Generator().manual_seed(T + k)
     ids = (torch.randn(T, k, generator=g) * E * 0.6).long()              # half of them elsewhere, experts of very different load
@@ -205,6 +205,21 @@ def test_embedding_of_odd_views():
     (d,) = torch.autograd.grad(ops.embedding(ids, leaf), leaf, dy)
     want, size = O.embedding_grad(ids.cpu(), dy.reshape(-1, 17).cpu(), 50, 0, 1.0)
     _within(d, want, 2.0 ** -8 * want.abs() + 40 * F * size, "gradient")
+
+
+@pytest.mark.parametrize("n", [1, 31, 1024, 1025, 4097, 16384, 16385, 40000])
+@pytest.mark.parametrize("V", [3, 1023, 1024, 151936, (1 << 18) - 1, 1 << 18, 1 << 20, 3000001])
+def test_embedding_sort(n, V):
+    """Every way of sorting: one launch or several, one pass or more, keys up to and beyond a power of two, runs that cross chunks."""
+    g = _gen(n + V)
+    ids = torch.randint(-1, V + 1, (n,), device="cuda", generator=g)
+    ids[: n // 2] = ids[: n // 2] % 40                       # half of the tokens share few rows
+    ids[-1] = V - 1
+    table = torch.zeros(V, 4, device="cuda").requires_grad_()
+    dy = torch.randint(-8, 9, (n, 4), device="cuda", generator=g).float()        # whole numbers: sums are exact in any order
+    (d,) = torch.autograd.grad(ops.embedding(ids, table), table, dy)
+    ok = (ids >= 0) & (ids < V)
+    assert torch.equal(d, torch.zeros(V, 4, device="cuda").index_add_(0, ids[ok], dy[ok]))
 
 
 # --------------------------------------------------------------------------- distillation
