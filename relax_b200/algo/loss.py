@@ -29,7 +29,8 @@ class LossConfig:
     kl_loss_coef: float = 0.0
     kl_loss_type: str = "k1"
     use_unbiased_kl: bool = False
-    # on-policy distillation as a loss term (the teacher's log-probs of the sampled tokens travel in LossBatch.extras)
+    # on-policy distillation as a loss term (the teacher's log-probs of the sampled tokens, or the divergence on top-K ids, travel in
+    # LossBatch.extras)
     opd_loss_coef: float = 0.0
     opd_kl_type: str = "reverse_kl"
     opd_per_token_clip: Optional[float] = None
@@ -198,14 +199,16 @@ def policy_loss(log_probs: torch.Tensor, entropy: torch.Tensor, b: LossBatch, cf
         loss = loss + cfg.kl_loss_coef * kl_loss
         metrics["kl_loss"] = kl_loss.detach()
 
-    if cfg.opd_loss_coef != 0.0 and b.extras.get("teacher_log_probs") is not None:
+    if cfg.opd_loss_coef != 0.0 and (b.extras.get("teacher_log_probs") is not None or b.extras.get("opd_divergence") is not None):
         # on-policy distillation as a differentiable loss term (relax/utils/opd/opd_utils.py compute_policy_opd_loss
-        # :1366-1455): per-token divergence of the sampled token, clipped from above, optionally weighted by the
-        # truncated importance ratio of the current to the old policy
+        # :1366-1455): per-token divergence - of the sampled token, or on the top-K ids where the forward pass computed it -, clipped
+        # from above, optionally weighted by the truncated importance ratio of the current to the old policy
         from . import opd as _opd
 
-        d = _opd.token_kl(log_probs, b.extras["teacher_log_probs"].detach(), kl_type=cfg.opd_kl_type,
-                          log_prob_min_clamp=cfg.opd_log_prob_min_clamp)
+        d = b.extras.get("opd_divergence")
+        if d is None:
+            d = _opd.token_kl(log_probs, b.extras["teacher_log_probs"].detach(), kl_type=cfg.opd_kl_type,
+                              log_prob_min_clamp=cfg.opd_log_prob_min_clamp)
         if cfg.opd_per_token_clip is not None:
             metrics["opd_per_token_clip_frac"] = red((d > cfg.opd_per_token_clip).float()).detach()
             d = d.clamp(max=float(cfg.opd_per_token_clip))

@@ -488,8 +488,6 @@ def validate_args(a: argparse.Namespace) -> argparse.Namespace:
         if a.opd_kl_coef not in (0.0, 1.0):          # 1.0 is the flag's default: loss mode overrides it
             raise ValueError("exactly one of --opd-kl-coef / --opd-loss-coef is non-zero (advantage mode or loss mode)")
         a.opd_kl_coef = 0.0
-        if a.opd_token_selection != "student_sampled":
-            raise ValueError("--opd-loss-coef (loss mode) is wired for the sampled token; top-K selections use --opd-kl-coef")
     for name in ("opd_per_token_clip", "opd_is_clip"):
         if getattr(a, name) is not None and getattr(a, name) <= 0:
             raise ValueError(f"--{name.replace('_', '-')} must be > 0")

@@ -350,6 +350,14 @@ class GPTModel(nn.Module):
             hidden = TP.copy_to_tp(hidden, self.ps.tp)
         return ops.fused_lm_head_logprob(hidden, w, targets, self.ps.tp.group, self.vocab_start, with_entropy, temperature)
 
+    def topk_distill(self, hidden, ids, teacher_log_probs, temperature: float = 1.0, **kw):
+        """Per-row divergence from a teacher known on ``ids [rows, K]`` (:func:`relax_b200.ops.topk_distill`), logits in pieces of rows."""
+        if self.ps.tp.size > 1:
+            raise NotImplementedError("distillation from top ids reads whole rows of logits: tp = 1")
+        w = self.lm_head_weight()
+        w = w if w.shape[0] == self.cfg.vocab_size else w[: self.cfg.vocab_size]
+        return ops.fused_lm_head_topk_distill(hidden, w, ids, teacher_log_probs, temperature=temperature, **kw)
+
     def class_logits(self, hidden):
         """Sequence-classification logits ``[rows, num_classes]`` from the given (last-token) hidden rows."""
         if self.sequence_parallel:

@@ -373,7 +373,9 @@ class TrainActor:
                               self.mcfg.num_query_groups // tp, self.mcfg.head_dim)
         return self.cp_comm
 
-    def _forward_logp(self, pb, with_entropy: bool):
+    def _forward_logp(self, pb, with_entropy: bool, distill: Optional[dict] = None):
+        """Log-probs and entropy per response position.  ``distill`` (``ids``, ``teacher``): the divergence from a teacher on those ids is
+        computed from the same hidden states and left in ``distill["divergence"]``."""
         if (self.cfg.use_routing_replay or self.cfg.use_rollout_routing_replay) and self.mcfg.is_moe:
             from ..models.moe import RoutingReplay
 
@@ -385,6 +387,11 @@ class TrainActor:
         emb = self._embed_multimodal(pb) if getattr(pb, "pixel_patches", None) is not None else None
         h = self.model(pb.tokens, pb.positions, pb.cu_seqlens, max_seqlen=pb.max_seqlen, inputs_embeds=emb)
         hr = h.index_select(0, pb.logit_rows)
+        if distill is not None:
+            c = self.cfg
+            distill["divergence"] = self.model.topk_distill(hr, distill["ids"], distill["teacher"], c.rollout_temperature, kl_type=c.opd_kl_type,
+                                                            alpha=c.opd_jsd_alpha, norm_mode=c.opd_norm_mode,
+                                                            log_prob_min_clamp=c.opd_log_prob_min_clamp)
         return self.model.log_probs(hr, pb.targets, self.cfg.rollout_temperature, with_entropy)
 
     def _forward_logp_mtp(self, pb, with_entropy: bool, lb):
@@ -540,6 +547,31 @@ class TrainActor:
                     out_ids[i] = piece
         self.switch_model("actor")
         return {"ids": out_ids if ids is None else list(ids), "log_probs": out_lp}
+
+    def _distill_ids(self, batch: dict):
+        """The token ids of every response position on which student and teacher are compared: the student's top-K, the teacher's, or their
+        union (rows of different width, padded with -1).  Returns ``(ids, lengths or None, student's log-probs or None, teacher's
+        log-probs)``, lists with one entry per sample."""
+        from ..algo import opd as OPD
+
+        sel, k = self.cfg.opd_token_selection, self.cfg.opd_log_prob_top_k
+        if "teacher" not in self.snapshots:
+            raise ValueError(f"--opd-token-selection {sel} needs the teacher's distribution: an in-process teacher "
+                             "(--opd-teacher-load); remote teachers return the sampled token's log-prob only")
+        if k <= 0:
+            raise ValueError(f"--opd-token-selection {sel} needs --opd-log-prob-top-k > 0")
+        own_s = self.compute_topk_log_probs(batch, "actor", k=k) if sel in ("student_topk", "union") else None
+        own_t = self.compute_topk_log_probs(batch, "teacher", k=k) if sel in ("teacher_topk", "union") else None
+        if sel == "teacher_topk":
+            return own_t["ids"], None, None, own_t["log_probs"]
+        if sel == "student_topk":
+            ids, lengths, s_lp = own_s["ids"], None, own_s["log_probs"]
+        else:
+            pairs = [OPD.union_ids(a, b) for a, b in zip(own_s["ids"], own_t["ids"])]
+            lengths, s_lp = [n for _, n in pairs], None
+            col = lambda u, n: torch.arange(u.shape[-1], device=u.device)[None, :] < n[:, None]      # noqa: E731
+            ids = [u.masked_fill(~col(u, n), -1) for u, n in pairs]
+        return ids, lengths, s_lp, self.compute_topk_log_probs(batch, "teacher", ids=ids)["log_probs"]
 
     # ------------------------------------------------------------------ pipeline parallelism
     def _stage_forward(self, pb, x):
@@ -778,7 +810,12 @@ class TrainActor:
             # pure distillation (relax/backends/megatron/loss.py:638-644): the task reward's contribution is removed
             batch["advantages"] = [torch.zeros_like(a) for a in batch["advantages"]]
             batch["returns"] = [torch.zeros_like(r_) for r_ in batch["returns"]]
-        if cfg.loss.opd_loss_coef != 0.0 and batch.get("teacher_log_probs") is None and "teacher" in self.snapshots:
+        if cfg.loss.opd_loss_coef != 0.0 and cfg.opd_token_selection != "sampled_token":
+            if self.ps.cp.size > 1 or self.ps.pp.size > 1 or self.mcfg.mtp_num_layers > 0 or cfg.loss.custom_loss_function is not None:
+                raise NotImplementedError("top-K distillation as a loss term: the policy loss of the plain decoder, trainer pp = cp = 1")
+            with self.timer.span("teacher_log_probs"):      # loss mode: the student's side is part of the training forward
+                batch["opd_topk_token_ids"], _, _, batch["opd_teacher_topk_log_probs"] = self._distill_ids(batch)
+        elif cfg.loss.opd_loss_coef != 0.0 and batch.get("teacher_log_probs") is None and "teacher" in self.snapshots:
             with self.timer.span("teacher_log_probs"):      # loss mode: the term itself is built in the policy loss
                 batch["teacher_log_probs"] = self.compute_log_prob(batch, "teacher")["log_probs"]
         if cfg.opd_kl_coef != 0.0 and (batch.get("teacher_log_probs") is not None or "teacher" in self.snapshots):
@@ -796,29 +833,11 @@ class TrainActor:
                                             teacher_lp=torch.as_tensor(b, dtype=torch.float32, device=dev), **kw)
                        for a, b in zip(student, batch["teacher_log_probs"])]
             else:
-                # both distributions on a set of K ids per position (relax/utils/opd/opd_utils.py:1275-1420): the set is
-                # the student's top-K, the teacher's, or their union (rows of different width, padded and masked)
-                if "teacher" not in self.snapshots:
-                    raise ValueError(f"--opd-token-selection {sel} needs the teacher's distribution: an in-process teacher "
-                                     "(--opd-teacher-load); remote teachers return the sampled token's log-prob only")
-                k = cfg.opd_log_prob_top_k
-                if k <= 0:
-                    raise ValueError(f"--opd-token-selection {sel} needs --opd-log-prob-top-k > 0")
+                # both distributions on a set of K ids per position (relax/utils/opd/opd_utils.py:1275-1420)
                 with self.timer.span("teacher_log_probs"):
-                    own_s = self.compute_topk_log_probs(batch, "actor", k=k) if sel in ("student_topk", "union") else None
-                    own_t = self.compute_topk_log_probs(batch, "teacher", k=k) if sel in ("teacher_topk", "union") else None
-                    lengths = None
-                    if sel == "student_topk":
-                        ids = own_s["ids"]
-                    elif sel == "teacher_topk":
-                        ids = own_t["ids"]
-                    else:
-                        pairs = [OPD.union_ids(a, b) for a, b in zip(own_s["ids"], own_t["ids"])]
-                        lengths = [n for _, n in pairs]
-                        col = lambda u, n: torch.arange(u.shape[-1], device=u.device)[None, :] < n[:, None]
-                        ids = [u.masked_fill(~col(u, n), -1) for u, n in pairs]
-                    s_lp = own_s["log_probs"] if sel == "student_topk" else self.compute_topk_log_probs(batch, "actor", ids=ids)["log_probs"]
-                    t_lp = own_t["log_probs"] if sel == "teacher_topk" else self.compute_topk_log_probs(batch, "teacher", ids=ids)["log_probs"]
+                    ids, lengths, s_lp, t_lp = self._distill_ids(batch)
+                    if s_lp is None:
+                        s_lp = self.compute_topk_log_probs(batch, "actor", ids=ids)["log_probs"]
                 sig = [OPD.per_token_signal(sel, student_topk_lp=a, teacher_topk_lp=b, k_lengths=(lengths[i] if lengths else None), **kw)
                        for i, (a, b) in enumerate(zip(s_lp, t_lp))]
                 batch["opd_topk_token_ids"] = ids
@@ -883,6 +902,16 @@ class TrainActor:
                            rollout_log_probs=f("rollout_log_probs"), returns=f("returns"), values=f("values"),
                            sample_denoms=denoms, extras=extras)
 
+    def _distill_batch(self, batch, ids) -> Optional[dict]:
+        """Ids and teacher log-probs of the packed rows of a micro-batch (top-K distillation as a loss term), padded to one width."""
+        if self.cfg.loss.opd_loss_coef == 0.0 or batch.get("opd_teacher_topk_log_probs") is None:
+            return None
+        dev, pad = self.device, torch.nn.functional.pad
+        rows = [torch.as_tensor(batch["opd_topk_token_ids"][i], dtype=torch.int64, device=dev) for i in ids]
+        lps = [torch.as_tensor(batch["opd_teacher_topk_log_probs"][i], dtype=torch.float32, device=dev) for i in ids]
+        k = max(t.shape[-1] for t in rows)
+        return {"ids": torch.cat([pad(t, (0, k - t.shape[-1]), value=-1) for t in rows]), "teacher": torch.cat([pad(t, (0, k - t.shape[-1])) for t in lps])}
+
     def _train_step(self, batch, idx):
         cfg, ps = self.cfg, self.ps
         opt = self.optimizer
@@ -928,8 +957,13 @@ class TrainActor:
                 lp, en = self._forward_logp(pb, cfg.compute_entropy)
                 loss, m = cfg.loss.custom_loss_function(lp, en, lb, cfg.loss)
             else:
-                lp, en = self._forward_logp(pb, cfg.compute_entropy)
+                distill = self._distill_batch(batch, ids)
+                lp, en = self._forward_logp(pb, cfg.compute_entropy, distill)
+                if distill is not None:
+                    lb.extras["opd_divergence"] = distill["divergence"]
                 loss, m = L.policy_loss(lp, en, lb, cfg.loss)
+                if distill is not None:
+                    lb.extras["opd_divergence"] = distill["divergence"].detach()
                 if self.replay.wants("loss", self._cur_rollout, self._cur_step) and ps.cp.size == 1:
                     # what the loss consumed and produced (post-forward statistics, no logits, no weights)
                     self.replay.capture("loss", self._cur_rollout, dict(log_probs=lp.detach(), entropy=en.detach(), batch=lb, cfg=cfg.loss),

@@ -90,13 +90,11 @@ def test_model_embedding_takes_the_configured_scale():
 
     from relax_b200.models.config import get_config
     from relax_b200.models.transformer import GPTModel
-    from relax_b200.rollout.weights import RolloutWeights
 
     cfg = dataclasses.replace(get_config("tiny"), embed_scale=3.0)
     m, plain = GPTModel(cfg, seed=1), GPTModel(get_config("tiny"), seed=1)
     tok = torch.tensor([1, 5, 1023])
     assert torch.equal(m.embedding.word_embeddings(tok, False), 3.0 * plain.embedding.word_embeddings(tok, False))
-    del RolloutWeights
 
 
 def _rows(R, V, K, seed, absent=True):
@@ -182,3 +180,43 @@ def test_fused_head_distill_chunks():
         assert torch.allclose(x, y, atol=1e-5, rtol=1e-5)
     assert torch.allclose(outs[0][0], ops.topk_distill(h @ wt.t(), ids, t, "jsd"), atol=1e-6)
     assert ops.fused_lm_head_topk_distill(h[:0], wt, ids[:0], t[:0]).shape == (0,)
+
+
+@pytest.mark.parametrize("selection", ["teacher_topk", "student_topk", "union"])
+def test_loss_mode_on_top_ids(tmp_path, selection):
+    """``--opd-loss-coef`` with a top-K selection: the step runs, the term is the only one that trains, and its gradient is that of the
+    divergence of the policy's own logits."""
+    from relax_b200.algo import opd
+    from relax_b200.checkpoint import hf as H
+    from relax_b200.config.arguments import parse_args
+    from relax_b200.models.config import get_config
+    from relax_b200.models.transformer import GPTModel
+    from relax_b200.orchestration.controller import Controller
+
+    cfg = get_config("tiny")
+    teacher = GPTModel(cfg, seed=77)
+    d = str(tmp_path / "teacher")
+    H.save_hf_checkpoint(d, cfg, H.convert_state_to_hf(cfg, {k: v.detach() for k, v in teacher.named_parameters()}))
+    a = parse_args(["--model-name", "tiny", "--colocate", "--rollout-batch-size", "2", "--n-samples-per-prompt", "2", "--global-batch-size", "4",
+                    "--num-rollout", "1", "--rollout-max-response-len", "6", "--use-opd", "--opd-teacher-load", d, "--lr", "1e-3", "--opd-loss-coef", "1.0",
+                    "--opd-only-reward", "--opd-token-selection", selection, "--opd-log-prob-top-k", "5", "--opd-kl-type", "jsd"])
+    assert a.opd_kl_coef == 0.0
+    c = Controller(a, device="cpu")
+    actor = c.runner.actor
+    seen = {}
+    plain = actor._distill_batch
+    actor._distill_batch = lambda batch, ids: seen.setdefault("made", plain(batch, ids))
+    hist = c.runner.step()
+    assert "opd_loss" in hist and math.isfinite(hist["grad_norm"]) and hist["grad_norm"] > 0
+    assert hist["pg_loss"] == 0.0 and hist["loss"] == pytest.approx(hist["opd_loss"], abs=1e-6)
+    made = seen["made"]
+    assert made["divergence"].requires_grad and (made["divergence"] >= -1e-6).all() and made["ids"].shape == made["teacher"].shape
+    assert selection == "union" or (made["ids"].shape[1] == 5 and (made["ids"] >= 0).all())
+    c.runner.close()
+    # the model's call against whole logits and the divergence on gathered log-probs
+    m = GPTModel(cfg, seed=5)
+    h = torch.randn(made["ids"].shape[0], cfg.hidden_size, generator=_gen(1))
+    got = m.topk_distill(h, made["ids"], made["teacher"], 0.8, kl_type="jsd", alpha=0.5, norm_mode="tail")
+    lp = torch.log_softmax(m.logits(h)[:, : cfg.vocab_size] / 0.8, -1).gather(1, made["ids"].clamp_min(0))
+    want = opd.token_kl(lp, made["teacher"].masked_fill(made["ids"] < 0, 0.0), "jsd", 0.5, "tail", mask=made["ids"] >= 0)
+    assert torch.allclose(got, want, atol=1e-5, rtol=1e-4)
