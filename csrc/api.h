@@ -227,8 +227,8 @@ int rb_expert_combine_bwd(const void* d_out, long long ld, const void* y, long l
 int rb_embedding(const void* ids, int wide, long long start, const void* table, long long ld, int rows, void* out, int n, int cols, float scale, int dtype,
                  cudaStream_t st);
 int rb_embedding_bwd_bins(int rows);
-int rb_embedding_bwd(const void* ids, int wide, long long start, const void* dy, long long ld, void* out, int add, int2* pairs, int* hist, float* part, int
-                     n, int rows, int cols, float scale, int dtype, cudaStream_t st);
+int rb_embedding_bwd(const void* ids, int wide, long long start, const void* dy, long long ld, void* out, int add, int2* pairs, int* hist, float* part,
+                     int* open, int n, int rows, int cols, float scale, int dtype, cudaStream_t st);
 int rb_topk_distill_parts(long long rows, int vocab);
 int rb_topk_distill(const void* z, long long ld, const long long* ids, const float* teacher, float* loss, float* coef, float* stats, float* log_probs,
                     float2* sums, long long rows, int vocab, int k, int kl, int norm, double alpha, double clamp, float inv_temp, int dtype, cudaStream_t

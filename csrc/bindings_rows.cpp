@@ -201,12 +201,13 @@ struct Embedding : Function<Embedding> {
     const auto dy = dense(g[0].reshape({ids.numel(), g[0].size(-1)}), "embedding");
     const int n = as_int(ids.numel(), "embedding: tokens"), V = as_int(rows, "embedding: table rows"), cols = as_int(dy.size(1), "embedding: columns");
     auto out = into.has_value() ? *into : at::empty({rows, cols}, dy.options());
-    // two buffers of (key, row), partial sums of runs (32-byte vectors), counters
-    const int64_t chunks = (n + 31) / 32, at_part = (4ll * n + 7) / 8 * 8, at_hist = at_part + (chunks > 1 ? chunks * 2 * cols : 0);
+    // two buffers of (key, row), partial sums of runs (32-byte vectors), the runs over several chunks, counters
+    const int64_t chunks = (n + 31) / 32, at_part = (4ll * n + 7) / 8 * 8, at_open = at_part + (chunks > 1 ? chunks * 2 * cols : 0);
+    const int64_t at_hist = at_open + 2 + chunks;
     const auto work = ints(at_hist + rb_sort_counters(n, rb_embedding_bwd_bins(V)), dy);
     int* p = work.data_ptr<int>();
     check(rb_embedding_bwd(ids.data_ptr(), ids.scalar_type() == at::kLong, ctx->saved_data["start"].toInt(), dy.data_ptr(), dy.stride(0), out.data_ptr(),
-                           into.has_value(), reinterpret_cast<int2*>(p), p + at_hist, reinterpret_cast<float*>(p + at_part), n, V, cols,
+                           into.has_value(), reinterpret_cast<int2*>(p), p + at_hist, reinterpret_cast<float*>(p + at_part), p + at_open, n, V, cols,
                            static_cast<float>(ctx->saved_data["scale"].toDouble()), code_of(dy, "embedding"), cur_stream()),
           "rb_embedding_bwd");
     return once({into.has_value() ? torch::Tensor() : out, torch::Tensor(), torch::Tensor(), torch::Tensor(), torch::Tensor()}, g);

@@ -82,8 +82,8 @@ __device__ __forceinline__ Pack<T, N> zeros() {
 
 // ----------------------------------------------------------------------------- stable counting sort
 // One pass puts rows in the order of a key with few values ("bins"), rows of a bin in their old order.  In place_kernel every warp of
-// a block has a run of rows and a counter per bin; 32 rows at a time find their equals with one match instruction, which gives
-// their rank in the warp and moves the counter.  Counters of warps in front, and of blocks in front (count_kernel's), are added then.
+// a block has a run of rows and a counter per bin; 32 rows at a time find their equals, which gives their rank in the warp and
+// moves the counter.  Counters of warps in front, and of blocks in front (count_kernel's), are added then.
 // Up to kOneBlock rows take place_kernel alone.
 
 struct ExpertKeys {      // expert ids; others than 0 .. bins - 1 live elsewhere and take no part
@@ -133,6 +133,7 @@ struct Fill {
   long long lo, hi;
   unsigned char* rest;      // the bytes behind the last whole vector
   int n_rest;
+  int* counter;             // two counters set to zero, for a kernel behind the sort
 };
 __device__ __forceinline__ void fill_near(const Fill& f, int blocks) {
   const long long t = blockIdx.x * static_cast<long long>(kThreads) + threadIdx.x, all = static_cast<long long>(blocks) * kThreads;
@@ -185,7 +186,8 @@ __device__ __forceinline__ int scan_block(int sum, int* part, int* all) {
   const int before = __shfl_sync(0xffffffffu, mine, (w + 31) & 31);
   return scan - sum + (w > 0 ? before : 0);
 }
-// the rank of this lane's digit among those of its warp so far; the warp's counters move on (digit -1: none)
+// The rank of this lane's digit among those of its warp so far; the warp's counters move on (digit -1: none).  (Equals found with a
+// ballot per bit instead: as fast for a text, slower where most digits are equal.)
 __device__ __forceinline__ int rank_in_warp(uint16_t* mine, int d) {
   const unsigned lane = threadIdx.x & 31, same = __match_any_sync(0xffffffffu, d);
   const int c = d >= 0 ? mine[d] : 0;
@@ -227,6 +229,7 @@ __global__ void __launch_bounds__(kThreads) place_kernel(Src src, Out out, int n
   int* first_row = total + bins;         // [bins] first output row of the bin
   uint16_t* cnt = reinterpret_cast<uint16_t*>(first_row + bins);      // [warps][bins]
   for (int i = t; i < warps * bins; i += kThreads) cnt[i] = 0;
+  if (blockIdx.x == 0 && t == 0 && fill.counter != nullptr) fill.counter[0] = fill.counter[1] = 0;
   int at[kSteps];      // digits, then digits and ranks
 #pragma unroll
   for (int s = 0; s < kSteps; ++s) {
@@ -309,6 +312,7 @@ __global__ void __launch_bounds__(kThreads) pack_sort_kernel(TokenKeys src, int2
   unsigned* a = reinterpret_cast<unsigned*>(sm);                       // [n] (between two barriers all of them are in registers)
   int* start = sm + n;                                                 // [bins]
   uint16_t* cnt = reinterpret_cast<uint16_t*>(start + bins);           // [warps][bins]
+  if (t == 0) fill.counter[0] = fill.counter[1] = 0;
   unsigned v[kSteps];
 #pragma unroll
   for (int s = 0; s < kSteps; ++s) {
@@ -427,6 +431,7 @@ int pack_sort_t(const TokenKeys& src, int2* pairs, int n, int pos_bits, int pass
 int pack_sort(const TokenKeys& src, int2* pairs, int n, int pos_bits, int passes, int each, const Fill& fill, cudaStream_t st) {
   if (n <= 1 * kThreads) return pack_sort_t<1>(src, pairs, n, pos_bits, passes, each, fill, st);
   if (n <= 4 * kThreads) return pack_sort_t<4>(src, pairs, n, pos_bits, passes, each, fill, st);
+  if (n <= 8 * kThreads) return pack_sort_t<8>(src, pairs, n, pos_bits, passes, each, fill, st);
   return pack_sort_t<16>(src, pairs, n, pos_bits, passes, each, fill, st);
 }
 
@@ -642,8 +647,8 @@ __global__ void __launch_bounds__(N == 1 ? kSingleThreads : 256) sum_bwd_kernel(
 // ----------------------------------------------------------------------------- gradient of a table by sorted rows
 // `pairs` holds (table row, input row) in order.  A warp walks 32 of them for 32 vectors of columns and keeps one running sum; a run
 // of equal keys that ends inside goes out at once, one that goes on in the next 32 (or came from those in front) leaves a partial
-// sum, and merge_kernel adds those of a run from left to right.  The longest run does not hold up one warp this way.
-constexpr int kRun = 32;
+// sum, and merge_kernel adds those of a run.
+constexpr int kRun = 32, kLongRun = 16;
 
 template <typename OutT, int N, bool kAdd>
 __device__ __forceinline__ void put_sum(OutT* out, long long row, int cols, int v, const float* acc, float scale) {
@@ -672,7 +677,7 @@ __device__ __forceinline__ void put_sum(OutT* out, long long row, int cols, int 
 
 template <typename T, int N, typename OutT, bool kAdd>
 __global__ void __launch_bounds__(256) run_kernel(const T* __restrict__ dy, long long ld, const int2* __restrict__ pairs, OutT* __restrict__ out,
-                                                  float* __restrict__ part, int n, int rows, int cols, int parts, float scale) {
+                                                  float* __restrict__ part, int* __restrict__ open, int n, int rows, int cols, int parts, float scale) {
   const long long unit = blockIdx.x * 8ll + (threadIdx.x >> 5);
   const int c = static_cast<int>(unit / parts);
   if (static_cast<long long>(c) * kRun >= n) return;
@@ -688,6 +693,12 @@ __global__ void __launch_bounds__(256) run_kernel(const T* __restrict__ dy, long
   const unsigned ends = __ballot_sync(0xffffffffu, pr.x != after) | 1u << 31;             // a run ends here, or at least its part in this chunk
   const bool from_front = __shfl_sync(0xffffffffu, pr.x, 0) == prev, goes_on = __shfl_sync(0xffffffffu, pr.x, 31) == next;
   const bool copies = std::is_same<T, OutT>::value && !kAdd && scale == 1.f;              // runs of one row go out as they are
+  if (lane == 0 && unit == static_cast<long long>(c) * parts && m == kRun && goes_on && !(from_front && ends == 1u << 31)) {
+    // a run that begins here goes on
+    const long long far = (static_cast<long long>(c) + kLongRun) * kRun, chunks = (static_cast<long long>(n) + kRun - 1) / kRun;
+    if (far < n && pairs[far].x == next) open[1 + chunks - atomicAdd(open + 1, 1)] = c;
+    else open[2 + atomicAdd(open, 1)] = c;
+  }
   float acc[N];
   bool fresh = true, head = true;      // nothing in `acc`; no run has ended in here yet
   constexpr int U = 8;
@@ -730,47 +741,77 @@ __global__ void __launch_bounds__(256) run_kernel(const T* __restrict__ dy, long
   }
 }
 
-template <int N, typename OutT, bool kAdd>
-__global__ void __launch_bounds__(256) merge_kernel(const int2* __restrict__ pairs, const float* __restrict__ part, OutT* __restrict__ out, int n, int rows,
-                                                    int cols, int parts, float scale) {
-  const long long unit = blockIdx.x * 8ll + (threadIdx.x >> 5);
-  const long long c = unit / parts;
-  if ((c + 1) * kRun >= n) return;      // nothing behind this chunk
-  const int key = pairs[c * kRun + kRun - 1].x;
-  if (key >= rows || pairs[(c + 1) * kRun].x != key) return;                         // no run goes on
-  if (c > 0 && pairs[c * kRun].x == key && pairs[c * kRun - 1].x == key) return;      // it came from in front: another warp's
-  const int lane = threadIdx.x & 31;
-  const int v = static_cast<int>(unit % parts) * 32 + lane;
-  const bool there = v < cols / N;
-  float acc[N];
+// acc += the partial sums d0 .. d1 - 1 of a run that begins in chunk c: the end of that chunk, the beginnings of the others
+template <int N>
+__device__ __forceinline__ void add_parts(const float* __restrict__ part, long long c, long long d0, long long d1, int cols, int v, float* acc) {
+  for (long long d = d0; d < d1; d += 8) {
+    Pack<float, N> p[8];
 #pragma unroll
-  for (int i = 0; i < N; ++i) acc[i] = 0.f;
-  const float* base = part + v * N;
-  if (there) {
+    for (int u = 0; u < 8; ++u)
+      if (d + u < d1) p[u] = *reinterpret_cast<const Pack<float, N>*>(part + ((d + u) * 2 + (d + u == c)) * cols + v * N);
 #pragma unroll
-    for (int i = 0; i < N; ++i) acc[i] = base[(c * 2 + 1) * cols + i];
-  }
-  for (long long d = c + 1;; d += 32) {      // 32 chunks at a time: how many of them begin with this key
-    const long long i = (d + lane) * kRun;
-    const unsigned in = __ballot_sync(0xffffffffu, i < n && pairs[i < n ? i : 0].x == key);
-    const int m = in == 0xffffffffu ? 32 : __ffs(~in) - 1;
-    if (there) {
-      for (int j = 0; j < m; j += 8) {
-        Pack<float, N> p[8];
+    for (int u = 0; u < 8; ++u)
+      if (d + u < d1) {
 #pragma unroll
-        for (int u = 0; u < 8; ++u)
-          if (j + u < m) p[u] = *reinterpret_cast<const Pack<float, N>*>(base + (d + j + u) * 2 * cols);
-#pragma unroll
-        for (int u = 0; u < 8; ++u)
-          if (j + u < m) {
-#pragma unroll
-            for (int i2 = 0; i2 < N; ++i2) acc[i2] += p[u].v[i2];
-          }
+        for (int i = 0; i < N; ++i) acc[i] += p[u].v[i];
       }
-    }
-    if (m < 32) break;
   }
-  if (there) put_sum<OutT, N, kAdd>(out, key, cols, v, acc, scale);
+}
+
+// the chunk behind the last of a run that begins in chunk c: 32 chunks side by side, then 32 at equal distances in what is left
+__device__ __forceinline__ long long run_end(const int2* __restrict__ pairs, int key, long long c, long long chunks) {
+  long long lo = c + 1, hi = chunks, step = 1;      // chunk lo begins with this key, chunk hi does not
+  for (;;) {
+    const long long x = lo + (threadIdx.x & 31) * step;
+    const int yes = __popc(__ballot_sync(0xffffffffu, x < hi && pairs[(x < hi ? x : lo) * kRun].x == key));
+    const long long next = lo + yes * step;
+    if (yes < 32 && next < hi) hi = next;
+    lo += (yes - 1) * step;
+    if (hi - lo <= 1) return hi;
+    step = (hi - lo + 31) / 32;
+  }
+}
+
+// Runs over several chunks; `open`: the number of those of up to kLongRun more chunks and of the others, then the chunks where they
+// begin, from the front and from the back, in no order.  A warp takes a part of the columns of a short run; of a long one a block
+// does, every warp a stretch, and the stretches are added from left to right.
+template <int N, typename OutT, bool kAdd>
+__global__ void __launch_bounds__(256) merge_kernel(const int2* __restrict__ pairs, const float* __restrict__ part, const int* __restrict__ open,
+                                                    OutT* __restrict__ out, int n, int cols, int parts, float scale) {
+  __shared__ Pack<float, N> sums[8][32];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const long long chunks = (static_cast<long long>(n) + kRun - 1) / kRun, items = static_cast<long long>(open[0]) * parts;
+  float acc[N];
+  for (long long item = blockIdx.x * 8ll + w; item < items; item += gridDim.x * 8ll) {
+    const long long c = open[2 + item / parts];
+    const int key = pairs[c * kRun + kRun - 1].x, v = static_cast<int>(item % parts) * 32 + lane;
+    const long long hi = run_end(pairs, key, c, chunks);
+    if (v >= cols / N) continue;
+#pragma unroll
+    for (int i = 0; i < N; ++i) acc[i] = 0.f;
+    add_parts<N>(part, c, c, hi, cols, v, acc);
+    put_sum<OutT, N, kAdd>(out, key, cols, v, acc, scale);
+  }
+  const long long longs = static_cast<long long>(open[1]) * parts;
+  for (long long item = gridDim.x - 1 - blockIdx.x; item < longs; item += gridDim.x) {      // (the last blocks have the fewest short ones)
+    const long long c = open[1 + chunks - item / parts];
+    const int key = pairs[c * kRun + kRun - 1].x, v = static_cast<int>(item % parts) * 32 + lane;
+    const bool there = v < cols / N;
+    const long long hi = run_end(pairs, key, c, chunks), each = (hi - c + 7) / 8, d0 = c + w * each, d1 = d0 + each < hi ? d0 + each : hi;
+#pragma unroll
+    for (int i = 0; i < N; ++i) acc[i] = 0.f;
+    if (there) add_parts<N>(part, c, d0, d1, cols, v, acc);
+    sums[w][lane].set(acc);
+    __syncthreads();
+    if (w == 0 && there) {
+#pragma unroll
+      for (int j = 1; j < 8; ++j)
+#pragma unroll
+        for (int i = 0; i < N; ++i) acc[i] += sums[j][lane].v[i];
+      put_sum<OutT, N, kAdd>(out, key, cols, v, acc, scale);
+    }
+    __syncthreads();
+  }
 }
 
 // ----------------------------------------------------------------------------- host
@@ -849,27 +890,28 @@ int sum_bwd_t(const void* d_out, long long ld, const void* y, long long ldy, con
 }
 
 template <typename T, int N, typename OutT, bool kAdd>
-int runs_t(const void* dy, long long ld, const int2* pairs, void* out, float* part, int n, int rows, int cols, float scale, cudaStream_t st) {
+int runs_t(const void* dy, long long ld, const int2* pairs, void* out, float* part, int* open, int n, int rows, int cols, float scale, cudaStream_t st) {
   const int per = 32 * N, parts = (cols + per - 1) / per;
   const long long chunks = (n + kRun - 1) / kRun, grid = grid_of(chunks * parts);
   if (grid > kMaxGrid) return -3;
-  run_kernel<T, N, OutT, kAdd><<<static_cast<int>(grid), 256, 0, st>>>(static_cast<const T*>(dy), ld, pairs, static_cast<OutT*>(out), part, n, rows, cols,
-                                                                       parts, scale);
+  run_kernel<T, N, OutT, kAdd><<<static_cast<int>(grid), 256, 0, st>>>(static_cast<const T*>(dy), ld, pairs, static_cast<OutT*>(out), part, open, n, rows,
+                                                                       cols, parts, scale);
   rb_note_launch(1);
   if (chunks > 1) {
-    merge_kernel<N, OutT, kAdd><<<static_cast<int>(grid), 256, 0, st>>>(pairs, part, static_cast<OutT*>(out), n, rows, cols, parts, scale);
+    const long long most = 8ll * num_sms(), blocks = (chunks / 2 + 1) * parts < most ? (chunks / 2 + 1) * parts : most;
+    merge_kernel<N, OutT, kAdd><<<static_cast<int>(blocks), 256, 0, st>>>(pairs, part, open, static_cast<OutT*>(out), n, cols, parts, scale);
     rb_note_launch(1);
   }
   return static_cast<int>(cudaGetLastError());
 }
 template <typename T>
-int runs_any(const void* dy, long long ld, const int2* pairs, void* out, float* part, int n, int rows, int cols, float scale, int add, cudaStream_t st) {
+int runs_any(const void* dy, long long ld, const int2* pairs, void* out, float* part, int* open, int n, int rows, int cols, float scale, int add, cudaStream_t st) {
   constexpr int NV = 16 / sizeof(T);
   const bool wide = wide_rows(dy, ld, cols, sizeof(T)) && wide_rows(out, cols, cols, add ? 4 : sizeof(T)) && wide_rows(part, cols, cols, 4);
-  if (add) return wide ? runs_t<T, NV, float, true>(dy, ld, pairs, out, part, n, rows, cols, scale, st)
-                       : runs_t<T, 1, float, true>(dy, ld, pairs, out, part, n, rows, cols, scale, st);
-  return wide ? runs_t<T, NV, T, false>(dy, ld, pairs, out, part, n, rows, cols, scale, st)
-              : runs_t<T, 1, T, false>(dy, ld, pairs, out, part, n, rows, cols, scale, st);
+  if (add) return wide ? runs_t<T, NV, float, true>(dy, ld, pairs, out, part, open, n, rows, cols, scale, st)
+                       : runs_t<T, 1, float, true>(dy, ld, pairs, out, part, open, n, rows, cols, scale, st);
+  return wide ? runs_t<T, NV, T, false>(dy, ld, pairs, out, part, open, n, rows, cols, scale, st)
+              : runs_t<T, 1, T, false>(dy, ld, pairs, out, part, open, n, rows, cols, scale, st);
 }
 
 inline int key_bits(int rows) {      // of the keys 0 .. rows
@@ -893,7 +935,7 @@ extern "C" int rb_expert_layout(const void* ids, int wide, int n, int experts, i
   const int tiles = align > 1 ? cap / align : 0;
   int at = 0;
   return sort_pass(ExpertKeys{ids, wide, experts}, ExpertOut{dest, source, align > 1 ? tile_expert : nullptr, bounds, cap, tiles}, n, experts, align, hist,
-                   Fill{source, cap, nullptr, 0, 0, nullptr, 0}, 1, &at, st);
+                   Fill{source, cap, nullptr, 0, 0, nullptr, 0, nullptr}, 1, &at, st);
 }
 
 extern "C" int rb_expert_dispatch(const void* x, long long ld, const int* source, void* out, int cap, int k, int cols, int dtype, cudaStream_t st) {
@@ -939,7 +981,7 @@ extern "C" int rb_embedding_bwd_bins(int rows) {      // counters of one block i
 }
 
 extern "C" int rb_embedding_bwd(const void* ids, int wide, long long start, const void* dy, long long ld, void* out, int add, int2* pairs, int* hist,
-                                float* part, int n, int rows, int cols, float scale, int dtype, cudaStream_t st) {
+                                float* part, int* open, int n, int rows, int cols, float scale, int dtype, cudaStream_t st) {
   if (n < 0 || n > kMaxSort || rows < 0 || rows > kMaxSort || cols < 0) return -1;
   if (rows == 0 || cols == 0) return 0;
   const size_t bytes = static_cast<size_t>(rows) * cols * (dtype == 2 ? 4 : 2);
@@ -947,6 +989,7 @@ extern "C" int rb_embedding_bwd(const void* ids, int wide, long long start, cons
   const int bits = key_bits(rows), passes = (bits + kPassBits - 1) / kPassBits, each = (bits + passes - 1) / passes;
   const int bins = 1 << each, mask = bins - 1;
   Fill fill{};
+  fill.counter = open;
   if (!add) {
     if (reinterpret_cast<uintptr_t>(out) % 16) return -4;
     fill.far = static_cast<uint4*>(out);
@@ -958,7 +1001,9 @@ extern "C" int rb_embedding_bwd(const void* ids, int wide, long long start, cons
   while (pos_bits < 31 && ((n - 1) >> pos_bits) != 0) ++pos_bits;
   int2* to = pairs;
   int2* from = pairs + n;
-  if (n <= kPackSort && pos_bits + bits <= 32) {
+  // one launch: few tokens, or a fill that takes longer than one block's sort (16384 tokens: 45 us, in four launches 18 us)
+  const bool one = n <= kOneBlock || (n <= kPackSort && !add && bytes >= static_cast<size_t>(n) * 20000);
+  if (one && pos_bits + bits <= 32) {
     const int rc = pack_sort(TokenKeys{ids, wide, rows, 0, mask, start}, from, n, pos_bits, passes, each, fill, st);
     if (rc) return rc;
   } else {
@@ -975,9 +1020,9 @@ extern "C" int rb_embedding_bwd(const void* ids, int wide, long long start, cons
     }
   }
   switch (dtype) {
-    case 0: return runs_any<__nv_bfloat16>(dy, ld, from, out, part, n, rows, cols, scale, add, st);
-    case 1: return runs_any<__half>(dy, ld, from, out, part, n, rows, cols, scale, add, st);
-    case 2: return runs_any<float>(dy, ld, from, out, part, n, rows, cols, scale, add, st);
+    case 0: return runs_any<__nv_bfloat16>(dy, ld, from, out, part, open, n, rows, cols, scale, add, st);
+    case 1: return runs_any<__half>(dy, ld, from, out, part, open, n, rows, cols, scale, add, st);
+    case 2: return runs_any<float>(dy, ld, from, out, part, open, n, rows, cols, scale, add, st);
   }
   return -1;
 }
