@@ -231,10 +231,10 @@ int rb_embedding_bwd(const void* ids, int wide, long long start, const void* dy,
                      int* open, int n, int rows, int cols, float scale, int dtype, cudaStream_t st);
 int rb_topk_distill_parts(long long rows, int vocab);
 int rb_topk_distill(const void* z, long long ld, const long long* ids, const float* teacher, float* loss, float* coef, float* stats, float* log_probs,
-                    float2* sums, long long rows, int vocab, int k, int kl, int norm, double alpha, double clamp, float inv_temp, int dtype, cudaStream_t
+                    double2* sums, long long rows, int vocab, int k, int kl, int norm, double alpha, double clamp, double inv_temp, int dtype, cudaStream_t
                     st);
 int rb_topk_distill_bwd(const void* z, long long ld, const long long* ids, const float* coef, const float* stats, const float* g, void* dz, long long rows,
-                        int vocab, int k, float inv_temp, int dtype, int out_dtype, cudaStream_t st);
+                        int vocab, int k, double inv_temp, int dtype, int out_dtype, cudaStream_t st);
 #ifdef __cplusplus
 }
 #endif

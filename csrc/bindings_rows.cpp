@@ -226,9 +226,9 @@ torch::Tensor embedding(const torch::Tensor& weight, const torch::Tensor& tokens
 // ----------------------------------------------------------------------------- distillation from top ids
 
 struct Distilled {
-  torch::Tensor loss, kept, log_probs;      // kept: statistics [R, 4], sums of parts (a workspace), slopes [R, K]
+  torch::Tensor loss, kept, log_probs;      // kept: statistics [R, 4], sums of parts (a workspace), slopes of the ids [R, K]
 };
-inline int64_t slopes_at(const torch::Tensor& z) { return z.size(0) * (4 + 2 * rb_topk_distill_parts(z.size(0), static_cast<int>(z.size(1)))); }
+inline int64_t slopes_at(const torch::Tensor& z) { return z.size(0) * (4 + 4 * rb_topk_distill_parts(z.size(0), static_cast<int>(z.size(1)))); }
 
 Distilled distill_rows(const torch::Tensor& z, const torch::Tensor& ids, const torch::Tensor& teacher, int64_t kl, int64_t norm, double alpha, double clamp,
                        double inv_temp, bool log_probs) {
@@ -248,8 +248,8 @@ Distilled distill_rows(const torch::Tensor& z, const torch::Tensor& ids, const t
   if (log_probs) d.log_probs = at::empty({R, K}, f32);
   check(rb_topk_distill(z.data_ptr(), z.stride(0), reinterpret_cast<const long long*>(ids.data_ptr<int64_t>()), teacher.data_ptr<float>(),
                         d.loss.data_ptr<float>(), kept + slopes, kept, log_probs ? d.log_probs.data_ptr<float>() : nullptr,
-                        reinterpret_cast<float2*>(kept + 4 * R), R, static_cast<int>(z.size(1)), static_cast<int>(K), static_cast<int>(kl),
-                        static_cast<int>(norm), alpha, clamp, static_cast<float>(inv_temp), code, cur_stream()),
+                        reinterpret_cast<double2*>(kept + 4 * R), R, static_cast<int>(z.size(1)), static_cast<int>(K), static_cast<int>(kl),
+                        static_cast<int>(norm), alpha, clamp, inv_temp, code, cur_stream()),
         "rb_topk_distill");
   return d;
 }
@@ -265,7 +265,7 @@ void distill_rows_bwd(const torch::Tensor& z, const torch::Tensor& ids, const to
                     "topk_distill: gradient or kept values of another shape");
   check(rb_topk_distill_bwd(z.data_ptr(), z.stride(0), reinterpret_cast<const long long*>(ids.data_ptr<int64_t>()), kept.data_ptr<float>() + slopes,
                             kept.data_ptr<float>(), g.data_ptr<float>(), out.data_ptr(), z.size(0), as_int(z.size(1), "topk_distill: vocabulary"),
-                            static_cast<int>(ids.size(1)), static_cast<float>(inv_temp), code_of(z, "topk_distill"), code_of(out, "topk_distill"),
+                            static_cast<int>(ids.size(1)), inv_temp, code_of(z, "topk_distill"), code_of(out, "topk_distill"),
                             cur_stream()),
         "rb_topk_distill_bwd");
 }

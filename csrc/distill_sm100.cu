@@ -30,7 +30,7 @@ constexpr int kMaxIds = 1024;      // eight per thread of id_kernel
 constexpr int kMaxVocab = 1 << 24;
 constexpr int kMaxParts = 32;      // blocks of a row
 constexpr int kStats = 4;      // per row: log2 reference, 1 / sum, sum of the slopes, (unused)
-constexpr double kLn2 = 0.6931471805599453;
+constexpr double kLn2 = 0.6931471805599453, kLog2e = 1.4426950408889634;
 constexpr double kLeastRest = 9.9999995e-08;      // 1 - exp(-1e-7)
 
 enum Kl { kReverse = 0, kForward = 1, kMixed = 2, kLowVar = 3 };
@@ -41,6 +41,14 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+
+// Logits in units of log2, z log2(e) / T, end at kLow: masks of a type's lowest value would pass it, and a row of nothing else is uniform.
+// Only rows whose largest logit is far down there look at it (`low` rows); elsewhere such logits have no mass either way.
+constexpr float kLow = -3.4e38f, kLowRows = -1e38f;
+__device__ __forceinline__ float low_mass(float z, float c2, float ref) { return z == -INFINITY ? 0.f : ex2(fmaxf(z * c2, kLow) - ref); }
+
+// the whole number at or above z log2(e) / T
+__device__ __forceinline__ float whole_ref(float z, float c2) { return z == -INFINITY ? z : ceilf(fmaxf(z * c2, kLow)); }
 
 // two 32-bit operations at a time
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
@@ -130,21 +138,24 @@ struct Params {
   const long long* ids;        // [rows, k]; outside 0 .. vocab - 1: no id
   const float* teacher;        // [rows, k] log-probs
   float* loss;                 // [rows]
-  float* coef;                 // [rows, k] dD / ds, added up over equal ids
+  float* coef;                 // [rows, k] logits of the ids (from one kernel to the other), then d D / d z of the ids, times T
   float* stats;                // [rows, kStats]
   float* log_probs;            // [rows, k] or null
-  float2* sums;                // [rows, parts] (reference, sum) of the parts of a row
+  double2* sums;               // [rows, parts] (reference, sum) of the parts of a row
   int vocab, k, kl, norm, parts;
-  float c2;                    // log2(e) / T
+  float c2, c2_low;            // log2(e) / T and what 32 bits leave of it
+  double scale;                // log2(e) / T
   double alpha, clamp;         // weight of the teacher; least log-prob
 };
 
-// (reference, sum): the sum of 2^(z c2) is sum 2^reference
+// (reference, sum): the sum of 2^(z c2) is sum 2^reference.  References are whole numbers, so that moving a sum to another one is exact
+// (each move by an approximate power took 5e-8 off the sum, 2.5e-7 in all).
 struct Sum {
-  float ref, sum;
-  __device__ __forceinline__ void add(float r, float s) {      // nothing yet: ref -inf, sum 0
+  float ref;
+  double sum;
+  __device__ __forceinline__ void add(float r, double s) {      // nothing yet: ref -inf, sum 0
     const float m = fmaxf(ref, r), at = m == -INFINITY ? 0.f : m;
-    sum = sum * ex2(ref - at) + s * ex2(r - at);
+    sum = sum * static_cast<double>(ex2(ref - at)) + s * static_cast<double>(ex2(r - at));
     ref = m;
   }
 };
@@ -174,9 +185,6 @@ __device__ __forceinline__ void block_sums(double (&v)[N], double (*sm)[kIdWarps
 __device__ __forceinline__ double least(double x, double c) { return x < c ? c : x; }      // (NaN stays)
 // 0 log 0 = 0: a term whose weight is nothing counts nothing
 __device__ __forceinline__ double weighted(double w, double x) { return w == 0.0 ? 0.0 : w * x; }
-// masses in 32 bits: off by 2^-22 like the exponentials of the sum, against which they are weighed
-__device__ __forceinline__ double mass_of(double log_prob) { return static_cast<double>(ex2(static_cast<float>(log_prob * 1.4426950408889634))); }
-
 struct Term {
   double d, slope;      // D's term and its derivative by P
 };
@@ -193,10 +201,10 @@ __device__ __forceinline__ Term term_of(int kl, double a, double p, double q, do
   } else {
     double pm, qm;      // log(p / m), log(q / m)
     if (l >= 0.0) {
-      pm = -static_cast<double>(log1pf(static_cast<float>(a) * expm1f(static_cast<float>(-l))));
+      pm = -log1p(a * expm1(-l));
       qm = pm - l;
     } else {
-      qm = -static_cast<double>(log1pf(static_cast<float>(1.0 - a) * expm1f(static_cast<float>(l))));
+      qm = -log1p((1.0 - a) * expm1(l));
       pm = l + qm;
     }
     r.d = (1.0 - a) * weighted(p, pm) + a * weighted(q, qm);
@@ -207,7 +215,7 @@ __device__ __forceinline__ Term term_of(int kl, double a, double p, double q, do
 
 // Sums over the vocabulary, `parts` blocks per row.  The row counts from the last address in front of it that is a multiple of eight
 // elements, so that all but its first and last group of eight are whole; groups are shared out to the blocks in runs.
-template <typename T, bool kMarks>
+template <typename T>
 __global__ void __launch_bounds__(kThreads, 4) sum_kernel(Params p) {
   const long long row = blockIdx.x / p.parts;
   const int part = static_cast<int>(blockIdx.x - row * p.parts), t = threadIdx.x;
@@ -220,10 +228,8 @@ __global__ void __launch_bounds__(kThreads, 4) sum_kernel(Params p) {
   const int g0 = min(groups, part * each), g1 = min(groups, g0 + each);
   const int w0 = g0 == 0 && skip ? 1 : g0, w1 = (g1 == groups && ((skip + p.vocab) & 7)) ? g1 - 1 : g1;      // whole groups
 
-  if constexpr (kMarks) {
-    for (int i = t; i < (each + 3) / 4; i += kThreads) marks[i] = 0;
-    __syncthreads();
-  }
+  for (int i = t; i < (each + 3) / 4; i += kThreads) marks[i] = 0;
+  __syncthreads();
   // logits of this part's ids, for the kernel behind this one: fetched here, where other blocks keep the memory busy meanwhile (K
   // scattered reads per row by themselves took 116 us for 4096 rows of 128), and put down at the end
   constexpr int kMine = kMaxIds / kThreads;
@@ -237,13 +243,13 @@ __global__ void __launch_bounds__(kThreads, 4) sum_kernel(Params p) {
     if (v >= 0 && v < p.vocab && b >= 0 && b < 8ll * (g1 - g0)) {
       here |= 1u << j;
       at_id[j] = up(z[v]);
-      if constexpr (kMarks) atomicOr(&marks[b >> 5], 1u << (b & 31));
+      atomicOr(&marks[b >> 5], 1u << (b & 31));
     }
   }
-  if constexpr (kMarks) __syncthreads();
+  __syncthreads();
   const unsigned char* mark = reinterpret_cast<const unsigned char*>(marks);
 
-  Sum s{-INFINITY, 0.f};
+  Sum s{-INFINITY, 0.0};
   constexpr int U = sizeof(T) == 4 ? 4 : 8;      // groups of a thread in one step: 128 bytes of it under way
   // U groups from g on, in strides of the block; the last step (kAll false) holds what is left
   auto step = [&](int g, auto all) {
@@ -254,20 +260,28 @@ __global__ void __launch_bounds__(kThreads, 4) sum_kernel(Params p) {
 #pragma unroll
     for (int u = 0; u < U; ++u)
       if (kAll || g + u * kThreads < w1) e[u].load(origin + 8ll * (g + u * kThreads));
-    if constexpr (kMarks) {
 #pragma unroll
-      for (int u = 0; u < U; ++u) m[u] = kAll || g + u * kThreads < w1 ? mark[g + u * kThreads - g0] : 0;
-    }
+    for (int u = 0; u < U; ++u) m[u] = kAll || g + u * kThreads < w1 ? mark[g + u * kThreads - g0] : 0;
 #pragma unroll
     for (int u = 0; u < U; ++u)
       if (kAll || g + u * kThreads < w1) big = fmaxf(big, e[u].max());
-    big *= p.c2;
+    big = whole_ref(big, p.c2);
     if (big > s.ref) {
-      s.sum *= ex2(s.ref - big);
+      s.sum *= static_cast<double>(ex2(s.ref - big));
       s.ref = big;
     }
     const float at = s.ref == -INFINITY ? 0.f : s.ref;
-    const float2 c = make_float2(p.c2, p.c2), o = make_float2(-at, -at);
+    if (at <= kLowRows) {
+#pragma unroll 1
+      for (int u = 0; u < U; ++u) {
+        const int q = g + u * kThreads;
+        if (q >= w1) break;
+        for (int i = 0; i < 8; ++i)
+          if (!((mark[q - g0] >> i) & 1)) s.sum += low_mass(up(origin[8ll * q + i]), p.c2, at);
+      }
+      return;
+    }
+    const float2 c = make_float2(p.c2, p.c2), l = make_float2(p.c2_low, p.c2_low), o = make_float2(-at, -at);
     float2 add = make_float2(0.f, 0.f);
 #pragma unroll
     for (int u = 0; u < U; ++u)
@@ -276,18 +290,16 @@ __global__ void __launch_bounds__(kThreads, 4) sum_kernel(Params p) {
         e[u].get(f);
 #pragma unroll
         for (int i = 0; i < 8; i += 2) {
-          const float2 x = fma2(make_float2(f[i], f[i + 1]), c, o);
+          const float2 y = make_float2(f[i], f[i + 1]), x = fma2(y, l, fma2(y, c, o));
           f[i] = ex2(x.x), f[i + 1] = ex2(x.y);
         }
-        if constexpr (kMarks) {
-          if (m[u]) {
+        if (m[u]) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) f[i] = (m[u] >> i) & 1 ? 0.f : f[i];
-          }
+          for (int i = 0; i < 8; ++i) f[i] = (m[u] >> i) & 1 ? 0.f : f[i];
         }
         add = add2(add, add2(add2(make_float2(f[0], f[1]), make_float2(f[2], f[3])), add2(make_float2(f[4], f[5]), make_float2(f[6], f[7]))));
       }
-    s.sum += add.x + add.y;
+    s.sum += static_cast<double>(add.x + add.y);
   };
   int g = w0 + t;
   for (; g + (U - 1) * kThreads < w1; g += U * kThreads) step(g, std::true_type{});
@@ -298,10 +310,10 @@ __global__ void __launch_bounds__(kThreads, 4) sum_kernel(Params p) {
     const long long v = 8ll * g + i - skip;
     const bool mine = t < 8 ? (g0 == 0 && skip) : (g1 == groups && ((skip + p.vocab) & 7) && !(groups == 1 && skip));
     if (mine && g0 < g1 && v >= 0 && v < p.vocab) {
-      bool counts = true;
-      if constexpr (kMarks) counts = !((mark[g - g0] >> i) & 1);
-      const float x = up(z[v]) * p.c2;
-      s.add(x, counts ? (x == -INFINITY ? 0.f : (x == x ? 1.f : x)) : 0.f);
+      const bool counts = !((mark[g - g0] >> i) & 1);
+      const float y = up(z[v]), x = y == y ? whole_ref(y, p.c2) : y;      // (NaN stays)
+      const double own = x == -INFINITY ? 0.0 : x == kLow ? 1.0 : static_cast<double>(ex2(fmaf(y, p.c2_low, fmaf(y, p.c2, -x))));
+      s.add(x, counts ? own : 0.0);
     }
   }
 #pragma unroll
@@ -312,7 +324,7 @@ __global__ void __launch_bounds__(kThreads, 4) sum_kernel(Params p) {
     Sum b = warp_sum[0];
 #pragma unroll
     for (int w = 1; w < kWarps; ++w) b.add(warp_sum[w].ref, warp_sum[w].sum);
-    p.sums[blockIdx.x] = make_float2(b.ref, b.sum);
+    p.sums[blockIdx.x] = make_double2(b.ref, b.sum);
   }
 #pragma unroll
   for (int j = 0; j < kMine; ++j)
@@ -326,27 +338,27 @@ __device__ __forceinline__ unsigned mixed(unsigned x) {
   return x ^ (x >> 16);
 }
 
-// The K ids of a row: the divergence, its slopes, the row's statistics.  Log-probs, their differences and the sums over the ids are in
-// 64 bits, exponentials in 32.  Equal ids are found with a hash table that keeps the first place of every id.
+// The K ids of a row: the divergence, its slopes, the row's statistics, in 64 bits: where student and teacher are near each other the
+// divergence is a small difference of its terms (32-bit masses left it 2e-5 off).  Equal ids are found with a hash table that keeps the first place of every id.
 __global__ void __launch_bounds__(kIdThreads) id_kernel(Params p, int slots) {
   const long long row = blockIdx.x;
   const int t = threadIdx.x, threads = blockDim.x;
   extern __shared__ __align__(16) unsigned char dyn[];
   double* lp = reinterpret_cast<double*>(dyn);                // [k] log-probs of the student, then slopes
-  int* id = reinterpret_cast<int*>(lp + p.k);                 // [k] the row's ids, -1: none
-  float* pm = reinterpret_cast<float*>(id + p.k);             // [k] masses of the student (before clamping)
-  float* tl = pm + p.k;                                       // [k] log-probs of the teacher
+  double* pm = lp + p.k;                                      // [k] places in the table, then probabilities of the student
+  int* id = reinterpret_cast<int*>(pm + p.k);                 // [k] the row's ids, -1: none
+  float* tl = reinterpret_cast<float*>(id + p.k);             // [k] log-probs of the teacher
   int* key = reinterpret_cast<int*>(tl + p.k);                // [slots] ids (a power of two, at least 2 k)
   int* place = key + slots;                                   // [slots] where they stand first
   __shared__ double red[4][kIdWarps];
   const bool tail = p.norm == kTail && p.kl != kLowVar, renorm = p.norm == kNorm && p.kl != kLowVar;
   for (int i = t; i < slots; i += threads) key[i] = -1, place[i] = p.k;
-  Sum all{-INFINITY, 0.f};
+  Sum all{-INFINITY, 0.0};
   for (int r = 0; r < p.parts; ++r) {
-    const float2 s = p.sums[row * p.parts + r];
-    all.add(s.x, s.y);
+    const double2 s = p.sums[row * p.parts + r];
+    all.add(static_cast<float>(s.x), s.y);
   }
-  const double ref = all.ref == -INFINITY ? 0.0 : static_cast<double>(all.ref), c2 = p.c2, counted = all.sum;
+  const double ref = all.ref == -INFINITY ? 0.0 : static_cast<double>(all.ref), rest_sum = all.sum;
   __syncthreads();
   for (int i0 = t; i0 < p.k; i0 += 4 * threads) {      // four ids at a time: they wait for memory
     int v[4];
@@ -369,57 +381,60 @@ __global__ void __launch_bounds__(kIdThreads) id_kernel(Params p, int slots) {
       if (i >= p.k) break;
       id[i] = v[u];
       if (v[u] < 0) continue;
-      lp[i] = (static_cast<double>(z[u]) * c2 - ref) * kLn2;      // z - reference in units of ln
+      const double y = static_cast<double>(z[u]) * p.scale, low = kLow;
+      lp[i] = ((y < low && z[u] != -INFINITY ? low : y) - ref) * kLn2;      // z - reference in units of ln
       unsigned h = mixed(v[u]);
       for (;; ++h) {      // (ends: no more than half the slots are taken)
         const int was = atomicCAS(&key[h & (slots - 1)], -1, v[u]);
         if (was == -1 || was == v[u]) break;
       }
       atomicMin(&place[h & (slots - 1)], i);
-      pm[i] = __int_as_float(static_cast<int>(h & (slots - 1)));
+      pm[i] = static_cast<double>(h & (slots - 1));
     }
   }
   __syncthreads();
   double one[1] = {0.0};
-  unsigned firsts = 0;      // a bit for each of this thread's ids
+  unsigned firsts = 0, moving = 0;      // a bit for each of this thread's ids
   for (int i = t, n = 0; i < p.k; i += threads, ++n) {
     if (id[i] < 0) continue;
-    const bool first = place[__float_as_int(pm[i])] == i;
+    const bool first = place[static_cast<int>(pm[i])] == i;
     firsts |= static_cast<unsigned>(first) << n;
-    const double e = mass_of(lp[i]);
-    pm[i] = static_cast<float>(e);
-    if (first && tail) one[0] += e;
+    pm[i] = exp(lp[i]);
+    if (first) one[0] += pm[i];
   }
-  if (tail) block_sums(one, red);      // the sum over the vocabulary left the ids out
-  const double total = counted + one[0], log_total = log(total), inv_total = 1.0 / total;
+  block_sums(one, red);      // the sum over the vocabulary left the ids out
+  const double total = rest_sum + one[0], log_total = log(total), inv_total = 1.0 / total;
 
-  // masses of the ids (renormalised: of all of them), and what the rest lacks: equal ids and clamped ones count as written
-  double mass[3] = {0.0, 0.0, 0.0};
+  // masses of the ids (renormalised: of all of them), what the rest lacks (equal ids and clamped ones count as written), ids in all
+  double mass[4] = {0.0, 0.0, 0.0, 0.0};
   bool twice = false;
   for (int i = t, n = 0; i < p.k; i += threads, ++n) {
     if (id[i] < 0) continue;
     const bool first = (firsts >> n) & 1;
     twice |= !first;
     lp[i] -= log_total;
+    pm[i] *= inv_total;
     if (p.log_probs) p.log_probs[row * p.k + i] = static_cast<float>(lp[i]);
     if (!tail && !renorm) continue;
-    const double used = least(lp[i], p.clamp), pi = pm[i] * inv_total, pu = used == lp[i] ? pi : used == used ? exp(used) : used;
+    const double used = least(lp[i], p.clamp), pu = used == lp[i] ? pm[i] : exp(used);
     mass[0] += pu;
-    mass[1] += exp(least(static_cast<double>(tl[i]), p.clamp));      // (64 bits: the rest is one minus their sum)
-    mass[2] += pu - (first ? pi : 0.0);
+    mass[1] += exp(least(static_cast<double>(tl[i]), p.clamp));
+    mass[2] += pu - (first ? pm[i] : 0.0);
+    mass[3] += 1.0;
   }
   if (tail || renorm) block_sums(mass, red);
   double rest_slope = 0.0, rest = 0.0;
   if (tail) {
-    const double free = counted / total - mass[2];      // (exactly one where there are no ids)
+    const double free = rest_sum / total - mass[2];      // (exactly one where there are no ids)
     const double pr = least(free, kLeastRest), qr = least(1.0 - mass[1], kLeastRest);
     const Term r = term_of(p.kl, p.alpha, pr, qr, log(pr / qr));
     rest = r.d;
     rest_slope = free >= kLeastRest ? r.slope : 0.0;
   }
+  const bool alone = renorm && mass[3] == 1.0;      // all mass is this id's, on both sides
   const double ls = renorm ? log(mass[0] / mass[1]) : 0.0, np = renorm ? 1.0 / mass[0] : 1.0, nq = renorm ? 1.0 / mass[1] : 1.0;
   double sums[4] = {0.0, 0.0, 0.0, 0.0};      // the divergence; slopes of all ids; slopes and masses of those that move
-  for (int i = t; i < p.k; i += threads) {
+  for (int i = t, n = 0; i < p.k; i += threads, ++n) {
     if (id[i] < 0) {
       if (p.log_probs) p.log_probs[row * p.k + i] = -INFINITY;
       continue;
@@ -432,9 +447,9 @@ __global__ void __launch_bounds__(kIdThreads) id_kernel(Params p, int slots) {
       sums[0] += x - 1.0 + r;
       c = 1.0 - x;
     } else {
-      const double qq = mass_of(t_i) * nq;
-      pp = (moves ? pm[i] * inv_total : exp(used)) * np;
-      const Term r = term_of(p.kl, p.alpha, pp, qq, used - t_i - ls);
+      const double qq = alone ? 1.0 : exp(t_i) * nq;
+      pp = alone ? 1.0 : (moves ? pm[i] : exp(used)) * np;
+      const Term r = term_of(p.kl, p.alpha, pp, qq, alone ? 0.0 : used - t_i - ls);
       sums[0] += r.d;
       c = (p.kl == kForward ? -qq : weighted(pp, r.slope)) - weighted(pp, rest_slope);
     }
@@ -442,30 +457,38 @@ __global__ void __launch_bounds__(kIdThreads) id_kernel(Params p, int slots) {
     if (moves) {
       sums[2] += c;
       sums[3] += pp;
+      moving |= 1u << n;
     }
     lp[i] = moves ? c : 0.0;
-    pm[i] = moves ? static_cast<float>(pp) : 0.f;
   }
   block_sums(sums, red);
   double move = sums[2];
   if (renorm) {      // c_i - P_i sum c
     move -= sums[1] * sums[3];
-    for (int i = t; i < p.k; i += threads)
-      if (id[i] >= 0) lp[i] -= pm[i] * sums[1];
+    for (int i = t, n = 0; i < p.k; i += threads, ++n)
+      if ((moving >> n) & 1) lp[i] -= (alone ? 1.0 : pm[i] * np) * sums[1];
   }
-  const bool sum_equals = __syncthreads_or(twice);      // equal ids move together
+  // what the logit of an id gets, its share of the sum of the slopes with it; equal ids move together
+  const bool sum_equals = __syncthreads_or(twice);
   for (int i = t; i < p.k; i += threads) {
-    double c = id[i] < 0 ? 0.0 : lp[i];
-    if (sum_equals && id[i] >= 0) {
-      c = 0.0;
-      for (int j = 0; j < p.k; ++j) c += id[j] == id[i] ? lp[j] : 0.0;
+    double c = 0.0;
+    if (id[i] >= 0) {
+      c = lp[i];
+      if (sum_equals) {
+        c = 0.0;
+        for (int j = 0; j < p.k; ++j) c += id[j] == id[i] ? lp[j] : 0.0;
+      }
+      c -= move * pm[i];
     }
     p.coef[row * p.k + i] = static_cast<float>(c);
   }
   if (t == 0) {
     p.loss[row] = static_cast<float>(sums[0] + rest);
+    // (the sum's power of two goes to the reference: 1 / sum is no less than a half, whatever the reference was)
+    int e = total > 0.0 && total < INFINITY ? ilogb(total) : 0;
+    if (static_cast<double>(static_cast<float>(ref + e)) - ref != e) e = 0;      // (a reference so large that it has no place for it)
     *reinterpret_cast<float4*>(p.stats + row * kStats) =
-        make_float4(static_cast<float>(ref), static_cast<float>(inv_total), static_cast<float>(move), 0.f);
+        make_float4(static_cast<float>(ref + e), static_cast<float>(ldexp(inv_total, e)), static_cast<float>(move), 0.f);
   }
 }
 
@@ -478,7 +501,7 @@ struct BwdParams {
   const float* g;          // [rows] gradient of the divergence
   void* dz;                // [rows, vocab] dense (may be z itself where types agree)
   int vocab, k, parts;
-  float c2, inv_t;
+  float c2, c2_low, inv_t;
 };
 
 // A block per part of a row: -g / T (sum c) P over its elements, then the K ids of that part in place of what stands there.
@@ -496,17 +519,10 @@ __global__ void __launch_bounds__(kThreads) bwd_kernel(BwdParams p) {
   const int g0 = min(groups, part * each), g1 = min(groups, g0 + each);
   const long long lo = max(0ll, 8ll * g0 - skip), hi = min(static_cast<long long>(p.vocab), 8ll * g1 - skip);
   if (lo >= hi) return;
-  // probabilities of this part's ids are read before they are overwritten (dz may be z)
-  extern __shared__ float at_id[];
-  if (g != 0.f) {
-    for (int i = t; i < p.k; i += kThreads) {
-      const long long v = p.ids[row * p.k + i];
-      if (v >= lo && v < hi) at_id[i] = g * p.coef[row * p.k + i] + f * ex2(fmaf(up(z[v]), p.c2, -ref));
-    }
-    __syncthreads();
-  }
-  auto one = [&](long long v) { put(d + v, g == 0.f ? 0.f : f * ex2(fmaf(up(z[v]), p.c2, -ref))); };
-  if constexpr (!kWhole) {
+  const bool low = ref <= kLowRows;
+  auto mass = [&](float x) { return ex2(fmaf(x, p.c2_low, fmaf(x, p.c2, -ref))); };
+  auto one = [&](long long v) { put(d + v, g == 0.f ? 0.f : f * (low ? low_mass(up(z[v]), p.c2, ref) : mass(up(z[v])))); };
+  if (!kWhole || (low && g != 0.f)) {
     for (long long v = lo + t; v < hi; v += kThreads) one(v);
   } else {
     const int w0 = g0 == 0 && skip ? 1 : g0, w1 = (g1 == groups && ((skip + p.vocab) & 7)) ? g1 - 1 : g1;
@@ -525,7 +541,7 @@ __global__ void __launch_bounds__(kThreads) bwd_kernel(BwdParams p) {
           if (g != 0.f) {
             e[u].get(x);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = f * ex2(fmaf(x[i], p.c2, -ref));
+            for (int i = 0; i < 8; ++i) x[i] = f * mass(x[i]);
           }
           Eight<O>::store(d + (8ll * (q + u * kThreads) - skip), x);
         }
@@ -541,7 +557,7 @@ __global__ void __launch_bounds__(kThreads) bwd_kernel(BwdParams p) {
   __syncthreads();
   for (int i = t; i < p.k; i += kThreads) {
     const long long v = p.ids[row * p.k + i];
-    if (v >= lo && v < hi) put(d + v, at_id[i]);
+    if (v >= lo && v < hi) put(d + v, g * p.coef[row * p.k + i]);
   }
 }
 
@@ -558,36 +574,34 @@ inline int parts_of(long long rows, int vocab, long long slots, int fixed) {
   }
   return best;
 }
-template <typename T, bool kMarks>
+template <typename T>
 int sums_t(const Params& p, long long rows, cudaStream_t st) {
   const int each = ((p.vocab + 14) / 8 + p.parts - 1) / p.parts + 1;
-  const size_t smem = kMarks ? (each + 3) / 4 * 4 + 16 : 0;
-  if (smem > 200 * 1024) return -4;      // (a vocabulary of more than a million ids, in one part)
-  auto kernel = sum_kernel<T, kMarks>;
+  const size_t smem = (each + 3) / 4 * 4 + 16;
+  constexpr size_t kMostSmem = 200 * 1024;      // (always the same limit: calls of several threads would lower one another's)
+  if (smem > kMostSmem) return -4;
   if (smem > 40 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    const cudaError_t e = cudaFuncSetAttribute(sum_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kMostSmem));
     if (e != cudaSuccess) return static_cast<int>(e);
   }
-  kernel<<<static_cast<unsigned>(rows * p.parts), kThreads, smem, st>>>(p);
+  sum_kernel<T><<<static_cast<unsigned>(rows * p.parts), kThreads, smem, st>>>(p);
   rb_note_launch(1);
   return static_cast<int>(cudaGetLastError());
-}
-template <typename T>
-int sums_any(const Params& p, long long rows, cudaStream_t st) {
-  return p.norm == kTail && p.kl != kLowVar ? sums_t<T, true>(p, rows, st) : sums_t<T, false>(p, rows, st);
 }
 
 template <typename T, typename O>
 int bwd_t(BwdParams p, long long rows, cudaStream_t st) {
+  // blocks of at least 24576 elements where rows are long (2048 rows of 151936 in bf16: six parts 201 us, one 221, sixteen 240)
+  const int most = p.vocab / 24576 < kMaxParts ? p.vocab / 24576 : kMaxParts;
   p.parts = parts_of(rows, p.vocab, 5ll * num_sms(), 500);
+  p.parts = p.parts > most ? p.parts : most;
   if (rows * p.parts > 2147483647ll) return -3;
   // groups of eight line up in both where rows keep their distance and begin alike
   const uintptr_t a = reinterpret_cast<uintptr_t>(p.z) / sizeof(T), b = reinterpret_cast<uintptr_t>(p.dz) / sizeof(O);
   const bool whole = (a - b) % 8 == 0 && (rows == 1 || (p.ld - p.vocab) % 8 == 0);
   const int grid = static_cast<int>(rows * p.parts);
-  const size_t smem = static_cast<size_t>(p.k) * 4 + 4;
-  if (whole) bwd_kernel<T, O, true><<<grid, kThreads, smem, st>>>(p);
-  else bwd_kernel<T, O, false><<<grid, kThreads, smem, st>>>(p);
+  if (whole) bwd_kernel<T, O, true><<<grid, kThreads, 0, st>>>(p);
+  else bwd_kernel<T, O, false><<<grid, kThreads, 0, st>>>(p);
   rb_note_launch(1);
   return static_cast<int>(cudaGetLastError());
 }
@@ -598,7 +612,7 @@ int bwd_t(BwdParams p, long long rows, cudaStream_t st) {
 using namespace rb;
 using namespace rb::distill;
 
-// Blocks per row, and so pairs of floats per row that rb_topk_distill takes as workspace.
+// Blocks per row, and so pairs of doubles per row that rb_topk_distill takes as workspace.
 extern "C" int rb_topk_distill_parts(long long rows, int vocab) {
   const int parts = parts_of(rows, vocab, 4ll * num_sms(), 1000);      // (a fixed 2 us of 4 blocks per SM)
   return vocab / parts > (1 << 20) ? kMaxParts : parts;                 // the bitmap of a part fits shared memory
@@ -606,35 +620,39 @@ extern "C" int rb_topk_distill_parts(long long rows, int vocab) {
 
 // dtype: 0 bf16, 1 fp16, 2 fp32.  kl: reverse, forward, mixed, low variance; norm: tail bin, renormalised, as they are.
 extern "C" int rb_topk_distill(const void* z, long long ld, const long long* ids, const float* teacher, float* loss, float* coef, float* stats,
-                               float* log_probs, float2* sums, long long rows, int vocab, int k, int kl, int norm, double alpha, double clamp,
-                               float inv_temp, int dtype, cudaStream_t st) {
-  if (rows < 0 || vocab < 1 || vocab > kMaxVocab || k < 0 || k > kMaxIds || kl < 0 || kl > 3 || norm < 0 || norm > 2 || !(inv_temp > 0.f)) return -1;
+                               float* log_probs, double2* sums, long long rows, int vocab, int k, int kl, int norm, double alpha, double clamp,
+                               double inv_temp, int dtype, cudaStream_t st) {
+  if (rows < 0 || vocab < 1 || vocab > kMaxVocab || k < 0 || k > kMaxIds || kl < 0 || kl > 3 || norm < 0 || norm > 2 || !(inv_temp > 0.0)) return -1;
   if (rows == 0) return 0;
   const int parts = rb_topk_distill_parts(rows, vocab);
   if (rows * parts > 2147483647ll) return -3;
-  const Params p{z, ld, ids, teacher, loss, coef, stats, log_probs, sums, vocab, k, kl, norm, parts, inv_temp * 1.4426950408889634f, alpha, clamp};
+  const double scale = inv_temp * kLog2e;
+  const float c2 = static_cast<float>(scale);
+  const Params p{z, ld, ids, teacher, loss, coef, stats, log_probs, sums, vocab, k, kl, norm, parts, c2, static_cast<float>(scale - c2), scale, alpha, clamp};
   int rc = -1;
   switch (dtype) {
-    case 0: rc = sums_any<__nv_bfloat16>(p, rows, st); break;
-    case 1: rc = sums_any<__half>(p, rows, st); break;
-    case 2: rc = sums_any<float>(p, rows, st); break;
+    case 0: rc = sums_t<__nv_bfloat16>(p, rows, st); break;
+    case 1: rc = sums_t<__half>(p, rows, st); break;
+    case 2: rc = sums_t<float>(p, rows, st); break;
   }
   if (rc) return rc;
   // many rows: a warp each, which spends the fewest instructions; few: a thread per id, for the shortest way
   int threads = rows >= 8ll * num_sms() ? 32 : (k + 31) / 32 * 32, slots = 32;
   threads = threads < 32 ? 32 : threads > kIdThreads ? kIdThreads : threads;
   while (slots < 2 * k) slots *= 2;
-  id_kernel<<<static_cast<unsigned>(rows), threads, static_cast<size_t>(k) * 20 + slots * 8, st>>>(p, slots);
+  id_kernel<<<static_cast<unsigned>(rows), threads, static_cast<size_t>(k) * 24 + slots * 8, st>>>(p, slots);
   rb_note_launch(1);
   return static_cast<int>(cudaGetLastError());
 }
 
 // out_dtype: that of the logits, or 0 (bf16) for logits in fp32
 extern "C" int rb_topk_distill_bwd(const void* z, long long ld, const long long* ids, const float* coef, const float* stats, const float* g, void* dz,
-                                   long long rows, int vocab, int k, float inv_temp, int dtype, int out_dtype, cudaStream_t st) {
-  if (rows < 0 || vocab < 1 || vocab > kMaxVocab || k < 0 || k > kMaxIds || !(inv_temp > 0.f)) return -1;
+                                   long long rows, int vocab, int k, double inv_temp, int dtype, int out_dtype, cudaStream_t st) {
+  if (rows < 0 || vocab < 1 || vocab > kMaxVocab || k < 0 || k > kMaxIds || !(inv_temp > 0.0)) return -1;
   if (rows == 0) return 0;
-  const BwdParams p{z, ld, ids, coef, stats, g, dz, vocab, k, 1, inv_temp * 1.4426950408889634f, inv_temp};
+  const double scale = inv_temp * kLog2e;
+  const float c2 = static_cast<float>(scale);
+  const BwdParams p{z, ld, ids, coef, stats, g, dz, vocab, k, 1, c2, static_cast<float>(scale - c2), static_cast<float>(inv_temp)};
   if (dtype == 0 && out_dtype == 0) return bwd_t<__nv_bfloat16, __nv_bfloat16>(p, rows, st);
   if (dtype == 1 && out_dtype == 1) return bwd_t<__half, __half>(p, rows, st);
   if (dtype == 2 && out_dtype == 2) return bwd_t<float, float>(p, rows, st);

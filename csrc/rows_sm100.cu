@@ -359,6 +359,7 @@ __global__ void __launch_bounds__(kThreads) pack_sort_kernel(TokenKeys src, int2
   for (int i = t; i < n; i += kThreads) pairs[i] = make_int2(static_cast<int>(a[i] >> pos_bits), static_cast<int>(a[i] & ((1u << pos_bits) - 1)));
 }
 
+constexpr size_t kMostSmem = 220 * 1024;
 constexpr int kMaxSort = 1 << 30;      // rows and keys of a sort (places are 32-bit)
 constexpr int kMostSteps = 16;         // counters of a warp's rows have 16 bits, and so have all of a block's
 constexpr int kOneBlock = 4096;        // rows that one block sorts by itself (9003 rows: 18 us, in nine blocks after a count 9 us)
@@ -375,9 +376,11 @@ inline int sort_blocks(long long n) {
 inline int fill_blocks(const Fill& f, long long vectors) {
   return f.far == nullptr ? 0 : static_cast<int>((vectors + kThreads * kFillRun - 1) / (kThreads * kFillRun)) + 1;
 }
+// Always the same limit: calls of several threads would lower one another's otherwise.
 template <typename K>
 int allow_smem(K kernel, size_t bytes) {
-  return bytes <= 48 * 1024 ? 0 : static_cast<int>(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)));
+  if (bytes <= 48 * 1024) return 0;
+  return bytes > kMostSmem ? -4 : static_cast<int>(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kMostSmem)));
 }
 
 template <int kSteps, typename Src, typename Out>

@@ -321,6 +321,32 @@ def test_distill_infinities():
     assert torch.isnan(out[3]) and torch.isinf(out[0]) and torch.isfinite(out[[1, 2]]).all()
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+def test_distill_masks_of_the_lowest_value(dtype):
+    """A mask may leave some tokens, or none: rows of nothing but the type's lowest value are uniform."""
+    z, ids, t, w = _case(5, 1003, 7, dtype, 14)
+    low = torch.finfo(DT[dtype]).min
+    z[0] = low
+    z[1, 10:] = low
+    z[2, ::2] = low
+    z[3, :] = -math.inf
+    z[3, 5] = 1.0
+    ids[1, :3] = torch.tensor([3, 500, 9], device="cuda")
+    for norm, temperature in (("tail", 1.0), ("norm", 1.0), ("trunc", 0.5)):
+        zl = z.detach().requires_grad_()
+        loss = ops.topk_distill(zl, ids, t, "forward_kl" if norm == "trunc" else "jsd", norm_mode=norm, temperature=temperature)
+        (d,) = torch.autograd.grad(loss, zl, w)
+        r = [0, 1, 2, 4]
+        zz = torch.where(z.double() <= -1e38, z.double() / 2 ** 20, z.double()) if dtype != "fp16" else z.double()      # (the same rows in exact arithmetic)
+        want, d_want, _ = O.distill(zz[r], ids[r], t[r], w[r], "forward_kl" if norm == "trunc" else "jsd", 0.5, norm, temperature)
+        fine = torch.isfinite(want)
+        assert torch.allclose(loss[r].double().cpu()[fine], want[fine], rtol=1e-5, atol=1e-5)
+        got = d[r].double().cpu()[fine]
+        assert float((got - d_want[fine]).abs().max()) <= 2 * _half_step(DT[dtype]) * float(d_want[fine].abs().max()) + 1e-5
+    lp = ops.topk_distill(z, ids, t, return_log_probs=True)[1]
+    assert torch.allclose(lp[0], torch.full((7,), -math.log(1003.0), device="cuda"), atol=1e-5)
+
+
 def test_distill_log_probs():
     z, ids, t, _ = _case(6, 5000, 20, "bf16", 3)
     ids[2, 4:] = -1
@@ -367,6 +393,117 @@ def test_fused_head_distill():
     ops.fused_lm_head_topk_distill(h2, wt, ids, t, "jsd", chunk_size=300).backward(w)
     assert wt.grad is None and float((wt.main_grad.double() - e_w).norm() / e_w.norm()) < 2.0 ** -7
     assert float((h2.grad.double() - e_h).norm() / e_h.norm()) < 2.0 ** -7
+
+
+# --------------------------------------------------------------------------- far offsets, one gradient only
+
+
+def test_offsets_beyond_32_bits():
+    g = _gen(3)
+    # a buffer of 2.2e9 elements
+    T, k, E, H = 66000, 8, 16, 4096
+    ids = torch.randint(0, E, (T, k), device="cuda", generator=g)
+    rows = ops.expert_layout(ids, E)
+    x = torch.randn(T, H, device="cuda", generator=g).bfloat16()
+    srt = ops.expert_dispatch(x, rows)
+    assert srt.numel() > 2 ** 31
+    last = int(rows.dest[:, 0].argmax())
+    assert torch.equal(srt[rows.dest[last].long()], x[last].expand(k, H)) and torch.equal(srt[int(rows.dest[0, 0])], x[0])
+    w = torch.full((T, k), 0.125, device="cuda")
+    out = ops.expert_combine(srt, w, rows)
+    assert torch.equal(out[[0, last, T - 1]], x[[0, last, T - 1]])            # eight eighths of a row
+    del srt, out
+    # logits of 2.4e9 elements: the last rows are those of a small call
+    R, V, K = 18000, 131072, 4
+    z = torch.empty(R, V, device="cuda", dtype=torch.bfloat16).normal_(generator=g)
+    ids = torch.randint(0, V, (R, K), device="cuda", generator=g)
+    t = torch.full((R, K), -3.0, device="cuda")
+    zl = z.requires_grad_()
+    loss = ops.topk_distill(zl, ids, t)
+    (d,) = torch.autograd.grad(loss.sum(), zl)
+    small = z.detach()[-3:].clone().requires_grad_()
+    part = ops.topk_distill(small, ids[-3:], t[-3:])
+    (ds,) = torch.autograd.grad(part.sum(), small)
+    assert torch.allclose(part, loss[-3:], rtol=1e-5, atol=1e-6) and torch.allclose(ds.float(), d[-3:].float(), rtol=2.0 ** -7, atol=1e-7)
+    del z, zl, d, loss
+    # a table of 2.2e9 elements
+    table = torch.zeros(550000, 4096, device="cuda", dtype=torch.bfloat16)
+    table[-1] = 1.0
+    tok = torch.tensor([549999, 0, 549999, 123], device="cuda")
+    leaf = table.requires_grad_()
+    out = ops.embedding(tok, leaf)
+    assert bool((out[0] == 1).all()) and not out[1].any()
+    (d,) = torch.autograd.grad(out, leaf, torch.ones_like(out))
+    assert bool((d[549999] == 2).all()) and bool((d[0] == 1).all()) and bool((d[123] == 1).all()) and int(d.count_nonzero()) == 3 * 4096
+
+
+def test_gradients_are_given_once():
+    z, ids, t, w = _case(3, 50, 4, "fp32", 1)
+    zl = z.requires_grad_()
+    wl = w.requires_grad_()
+    (d,) = torch.autograd.grad(ops.topk_distill(zl, ids, t), zl, wl, create_graph=True)
+    with pytest.raises(RuntimeError, match="once"):
+        d.sum().backward()
+    rows = ops.expert_layout(torch.zeros(4, 2, dtype=torch.int64, device="cuda"), 2)
+    x = torch.randn(4, 8, device="cuda").requires_grad_()
+    up = torch.randn(rows.source.numel(), 8, device="cuda").requires_grad_()
+    (d,) = torch.autograd.grad(ops.expert_dispatch(x, rows), x, up, create_graph=True)
+    with pytest.raises(RuntimeError, match="once"):
+        d.sum().backward()
+
+
+def test_combine_in_fp32_passes_gradients_on():
+    g = _gen(4)
+    ids = torch.randint(0, 5, (60, 3), device="cuda", generator=g)
+    rows = ops.expert_layout(ids, 5)
+    y = torch.randn(rows.source.numel(), 40, device="cuda", generator=g).bfloat16().requires_grad_()
+    w = torch.rand(60, 3, device="cuda", generator=g).bfloat16().requires_grad_()
+    up = torch.randn(60, 40, device="cuda", generator=g).bfloat16()
+    a = torch.autograd.grad(ops.expert_combine(y, w, rows, torch.float32), [y, w], up.float())
+    b = torch.autograd.grad(ops.expert_combine(y, w, rows), [y, w], up)
+    assert a[0].dtype == torch.bfloat16 and a[1].dtype == torch.bfloat16 and all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+def test_calls_of_two_threads():
+    """Threads on streams of their own: no workspace, counter or limit is shared."""
+    import threading
+
+    g = _gen(6)
+    cases = []
+    for n, E in ((3000, 2048), (16000, 64)):
+        ids = torch.randint(0, E, (n, 2), device="cuda", generator=g)
+        x = torch.randn(n, 64, device="cuda", generator=g).bfloat16()
+        tok = torch.randint(0, 700, (n,), device="cuda", generator=g)
+        cases.append((ids, E, x, tok, torch.randn(n, 64, device="cuda", generator=g).bfloat16(), torch.randn(n // 50, 1000, device="cuda", generator=g)))
+
+    def run(ids, E, x, tok, dy, z):
+        rows = ops.expert_layout(ids, E)
+        out = [rows.dest, ops.expert_combine(ops.expert_dispatch(x, rows), None, rows)]
+        table = torch.zeros(700, 64, device="cuda", dtype=torch.bfloat16).requires_grad_()
+        out += torch.autograd.grad(ops.embedding(tok, table), table, dy)
+        at = tok[: 4 * z.shape[0]].view(-1, 4)
+        return out + [ops.topk_distill(z, at, torch.full(at.shape, -4.0, device="cuda"))]
+
+    want = [[t.clone() for t in run(*c)] for c in cases]
+    torch.cuda.synchronize()
+    got, failed = {}, []
+
+    def work(i):
+        try:
+            s = torch.cuda.Stream()
+            with torch.cuda.stream(s):
+                for _ in range(20):
+                    got[i] = run(*cases[i])
+            s.synchronize()
+        except Exception as e:   # noqa: BLE001
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    torch.cuda.synchronize()
+    assert not failed, failed
+    assert all(torch.equal(a, b) for i in range(2) for a, b in zip(want[i], got[i]))
 
 
 # --------------------------------------------------------------------------- together
