@@ -304,6 +304,7 @@ __global__ void __launch_bounds__(kThreads, 4) sum_kernel(Params p) {
   int g = w0 + t;
   for (; g + (U - 1) * kThreads < w1; g += U * kThreads) step(g, std::true_type{});
   if (g < w1) step(g, std::false_type{});
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");      // the small kernel may come in and set up its table
   // the row's first and last group, where they are not whole: one element per thread
   if (t < 16) {
     const int g = t < 8 ? 0 : groups - 1, i = t & 7;
@@ -353,6 +354,7 @@ __global__ void __launch_bounds__(kIdThreads) id_kernel(Params p, int slots) {
   __shared__ double red[4][kIdWarps];
   const bool tail = p.norm == kTail && p.kl != kLowVar, renorm = p.norm == kNorm && p.kl != kLowVar;
   for (int i = t; i < slots; i += threads) key[i] = -1, place[i] = p.k;
+  asm volatile("griddepcontrol.wait;" ::: "memory");      // the streaming kernel is done, and what it wrote can be seen
   Sum all{-INFINITY, 0.0};
   for (int r = 0; r < p.parts; ++r) {
     const double2 s = p.sums[row * p.parts + r];
@@ -640,9 +642,19 @@ extern "C" int rb_topk_distill(const void* z, long long ld, const long long* ids
   int threads = rows >= 8ll * num_sms() ? 32 : (k + 31) / 32 * 32, slots = 32;
   threads = threads < 32 ? 32 : threads > kIdThreads ? kIdThreads : threads;
   while (slots < 2 * k) slots *= 2;
-  id_kernel<<<static_cast<unsigned>(rows), threads, static_cast<size_t>(k) * 24 + slots * 8, st>>>(p, slots);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(rows));
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = static_cast<size_t>(k) * 24 + slots * 8;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, id_kernel, p, slots);
   rb_note_launch(1);
-  return static_cast<int>(cudaGetLastError());
+  return static_cast<int>(e != cudaSuccess ? e : cudaGetLastError());
 }
 
 // out_dtype: that of the logits, or 0 (bf16) for logits in fp32
