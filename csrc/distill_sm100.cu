@@ -6,15 +6,20 @@
 //   bin with all other mass (no less than 1 - exp(-1e-7) of it).
 //   d z_v = g / T (sum_i c_i [v = id_i] - P_v sum_i c_i)  with  c_i = dD / ds_i
 //
-// Both directions are bound by memory: the forward kernel reads the logits once (maximum and sum together, the sum rescaled when
-// the maximum grows), the backward kernel reads them once more and writes the gradient; everything about the K ids is a few
-// values per row.  The mass outside the ids is summed by itself - the ids are marked in a bitmap and left out - because 1 - sum P
-// loses all digits where the ids hold nearly everything.  The forward pass is two kernels: one that streams the rows (several blocks
-// per row where there are few of them) and a small one with the 64-bit arithmetic, which would cost the first its occupancy.
-// Arithmetic: 32-bit exponentials and sums over the vocabulary, 64 bits for the K ids (a few hundred values per row).
+// Both directions are bound by memory: the forward pass reads the logits once (maximum and sum together, the sum rescaled when the
+// maximum grows), the backward pass reads them once more and writes the gradient; everything about the K ids is a few values per
+// row.  The mass outside the ids is summed by itself - the ids are marked in a bitmap and left out - because 1 - sum P loses all
+// digits where the ids hold nearly everything.  The forward pass is two kernels: one that streams the rows (several blocks per row
+// where there are few of them) and a small one with the 64-bit arithmetic, which would cost the first its occupancy.
+// Arithmetic: 32-bit exponentials (the instruction is off by 1.5e-7 at most, 5e-8 on average), 64 of them added in 32 bits, the rest of
+// the sum and everything about the ids in 64.
+// Measured (copy: 6.47 TB/s): 2048 rows of 151936 in bf16 125 us forward, where memory (96 us) and the exponentials (69 us) meet, and
+// 177 us backward (193 us of a copy); 4096 rows in fp32 367 us (385) and 736 us (770); the ids 8 to 22 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
+#include <float.h>
+#include <math.h>
 #include <stdint.h>
 
 #include <type_traits>
@@ -29,7 +34,7 @@ constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kMaxIds = 1024;      // eight per thread of id_kernel
 constexpr int kMaxVocab = 1 << 24;
 constexpr int kMaxParts = 32;      // blocks of a row
-constexpr int kStats = 4;      // per row: log2 reference, 1 / sum, sum of the slopes, (unused)
+constexpr int kStats = 4;      // per row: log2 reference, 1 / sum, sum of the slopes (and one to fill 16 bytes)
 constexpr double kLn2 = 0.6931471805599453, kLog2e = 1.4426950408889634;
 constexpr double kLeastRest = 9.9999995e-08;      // 1 - exp(-1e-7)
 
@@ -45,7 +50,10 @@ __device__ __forceinline__ float ex2(float x) {
 // Logits in units of log2, z log2(e) / T, end at kLow: masks of a type's lowest value would pass it, and a row of nothing else is uniform.
 // Only rows whose largest logit is far down there look at it (`low` rows); elsewhere such logits have no mass either way.
 constexpr float kLow = -3.4e38f, kLowRows = -1e38f;
-__device__ __forceinline__ float low_mass(float z, float c2, float ref) { return z == -INFINITY ? 0.f : ex2(fmaxf(z * c2, kLow) - ref); }
+__device__ __forceinline__ float low_mass(float z, float c2, float ref) {
+  const float x = z * c2;
+  return z == -INFINITY ? 0.f : ex2((x < kLow ? kLow : x) - ref);      // (NaN stays)
+}
 
 // the whole number at or above z log2(e) / T
 __device__ __forceinline__ float whole_ref(float z, float c2) { return z == -INFINITY ? z : ceilf(fmaxf(z * c2, kLow)); }
@@ -564,8 +572,8 @@ __global__ void __launch_bounds__(kThreads) bwd_kernel(BwdParams p) {
 }
 
 // Blocks of a row for kernels of `slots` blocks at a time: the number with the shortest waves, where a block costs as much as `fixed`
-// groups of eight beside its own.  (2048 rows of 151936: two parts in 7 waves, 108 us; one part in 4 waves, the last of them less
-// than half full, 115 us; four parts 127 us.)
+// groups of eight beside its own.  (2048 rows of 151936, while a block's own part of the work was smaller: two parts in 7 waves 108 us;
+// one part in 4 waves, the last of them less than half full, 115 us; four parts 127 us.)
 inline int parts_of(long long rows, int vocab, long long slots, int fixed) {
   const long long groups = (vocab + 7) / 8;
   int best = 1;
@@ -576,6 +584,13 @@ inline int parts_of(long long rows, int vocab, long long slots, int fixed) {
   }
   return best;
 }
+// log2(e) / T in two 32-bit numbers.  Both are above zero: a logit of -inf stays -inf in z c2 + z c2_low.
+inline void two_floats(double scale, float& c2, float& c2_low) {
+  c2 = static_cast<float>(scale);
+  if (static_cast<double>(c2) > scale) c2 = nextafterf(c2, 0.f);
+  c2_low = fmaxf(static_cast<float>(scale - c2), FLT_MIN);
+}
+
 template <typename T>
 int sums_t(const Params& p, long long rows, cudaStream_t st) {
   const int each = ((p.vocab + 14) / 8 + p.parts - 1) / p.parts + 1;
@@ -629,8 +644,9 @@ extern "C" int rb_topk_distill(const void* z, long long ld, const long long* ids
   const int parts = rb_topk_distill_parts(rows, vocab);
   if (rows * parts > 2147483647ll) return -3;
   const double scale = inv_temp * kLog2e;
-  const float c2 = static_cast<float>(scale);
-  const Params p{z, ld, ids, teacher, loss, coef, stats, log_probs, sums, vocab, k, kl, norm, parts, c2, static_cast<float>(scale - c2), scale, alpha, clamp};
+  float c2, c2_low;
+  two_floats(scale, c2, c2_low);
+  const Params p{z, ld, ids, teacher, loss, coef, stats, log_probs, sums, vocab, k, kl, norm, parts, c2, c2_low, scale, alpha, clamp};
   int rc = -1;
   switch (dtype) {
     case 0: rc = sums_t<__nv_bfloat16>(p, rows, st); break;
@@ -663,8 +679,9 @@ extern "C" int rb_topk_distill_bwd(const void* z, long long ld, const long long*
   if (rows < 0 || vocab < 1 || vocab > kMaxVocab || k < 0 || k > kMaxIds || !(inv_temp > 0.0)) return -1;
   if (rows == 0) return 0;
   const double scale = inv_temp * kLog2e;
-  const float c2 = static_cast<float>(scale);
-  const BwdParams p{z, ld, ids, coef, stats, g, dz, vocab, k, 1, c2, static_cast<float>(scale - c2), static_cast<float>(inv_temp)};
+  float c2, c2_low;
+  two_floats(scale, c2, c2_low);
+  const BwdParams p{z, ld, ids, coef, stats, g, dz, vocab, k, 1, c2, c2_low, static_cast<float>(inv_temp)};
   if (dtype == 0 && out_dtype == 0) return bwd_t<__nv_bfloat16, __nv_bfloat16>(p, rows, st);
   if (dtype == 1 && out_dtype == 1) return bwd_t<__half, __half>(p, rows, st);
   if (dtype == 2 && out_dtype == 2) return bwd_t<float, float>(p, rows, st);

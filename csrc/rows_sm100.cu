@@ -1,8 +1,10 @@
 // Rows moved by key: the layout of routed rows sorted by expert, their way there and back (with weights), the rows of an
 // embedding table and the table's gradient by sorted tokens.
 //
-// All of it is bound by memory: every kernel touches each row it needs once, in 16-byte vectors where rows allow it, one warp
-// per row or part of a row, sums in 32 bits in a fixed order (no floating-point atomics, so reruns give the same bits).
+// All of it is bound by memory: every kernel touches each row it needs once, in 16-byte vectors where rows allow it, a warp per part
+// of a row or a block per token, sums in 32 bits in a fixed order (no floating-point atomics, so reruns give the same bits).
+// Measured against a copy's 6.47 TB/s (bf16): 8192 tokens to 8 of 128 experts, width 2048, 62 us there (57 us of memory), 54 us back (47),
+// 96 us for the gradients of rows and weights (98); 16384 tokens from a table of 4096 columns 29 us (27).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -299,8 +301,8 @@ __global__ void __launch_bounds__(kThreads) place_kernel(Src src, Out out, int n
   }
 }
 
-// Tokens sorted by table row in one launch: (key, position) in 32 bits, all passes in the shared memory of one block (two passes of
-// 16384 tokens 13 us, four launches of the kernels above 16 us).
+// Tokens sorted by table row in one launch: (key, position) in 32 bits, all passes in the shared memory of one block, the other blocks
+// fill the gradient meanwhile (16384 tokens of a text 45 us, hidden behind a fill of 1.2 GB that takes 166 us; 300 tokens 4 us).
 template <int kSteps>
 __global__ void __launch_bounds__(kThreads) pack_sort_kernel(TokenKeys src, int2* __restrict__ pairs, int n, int pos_bits, int passes, int each, Fill fill) {
   extern __shared__ int sm[];
@@ -494,7 +496,7 @@ __global__ void __launch_bounds__(256) move_kernel(const T* __restrict__ in, lon
 
 constexpr int kSingleThreads = 128;      // of a block that works on a row of single elements
 // out[t] = sum_j w[t, j] in[dest[t, j]] in 32 bits, j ascending.  A block per token: its places are read once, and the rows that follow
-// from them in vectors of all threads, eight rows in flight (single elements: four rows, eight elements of a thread).  Measured for
+// from them in vectors of all threads, eight rows in flight (single elements: four rows, four elements of a thread).  Measured for
 // 65536 rows of 4 KB, 47 us of memory: 54 us; a warp per part of a row, which waits for its places as long as for the rows, 61 us; blocks
 // that fetch the places of their next token meanwhile, but wait for one another between tokens, 63 us.
 template <typename T, int N, bool kWeight, typename OutT>
@@ -650,7 +652,8 @@ __global__ void __launch_bounds__(N == 1 ? kSingleThreads : 256) sum_bwd_kernel(
 // ----------------------------------------------------------------------------- gradient of a table by sorted rows
 // `pairs` holds (table row, input row) in order.  A warp walks 32 of them for 32 vectors of columns and keeps one running sum; a run
 // of equal keys that ends inside goes out at once, one that goes on in the next 32 (or came from those in front) leaves a partial
-// sum, and merge_kernel adds those of a run.
+// sum, and merge_kernel adds those of a run.  16384 tokens of a text, 4096 columns in bf16: 39 us for 28 us of memory and 9 us for the
+// merge; added to fp32 rows 69 us for 48.
 constexpr int kRun = 32, kLongRun = 16;
 
 template <typename OutT, int N, bool kAdd>

@@ -499,6 +499,12 @@ def validate_args(a: argparse.Namespace) -> argparse.Namespace:
                              "the sampled token's log-prob only")
         if a.opd_kl_type == "low_var_kl" and a.opd_token_selection == "union":
             pass
+        if (a.opd_loss_coef or 0.0) != 0.0:
+            if max(a.tensor_model_parallel_size, a.context_parallel_size, a.pipeline_model_parallel_size) > 1:
+                raise ValueError("--opd-loss-coef with a top-K selection reads whole rows of logits: trainer tp = cp = pp = 1")
+            most = 512 if a.opd_token_selection == "union" else 1024
+            if a.opd_log_prob_top_k > most:
+                raise ValueError(f"--opd-loss-coef with --opd-token-selection {a.opd_token_selection}: --opd-log-prob-top-k up to {most}")
     elif a.opd_kl_type in ("forward_kl", "jsd"):
         raise ValueError(f"--opd-kl-type {a.opd_kl_type} needs both distributions: choose a top-K --opd-token-selection")
     if a.engine_speculative_algorithm:

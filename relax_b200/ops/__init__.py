@@ -346,12 +346,15 @@ def expert_combine(y, weights, rows, dtype=None):
     return (_cuda() if _use_cuda(y) else ref).expert_combine(y, weights, rows, dtype)
 
 
-def embedding(tokens, weight, scale: float = 1.0, vocab_start: int = 0):
+def embedding(tokens, weight, scale: float = 1.0, vocab_start: int = 0, whole: bool = False):
     """``scale * weight[tokens - vocab_start]``, zeros for tokens outside the table's rows (those of other shards).  The gradient sorts the
-    tokens and sums every table row's incoming rows in 32 bits in the order of the tokens, so reruns give the same bits; it is added to
-    the weight's fp32 ``main_grad`` where there is one, which touches only rows that were looked up."""
+    tokens and sums every table row's incoming rows in 32 bits in a fixed order, so reruns give the same bits; it is added to the
+    weight's fp32 ``main_grad`` where there is one at the time of the lookup, which touches only rows that were looked up.  ``whole``: the table
+    is the whole vocabulary, and on the CPU a token outside it raises (on a GPU nothing is read back)."""
     if tokens.dtype not in (torch.int64, torch.int32) or weight.dim() != 2:
         raise ValueError(f"embedding: int64 or int32 tokens and a matrix, got {tokens.dtype} and {weight.dim()} dimensions")
+    if whole and not tokens.is_cuda and tokens.numel() and not 0 <= int(tokens.min()) - vocab_start <= int(tokens.max()) - vocab_start < weight.shape[0]:
+        raise IndexError(f"embedding: token ids {int(tokens.min())} .. {int(tokens.max())} for a table of {weight.shape[0]} rows from {vocab_start}")
     return (_cuda() if _use_cuda(weight) else ref).embedding(tokens, weight, float(scale), int(vocab_start))
 
 
@@ -367,8 +370,8 @@ def _distill_args(what, rows, ids, teacher_log_probs, kl_type, alpha, norm_mode,
         raise ValueError(f"{what}: norm_mode is tail, norm or trunc, got {norm_mode!r}")
     if not 0.0 <= alpha <= 1.0:
         raise ValueError(f"{what}: alpha must lie in [0, 1], got {alpha}")
-    if not 0.0 < temperature < float("inf"):
-        raise ValueError(f"{what}: temperature must be positive, got {temperature}")
+    if not 1e-20 <= temperature <= 1e20:
+        raise ValueError(f"{what}: temperature must be positive, 1e-20 to 1e20, got {temperature}")
 
 
 def topk_distill(logits, ids, teacher_log_probs, kl_type: str = "reverse_kl", alpha: float = 0.5, norm_mode: str = "tail", temperature: float = 1.0,

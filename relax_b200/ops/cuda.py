@@ -1283,18 +1283,21 @@ class _FusedHeadDistill(torch.autograd.Function):
         inv_temp, chunk, weight = ctx.meta
         g = g.float().contiguous()
         R, V = h.shape[0], w.shape[0]
-        dh = torch.empty_like(h)
+        learn_h, learn_w = ctx.needs_input_grad[:2]
+        dh = torch.empty_like(h) if learn_h else None
         mg = main_grad_of(weight)
         direct = mg is not None and mg.is_contiguous()
-        dw = mg if direct else torch.zeros(w.shape, dtype=torch.float32, device=h.device)
+        dw = (mg if direct else torch.zeros(w.shape, dtype=torch.float32, device=h.device)) if learn_w else None
         for k, s in zip(kept, range(0, R, chunk)):
             e = min(R, s + chunk)
             z = matmul_nt(h[s:e], w, out_dtype=torch.float32)
             d = torch.empty(e - s, V, dtype=h.dtype, device=h.device)
             _load().topk_distill_rows_bwd(z, ids[s:e], k, g[s:e], inv_temp, d)
-            matmul_nn(d, w, out=dh[s:e])
-            matmul_tn(d, h[s:e], out=dw, accumulate=True)
-        return dh, None if direct else dw.to(weight.dtype), None, None, None, None
+            if learn_h:
+                matmul_nn(d, w, out=dh[s:e])
+            if learn_w:
+                matmul_tn(d, h[s:e], out=dw, accumulate=True)
+        return dh, dw.to(weight.dtype) if learn_w and not direct else None, None, None, None, None
 
 
 def fused_lm_head_topk_distill(hidden, weight, ids, teacher, kl_type, alpha, norm_mode, temperature, clamp, chunk):

@@ -217,7 +217,7 @@ class RolloutWeights(ComposedForward):
     # ------------------------------------------------------------------ model pieces
     def _embed(self, tokens, tp: GroupInfo):
         if tp.size == 1:
-            return ops.embedding(tokens, self.p["embed"], self.cfg.embed_scale)
+            return ops.embedding(tokens, self.p["embed"], self.cfg.embed_scale, whole=True)
         e = ops.embedding(tokens, self.p["embed"], self.cfg.embed_scale, self.vocab_start)
         dist.all_reduce(e, group=tp.group)
         return e

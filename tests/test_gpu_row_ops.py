@@ -321,6 +321,73 @@ def test_distill_infinities():
     assert torch.isnan(out[3]) and torch.isinf(out[0]) and torch.isfinite(out[[1, 2]]).all()
 
 
+@pytest.mark.parametrize("temperature", [0.7, 1.0, 1.5, 3.0])      # (what 32 bits leave of log2(e) / T is below zero at the first, third and last)
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+def test_distill_masks_at_any_temperature(dtype, temperature):
+    """Tokens masked with -inf have no mass and no gradient; the others are as if they stood alone."""
+    z, ids, t, w = _case(6, 1500, 9, dtype, 16)
+    want, d_want = _check(z, ids, t, w, kl="jsd", temperature=temperature)
+    masked = torch.nn.functional.pad(z, (0, 700), value=-math.inf).requires_grad_()
+    loss = ops.topk_distill(masked, ids, t, "jsd", temperature=temperature)
+    (d,) = torch.autograd.grad(loss, masked, w)
+    assert bool((d[:, 1500:] == 0).all())
+    assert torch.allclose(loss, want, rtol=1e-5, atol=1e-6)      # (other parts of a row: other orders of the sum, 2e-6 of it)
+    assert torch.allclose(d[:, :1500].float(), d_want.float(), rtol=4 * _half_step(d.dtype) + 1e-5, atol=1e-6)
+
+
+@pytest.mark.parametrize("at", [0, 1, 800, 1002])
+def test_distill_nan_between_masks(at):
+    """A NaN is not lost in a row of nothing but the type's lowest value, nor is a row of NaN."""
+    z, ids, t, w = _case(3, 1003, 4, "fp32", 17)
+    ids[:] = torch.tensor([5, 6, 7, 9], device="cuda")
+    z[0] = torch.finfo(torch.float32).min
+    z[0, at] = math.nan
+    z[1] = math.nan
+    loss, lp = ops.topk_distill(z, ids, t, return_log_probs=True)
+    assert torch.isnan(loss[:2]).all() and torch.isnan(lp[:2]).all() and torch.isfinite(loss[2])
+
+
+@pytest.mark.parametrize("kl", ["reverse_kl", "forward_kl", "jsd"])
+def test_distill_a_single_renormalised_id(kl):
+    """All mass is the one id's on both sides: exactly nothing to learn, wherever the other entries stand and however the id is clamped."""
+    z, ids, t, w = _case(4, 900, 5, "fp32", 18)
+    ids[:3, 1:] = -1
+    ids[1] = ids[1].roll(2)
+    t[1, 2] = -30.0
+    for clamp in (None, -4.0):
+        zl = z.detach().requires_grad_()
+        loss = ops.topk_distill(zl, ids, t, kl, norm_mode="norm", log_prob_min_clamp=clamp)
+        (d,) = torch.autograd.grad(loss, zl, w)
+        assert bool((loss[:3] == 0).all()) and bool((d[:3] == 0).all()) and float(loss[3]) > 0
+
+
+def test_distill_mixture_at_its_ends():
+    z, ids, t, w = _case(20, 3001, 8, "bf16", 19)
+    for alpha, kl in ((0.0, "reverse_kl"), (1.0, "forward_kl")):
+        assert torch.equal(ops.topk_distill(z, ids, t, "jsd", alpha), ops.topk_distill(z, ids, t, kl))
+
+
+def test_fused_head_of_frozen_weights():
+    """A head that does not learn keeps its buffer, hidden states that need no gradient get none."""
+    g = _gen(21)
+    h = torch.randn(33, 64, device="cuda", generator=g).bfloat16()
+    weight = torch.randn(512, 64, device="cuda", generator=g).bfloat16()
+    _, ids, t, w = _case(33, 512, 6, "bf16", 22)
+    want = []
+    for freeze in (False, True):
+        hl, wl = h.detach().requires_grad_(), weight.detach().requires_grad_(not freeze)
+        wl.main_grad = torch.full((512, 64), 0.25, device="cuda")
+        (ops.fused_lm_head_topk_distill(hl, wl, ids, t, chunk_size=16) * w).sum().backward()
+        want.append(hl.grad)
+        assert bool((wl.main_grad == 0.25).all()) == freeze
+        learned = wl.main_grad if not freeze else learned
+    assert torch.equal(*want)
+    wl = weight.detach().requires_grad_()
+    wl.main_grad = torch.full((512, 64), 0.25, device="cuda")
+    (ops.fused_lm_head_topk_distill(h, wl, ids, t, chunk_size=16) * w).sum().backward()
+    assert torch.equal(wl.main_grad, learned)
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
 def test_distill_masks_of_the_lowest_value(dtype):
     """A mask may leave some tokens, or none: rows of nothing but the type's lowest value are uniform."""
@@ -356,6 +423,34 @@ def test_distill_log_probs():
     there = ids >= 0
     # the sum's error (2^-22 and A 2^-23 with |A| < 60, 45 additions) and the value's own rounding
     assert ((lp.double() - want).abs()[there] <= 2.0 ** -22 + 170 * F + F * want.abs()[there]).all()
+
+
+def test_distill_captured():
+    """Forward and backward in a graph, replayed on other inputs; the small kernel follows the streaming one as a programmatic dependent."""
+    z, ids, t, w = _case(40, 20000, 16, "bf16", 9)
+    zl = z.clone().requires_grad_()
+
+    def both():
+        loss, lp = ops.topk_distill(zl, ids, t, "jsd", return_log_probs=True)
+        return loss, lp, torch.autograd.grad(loss, zl, w)[0]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        both()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = both()
+    for seed in (1, 2, 3):
+        other, ids2, t2, w2 = _case(40, 20000, 16, "bf16", 20 + seed)
+        with torch.no_grad():
+            zl.copy_(other)
+        ids.copy_(ids2), t.copy_(t2), w.copy_(w2)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [x.clone() for x in held]
+        assert all(torch.equal(a, b) for a, b in zip(got, both()))
 
 
 def test_distill_gradient_against_differences():

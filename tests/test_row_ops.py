@@ -83,6 +83,9 @@ def test_embedding_statement(scale, start):
     assert w.grad is None and torch.allclose(w.main_grad, got + 0.5, rtol=2.0 ** -20, atol=2.0 ** -20 * float(size.max()))
     with pytest.raises(ValueError, match="tokens"):
         ops.embedding(tok.float(), w)
+    with pytest.raises(IndexError, match="table of 20 rows"):
+        ops.embedding(tok, w, scale, start, whole=True)
+    assert ops.embedding(tok[:0], w, whole=True).shape == (0, 11, 5)
 
 
 def test_model_embedding_takes_the_configured_scale():
@@ -220,3 +223,22 @@ def test_loss_mode_on_top_ids(tmp_path, selection):
     lp = torch.log_softmax(m.logits(h)[:, : cfg.vocab_size] / 0.8, -1).gather(1, made["ids"].clamp_min(0))
     want = opd.token_kl(lp, made["teacher"].masked_fill(made["ids"] < 0, 0.0), "jsd", 0.5, "tail", mask=made["ids"] >= 0)
     assert torch.allclose(got, want, atol=1e-5, rtol=1e-4)
+
+
+@pytest.mark.parametrize("extra,match", [(["--tensor-model-parallel-size", "2"], "tp = cp = pp = 1"), (["--context-parallel-size", "2"], "tp = cp = pp = 1"),
+                                         (["--opd-log-prob-top-k", "600"], "up to 512")])
+def test_loss_mode_refusals(extra, match):
+    from relax_b200.config.arguments import parse_args
+
+    base = ["--model-name", "tiny", "--colocate", "--rollout-batch-size", "2", "--use-opd", "--opd-teacher-load", "somewhere", "--opd-loss-coef", "1.0",
+            "--opd-token-selection", "union", "--opd-log-prob-top-k", "512"]
+    assert parse_args(base).opd_loss_coef == 1.0
+    with pytest.raises(ValueError, match=match):
+        parse_args(base + extra)
+
+
+def test_distill_temperatures():
+    z, ids, t = _rows(3, 50, 4, 2)[:3]
+    for bad in (0.0, -1.0, math.inf, math.nan, 1e-21):
+        with pytest.raises(ValueError, match="temperature"):
+            ops.topk_distill(z, ids, t, temperature=bad)
