@@ -34,7 +34,7 @@ constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kMaxIds = 1024;      // eight per thread of id_kernel
 constexpr int kMaxVocab = 1 << 24;
 constexpr int kMaxParts = 32;      // blocks of a row
-constexpr int kStats = 4;      // per row: log2 reference, 1 / sum, sum of the slopes (and one to fill 16 bytes)
+constexpr int kStats = 4;      // per row: log2 reference, 1 / sum, sum of the slopes, power of two of a far row's sum and a half (or 0)
 constexpr double kLn2 = 0.6931471805599453, kLog2e = 1.4426950408889634;
 constexpr double kLeastRest = 9.9999995e-08;      // 1 - exp(-1e-7)
 
@@ -47,16 +47,32 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// Logits in units of log2, z log2(e) / T, end at kLow: masks of a type's lowest value would pass it, and a row of nothing else is uniform.
-// Only rows whose largest logit is far down there look at it (`low` rows); elsewhere such logits have no mass either way.
-constexpr float kLow = -3.4e38f, kLowRows = -1e38f;
-__device__ __forceinline__ float low_mass(float z, float c2, float ref) {
+// Rows are summed against a whole number near their largest z log2(e) / T.  As far as kFar, 32 bits in two parts tell z log2(e) / T from it;
+// rows (and steps) whose largest logit is further away - masks of -1e9, say, that leave nothing - are taken in 64 bits.  Beyond kBeyond, where
+// neighbouring 32-bit numbers lie 512 apart, a logit is what its 32-bit product is, and the products end at kLow: a type's lowest value would
+// pass it.  A row of nothing but one such value is uniform, and beside other logits it has no mass either way.
+constexpr float kFar = 1048576.f, kBeyond = 4294967296.f, kLow = -3.4e38f;
+__device__ __noinline__ double far_mass(float z, double scale, float c2, float ref) {      // 2^(z scale - ref), NaN stays
+  if (z == -INFINITY) return 0.0;
   const float x = z * c2;
-  return z == -INFINITY ? 0.f : ex2((x < kLow ? kLow : x) - ref);      // (NaN stays)
+  if (fabsf(ref) > kBeyond) return static_cast<double>(ex2((x < kLow ? kLow : x) - ref));
+  return exp2(static_cast<double>(z) * scale - static_cast<double>(ref));      // (2^512 at most)
+}
+// s 2^d for a whole number d, at most 0 (from 2^-1022 on there is nothing left of sums that begin at 2^512)
+__device__ __forceinline__ double moved(double s, float d) {
+  return s * __hiloint2double((1023 + static_cast<int>(fmaxf(d, -1022.f))) << 20, 0);
 }
 
 // the whole number at or above z log2(e) / T
-__device__ __forceinline__ float whole_ref(float z, float c2) { return z == -INFINITY ? z : ceilf(fmaxf(z * c2, kLow)); }
+__device__ __forceinline__ float whole_ref(float z, float c2) {
+  const float x = z * c2;
+  return z == -INFINITY ? z : ceilf(x < kLow ? kLow : x);      // (NaN stays)
+}
+__device__ __forceinline__ float max_nan(float a, float b) {      // (fmaxf would drop a NaN)
+  float m;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+  return m;
+}
 
 // two 32-bit operations at a time
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
@@ -80,7 +96,9 @@ template <> struct Eight<float> {
     a = reinterpret_cast<const float4*>(p)[0];
     b = reinterpret_cast<const float4*>(p)[1];
   }
-  __device__ __forceinline__ float max() const { return fmaxf(fmaxf(fmaxf(a.x, a.y), fmaxf(a.z, a.w)), fmaxf(fmaxf(b.x, b.y), fmaxf(b.z, b.w))); }
+  __device__ __forceinline__ float max() const {
+    return max_nan(max_nan(max_nan(a.x, a.y), max_nan(a.z, a.w)), max_nan(max_nan(b.x, b.y), max_nan(b.z, b.w)));
+  }
   __device__ __forceinline__ void get(float* f) const {
     f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
   }
@@ -93,8 +111,8 @@ template <> struct Eight<__nv_bfloat16> {
   __nv_bfloat162 h[4];
   __device__ __forceinline__ void load(const __nv_bfloat16* p) { *reinterpret_cast<uint4*>(h) = *reinterpret_cast<const uint4*>(p); }
   __device__ __forceinline__ float max() const {
-    const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
-    return fmaxf(__low2float(m), __high2float(m));
+    const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
+    return max_nan(__low2float(m), __high2float(m));
   }
   __device__ __forceinline__ void get(float* f) const {
 #pragma unroll
@@ -115,8 +133,8 @@ template <> struct Eight<__half> {
   __half2 h[4];
   __device__ __forceinline__ void load(const __half* p) { *reinterpret_cast<uint4*>(h) = *reinterpret_cast<const uint4*>(p); }
   __device__ __forceinline__ float max() const {
-    const __half2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
-    return fmaxf(__low2float(m), __high2float(m));
+    const __half2 m = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
+    return max_nan(__low2float(m), __high2float(m));
   }
   __device__ __forceinline__ void get(float* f) const {
 #pragma unroll
@@ -163,7 +181,7 @@ struct Sum {
   double sum;
   __device__ __forceinline__ void add(float r, double s) {      // nothing yet: ref -inf, sum 0
     const float m = fmaxf(ref, r), at = m == -INFINITY ? 0.f : m;
-    sum = sum * static_cast<double>(ex2(ref - at)) + s * static_cast<double>(ex2(r - at));
+    sum = moved(sum, ref - at) + moved(s, r - at);
     ref = m;
   }
 };
@@ -188,6 +206,25 @@ __device__ __forceinline__ void block_sums(double (&v)[N], double (*sm)[kIdWarps
     v[i] = 0.0;
     for (int w = 0; w < warps; ++w) v[i] += sm[i][w];
   }
+}
+
+template <int N>
+__device__ __forceinline__ void block_max(double (&v)[N], double (*sm)[kIdWarps]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v[i] = fmax(v[i], __shfl_xor_sync(0xffffffffu, v[i], o));
+  const int warps = blockDim.x >> 5;
+  if (warps == 1) return;
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) sm[i][threadIdx.x >> 5] = v[i];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    for (int w = 0; w < warps; ++w) v[i] = fmax(v[i], sm[i][w]);
 }
 
 __device__ __forceinline__ double least(double x, double c) { return x < c ? c : x; }      // (NaN stays)
@@ -258,6 +295,7 @@ __global__ void __launch_bounds__(kThreads, 4) sum_kernel(Params p) {
   const unsigned char* mark = reinterpret_cast<const unsigned char*>(marks);
 
   Sum s{-INFINITY, 0.0};
+  unsigned far = 0;      // steps left out: 1 below, 2 above
   constexpr int U = sizeof(T) == 4 ? 4 : 8;      // groups of a thread in one step: 128 bytes of it under way
   // U groups from g on, in strides of the block; the last step (kAll false) holds what is left
   auto step = [&](int g, auto all) {
@@ -272,23 +310,17 @@ __global__ void __launch_bounds__(kThreads, 4) sum_kernel(Params p) {
     for (int u = 0; u < U; ++u) m[u] = kAll || g + u * kThreads < w1 ? mark[g + u * kThreads - g0] : 0;
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (kAll || g + u * kThreads < w1) big = fmaxf(big, e[u].max());
+      if (kAll || g + u * kThreads < w1) big = max_nan(big, e[u].max());
     big = whole_ref(big, p.c2);
+    if (fabsf(big) > kFar) {      // nothing there (-inf), or for the loop behind this one
+      far |= big > 0.f ? 2u : big != -INFINITY;
+      return;
+    }
     if (big > s.ref) {
-      s.sum *= static_cast<double>(ex2(s.ref - big));
+      s.sum = moved(s.sum, s.ref - big);
       s.ref = big;
     }
     const float at = s.ref == -INFINITY ? 0.f : s.ref;
-    if (at <= kLowRows) {
-#pragma unroll 1
-      for (int u = 0; u < U; ++u) {
-        const int q = g + u * kThreads;
-        if (q >= w1) break;
-        for (int i = 0; i < 8; ++i)
-          if (!((mark[q - g0] >> i) & 1)) s.sum += low_mass(up(origin[8ll * q + i]), p.c2, at);
-      }
-      return;
-    }
     const float2 c = make_float2(p.c2, p.c2), l = make_float2(p.c2_low, p.c2_low), o = make_float2(-at, -at);
     float2 add = make_float2(0.f, 0.f);
 #pragma unroll
@@ -312,6 +344,25 @@ __global__ void __launch_bounds__(kThreads, 4) sum_kernel(Params p) {
   int g = w0 + t;
   for (; g + (U - 1) * kThreads < w1; g += U * kThreads) step(g, std::true_type{});
   if (g < w1) step(g, std::false_type{});
+  // steps whose largest logit is far away, once more; those far below are nothing where some other logit is not
+  if (__syncthreads_or(s.ref > 4096.f - kFar)) far &= 2;
+  if (far) {
+#pragma unroll 1
+    for (g = w0 + t; g < w1; g += U * kThreads) {
+      float big = -INFINITY;
+#pragma unroll 1
+      for (int q = g; q < w1 && q < g + U * kThreads; q += kThreads)
+        for (int i = 0; i < 8; ++i) big = max_nan(big, up(origin[8ll * q + i]));
+      big = whole_ref(big, p.c2);
+      if (!(fabsf(big) > kFar) || big == -INFINITY || (far == 2 && big < 0.f)) continue;
+      Sum some{big, 0.0};
+#pragma unroll 1
+      for (int q = g; q < w1 && q < g + U * kThreads; q += kThreads)
+        for (int i = 0; i < 8; ++i)
+          if (!((mark[q - g0] >> i) & 1)) some.sum += far_mass(up(origin[8ll * q + i]), p.scale, p.c2, big);
+      s.add(some.ref, some.sum);
+    }
+  }
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");      // the small kernel may come in and set up its table
   // the row's first and last group, where they are not whole: one element per thread
   if (t < 16) {
@@ -320,8 +371,8 @@ __global__ void __launch_bounds__(kThreads, 4) sum_kernel(Params p) {
     const bool mine = t < 8 ? (g0 == 0 && skip) : (g1 == groups && ((skip + p.vocab) & 7) && !(groups == 1 && skip));
     if (mine && g0 < g1 && v >= 0 && v < p.vocab) {
       const bool counts = !((mark[g - g0] >> i) & 1);
-      const float y = up(z[v]), x = y == y ? whole_ref(y, p.c2) : y;      // (NaN stays)
-      const double own = x == -INFINITY ? 0.0 : x == kLow ? 1.0 : static_cast<double>(ex2(fmaf(y, p.c2_low, fmaf(y, p.c2, -x))));
+      const float y = up(z[v]), x = whole_ref(y, p.c2);
+      const double own = x == -INFINITY ? 0.0 : fabsf(x) > kFar ? far_mass(y, p.scale, p.c2, x) : static_cast<double>(ex2(fmaf(y, p.c2_low, fmaf(y, p.c2, -x))));
       s.add(x, counts ? own : 0.0);
     }
   }
@@ -369,6 +420,8 @@ __global__ void __launch_bounds__(kIdThreads) id_kernel(Params p, int slots) {
     all.add(static_cast<float>(s.x), s.y);
   }
   const double ref = all.ref == -INFINITY ? 0.0 : static_cast<double>(all.ref), rest_sum = all.sum;
+  const bool beyond = fabs(ref) > kBeyond;
+  bool some = false;
   __syncthreads();
   for (int i0 = t; i0 < p.k; i0 += 4 * threads) {      // four ids at a time: they wait for memory
     int v[4];
@@ -391,8 +444,10 @@ __global__ void __launch_bounds__(kIdThreads) id_kernel(Params p, int slots) {
       if (i >= p.k) break;
       id[i] = v[u];
       if (v[u] < 0) continue;
-      const double y = static_cast<double>(z[u]) * p.scale, low = kLow;
-      lp[i] = ((y < low && z[u] != -INFINITY ? low : y) - ref) * kLn2;      // z - reference in units of ln
+      some = true;
+      const float x = z[u] * p.c2;
+      const double y = beyond ? static_cast<double>(x < kLow && z[u] != -INFINITY ? kLow : x) : static_cast<double>(z[u]) * p.scale;
+      lp[i] = (y - ref) * kLn2;      // z - reference in units of ln
       unsigned h = mixed(v[u]);
       for (;; ++h) {      // (ends: no more than half the slots are taken)
         const int was = atomicCAS(&key[h & (slots - 1)], -1, v[u]);
@@ -402,7 +457,14 @@ __global__ void __launch_bounds__(kIdThreads) id_kernel(Params p, int slots) {
       pm[i] = static_cast<double>(h & (slots - 1));
     }
   }
-  __syncthreads();
+  if (!__syncthreads_or(some)) {      // no ids: nothing to compare, whatever the logits are
+    for (int i = t; i < p.k; i += threads) {
+      p.coef[row * p.k + i] = 0.f;
+      if (p.log_probs) p.log_probs[row * p.k + i] = -INFINITY;
+    }
+    if (t == 0) p.loss[row] = 0.f, *reinterpret_cast<float4*>(p.stats + row * kStats) = make_float4(0.f, 0.f, 0.f, 0.f);
+    return;
+  }
   double one[1] = {0.0};
   unsigned firsts = 0, moving = 0;      // a bit for each of this thread's ids
   for (int i = t, n = 0; i < p.k; i += threads, ++n) {
@@ -415,8 +477,8 @@ __global__ void __launch_bounds__(kIdThreads) id_kernel(Params p, int slots) {
   block_sums(one, red);      // the sum over the vocabulary left the ids out
   const double total = rest_sum + one[0], log_total = log(total), inv_total = 1.0 / total;
 
-  // masses of the ids (renormalised: of all of them), what the rest lacks (equal ids and clamped ones count as written), ids in all
-  double mass[4] = {0.0, 0.0, 0.0, 0.0};
+  // masses of the ids (renormalised), what the rest lacks (equal ids and clamped ones count as written), ids in all
+  double mass[4] = {0.0, 0.0, 0.0, 0.0}, most[2] = {-INFINITY, -INFINITY};
   bool twice = false;
   for (int i = t, n = 0; i < p.k; i += threads, ++n) {
     if (id[i] < 0) continue;
@@ -426,11 +488,26 @@ __global__ void __launch_bounds__(kIdThreads) id_kernel(Params p, int slots) {
     pm[i] *= inv_total;
     if (p.log_probs) p.log_probs[row * p.k + i] = static_cast<float>(lp[i]);
     if (!tail && !renorm) continue;
-    const double used = least(lp[i], p.clamp), pu = used == lp[i] ? pm[i] : exp(used);
-    mass[0] += pu;
-    mass[1] += exp(least(static_cast<double>(tl[i]), p.clamp));
-    mass[2] += pu - (first ? pm[i] : 0.0);
-    mass[3] += 1.0;
+    const double used = least(lp[i], p.clamp), t_i = least(static_cast<double>(tl[i]), p.clamp);
+    if (tail) {
+      const double pu = used == lp[i] ? pm[i] : exp(used);
+      mass[1] += exp(t_i);
+      mass[2] += pu - (first ? pm[i] : 0.0);
+    } else {
+      most[0] = used > most[0] ? used : most[0];
+      most[1] = t_i > most[1] ? t_i : most[1];
+    }
+  }
+  double* pn = reinterpret_cast<double*>(key);      // [k] renormalised masses of the student (the table is no longer needed)
+  if (renorm) {      // against the largest of them: ids far behind the others would have no mass left to renormalise
+    block_max(most, red);
+    for (int i = t; i < p.k; i += threads) {
+      if (id[i] < 0) continue;
+      pn[i] = exp(least(lp[i], p.clamp) - most[0]);
+      mass[0] += pn[i];
+      mass[1] += exp(least(static_cast<double>(tl[i]), p.clamp) - most[1]);
+      mass[3] += pn[i] == 1.0 ? 1.0 : 2.0;
+    }
   }
   if (tail || renorm) block_sums(mass, red);
   double rest_slope = 0.0, rest = 0.0;
@@ -441,7 +518,7 @@ __global__ void __launch_bounds__(kIdThreads) id_kernel(Params p, int slots) {
     rest = r.d;
     rest_slope = free >= kLeastRest ? r.slope : 0.0;
   }
-  const bool alone = renorm && mass[3] == 1.0;      // all mass is this id's, on both sides
+  const bool alone = renorm && mass[3] == 1.0 && mass[1] == 1.0;      // all mass is this id's, on both sides
   const double ls = renorm ? log(mass[0] / mass[1]) : 0.0, np = renorm ? 1.0 / mass[0] : 1.0, nq = renorm ? 1.0 / mass[1] : 1.0;
   double sums[4] = {0.0, 0.0, 0.0, 0.0};      // the divergence; slopes of all ids; slopes and masses of those that move
   for (int i = t, n = 0; i < p.k; i += threads, ++n) {
@@ -457,9 +534,9 @@ __global__ void __launch_bounds__(kIdThreads) id_kernel(Params p, int slots) {
       sums[0] += x - 1.0 + r;
       c = 1.0 - x;
     } else {
-      const double qq = alone ? 1.0 : exp(t_i) * nq;
-      pp = alone ? 1.0 : (moves ? pm[i] : exp(used)) * np;
-      const Term r = term_of(p.kl, p.alpha, pp, qq, alone ? 0.0 : used - t_i - ls);
+      const double qq = renorm ? exp(t_i - most[1]) * nq : exp(t_i);
+      pp = renorm ? pn[i] * np : moves ? pm[i] : exp(used);
+      const Term r = term_of(p.kl, p.alpha, pp, qq, alone ? 0.0 : renorm ? (used - most[0]) - (t_i - most[1]) - ls : used - t_i);
       sums[0] += r.d;
       c = (p.kl == kForward ? -qq : weighted(pp, r.slope)) - weighted(pp, rest_slope);
     }
@@ -476,7 +553,7 @@ __global__ void __launch_bounds__(kIdThreads) id_kernel(Params p, int slots) {
   if (renorm) {      // c_i - P_i sum c
     move -= sums[1] * sums[3];
     for (int i = t, n = 0; i < p.k; i += threads, ++n)
-      if ((moving >> n) & 1) lp[i] -= (alone ? 1.0 : pm[i] * np) * sums[1];
+      if ((moving >> n) & 1) lp[i] -= pn[i] * np * sums[1];
   }
   // what the logit of an id gets, its share of the sum of the slopes with it; equal ids move together
   const bool sum_equals = __syncthreads_or(twice);
@@ -494,11 +571,11 @@ __global__ void __launch_bounds__(kIdThreads) id_kernel(Params p, int slots) {
   }
   if (t == 0) {
     p.loss[row] = static_cast<float>(sums[0] + rest);
-    // (the sum's power of two goes to the reference: 1 / sum is no less than a half, whatever the reference was)
-    int e = total > 0.0 && total < INFINITY ? ilogb(total) : 0;
-    if (static_cast<double>(static_cast<float>(ref + e)) - ref != e) e = 0;      // (a reference so large that it has no place for it)
+    // the sum's power of two goes to the reference: 1 / sum is no less than a half.  Far references have no place for it.
+    const int e = total > 0.0 && total < INFINITY ? ilogb(total) : 0;
+    const bool far = fabs(ref) > kFar;
     *reinterpret_cast<float4*>(p.stats + row * kStats) =
-        make_float4(static_cast<float>(ref + e), static_cast<float>(ldexp(inv_total, e)), static_cast<float>(move), 0.f);
+        make_float4(static_cast<float>(far ? ref : ref + e), static_cast<float>(ldexp(inv_total, e)), static_cast<float>(move), far ? e + 0.5f : 0.f);
   }
 }
 
@@ -512,6 +589,7 @@ struct BwdParams {
   void* dz;                // [rows, vocab] dense (may be z itself where types agree)
   int vocab, k, parts;
   float c2, c2_low, inv_t;
+  double scale;
 };
 
 // A block per part of a row: -g / T (sum c) P over its elements, then the K ids of that part in place of what stands there.
@@ -523,23 +601,25 @@ __global__ void __launch_bounds__(kThreads) bwd_kernel(BwdParams p) {
   O* d = static_cast<O*>(p.dz) + row * p.vocab;
   const float g = p.g[row] * p.inv_t;
   const float ref = p.stats[row * kStats], inv = p.stats[row * kStats + 1], csum = p.stats[row * kStats + 2];
-  const float f = g == 0.f ? 0.f : -g * csum * inv;
+  const float f = g == 0.f ? 0.f : -g * csum * inv, power = p.stats[row * kStats + 3];
+  const bool far = power != 0.f;
   const int skip = kWhole ? static_cast<int>((reinterpret_cast<uintptr_t>(z) / sizeof(T)) & 7) : 0;
   const int groups = (skip + p.vocab + 7) >> 3, each = (groups + p.parts - 1) / p.parts;
   const int g0 = min(groups, part * each), g1 = min(groups, g0 + each);
   const long long lo = max(0ll, 8ll * g0 - skip), hi = min(static_cast<long long>(p.vocab), 8ll * g1 - skip);
   if (lo >= hi) return;
-  const bool low = ref <= kLowRows;
   auto mass = [&](float x) { return ex2(fmaf(x, p.c2_low, fmaf(x, p.c2, -ref))); };
-  auto one = [&](long long v) { put(d + v, g == 0.f ? 0.f : f * (low ? low_mass(up(z[v]), p.c2, ref) : mass(up(z[v])))); };
-  if (!kWhole || (low && g != 0.f)) {
+  auto one = [&](long long v) {
+    put(d + v, f == 0.f ? 0.f : far ? static_cast<float>(f * ldexp(far_mass(up(z[v]), p.scale, p.c2, ref), -static_cast<int>(floorf(power)))) : f * mass(up(z[v])));
+  };
+  if (!kWhole || (far && f != 0.f)) {
     for (long long v = lo + t; v < hi; v += kThreads) one(v);
   } else {
     const int w0 = g0 == 0 && skip ? 1 : g0, w1 = (g1 == groups && ((skip + p.vocab) & 7)) ? g1 - 1 : g1;
     constexpr int U = sizeof(T) == 4 ? 2 : 4;
     for (int q = w0 + t; q < w1; q += kThreads * U) {
       Eight<T> e[U];
-      if (g != 0.f) {
+      if (f != 0.f) {
 #pragma unroll
         for (int u = 0; u < U; ++u)
           if (q + u * kThreads < w1) e[u].load(z + (8ll * (q + u * kThreads) - skip));
@@ -548,7 +628,7 @@ __global__ void __launch_bounds__(kThreads) bwd_kernel(BwdParams p) {
       for (int u = 0; u < U; ++u)
         if (q + u * kThreads < w1) {
           float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-          if (g != 0.f) {
+          if (f != 0.f) {
             e[u].get(x);
 #pragma unroll
             for (int i = 0; i < 8; ++i) x[i] = f * mass(x[i]);
@@ -681,7 +761,7 @@ extern "C" int rb_topk_distill_bwd(const void* z, long long ld, const long long*
   const double scale = inv_temp * kLog2e;
   float c2, c2_low;
   two_floats(scale, c2, c2_low);
-  const BwdParams p{z, ld, ids, coef, stats, g, dz, vocab, k, 1, c2, c2_low, static_cast<float>(inv_temp)};
+  const BwdParams p{z, ld, ids, coef, stats, g, dz, vocab, k, 1, c2, c2_low, static_cast<float>(inv_temp), scale};
   if (dtype == 0 && out_dtype == 0) return bwd_t<__nv_bfloat16, __nv_bfloat16>(p, rows, st);
   if (dtype == 1 && out_dtype == 1) return bwd_t<__half, __half>(p, rows, st);
   if (dtype == 2 && out_dtype == 2) return bwd_t<float, float>(p, rows, st);

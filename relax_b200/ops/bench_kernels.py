@@ -273,6 +273,67 @@ def bench_moe(args, pk):
     print(f"  grouped GEMMs + SwiGLU (3 launches)   {t:7.3f} ms {pk.flops(fl / t)} | loop of library GEMMs ({3 * E} launches) {tl:7.3f} ms")
 
 
+def bench_rows(args, pk):
+    """Rows moved by key: the way of routed rows to their experts and back (128 experts, top 8, width 2048), an embedding table and its
+    gradient.  Bytes are those of every row read or written once."""
+    from .. import ops
+
+    dev, T, k, E, H, V = "cuda", args.tokens, 8, 128, 2048, 151936
+    g = torch.Generator(device=dev).manual_seed(0)
+    idx = torch.rand(T, E, device=dev, generator=g).topk(k, -1).indices
+    x = torch.randn(T, H, device=dev, generator=g).bfloat16()
+    w = torch.rand(T, k, device=dev, generator=g)
+    rows = ops.expert_layout(idx, E)
+    y = ops.expert_dispatch(x, rows)
+    cap, row = y.shape[0], 2 * H
+    print(f"== routed rows, {T} tokens to {k} of {E} experts, width {H} ({cap} buffer rows)")
+    yl, wl, dy = y.detach().requires_grad_(), w.detach().requires_grad_(), torch.randn_like(x)
+    back = ops.expert_combine(yl, wl, rows)
+    for name, fn, nbytes in [("layout", lambda: ops.expert_layout(idx, E), 8 * T * k + 4 * (T * k + cap)),
+                             ("dispatch", lambda: ops.expert_dispatch(x, rows), (T + cap) * row),
+                             ("combine", lambda: ops.expert_combine(y, w, rows), (T * k + T) * row),
+                             ("combine bwd", lambda: torch.autograd.grad(back, (yl, wl), dy, retain_graph=True), (T + T * k + cap) * row)]:
+        t = _timeit(fn, args.iters, args.warmup)
+        print(f"  {name:12s} {t:7.3f} ms {pk.bytes(nbytes / t / 1e6)}")
+    table = torch.randn(V, 2 * H, device=dev, generator=g).bfloat16().requires_grad_()
+    tokens = (V ** torch.rand(T, device=dev, generator=g)).long().clamp_max(V - 1) * 7919 % V      # few tokens often, most of them rarely
+    out = ops.embedding(tokens, table)
+    dy = torch.randn_like(out)
+    print(f"== embedding, {T} tokens from {V} x {2 * H}")
+    t = _timeit(lambda: ops.embedding(tokens, table.detach()), args.iters, args.warmup)
+    print(f"  {'lookup':12s} {t:7.3f} ms {pk.bytes(2 * T * 4 * H / t / 1e6)}")
+    t = _timeit(lambda: torch.autograd.grad(out, table, dy, retain_graph=True), args.iters, args.warmup)
+    print(f"  {'gradient':12s} {t:7.3f} ms {pk.bytes((T + V) * 4 * H / t / 1e6)}")
+    table.main_grad = torch.zeros(V, 2 * H, device=dev)
+    out = ops.embedding(tokens, table)
+    t = _timeit(lambda: torch.autograd.backward(out, dy, retain_graph=True), args.iters, args.warmup)
+    print(f"  {'into fp32':12s} {t:7.3f} ms {pk.bytes((T + 4 * len(tokens.unique())) * 4 * H / t / 1e6)}")
+
+
+def bench_distill(args, pk):
+    """Divergence from a teacher's top 64 ids on whole rows of logits (vocabulary 151936), and from hidden states (width 4096)."""
+    from .. import ops
+
+    dev, V, K, H = "cuda", 151936, 64, 4096
+    g = torch.Generator(device=dev).manual_seed(0)
+    for T, dtype in ((min(2048, args.tokens), torch.bfloat16), (min(4096, args.tokens), torch.float32)):
+        z = torch.randn(T, V, device=dev, generator=g).to(dtype).requires_grad_()
+        ids = torch.randint(0, V, (T, K), device=dev, generator=g)
+        teacher = torch.log_softmax(torch.randn(T, K + 1, device=dev, generator=g), -1)[:, :K].contiguous()
+        loss, dy = ops.topk_distill(z, ids, teacher), torch.ones(T, device=dev)
+        print(f"== distillation from {K} ids, {T} rows of {V}, {dtype}")
+        t = _timeit(lambda: ops.topk_distill(z.detach(), ids, teacher), args.iters, args.warmup)
+        print(f"  {'forward':12s} {t:7.3f} ms {pk.bytes(z.numel() * z.element_size() / t / 1e6)}")
+        t = _timeit(lambda: torch.autograd.grad(loss, z, dy, retain_graph=True), args.iters, args.warmup)
+        print(f"  {'backward':12s} {t:7.3f} ms {pk.bytes(2 * z.numel() * z.element_size() / t / 1e6)}")
+        del z, loss
+    h = torch.randn(T, H, device=dev, generator=g).bfloat16().requires_grad_()
+    w = (torch.randn(V, H, device=dev, generator=g) * 0.02).bfloat16().requires_grad_()
+    w.main_grad = torch.zeros(V, H, device=dev)
+    t = _timeit(lambda: ops.fused_lm_head_topk_distill(h, w, ids, teacher).sum().backward(), args.iters, args.warmup)
+    print(f"  {'fused head, forward and backward':32s} {t:7.3f} ms {pk.flops(8 * T * V * H / t / 1e9)}")
+
+
 def bench_decode_step(args, pk):
     """One whole decode step of the rollout engine (all layers + LM head + sampling + device-side advance) as the
     engine runs it: a CUDA graph replayed back to back.  Reports ms per step against the bytes a step must read
@@ -331,7 +392,7 @@ def bench_decode_step(args, pk):
 
 
 SECTIONS = {"decode_step": bench_decode_step, "moe": bench_moe, "gemm": bench_gemm, "gemm_fp8": bench_gemm_fp8, "attention": bench_attention, "decode": bench_decode, "lm_head": bench_lm_head,
-            "elementwise": bench_elementwise, "train_step": bench_train_step}
+            "elementwise": bench_elementwise, "rows": bench_rows, "distill": bench_distill, "train_step": bench_train_step}
 
 
 def main():

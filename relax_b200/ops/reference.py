@@ -815,9 +815,9 @@ def embedding(tokens, weight, scale: float = 1.0, vocab_start: int = 0):
 
 
 def topk_distill(logits, ids, teacher_log_probs, kl_type, alpha, norm_mode, temperature, log_prob_min_clamp, return_log_probs):
-    z = logits.double() / temperature
-    away = (ids < 0) | (ids >= z.shape[1])
-    lp = (z - torch.logsumexp(z, -1, keepdim=True)).gather(1, torch.where(away, 0, ids))
+    away = (ids < 0) | (ids >= logits.shape[1])
+    z = (logits.double() / temperature).masked_fill(away.all(1, keepdim=True), 0.0)       # (a row without ids has nothing to compare)
+    lp = torch.log_softmax(z, -1).gather(1, torch.where(away, 0, ids))
     found = lp.masked_fill(away, float("-inf")).float()
     t = teacher_log_probs.double()
     if log_prob_min_clamp is not None:
@@ -828,18 +828,21 @@ def topk_distill(logits, ids, teacher_log_probs, kl_type, alpha, norm_mode, temp
         loss = (torch.exp(-r) - 1.0 + r).sum(-1)
     else:
         a = {"reverse_kl": 0.0, "forward_kl": 1.0}.get(kl_type, alpha)
-        gone = -1e30                                             # (finite: gradients of absent ids are zeros)
+        gone = -1e300                                            # (finite: gradients of absent ids are zeros)
         s, t = lp.masked_fill(away, gone), t.masked_fill(away, gone)
         keep = ~away
         if norm_mode == "norm":
-            s, t = torch.log_softmax(s, -1), torch.log_softmax(t, -1)
+            def shares(l):      # (of ids without any mass: there are none)
+                return torch.log_softmax(l, -1).masked_fill(((l == float("-inf")) | away).all(1, keepdim=True) & keep, float("nan"))
+
+            s, t = shares(s), shares(t)
         elif norm_mode == "tail":
             rest = lambda l: torch.log(-torch.expm1(torch.logsumexp(l, -1, keepdim=True).clamp(max=-1e-7)))      # noqa: E731
             s, t = torch.cat([s, rest(s)], -1), torch.cat([t, rest(t)], -1)
             keep = torch.cat([keep, torch.ones_like(keep[:, :1])], -1)
 
         def kl(p, q):      # sum exp(p) (p - q); an outcome without mass counts nothing
-            keep_p = keep & (p > float("-inf"))
+            keep_p = keep & (p != float("-inf"))      # (NaN stays)
             d = torch.where(keep_p, p, none) - torch.where(keep_p, q, none)
             return torch.where(keep_p, torch.where(keep_p, p, none).exp() * d, none).sum(-1)
 

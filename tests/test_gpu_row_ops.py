@@ -347,6 +347,83 @@ def test_distill_nan_between_masks(at):
     assert torch.isnan(loss[:2]).all() and torch.isnan(lp[:2]).all() and torch.isfinite(loss[2])
 
 
+@pytest.mark.parametrize("temperature", [0.3, 1.0, 5.03])
+@pytest.mark.parametrize("mask", [-1e5, -3e6, -1e9, -2e10, -1e30, -3.3e38])
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_distill_masks_of_any_value(dtype, mask, temperature):
+    """Masked tokens have no mass beside others, wherever they lie and however many follow one another; rows of nothing else are uniform."""
+    z, ids, t, w = _case(5, 20003, 12, dtype, 23)
+    z[0] = mask
+    z[1, 40:] = mask
+    z[2, ::2] = mask
+    z[3, :19000] = mask
+    ids[1] = torch.arange(4, 28, 2, device="cuda")
+    ids[3] += 100      # (masked ones among them)
+    ids.remainder_(20003)
+    for kl, norm in (("forward_kl", "trunc"), ("jsd", "tail")):
+        zl = z.detach().requires_grad_()
+        loss = ops.topk_distill(zl, ids, t, kl, norm_mode=norm, temperature=temperature, log_prob_min_clamp=-30.0)
+        (d,) = torch.autograd.grad(loss, zl, w)
+        want, d_want, _ = O.distill(z, ids, t, w, kl, 0.5, norm, temperature, -30.0)
+        # far rows: logits of one value, whose 64-bit exponents are alike but for 2^-53 of 1e10; others as in the tests above
+        assert torch.allclose(loss.double().cpu(), want, rtol=3e-5, atol=1e-5)
+        top = d_want.abs().amax(1, keepdim=True)
+        assert bool(((d.double().cpu() - d_want).abs() <= (2 * _half_step(d.dtype) + 1e-4) * d_want.abs() + 1e-6 * top + 1e-30).all())
+
+
+def test_distill_far_logits_are_told_apart():
+    """Rows whose logits lie around 1e7 (32-bit numbers one apart): the distribution is that of their differences."""
+    z, ids, t, w = _case(6, 5000, 8, "fp32", 24)
+    near = z.round()
+    for off in (1e7, -1.5e7):
+        want = ops.topk_distill(near, ids, t, "jsd", return_log_probs=True)
+        got = ops.topk_distill(near + off, ids, t, "jsd", return_log_probs=True)
+        assert all(torch.allclose(a, b, rtol=1e-5, atol=1e-6) for a, b in zip(got, want))
+        grads = [torch.autograd.grad(ops.topk_distill(x, ids, t, "jsd"), x, w)[0] for x in (near.clone().requires_grad_(), (near + off).requires_grad_())]
+        assert torch.allclose(*grads, rtol=2e-5, atol=1e-9)
+
+
+@pytest.mark.parametrize("kl", ["reverse_kl", "forward_kl", "jsd"])
+def test_distill_renormalised_ids_far_behind(kl):
+    """Ids whose mass is nothing to 64 bits beside the rest of the row still have their shares of one another's."""
+    z, ids, t, w = _case(4, 700, 6, "fp32", 25)
+    z.scatter_add_(1, ids, torch.full_like(t, -900.0))
+    got = []
+    for x, i, tt, ww in ((z, ids, t, w), (z.cpu().double(), ids.cpu(), t.cpu(), w.cpu())):      # (the CPU's log-softmax is in 64 bits)
+        zl = x.detach().requires_grad_()
+        loss = ops.topk_distill(zl, i, tt, kl, norm_mode="norm")
+        got.append((loss.detach().cpu(), torch.autograd.grad(loss, zl, ww)[0].cpu().double()))
+    # logits of 900 are off by 900 * 2^-24 in 32 bits, but the CPU reads the same ones: what is left are roundings of the results
+    assert torch.allclose(got[0][0], got[1][0], rtol=1e-6, atol=1e-9)
+    assert torch.allclose(got[0][1], got[1][1], rtol=1e-6, atol=1e-9)
+
+
+@pytest.mark.parametrize("kl", ["reverse_kl", "forward_kl", "jsd"])
+def test_distill_shares_of_nothing(kl):
+    z, ids, t, _ = _case(4, 50, 3, "fp32", 27)
+    z[:2].scatter_(1, ids[:2], -math.inf)
+    ids[1, 1:] = -1
+    ids[2, 1:] = 70
+    t[2] = -math.inf
+    assert torch.isnan(ops.topk_distill(z, ids, t, kl, norm_mode="norm")).tolist() == [True, True, True, False]
+
+
+def test_distill_rows_without_ids():
+    """Nothing to compare: no loss and no gradient, whatever the row holds."""
+    z, ids, t, w = _case(5, 1200, 6, "fp32", 26)
+    ids[:4] = -1
+    ids[3] = 1200
+    z[0], z[1, 5], z[2] = -math.inf, math.nan, torch.finfo(torch.float32).min
+    for norm in ("tail", "norm", "trunc"):
+        for x, i, tt, ww in ((z, ids, t, w), (z.cpu(), ids.cpu(), t.cpu(), w.cpu())):
+            zl = x.detach().requires_grad_()
+            loss, lp = ops.topk_distill(zl, i, tt, "jsd", norm_mode=norm, return_log_probs=True)
+            (d,) = torch.autograd.grad(loss, zl, ww)
+            assert bool((loss[:4] == 0).all()) and bool((d[:4] == 0).all()) and bool((lp[:4] == -math.inf).all()) and float(loss[4]) > 0
+    loss = ops.topk_distill(z, ids[:, :0], t[:, :0])
+    assert bool((loss == 0).all())
+
+
 @pytest.mark.parametrize("kl", ["reverse_kl", "forward_kl", "jsd"])
 def test_distill_a_single_renormalised_id(kl):
     """All mass is the one id's on both sides: exactly nothing to learn, wherever the other entries stand and however the id is clamped."""

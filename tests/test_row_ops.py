@@ -242,3 +242,33 @@ def test_distill_temperatures():
     for bad in (0.0, -1.0, math.inf, math.nan, 1e-21):
         with pytest.raises(ValueError, match="temperature"):
             ops.topk_distill(z, ids, t, temperature=bad)
+
+
+@pytest.mark.parametrize("norm", ["tail", "norm", "trunc"])
+@pytest.mark.parametrize("kl", ["reverse_kl", "forward_kl", "jsd", "low_var_kl"])
+def test_distill_keeps_nan(kl, norm):
+    """A row without a distribution (all masked, or a NaN among its logits) has no divergence."""
+    z, ids, t, _ = _rows(4, 50, 4, 2, absent=False)
+    z[1] = -math.inf
+    z[2, 7] = math.nan
+    loss = ops.topk_distill(z, ids, t, kl, norm_mode=norm)
+    assert torch.isnan(loss).tolist() == [False, True, True, False]
+
+
+@pytest.mark.parametrize("kl", ["reverse_kl", "forward_kl", "jsd"])
+def test_distill_shares_of_nothing(kl):
+    """Renormalising ids without any mass gives no shares, whether absent ids stand beside them or not."""
+    z, ids, t, _ = _rows(4, 50, 3, 2, absent=False)
+    z[:2].scatter_(1, ids[:2], -math.inf)
+    ids[1, 1:] = -1
+    ids[2, 1:] = 70
+    t[2] = -math.inf
+    loss = ops.topk_distill(z, ids, t, kl, norm_mode="norm")
+    assert torch.isnan(loss).tolist() == [True, True, True, False]
+    z = torch.full((1, 9), torch.finfo(torch.float32).min)       # ids far below absent ones share their mass all the same
+    z[0, 8] = 0.0
+    ids = torch.tensor([[3, -1, 5]])
+    t = torch.tensor([[0.25, 0.5, 0.75]]).log()
+    want = {"reverse_kl": 0.5 * math.log(0.5 / 0.25) + 0.5 * math.log(0.5 / 0.75), "forward_kl": 0.25 * math.log(0.5) + 0.75 * math.log(1.5)}
+    if kl in want:
+        assert float(ops.topk_distill(z, ids, t, kl, norm_mode="norm")) == pytest.approx(want[kl], rel=1e-6)
