@@ -13,8 +13,9 @@
 // where there are few of them) and a small one with the 64-bit arithmetic, which would cost the first its occupancy.
 // Arithmetic: 32-bit exponentials (the instruction is off by 1.5e-7 at most, 5e-8 on average), 64 of them added in 32 bits, the rest of
 // the sum and everything about the ids in 64.
-// Measured (copy: 6.47 TB/s): 2048 rows of 151936 in bf16 125 us forward, where memory (96 us) and the exponentials (69 us) meet, and
-// 177 us backward (193 us of a copy); 4096 rows in fp32 367 us (385) and 736 us (770); the ids 8 to 22 us.
+// Measured (copy: 6.47 TB/s): 2048 rows of 151936 in bf16 124 us forward, where memory (96 us) and the exponentials (69 us) meet, and
+// 174 us backward (193 us of a copy); 4096 rows in fp32 369 us (385) and 733 us (770); the ids 10 to 24 us.  A polynomial on the multiply-add
+// pipe for a quarter of the exponentials made the first 6 us slower: instructions are no less scarce.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
