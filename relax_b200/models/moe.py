@@ -4,9 +4,10 @@ Softmax router in fp32, top-k, token permutation, all-to-all dispatch to the
 ranks that own the experts, grouped SwiGLU expert GEMMs, all-to-all combine and
 weighted un-permutation - the pipeline the reference configures through
 Megatron (scripts/models/qwen3-30B-A3B.sh:40-50: alltoall dispatcher, grouped
-GEMM, permute fusion).  This file is the unfused statement over
-``torch.distributed``; on CUDA the dispatch+permute+grouped-GEMM and
-GEMM+unpermute+combine pairs are fused kernels (:mod:`relax_b200.ops.fused_comm`).
+GEMM, permute fusion).  Rows go to their experts and back through
+:func:`relax_b200.ops.expert_layout` / ``expert_dispatch`` / ``expert_combine``;
+ranks exchange them over ``torch.distributed`` or, on CUDA, by peer stores
+(:mod:`relax_b200.parallel.ep_peer`).
 
 Routing replay (relax/utils/training/routing_replay.py:17-106): when a
 :class:`RoutingReplay` is active the top-k indices recorded by an earlier
