@@ -55,6 +55,16 @@ def _run(cmd: list, log_path: str | None = None):
     return p.stdout
 
 
+def _shared_libstdcxx(cxx: str) -> list:
+    """The shared C++ runtime by its path.  A compiler that has only the archive would link a second runtime into the extension, whose
+    streams then meet the facets of the first: numbers in a refusal's message ended the process."""
+    for name in ("libstdc++.so", "libstdc++.so.6"):
+        path = _run([cxx, f"-print-file-name={name}"]).strip()
+        if os.path.isabs(path) and os.path.exists(path):
+            return [path]
+    return []
+
+
 def ensure_serving(verbose: bool = False) -> str:
     """The extension a serving process needs: the full one when it is there and newer than the sources, else the serving
     subset (built if missing or stale).  Concurrent callers take turns."""
@@ -106,10 +116,10 @@ def build_extension(verbose: bool = False, force: bool = False, serving: bool = 
             print(f"[relax_b200.build] compiling {len(jobs)} translation unit(s) for sm_100a", flush=True)
         with ThreadPoolExecutor(max_workers=min(8, len(jobs))) as ex:
             list(ex.map(lambda j: _run(*j), sorted(jobs, key=lambda j: -os.path.getsize(j[0][j[0].index("-c") + 1]))))
-    if jobs or force or _stale(so_path, objs):
+    if jobs or force or _stale(so_path, objs + [os.path.abspath(__file__)]):
         tlib = os.path.join(os.path.dirname(torch.__file__), "lib")
         cuda_lib = os.path.join(os.environ.get("CUDA_HOME", "/usr/local/cuda"), "lib64")
-        cmd = [cxx, "-shared", "-o", so_path] + objs + [
+        cmd = [cxx, "-shared", "-o", so_path] + objs + _shared_libstdcxx(cxx) + [
             f"-L{tlib}", "-lc10", "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10_cuda", "-ltorch_cuda",
             f"-L{cuda_lib}", "-lcudart", f"-Wl,-rpath,{tlib}", f"-Wl,-rpath,{cuda_lib}",
         ]

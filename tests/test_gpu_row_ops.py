@@ -408,6 +408,45 @@ def test_distill_shares_of_nothing(kl):
     assert torch.isnan(ops.topk_distill(z, ids, t, kl, norm_mode="norm")).tolist() == [True, True, True, False]
 
 
+def test_refusals_name_numbers():
+    """The extension's own checks, for callers that come without the package's."""
+    from relax_b200.ops import cuda as C
+
+    m, ids = C._load(), torch.zeros(3, 2, dtype=torch.int64, device="cuda")
+    for bad, text in (((0, 1), "got 0"), ((2049, 1), "got 2049"), ((3, 0), "got 0"), ((3, 65537), "got 65537")):
+        with pytest.raises(ValueError, match=text):
+            m.expert_layout(ids, *bad)
+    wide = torch.zeros(3, 1025, dtype=torch.int64, device="cuda")
+    with pytest.raises(ValueError, match="got 1025"):
+        m.topk_distill(torch.zeros(3, 8, device="cuda"), wide, wide.float(), 0, 0, 0.5, -math.inf, 1.0, False)
+    with pytest.raises(RuntimeError, match="code -1"):
+        m.topk_distill(torch.zeros(3, 8, device="cuda"), ids, ids.float(), 9, 0, 0.5, -math.inf, 1.0, False)
+
+
+@pytest.mark.parametrize("V", [(1 << 20) + 5, (1 << 23) - 1, 1 << 24])
+def test_distill_vocabularies_of_any_size(V):
+    """Parts of a row are as long as a bitmap in shared memory has room for."""
+    z, ids, t, w = _case(1, 1000, 5, "bf16", 28)
+    big = torch.full((1, V), -8.0, device="cuda", dtype=torch.bfloat16)
+    big[:, -1000:] = z
+    ids += V - 1000
+    zl = big.requires_grad_()
+    loss, lp = ops.topk_distill(zl, ids, t, "jsd", return_log_probs=True)
+    (d,) = torch.autograd.grad(loss, zl, w)
+    lse = torch.logaddexp(torch.logsumexp(z.double(), 1), torch.tensor(math.log(V - 1000.0) - 8.0, device="cuda", dtype=torch.float64))
+    want = z.double().gather(1, ids - (V - 1000)) - lse[:, None]
+    assert torch.allclose(lp.double(), want, rtol=1e-6, atol=2e-6)
+    p, q = torch.cat([want.exp(), 1 - want.exp().sum(1, keepdim=True)], 1), torch.cat([t.double().exp(), 1 - t.double().exp().sum(1, keepdim=True)], 1)
+    m = (p + q) / 2
+    assert torch.allclose(loss.double(), ((p * (p / m).log() + q * (q / m).log()) / 2).sum(1), rtol=2e-5, atol=1e-7)
+    slope = ((p / m).log() / 2)
+    c = p[:, :5] * (slope[:, :5] - slope[:, 5:])
+    assert torch.allclose(d[0, 0].double(), (-w[0] * c.sum() * math.exp(-8.0 - float(lse))).double(), rtol=1e-2)
+    assert torch.equal(d[0, : V - 1000], d[0, 0].expand(V - 1000))
+    with pytest.raises(ValueError, match="2.24"):
+        ops.topk_distill(torch.empty(1, (1 << 24) + 1, device="cuda", dtype=torch.bfloat16), ids, t)
+
+
 def test_distill_rows_without_ids():
     """Nothing to compare: no loss and no gradient, whatever the row holds."""
     z, ids, t, w = _case(5, 1200, 6, "fp32", 26)

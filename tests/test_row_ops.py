@@ -272,3 +272,16 @@ def test_distill_shares_of_nothing(kl):
     want = {"reverse_kl": 0.5 * math.log(0.5 / 0.25) + 0.5 * math.log(0.5 / 0.75), "forward_kl": 0.25 * math.log(0.5) + 0.75 * math.log(1.5)}
     if kl in want:
         assert float(ops.topk_distill(z, ids, t, kl, norm_mode="norm")) == pytest.approx(want[kl], rel=1e-6)
+
+
+def test_extension_uses_the_process_s_cxx_runtime():
+    """Two C++ runtimes in one process: a refusal that names a number would end it."""
+    import shutil
+    import subprocess
+
+    from relax_b200.ops.build import build_extension
+
+    if not (shutil.which("readelf") and (shutil.which("nvcc") or shutil.which("/usr/local/cuda/bin/nvcc"))):
+        pytest.skip("readelf and nvcc")
+    found = subprocess.run(["readelf", "-d", build_extension()], capture_output=True, text=True, check=True).stdout
+    assert "[libstdc++.so" in found
