@@ -31,8 +31,8 @@
 namespace rb {
 namespace distill {
 
-constexpr int kThreads = 256, kWarps = kThreads / 32;
-constexpr int kMaxIds = 1024;      // eight per thread of id_kernel
+constexpr int kThreads = 256, kFewThreads = 64;      // of a block that streams a row or a part of it; of one with a short row
+constexpr int kMaxIds = 1024, kMine = kMaxIds / kThreads;      // ids of a row; of a thread of a streaming block
 constexpr int kMaxVocab = 1 << 24;
 constexpr int kMaxParts = 32;      // blocks of a row
 constexpr int kStats = 4;      // per row: log2 reference, 1 / sum, sum of the slopes, power of two of a far row's sum and a half (or 0)
@@ -261,12 +261,12 @@ __device__ __forceinline__ Term term_of(int kl, double a, double p, double q, do
 
 // Sums over the vocabulary, `parts` blocks per row.  The row counts from the last address in front of it that is a multiple of eight
 // elements, so that all but its first and last group of eight are whole; groups are shared out to the blocks in runs.
-template <typename T>
-__global__ void __launch_bounds__(kThreads, 4) sum_kernel(Params p) {
+template <typename T, int kBlock>
+__global__ void __launch_bounds__(kBlock, 1024 / kBlock) sum_kernel(Params p) {
   const long long row = blockIdx.x / p.parts;
   const int part = static_cast<int>(blockIdx.x - row * p.parts), t = threadIdx.x;
   extern __shared__ unsigned marks[];      // a bit per element of this block's groups
-  __shared__ Sum warp_sum[kWarps];
+  __shared__ Sum warp_sum[kBlock / 32];
   const T* z = static_cast<const T*>(p.z) + row * p.ld;
   const int skip = static_cast<int>((reinterpret_cast<uintptr_t>(z) / sizeof(T)) & 7);      // elements in front of the row in its first group
   const T* origin = z - skip;
@@ -274,16 +274,15 @@ __global__ void __launch_bounds__(kThreads, 4) sum_kernel(Params p) {
   const int g0 = min(groups, part * each), g1 = min(groups, g0 + each);
   const int w0 = g0 == 0 && skip ? 1 : g0, w1 = (g1 == groups && ((skip + p.vocab) & 7)) ? g1 - 1 : g1;      // whole groups
 
-  for (int i = t; i < (each + 3) / 4; i += kThreads) marks[i] = 0;
+  for (int i = t; i < (each + 3) / 4; i += kBlock) marks[i] = 0;
   __syncthreads();
   // logits of this part's ids, for the kernel behind this one: fetched here, where other blocks keep the memory busy meanwhile (K
   // scattered reads per row by themselves took 116 us for 4096 rows of 128), and put down at the end
-  constexpr int kMine = kMaxIds / kThreads;
   float at_id[kMine];
   unsigned here = 0;
 #pragma unroll
   for (int j = 0; j < kMine; ++j) {
-    const int i = t + j * kThreads;
+    const int i = t + j * kBlock;
     if (i >= p.k) break;
     const long long v = p.ids[row * p.k + i], b = v + skip - 8ll * g0;
     if (v >= 0 && v < p.vocab && b >= 0 && b < 8ll * (g1 - g0)) {
@@ -306,12 +305,12 @@ __global__ void __launch_bounds__(kThreads, 4) sum_kernel(Params p) {
     float big = -INFINITY;
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (kAll || g + u * kThreads < w1) e[u].load(origin + 8ll * (g + u * kThreads));
+      if (kAll || g + u * kBlock < w1) e[u].load(origin + 8ll * (g + u * kBlock));
 #pragma unroll
-    for (int u = 0; u < U; ++u) m[u] = kAll || g + u * kThreads < w1 ? mark[g + u * kThreads - g0] : 0;
+    for (int u = 0; u < U; ++u) m[u] = kAll || g + u * kBlock < w1 ? mark[g + u * kBlock - g0] : 0;
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (kAll || g + u * kThreads < w1) big = max_nan(big, e[u].max());
+      if (kAll || g + u * kBlock < w1) big = max_nan(big, e[u].max());
     big = whole_ref(big, p.c2);
     if (fabsf(big) > kFar) {      // nothing there (-inf), or for the loop behind this one
       far |= big > 0.f ? 2u : big != -INFINITY;
@@ -326,7 +325,7 @@ __global__ void __launch_bounds__(kThreads, 4) sum_kernel(Params p) {
     float2 add = make_float2(0.f, 0.f);
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (kAll || g + u * kThreads < w1) {
+      if (kAll || g + u * kBlock < w1) {
         float f[8];
         e[u].get(f);
 #pragma unroll
@@ -343,22 +342,22 @@ __global__ void __launch_bounds__(kThreads, 4) sum_kernel(Params p) {
     s.sum += static_cast<double>(add.x + add.y);
   };
   int g = w0 + t;
-  for (; g + (U - 1) * kThreads < w1; g += U * kThreads) step(g, std::true_type{});
+  for (; g + (U - 1) * kBlock < w1; g += U * kBlock) step(g, std::true_type{});
   if (g < w1) step(g, std::false_type{});
   // steps whose largest logit is far away, once more; those far below are nothing where some other logit is not
   if (__syncthreads_or(s.ref > 4096.f - kFar)) far &= 2;
   if (far) {
 #pragma unroll 1
-    for (g = w0 + t; g < w1; g += U * kThreads) {
+    for (g = w0 + t; g < w1; g += U * kBlock) {
       float big = -INFINITY;
 #pragma unroll 1
-      for (int q = g; q < w1 && q < g + U * kThreads; q += kThreads)
+      for (int q = g; q < w1 && q < g + U * kBlock; q += kBlock)
         for (int i = 0; i < 8; ++i) big = max_nan(big, up(origin[8ll * q + i]));
       big = whole_ref(big, p.c2);
       if (!(fabsf(big) > kFar) || big == -INFINITY || (far == 2 && big < 0.f)) continue;
       Sum some{big, 0.0};
 #pragma unroll 1
-      for (int q = g; q < w1 && q < g + U * kThreads; q += kThreads)
+      for (int q = g; q < w1 && q < g + U * kBlock; q += kBlock)
         for (int i = 0; i < 8; ++i)
           if (!((mark[q - g0] >> i) & 1)) some.sum += far_mass(up(origin[8ll * q + i]), p.scale, p.c2, big);
       s.add(some.ref, some.sum);
@@ -384,12 +383,12 @@ __global__ void __launch_bounds__(kThreads, 4) sum_kernel(Params p) {
   if (t == 0) {
     Sum b = warp_sum[0];
 #pragma unroll
-    for (int w = 1; w < kWarps; ++w) b.add(warp_sum[w].ref, warp_sum[w].sum);
+    for (int w = 1; w < kBlock / 32; ++w) b.add(warp_sum[w].ref, warp_sum[w].sum);
     p.sums[blockIdx.x] = make_double2(b.ref, b.sum);
   }
 #pragma unroll
   for (int j = 0; j < kMine; ++j)
-    if ((here >> j) & 1) p.coef[row * p.k + t + j * kThreads] = at_id[j];
+    if ((here >> j) & 1) p.coef[row * p.k + t + j * kBlock] = at_id[j];
 }
 
 // every bit of an id in every bit of its slot: ids at even distances would fill one stretch of the table otherwise
@@ -594,8 +593,8 @@ struct BwdParams {
 };
 
 // A block per part of a row: -g / T (sum c) P over its elements, then the K ids of that part in place of what stands there.
-template <typename T, typename O, bool kWhole>
-__global__ void __launch_bounds__(kThreads) bwd_kernel(BwdParams p) {
+template <typename T, typename O, bool kWhole, int kBlock>
+__global__ void __launch_bounds__(kBlock) bwd_kernel(BwdParams p) {
   const long long row = blockIdx.x / p.parts;
   const int part = static_cast<int>(blockIdx.x - row * p.parts), t = threadIdx.x;
   const T* z = static_cast<const T*>(p.z) + row * p.ld;
@@ -614,27 +613,27 @@ __global__ void __launch_bounds__(kThreads) bwd_kernel(BwdParams p) {
     put(d + v, f == 0.f ? 0.f : far ? static_cast<float>(f * ldexp(far_mass(up(z[v]), p.scale, p.c2, ref), -static_cast<int>(floorf(power)))) : f * mass(up(z[v])));
   };
   if (!kWhole || (far && f != 0.f)) {
-    for (long long v = lo + t; v < hi; v += kThreads) one(v);
+    for (long long v = lo + t; v < hi; v += kBlock) one(v);
   } else {
     const int w0 = g0 == 0 && skip ? 1 : g0, w1 = (g1 == groups && ((skip + p.vocab) & 7)) ? g1 - 1 : g1;
     constexpr int U = sizeof(T) == 4 ? 2 : 4;
-    for (int q = w0 + t; q < w1; q += kThreads * U) {
+    for (int q = w0 + t; q < w1; q += kBlock * U) {
       Eight<T> e[U];
       if (f != 0.f) {
 #pragma unroll
         for (int u = 0; u < U; ++u)
-          if (q + u * kThreads < w1) e[u].load(z + (8ll * (q + u * kThreads) - skip));
+          if (q + u * kBlock < w1) e[u].load(z + (8ll * (q + u * kBlock) - skip));
       }
 #pragma unroll
       for (int u = 0; u < U; ++u)
-        if (q + u * kThreads < w1) {
+        if (q + u * kBlock < w1) {
           float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
           if (f != 0.f) {
             e[u].get(x);
 #pragma unroll
             for (int i = 0; i < 8; ++i) x[i] = f * mass(x[i]);
           }
-          Eight<O>::store(d + (8ll * (q + u * kThreads) - skip), x);
+          Eight<O>::store(d + (8ll * (q + u * kBlock) - skip), x);
         }
     }
     if (t < 16) {
@@ -646,7 +645,7 @@ __global__ void __launch_bounds__(kThreads) bwd_kernel(BwdParams p) {
   }
   if (g == 0.f) return;
   __syncthreads();
-  for (int i = t; i < p.k; i += kThreads) {
+  for (int i = t; i < p.k; i += kBlock) {
     const long long v = p.ids[row * p.k + i];
     if (v >= lo && v < hi) put(d + v, g * p.coef[row * p.k + i]);
   }
@@ -672,19 +671,26 @@ inline void two_floats(double scale, float& c2, float& c2_low) {
   c2_low = fmaxf(static_cast<float>(scale - c2), FLT_MIN);
 }
 
-template <typename T>
+template <typename T, int kBlock>
 int sums_t(const Params& p, long long rows, cudaStream_t st) {
   const int each = ((p.vocab + 14) / 8 + p.parts - 1) / p.parts + 1;
   const size_t smem = (each + 3) / 4 * 4 + 16;
   constexpr size_t kMostSmem = 200 * 1024;      // (always the same limit: calls of several threads would lower one another's)
   if (smem > kMostSmem) return -4;
   if (smem > 40 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(sum_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kMostSmem));
+    const cudaError_t e = cudaFuncSetAttribute(sum_kernel<T, kBlock>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kMostSmem));
     if (e != cudaSuccess) return static_cast<int>(e);
   }
-  sum_kernel<T><<<static_cast<unsigned>(rows * p.parts), kThreads, smem, st>>>(p);
+  sum_kernel<T, kBlock><<<static_cast<unsigned>(rows * p.parts), kBlock, smem, st>>>(p);
   rb_note_launch(1);
   return static_cast<int>(cudaGetLastError());
+}
+// Many short rows: small blocks, so that more rows are under way and wait for their ids and their sums side by side (8192 rows of 4096 in
+// bf16, ids included: 50 us against 91 with large blocks; of 12000: 81 against 108; of 32000: 134 against 149, but 204 against 189 in fp32).
+template <typename T>
+int sums_of(const Params& p, long long rows, cudaStream_t st) {
+  if (p.vocab <= 16384 && rows >= 8ll * num_sms() && p.parts == 1 && p.k <= kMine * kFewThreads) return sums_t<T, kFewThreads>(p, rows, st);
+  return sums_t<T, kThreads>(p, rows, st);
 }
 
 template <typename T, typename O>
@@ -698,8 +704,11 @@ int bwd_t(BwdParams p, long long rows, cudaStream_t st) {
   const uintptr_t a = reinterpret_cast<uintptr_t>(p.z) / sizeof(T), b = reinterpret_cast<uintptr_t>(p.dz) / sizeof(O);
   const bool whole = (a - b) % 8 == 0 && (rows == 1 || (p.ld - p.vocab) % 8 == 0);
   const int grid = static_cast<int>(rows * p.parts);
-  if (whole) bwd_kernel<T, O, true><<<grid, kThreads, 0, st>>>(p);
-  else bwd_kernel<T, O, false><<<grid, kThreads, 0, st>>>(p);
+  // many short rows: small blocks (8192 rows of 1024 in bf16 19 us against 33, of 4096 31 against 41, in fp32 53 both; of 12000 fp32 152 against 130)
+  const bool few = p.vocab <= 4096 && rows >= 8ll * num_sms();
+  if (whole && few) bwd_kernel<T, O, true, kFewThreads><<<grid, kFewThreads, 0, st>>>(p);
+  else if (whole) bwd_kernel<T, O, true, kThreads><<<grid, kThreads, 0, st>>>(p);
+  else bwd_kernel<T, O, false, kThreads><<<grid, kThreads, 0, st>>>(p);
   rb_note_launch(1);
   return static_cast<int>(cudaGetLastError());
 }
@@ -730,12 +739,13 @@ extern "C" int rb_topk_distill(const void* z, long long ld, const long long* ids
   const Params p{z, ld, ids, teacher, loss, coef, stats, log_probs, sums, vocab, k, kl, norm, parts, c2, c2_low, scale, alpha, clamp};
   int rc = -1;
   switch (dtype) {
-    case 0: rc = sums_t<__nv_bfloat16>(p, rows, st); break;
-    case 1: rc = sums_t<__half>(p, rows, st); break;
-    case 2: rc = sums_t<float>(p, rows, st); break;
+    case 0: rc = sums_of<__nv_bfloat16>(p, rows, st); break;
+    case 1: rc = sums_of<__half>(p, rows, st); break;
+    case 2: rc = sums_of<float>(p, rows, st); break;
   }
   if (rc) return rc;
-  // many rows: a warp each, which spends the fewest instructions; few: a thread per id, for the shortest way
+  // many rows: a warp each, which spends the fewest instructions (8192 rows of 4096 and 128 ids, streaming included: 112 us, a thread per id
+  // 157); few: a thread per id, for the shortest way (the same time up to 64 ids)
   int threads = rows >= 8ll * num_sms() ? 32 : (k + 31) / 32 * 32, slots = 32;
   threads = threads < 32 ? 32 : threads > kIdThreads ? kIdThreads : threads;
   while (slots < 2 * k) slots *= 2;

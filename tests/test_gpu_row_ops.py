@@ -447,6 +447,26 @@ def test_distill_vocabularies_of_any_size(V):
         ops.topk_distill(torch.empty(1, (1 << 24) + 1, device="cuda", dtype=torch.bfloat16), ids, t)
 
 
+@pytest.mark.parametrize("R,V,K", [(1300, 515, 20), (1184, 1024, 256), (1184, 1024, 257), (1190, 4099, 8), (1200, 33, 33)])
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_distill_many_short_rows(R, V, K, dtype):
+    """Blocks of fewer threads: rows of every alignment, up to the most ids that such a block takes and beyond."""
+    z, ids, t, w = _case(R, V, K, dtype, 29)
+    z[7, 1:] = -1e30
+    z[8, :] = -1e9
+    zl = z.detach().requires_grad_()
+    loss, lp = ops.topk_distill(zl, ids, t, "jsd", return_log_probs=True)
+    (d,) = torch.autograd.grad(loss, zl, w)
+    some = torch.cat([torch.arange(20), torch.arange(R - 4, R)])
+    zl = z[some.cuda()].clone().requires_grad_()      # the same rows, few of them: in blocks of more threads
+    loss2, lp2 = ops.topk_distill(zl, ids[some.cuda()], t[some.cuda()], "jsd", return_log_probs=True)
+    (d2,) = torch.autograd.grad(loss2, zl, w[some.cuda()])
+    assert torch.allclose(loss[some.cuda()], loss2, rtol=1e-5, atol=1e-6) and torch.allclose(lp[some.cuda()], lp2, rtol=1e-6, atol=2e-6)
+    assert torch.allclose(d[some.cuda()].float(), d2.float(), rtol=2 * _half_step(d.dtype) + 2e-5, atol=1e-8)
+    plain = some[(some != 7) & (some != 8)].cuda()      # (which are those of the statement)
+    _check(z[plain], ids[plain], t[plain], w[plain], kl="jsd")
+
+
 def test_distill_rows_without_ids():
     """Nothing to compare: no loss and no gradient, whatever the row holds."""
     z, ids, t, w = _case(5, 1200, 6, "fp32", 26)
