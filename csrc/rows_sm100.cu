@@ -460,6 +460,12 @@ struct TokenRow {      // row r <- table row of its token
 };
 
 template <int N> constexpr int kMove = N == 1 ? 8 : 4;      // vectors of a lane in flight
+// A vector that leaves the L2 first: what is read again and again (a token's row by its experts) stays there meanwhile.
+template <typename T, int N>
+__device__ __forceinline__ void put_away(Pack<T, N>* o, const Pack<T, N>& p) {
+  if constexpr (sizeof(p) == 16) __stcs(reinterpret_cast<uint4*>(o), *reinterpret_cast<const uint4*>(&p));
+  else *o = p;
+}
 // out[r] = scale * in[row(r)], zeros where there is no such row; a warp takes 32 x kMove vectors of a row
 template <typename T, int N, bool kScale, typename Row>
 __global__ void __launch_bounds__(256) move_kernel(const T* __restrict__ in, long long ld, Row src, T* __restrict__ out, long long n, int cols, int parts,
@@ -490,7 +496,36 @@ __global__ void __launch_bounds__(256) move_kernel(const T* __restrict__ in, lon
       for (int i = 0; i < N; ++i) f[i] *= scale;
       p[u].set(f);
     }
-    o[v] = p[u];
+    put_away(o + v, p[u]);
+  }
+}
+
+// The same for rows that would leave many of those lanes idle: vectors of the output one after the other, over the ends of rows.
+template <typename T, int N, bool kScale, typename Row>
+__global__ void __launch_bounds__(256) move_flat_kernel(const T* __restrict__ in, long long ld, Row src, T* __restrict__ out, unsigned all, unsigned vecs,
+                                                        float scale) {
+  const unsigned q0 = (blockIdx.x * 8u + (threadIdx.x >> 5)) * (32 * kMove<N>) + (threadIdx.x & 31);
+  Pack<T, N> p[kMove<N>];
+#pragma unroll
+  for (int u = 0; u < kMove<N>; ++u) {
+    const unsigned q = q0 + u * 32, r = q / vecs;
+    p[u] = zeros<T, N>();
+    if (q >= all) break;
+    const long long s = src.row(r);
+    if (s >= 0) p[u] = reinterpret_cast<const Pack<T, N>*>(in + s * ld)[q - r * vecs];
+  }
+#pragma unroll
+  for (int u = 0; u < kMove<N>; ++u) {
+    const unsigned q = q0 + u * 32;
+    if (q >= all) break;
+    if constexpr (kScale) {
+      float f[N];
+      p[u].get(f);
+#pragma unroll
+      for (int i = 0; i < N; ++i) f[i] *= scale;
+      p[u].set(f);
+    }
+    put_away(reinterpret_cast<Pack<T, N>*>(out) + q, p[u]);
   }
 }
 
@@ -554,11 +589,14 @@ __global__ void __launch_bounds__(N == 1 ? kSingleThreads : 256) sum_bwd_kernel(
                                                       T* __restrict__ d_y, float* __restrict__ d_w, long long cap, long long n, int k, int cols) {
   const int t = threadIdx.x, lane = t & 31, w = t >> 5, warps = blockDim.x >> 5, vecs = cols / N;
   const long long row = blockIdx.x;
-  if (row >= n) {
-    const long long r = (row - n) * warps + w;
-    if (r >= cap || source[r] >= 0) return;
+  if (row >= n) {      // a warp looks at 32 rows far from one another: padding rows lie together
+    const long long units = (cap + 31) / 32, unit = (row - n) * warps + w, r = unit + lane * units;
+    unsigned empty = __ballot_sync(0xffffffffu, unit < units && r < cap && source[r < cap ? r : 0] < 0);
     const Pack<T, N> z = zeros<T, N>();
-    for (int v = lane; v < vecs; v += 32) reinterpret_cast<Pack<T, N>*>(d_y + r * cols)[v] = z;
+    for (; empty; empty &= empty - 1) {
+      Pack<T, N>* o = reinterpret_cast<Pack<T, N>*>(d_y + (unit + (__ffs(empty) - 1) * units) * cols);
+      for (int v = lane; v < vecs; v += 32) o[v] = z;
+    }
     return;
   }
   __shared__ float red[8][8];
@@ -837,7 +875,12 @@ int move_t(const void* in, long long ld, const Row& src, void* out, long long n,
   const T* a = static_cast<const T*>(in);
   T* o = static_cast<T*>(out);
   const int g = static_cast<int>(grid);
-  if (wide && scale == 1.f) move_kernel<T, NV, false><<<g, 256, 0, st>>>(a, ld, src, o, n, cols, parts, scale);
+  const long long vecs = cols / NV, all = n * vecs;
+  if (wide && parts * 128ll * 8 > vecs * 9 && all < 1ll << 31) {
+    const int blocks = static_cast<int>((all + 8 * 32 * kMove<NV> - 1) / (8 * 32 * kMove<NV>));
+    if (scale == 1.f) move_flat_kernel<T, NV, false><<<blocks, 256, 0, st>>>(a, ld, src, o, static_cast<unsigned>(all), static_cast<unsigned>(vecs), scale);
+    else move_flat_kernel<T, NV, true><<<blocks, 256, 0, st>>>(a, ld, src, o, static_cast<unsigned>(all), static_cast<unsigned>(vecs), scale);
+  } else if (wide && scale == 1.f) move_kernel<T, NV, false><<<g, 256, 0, st>>>(a, ld, src, o, n, cols, parts, scale);
   else if (wide) move_kernel<T, NV, true><<<g, 256, 0, st>>>(a, ld, src, o, n, cols, parts, scale);
   else if (scale == 1.f) move_kernel<T, 1, false><<<g, 256, 0, st>>>(a, ld, src, o, n, cols, parts, scale);
   else move_kernel<T, 1, true><<<g, 256, 0, st>>>(a, ld, src, o, n, cols, parts, scale);
@@ -884,7 +927,7 @@ int sum_bwd_t(const void* d_out, long long ld, const void* y, long long ldy, con
               long long cap, long long n, int k, int cols, cudaStream_t st) {
   const bool wide = wide_rows(d_out, ld, cols, sizeof(T)) && wide_rows(y, ldy, cols, sizeof(T)) && wide_rows(d_y, cols, cols, sizeof(T));
   const int threads = row_threads(cols / (wide ? 16 / static_cast<int>(sizeof(T)) : 1), !wide);
-  const long long warps = threads / 32, grid = n + (cap + warps - 1) / warps;
+  const long long warps = threads / 32, grid = n + ((cap + 31) / 32 + warps - 1) / warps;
   if (grid > kMaxGrid) return -3;
   const T *a = static_cast<const T*>(d_out), *b = static_cast<const T*>(y);
   T* o = static_cast<T*>(d_y);
