@@ -219,7 +219,8 @@ int rb_moe_gemm(const void* X, const void* W, void* out, const int* tiles, const
 int rb_sort_counters(long long n, int bins);
 int rb_expert_layout(const void* ids, int wide, int n, int experts, int align, int cap, int* dest, int* source, int* tile_expert, int* bounds, int* hist,
                      cudaStream_t st);
-int rb_expert_dispatch(const void* x, long long ld, const int* source, void* out, int cap, int k, int cols, int dtype, cudaStream_t st);
+int rb_expert_dispatch(const void* x, long long ld, const int* source, const int* dest, void* out, int cap, int n, int k, int cols, int dtype,
+                       cudaStream_t st);
 int rb_expert_combine(const void* y, long long ld, const int* dest, const float* weight, void* out, int n, int k, int cols, int dtype, int out_fp32,
                       cudaStream_t st);
 int rb_expert_combine_bwd(const void* d_out, long long ld, const void* y, long long ldy, const int* source, const int* dest, const float* weight, void* d_y,

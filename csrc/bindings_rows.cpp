@@ -95,13 +95,13 @@ py::tuple expert_layout(torch::Tensor ids, int64_t experts, int64_t align) {
                         part_of(all, at_bounds, {experts + 1}));
 }
 
-torch::Tensor scatter_rows(const torch::Tensor& in, const torch::Tensor& source, int64_t k, const char* what) {
+torch::Tensor scatter_rows(const torch::Tensor& in, const torch::Tensor& source, const torch::Tensor& dest, const char* what) {
   const c10::cuda::CUDAGuard guard(in.device());
   const auto x = dense(in, what);
   same_device(source, x, "expert_dispatch: the layout");
   auto out = at::empty({source.numel(), x.size(1)}, x.options());
-  check(rb_expert_dispatch(x.data_ptr(), x.stride(0), source.data_ptr<int>(), out.data_ptr(), as_int(source.numel(), what), as_int(k, what),
-                           as_int(x.size(1), what), code_of(x, what), cur_stream()),
+  check(rb_expert_dispatch(x.data_ptr(), x.stride(0), source.data_ptr<int>(), dest.data_ptr<int>(), out.data_ptr(), as_int(source.numel(), what),
+                           as_int(dest.size(0), what), as_int(dest.size(1), what), as_int(x.size(1), what), code_of(x, what), cur_stream()),
         "rb_expert_dispatch");
   return out;
 }
@@ -121,7 +121,7 @@ torch::Tensor gather_rows(const torch::Tensor& in, const torch::Tensor& dest, co
 struct Dispatch : Function<Dispatch> {
   static torch::Tensor forward(AutogradContext* ctx, const torch::Tensor& x, const torch::Tensor& dest, const torch::Tensor& source) {
     ctx->save_for_backward({dest});
-    return scatter_rows(x, source, dest.size(1), "expert_dispatch");
+    return scatter_rows(x, source, dest, "expert_dispatch");
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     const auto saved = ctx->get_saved_variables();
@@ -129,7 +129,7 @@ struct Dispatch : Function<Dispatch> {
   }
 };
 torch::Tensor expert_dispatch(const torch::Tensor& x, const torch::Tensor& dest, const torch::Tensor& source) {
-  return recorded(x) ? Dispatch::apply(x, dest, source) : scatter_rows(x, source, dest.size(1), "expert_dispatch");
+  return recorded(x) ? Dispatch::apply(x, dest, source) : scatter_rows(x, source, dest, "expert_dispatch");
 }
 
 struct Combine : Function<Combine> {
@@ -148,7 +148,7 @@ struct Combine : Function<Combine> {
     const c10::cuda::CUDAGuard guard(g[0].device());
     const auto d = dense(g[0].to(static_cast<at::ScalarType>(ctx->saved_data["type"].toInt())), "expert_combine");
     if (!w.defined())
-      return once({scatter_rows(d, source, dest.size(1), "expert_combine"), torch::Tensor(), torch::Tensor(), torch::Tensor(), torch::Tensor()}, g);
+      return once({scatter_rows(d, source, dest, "expert_combine"), torch::Tensor(), torch::Tensor(), torch::Tensor(), torch::Tensor()}, g);
     const auto y = dense(saved[0], "expert_combine");
     auto d_y = at::empty({y.size(0), y.size(1)}, y.options()), d_w = at::empty_like(w);
     check(rb_expert_combine_bwd(d.data_ptr(), d.stride(0), y.data_ptr(), y.stride(0), source.data_ptr<int>(), dest.data_ptr<int>(), w.data_ptr<float>(),

@@ -95,6 +95,19 @@ def test_dispatch_and_combine(T, k, E, H, dtype):
     _within(d_w.reshape(-1), want_w, (H / 32 + 8) * F * size_w, "d weights")      # a lane sums H / 32 terms, five more additions join the lanes
 
 
+@pytest.mark.parametrize("T,k,E,H,align,dtype", [(8193, 3, 40, 1552, 128, "bf16"), (6200, 33, 300, 2048, 4, "fp16"), (26000, 2, 7, 520, 1, "bf16"), (3000, 5, 64, 2100, 128, "fp32")])
+def test_dispatch_of_many_rows(T, k, E, H, align, dtype):
+    """Rows that are read once and put down at all their places: every row of the buffer is written, padding with zeros."""
+    g = _gen(31)
+    ids = torch.randint(-1, E + 1, (T, k), device="cuda", generator=g)      # (some live elsewhere, some come twice)
+    x = torch.randn(T, H + 8, device="cuda", generator=g).to(DT[dtype])[:, 8 * (k % 2): 8 * (k % 2) + H]
+    rows = ops.expert_layout(ids, E, align)
+    out = ops.expert_dispatch(x, rows)
+    s = rows.source.long()
+    want = torch.where((s >= 0)[:, None], x[torch.div(s.clamp_min(0), k, rounding_mode="floor")], torch.zeros((), device="cuda", dtype=DT[dtype]))
+    assert torch.equal(out, want)
+
+
 def test_rows_again_give_the_same_bits_and_may_be_captured():
     g = _gen(5)
     ids = torch.randint(0, 16, (700, 4), device="cuda", generator=g)
