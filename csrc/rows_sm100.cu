@@ -619,6 +619,9 @@ __global__ void __launch_bounds__(N == 1 ? kSingleThreads : 256) sum_kernel(cons
   }
 }
 
+// buffer rows that a warp looks at for padding: long ones take their time, short ones would be more warps than tokens
+__host__ __device__ inline int padding_rows(int vecs) { return vecs >= 128 ? 8 : 32; }
+
 // Backward of the weighted sum: d_y[dest] = w d_out[t] and d_w = <d_out[t], y[dest]>.  A block per token holds its row of d_out while
 // it walks over the token's rows of y, so that all of them pass once; blocks behind the tokens write the zeros of padding rows.
 template <typename T, int N>
@@ -627,9 +630,10 @@ __global__ void __launch_bounds__(N == 1 ? kSingleThreads : 256) sum_bwd_kernel(
                                                       T* __restrict__ d_y, float* __restrict__ d_w, long long cap, long long n, int k, int cols) {
   const int t = threadIdx.x, lane = t & 31, w = t >> 5, warps = blockDim.x >> 5, vecs = cols / N;
   const long long row = blockIdx.x;
-  if (row >= n) {      // a warp looks at 32 rows far from one another: padding rows lie together
-    const long long units = (cap + 31) / 32, unit = (row - n) * warps + w, r = unit + lane * units;
-    unsigned empty = __ballot_sync(0xffffffffu, unit < units && r < cap && source[r < cap ? r : 0] < 0);
+  if (row >= n) {      // a warp looks at some rows far from one another: padding rows lie together
+    const int some = padding_rows(vecs);
+    const long long units = (cap + some - 1) / some, unit = (row - n) * warps + w, r = unit + lane * units;
+    unsigned empty = __ballot_sync(0xffffffffu, lane < some && unit < units && r < cap && source[r < cap ? r : 0] < 0);
     const Pack<T, N> z = zeros<T, N>();
     for (; empty; empty &= empty - 1) {
       Pack<T, N>* o = reinterpret_cast<Pack<T, N>*>(d_y + (unit + (__ffs(empty) - 1) * units) * cols);
@@ -965,7 +969,8 @@ int sum_bwd_t(const void* d_out, long long ld, const void* y, long long ldy, con
               long long cap, long long n, int k, int cols, cudaStream_t st) {
   const bool wide = wide_rows(d_out, ld, cols, sizeof(T)) && wide_rows(y, ldy, cols, sizeof(T)) && wide_rows(d_y, cols, cols, sizeof(T));
   const int threads = row_threads(cols / (wide ? 16 / static_cast<int>(sizeof(T)) : 1), !wide);
-  const long long warps = threads / 32, grid = n + ((cap + 31) / 32 + warps - 1) / warps;
+  const long long warps = threads / 32, some = padding_rows(cols / (wide ? 16 / static_cast<int>(sizeof(T)) : 1)),
+                  grid = n + ((cap + some - 1) / some + warps - 1) / warps;
   if (grid > kMaxGrid) return -3;
   const T *a = static_cast<const T*>(d_out), *b = static_cast<const T*>(y);
   T* o = static_cast<T*>(d_y);
