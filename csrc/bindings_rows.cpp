@@ -228,7 +228,7 @@ torch::Tensor embedding(const torch::Tensor& weight, const torch::Tensor& tokens
 struct Distilled {
   torch::Tensor loss, kept, log_probs;      // kept: statistics [R, 4], sums of parts (a workspace), slopes of the ids [R, K]
 };
-inline int64_t slopes_at(const torch::Tensor& z) { return z.size(0) * (4 + 4 * rb_topk_distill_parts(z.size(0), static_cast<int>(z.size(1)))); }
+inline int64_t slopes_at(const torch::Tensor& z) { return z.size(0) * (4 + 4 * rb_topk_distill_parts(z.size(0), static_cast<int>(z.size(1)), static_cast<int>(z.element_size()))); }
 
 Distilled distill_rows(const torch::Tensor& z, const torch::Tensor& ids, const torch::Tensor& teacher, int64_t kl, int64_t norm, double alpha, double clamp,
                        double inv_temp, bool log_probs) {

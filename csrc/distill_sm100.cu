@@ -31,7 +31,7 @@
 namespace rb {
 namespace distill {
 
-constexpr int kThreads = 256, kFewThreads = 64;      // of a block that streams a row or a part of it; of one with a short row
+constexpr int kThreads = 256, kHalfThreads = 128, kFewThreads = 64;      // of a block that streams a row or a part of it; of smaller ones
 constexpr int kMaxIds = 1024, kMine = kMaxIds / kThreads;      // ids of a row; of a thread of a streaming block
 constexpr int kMaxVocab = 1 << 24;
 constexpr int kMaxParts = 32;      // blocks of a row
@@ -685,11 +685,17 @@ int sums_t(const Params& p, long long rows, cudaStream_t st) {
   rb_note_launch(1);
   return static_cast<int>(cudaGetLastError());
 }
+// Rows that take more than one wave of large blocks but one of blocks half their size: the second wave is mostly empty (777 rows of 32003 in
+// bf16, ids included: 30 us against 39 with large blocks; of 151936 68 against 72; fp32 38 against 41, but 106 against 100, of 65536 57 both).
+inline bool one_wave_of_halves(long long rows, int vocab, int size) {
+  return rows > 4ll * num_sms() && rows <= 8ll * num_sms() && vocab <= (size == 2 ? 200000 : 65536);      // (eight bitmaps fit shared memory)
+}
 // Many short rows: small blocks, so that more rows are under way and wait for their ids and their sums side by side (8192 rows of 4096 in
 // bf16, ids included: 50 us against 91 with large blocks; of 12000: 81 against 108; of 32000: 134 against 149, but 204 against 189 in fp32).
 template <typename T>
 int sums_of(const Params& p, long long rows, cudaStream_t st) {
   if (p.vocab <= 16384 && rows >= 8ll * num_sms() && p.parts == 1 && p.k <= kMine * kFewThreads) return sums_t<T, kFewThreads>(p, rows, st);
+  if (one_wave_of_halves(rows, p.vocab, sizeof(T)) && p.k <= kMine * kHalfThreads) return sums_t<T, kHalfThreads>(p, rows, st);
   return sums_t<T, kThreads>(p, rows, st);
 }
 
@@ -719,8 +725,9 @@ int bwd_t(BwdParams p, long long rows, cudaStream_t st) {
 using namespace rb;
 using namespace rb::distill;
 
-// Blocks per row, and so pairs of doubles per row that rb_topk_distill takes as workspace.
-extern "C" int rb_topk_distill_parts(long long rows, int vocab) {
+// Blocks per row, and so pairs of doubles per row that rb_topk_distill takes as workspace.  size: bytes of a logit.
+extern "C" int rb_topk_distill_parts(long long rows, int vocab, int size) {
+  if (one_wave_of_halves(rows, vocab, size)) return 1;
   const int parts = parts_of(rows, vocab, 4ll * num_sms(), 1000);      // (a fixed 2 us of 4 blocks per SM)
   return vocab / parts > (1 << 20) ? kMaxParts : parts;                 // the bitmap of a part fits shared memory
 }
@@ -731,7 +738,7 @@ extern "C" int rb_topk_distill(const void* z, long long ld, const long long* ids
                                double inv_temp, int dtype, cudaStream_t st) {
   if (rows < 0 || vocab < 1 || vocab > kMaxVocab || k < 0 || k > kMaxIds || kl < 0 || kl > 3 || norm < 0 || norm > 2 || !(inv_temp > 0.0)) return -1;
   if (rows == 0) return 0;
-  const int parts = rb_topk_distill_parts(rows, vocab);
+  const int parts = rb_topk_distill_parts(rows, vocab, dtype == 2 ? 4 : 2);
   if (rows * parts > 2147483647ll) return -3;
   const double scale = inv_temp * kLog2e;
   float c2, c2_low;

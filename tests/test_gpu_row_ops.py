@@ -460,10 +460,11 @@ def test_distill_vocabularies_of_any_size(V):
         ops.topk_distill(torch.empty(1, (1 << 24) + 1, device="cuda", dtype=torch.bfloat16), ids, t)
 
 
-@pytest.mark.parametrize("R,V,K", [(1300, 515, 20), (1184, 1024, 256), (1184, 1024, 257), (1190, 4099, 8), (1200, 33, 33)])
+@pytest.mark.parametrize("R,V,K", [(1300, 515, 20), (1184, 1024, 256), (1184, 1024, 257), (1190, 4099, 8), (1200, 33, 33), (593, 4099, 512), (600, 2003, 513),
+                                   (1184, 20001, 9), (700, 70007, 5)])
 @pytest.mark.parametrize("dtype", ["bf16", "fp32"])
 def test_distill_many_short_rows(R, V, K, dtype):
-    """Blocks of fewer threads: rows of every alignment, up to the most ids that such a block takes and beyond."""
+    """Blocks of fewer threads: rows of every alignment, up to the most ids that such blocks take and beyond."""
     z, ids, t, w = _case(R, V, K, dtype, 29)
     z[7, 1:] = -1e30
     z[8, :] = -1e9
