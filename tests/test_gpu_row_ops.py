@@ -786,3 +786,36 @@ def test_step_of_a_routed_student():
     assert abs(float(loss) - float(ld)) < 2e-2 * abs(float(ld))      # bf16 activations: four roundings of 2^-8 in front of the logits
     for got, ref in zip(grads, want):
         assert float((got.double() - ref).norm() / ref.norm()) < 5e-2, got.shape
+
+
+@pytest.mark.parametrize("selection", ["teacher_topk", "student_topk", "union"])
+def test_loss_mode_of_a_routed_student(tmp_path, monkeypatch, selection):
+    """The training loop with ``--opd-loss-coef`` on top ids: every operator of this file in one step, as a user runs them."""
+    import dataclasses
+
+    from relax_b200.checkpoint import hf as H
+    from relax_b200.config.arguments import parse_args
+    from relax_b200.models import config as MC
+    from relax_b200.models.transformer import GPTModel
+    from relax_b200.orchestration.controller import Controller
+
+    cfg = dataclasses.replace(MC.get_config("tiny-moe"), name="tiny-moe-wide-heads", head_dim=128, vocab_size=1024, dtype="bf16")
+    monkeypatch.setitem(MC.PRESETS, cfg.name, cfg)
+    teacher = GPTModel(cfg, seed=77)
+    d = str(tmp_path / "teacher")
+    H.save_hf_checkpoint(d, cfg, H.convert_state_to_hf(cfg, {k: v.detach() for k, v in teacher.named_parameters()}))
+    a = parse_args(["--model-name", cfg.name, "--colocate", "--rollout-batch-size", "2", "--n-samples-per-prompt", "2", "--global-batch-size", "4",
+                    "--num-rollout", "1", "--rollout-max-response-len", "24", "--use-opd", "--opd-teacher-load", d, "--lr", "1e-3", "--opd-loss-coef", "1.0",
+                    "--opd-only-reward", "--opd-token-selection", selection, "--opd-log-prob-top-k", "16", "--opd-kl-type", "jsd"])
+    c = Controller(a, device="cuda")
+    actor, seen = c.runner.actor, {}
+    plain = actor._distill_batch
+    actor._distill_batch = lambda batch, ids: seen.setdefault("made", plain(batch, ids))
+    hist = c.runner.step()
+    made = seen["made"]
+    assert made["divergence"].dtype == torch.float32 and bool((made["divergence"] >= 0).all())
+    assert math.isfinite(hist["grad_norm"]) and hist["grad_norm"] > 0 and hist["opd_loss"] > 0
+    assert hist["pg_loss"] == 0.0 and hist["loss"] == pytest.approx(hist["opd_loss"], rel=1e-6)
+    assert made["ids"].shape[1] == 16 if selection != "union" else 16 < made["ids"].shape[1] <= 32
+    assert c.runner.step()["opd_loss"] > 0
+    c.runner.close()
