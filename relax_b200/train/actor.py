@@ -11,6 +11,7 @@ reference log-probs -> old-policy log-probs -> advantages -> optimizer steps.
 """
 from __future__ import annotations
 
+import contextlib
 import math
 import os
 import time
@@ -373,13 +374,17 @@ class TrainActor:
                               self.mcfg.num_query_groups // tp, self.mcfg.head_dim)
         return self.cp_comm
 
-    def _forward_logp(self, pb, with_entropy: bool, distill: Optional[dict] = None):
-        """Log-probs and entropy per response position.  ``distill`` (``ids``, ``teacher``): the divergence from a teacher on those ids is
-        computed from the same hidden states and left in ``distill["divergence"]``."""
+    def _set_replay_layout(self, pb):
+        """Whose tokens the next pass routes, for routing replay."""
         if (self.cfg.use_routing_replay or self.cfg.use_rollout_routing_replay) and self.mcfg.is_moe:
             from ..models.moe import RoutingReplay
 
             RoutingReplay.set_layout(getattr(self, "_cur_ids", None), pb.total_lengths)
+
+    def _forward_logp(self, pb, with_entropy: bool, distill: Optional[dict] = None):
+        """Log-probs and entropy per response position.  ``distill`` (``ids``, ``teacher``): the divergence from a teacher on those ids is
+        computed from the same hidden states and left in ``distill["divergence"]``."""
+        self._set_replay_layout(pb)
         if self.ps.pp.size > 1:
             return self._forward_logp_pp(pb, with_entropy)
         if self.ps.cp.size > 1:
@@ -462,33 +467,39 @@ class TrainActor:
             mbs.append([])
         return mbs
 
+    @contextlib.contextmanager
+    def _as_model(self, tag: str):
+        """The weights of ``tag`` for the passes inside, those of the actor afterwards.  Reference and teacher choose their experts
+        themselves: routing replay is suspended for them."""
+        own_routing = tag not in ("actor", "old_actor") and (self.cfg.use_routing_replay or self.cfg.use_rollout_routing_replay) and self.mcfg.is_moe
+        if own_routing:
+            from ..models.moe import RoutingReplay
+
+            suspended, RoutingReplay.mode = RoutingReplay.mode, None
+        try:
+            self.switch_model(tag)
+            yield
+        finally:
+            if own_routing:
+                RoutingReplay.mode = suspended
+            self.switch_model("actor")
+
     @torch.no_grad()
     def compute_log_prob(self, batch: dict, tag: str = "actor", with_entropy: bool = False) -> dict:
         """Forward-only pass; returns per-sample lists ``log_probs`` (and ``entropy``)."""
-        self.switch_model(tag)
-        suspended = None
-        if tag not in ("actor", "old_actor") and (self.cfg.use_routing_replay or self.cfg.use_rollout_routing_replay) and self.mcfg.is_moe:
-            from ..models.moe import RoutingReplay
-
-            suspended, RoutingReplay.mode = RoutingReplay.mode, None     # reference / teacher route for themselves
-        toks, rl = batch["tokens"], batch["response_lengths"]
-        mbs = self._microbatches([len(t) for t in toks])
+        toks = batch["tokens"]
         out_lp = [None] * len(toks)
         out_en = [None] * len(toks)
-        for mb in mbs:
-            if not mb:
-                self._dummy_forward()
-                continue
-            pb = self._pack_batch(batch, mb)
-            self._cur_ids = list(mb)
-            lp, en = self._forward_logp(pb, with_entropy)
-            for i, a, b in zip(mb, torch.split(lp, pb.response_lengths), torch.split(en, pb.response_lengths)):
-                out_lp[i], out_en[i] = a, b
-        self.switch_model("actor")
-        if suspended is not None:
-            from ..models.moe import RoutingReplay
-
-            RoutingReplay.mode = suspended
+        with self._as_model(tag):
+            for mb in self._microbatches([len(t) for t in toks]):
+                if not mb:
+                    self._dummy_forward()
+                    continue
+                pb = self._pack_batch(batch, mb)
+                self._cur_ids = list(mb)
+                lp, en = self._forward_logp(pb, with_entropy)
+                for i, a, b in zip(mb, torch.split(lp, pb.response_lengths), torch.split(en, pb.response_lengths)):
+                    out_lp[i], out_en[i] = a, b
         res = {"log_probs": out_lp}
         if with_entropy:
             res["entropy"] = out_en
@@ -507,45 +518,46 @@ class TrainActor:
             raise NotImplementedError("top-K distillation reads full-vocabulary rows: trainer tp = pp = cp = 1")
         if ids is None and k <= 0:
             raise ValueError("either k > 0 or ids")
-        self.switch_model(tag)
         toks = batch["tokens"]
         out_ids, out_lp = [None] * len(toks), [None] * len(toks)
-        w = self.model.lm_head_weight()[: self.mcfg.vocab_size].float()
-        inv_t = 1.0 / float(self.cfg.rollout_temperature or 1.0)
-        for mb in self._microbatches([len(t) for t in toks]):
-            if not mb:
-                self._dummy_forward()
-                continue
-            pb = self._pack_batch(batch, mb)
-            emb = self._embed_multimodal(pb) if getattr(pb, "pixel_patches", None) is not None else None
-            h = self.model(pb.tokens, pb.positions, pb.cu_seqlens, max_seqlen=pb.max_seqlen, inputs_embeds=emb)
-            hr = h.index_select(0, pb.logit_rows).float()
-            want = None
-            if ids is not None:
-                rows = [torch.as_tensor(ids[i], dtype=torch.long, device=self.device) for i in mb]
-                kmax = max(t.shape[-1] for t in rows)          # union sets differ in width: pad with -1
-                want = torch.cat([torch.nn.functional.pad(t, (0, kmax - t.shape[-1]), value=-1) for t in rows])
-                if want.shape[0] != hr.shape[0]:
-                    raise ValueError("ids must hold one row per response position")
-            got_ids, got_lp = [], []
-            for a in range(0, hr.shape[0], row_chunk):
-                logits = (hr[a:a + row_chunk] @ w.t()) * inv_t
-                lse = torch.logsumexp(logits, -1, keepdim=True)
+        with self._as_model(tag):
+            w = self.model.lm_head_weight()[: self.mcfg.vocab_size].float()
+            inv_t = 1.0 / float(self.cfg.rollout_temperature or 1.0)
+            for mb in self._microbatches([len(t) for t in toks]):
+                if not mb:
+                    self._dummy_forward()
+                    continue
+                pb = self._pack_batch(batch, mb)
+                self._cur_ids = list(mb)
+                self._set_replay_layout(pb)
+                emb = self._embed_multimodal(pb) if getattr(pb, "pixel_patches", None) is not None else None
+                h = self.model(pb.tokens, pb.positions, pb.cu_seqlens, max_seqlen=pb.max_seqlen, inputs_embeds=emb)
+                hr = h.index_select(0, pb.logit_rows).float()
+                want = None
+                if ids is not None:
+                    rows = [torch.as_tensor(ids[i], dtype=torch.long, device=self.device) for i in mb]
+                    kmax = max(t.shape[-1] for t in rows)          # union sets differ in width: pad with -1
+                    want = torch.cat([torch.nn.functional.pad(t, (0, kmax - t.shape[-1]), value=-1) for t in rows])
+                    if want.shape[0] != hr.shape[0]:
+                        raise ValueError("ids must hold one row per response position")
+                got_ids, got_lp = [], []
+                for a in range(0, hr.shape[0], row_chunk):
+                    logits = (hr[a:a + row_chunk] @ w.t()) * inv_t
+                    lse = torch.logsumexp(logits, -1, keepdim=True)
+                    if want is None:
+                        val, idx = logits.topk(k, -1)
+                        got_ids.append(idx)
+                        got_lp.append(val - lse)
+                    else:
+                        q = want[a:a + row_chunk]
+                        lp = logits.gather(-1, q.clamp_min(0)) - lse
+                        got_lp.append(lp.masked_fill(q < 0, float("-inf")))
+                lp_all = torch.cat(got_lp) if got_lp else hr.new_zeros(0, k)
+                for j, (i, piece) in enumerate(zip(mb, torch.split(lp_all, pb.response_lengths))):
+                    out_lp[i] = piece if ids is None else piece[:, : torch.as_tensor(ids[i]).shape[-1]]
                 if want is None:
-                    val, idx = logits.topk(k, -1)
-                    got_ids.append(idx)
-                    got_lp.append(val - lse)
-                else:
-                    q = want[a:a + row_chunk]
-                    lp = logits.gather(-1, q.clamp_min(0)) - lse
-                    got_lp.append(lp.masked_fill(q < 0, float("-inf")))
-            lp_all = torch.cat(got_lp) if got_lp else hr.new_zeros(0, k)
-            for j, (i, piece) in enumerate(zip(mb, torch.split(lp_all, pb.response_lengths))):
-                out_lp[i] = piece if ids is None else piece[:, : torch.as_tensor(ids[i]).shape[-1]]
-            if want is None:
-                for i, piece in zip(mb, torch.split(torch.cat(got_ids), pb.response_lengths)):
-                    out_ids[i] = piece
-        self.switch_model("actor")
+                    for i, piece in zip(mb, torch.split(torch.cat(got_ids), pb.response_lengths)):
+                        out_ids[i] = piece
         return {"ids": out_ids if ids is None else list(ids), "log_probs": out_lp}
 
     def _distill_ids(self, batch: dict):

@@ -1,0 +1,138 @@
+"""Distillation on top ids as a loss term: whose experts route the teacher's passes, which rows reach the loss, and what the step trains on."""
+import math
+
+import pytest
+import torch
+
+from relax_b200.algo.loss import LossConfig
+from relax_b200.models.config import get_config
+from relax_b200.models.moe import RoutingReplay
+from relax_b200.models.transformer import GPTModel
+from relax_b200.train.actor import TrainActor, TrainConfig
+from relax_b200.train.optimizer import OptimizerConfig
+
+SEL = ["teacher_topk", "student_topk", "union"]
+
+
+@pytest.fixture(autouse=True)
+def _no_replay_left():
+    yield
+    RoutingReplay.end()
+    RoutingReplay.per_sample = {}
+
+
+def _actor(model="tiny-moe", micro=2, selection="teacher_topk", coef=1.0, lr=0.0, **kw):
+    cfg = TrainConfig(advantage_estimator="grpo", global_batch_size=4, n_samples_per_prompt=2, use_dynamic_batch_size=False, micro_batch_size=micro,
+                      pad_multiple=1, opd_token_selection=selection, opd_log_prob_top_k=5, opd_kl_type="jsd",
+                      loss=LossConfig(opd_loss_coef=coef, opd_kl_type="jsd"), optim=OptimizerConfig(lr=lr), **kw)
+    actor = TrainActor(get_config(model), cfg, role="actor", seed=0)
+    g = torch.Generator().manual_seed(3)
+    teacher = actor.param_buf + 0.1 * torch.randn(actor.param_buf.shape, generator=g)      # (the norms' weights too)
+    actor.snapshots["teacher"] = teacher
+    return actor
+
+
+def _batch(actor, routed=False):
+    g = torch.Generator().manual_seed(1)
+    lens, rl = (12, 9, 14, 10), [5, 4, 6, 3]
+    toks = [torch.randint(3, 1000, (n,), generator=g).tolist() for n in lens]
+    batch = {"tokens": toks, "response_lengths": rl, "loss_masks": [[1.0] * r for r in rl], "rewards": [1.0, 0.0, 0.0, 1.0]}
+    if routed:      # as recorded by an engine, other than what either router would choose
+        c = actor.mcfg
+        moe = [i for i in range(c.num_layers) if c.is_moe_layer(i)]
+        batch["rollout_routed_experts"] = [torch.stack([torch.randperm(c.num_experts, generator=g)[: c.moe_top_k] for _ in range((n - 1) * len(moe))])
+                                           .view(n - 1, len(moe), c.moe_top_k).tolist() for n in lens]
+    return batch
+
+
+def _teacher_alone(actor, batch, ids=None, k=5):
+    """The teacher's top ids and log-probs, or its log-probs of given ids, by whole logits of one sample after the other, without replay."""
+    m = GPTModel(actor.mcfg, seed=0)
+    named = dict(actor.model.named_parameters())
+    off = {id(p): o for p, o in actor._bound_params()}
+    m.load_state_dict({n: actor.snapshots["teacher"][off[id(p)]: off[id(p)] + p.numel()].view_as(p) for n, p in named.items()}, strict=False)
+    out = []
+    for i, (t, r) in enumerate(zip(batch["tokens"], batch["response_lengths"])):
+        with torch.no_grad():
+            h = m(torch.tensor(t), torch.arange(len(t)), torch.tensor([0, len(t)], dtype=torch.int32), max_seqlen=len(t))
+            lp = torch.log_softmax(m.logits(h)[len(t) - r - 1:len(t) - 1, : actor.mcfg.vocab_size].double(), -1)
+        if ids is None:
+            out.append(lp.topk(k, -1)[::-1])
+        else:
+            q = torch.as_tensor(ids[i])
+            out.append((q, lp.gather(-1, q.clamp_min(0)).masked_fill(q < 0, -math.inf)))
+    return out
+
+
+@pytest.mark.parametrize("flags", [dict(use_routing_replay=True), dict(use_rollout_routing_replay=True),
+                                   dict(use_rollout_routing_replay=True, use_rollout_logprobs=True)])
+@pytest.mark.parametrize("selection", SEL)
+def test_teacher_routes_for_itself(selection, flags):
+    """With routing replay on, ids and log-probs that reach the loss are those of a teacher that chooses its experts itself, sample by sample
+    over several micro-batches; the policy's passes replay what was recorded for them."""
+    actor = _actor(selection=selection, **flags)
+    batch = _batch(actor, routed="use_rollout_routing_replay" in flags)
+    if flags.get("use_rollout_logprobs"):
+        batch["rollout_log_probs"] = [[-7.0] * r for r in batch["response_lengths"]]
+    seen, made, plain = [], [], actor._distill_ids
+    orig = RoutingReplay.route.__func__
+
+    def spy(cls, layer, idx):
+        out = orig(cls, layer, idx)
+        seen.append((actor._active_tag, cls.mode, bool((out != idx).any())))
+        return out
+
+    actor._distill_ids = lambda b: made.append(plain(b)) or made[-1]
+    RoutingReplay.route = classmethod(spy)
+    try:
+        m = actor.train(0, batch)
+    finally:
+        RoutingReplay.route = classmethod(orig)
+    assert RoutingReplay.mode is None and m["opd_loss"] > 0
+    assert {mode for tag, mode, _ in seen if tag == "teacher"} == {None}
+    assert "replay" in {mode for tag, mode, _ in seen if tag == "actor"}
+    ids, _, _, t_lp = made[0]
+    for i, (q, lp) in enumerate(_teacher_alone(actor, batch, None if selection == "teacher_topk" else ids)):
+        assert torch.equal(ids[i], q)
+        there = q >= 0
+        # 32-bit logits and their logsumexp against 64-bit ones of the same hidden states, packed differently
+        assert torch.allclose(t_lp[i][there].double(), lp[there], atol=1e-4, rtol=0)
+
+
+def test_policy_passes_on_sets_of_ids_replay_what_was_recorded():
+    """The student's own log-probs on its ids come from the experts that the training forward will use, however samples are packed."""
+    actor = _actor(use_routing_replay=True)
+    batch = _batch(actor)
+    RoutingReplay.begin_record()
+    want = actor.compute_topk_log_probs(batch, k=5)["ids"]
+    kept = dict(RoutingReplay.per_sample)
+    assert len(kept) == 4 * sum(actor.mcfg.is_moe_layer(i) for i in range(actor.mcfg.num_layers))
+    RoutingReplay.end()
+    RoutingReplay.begin_replay()
+    for p in actor.model.parameters():      # another router: without replay other experts
+        if p.shape == (actor.mcfg.num_experts, actor.mcfg.hidden_size):
+            p.data.neg_()
+    actor.cfg.micro_batch_size = 3
+    calls, orig = [], RoutingReplay.route.__func__
+
+    def spy(cls, layer, idx):
+        calls.append(torch.equal(orig(cls, layer, idx), torch.cat([kept[(layer, s)] for s in cls.layout[0]])))
+        return orig(cls, layer, idx)
+
+    RoutingReplay.route = classmethod(spy)
+    try:
+        got = actor.compute_topk_log_probs(batch, ids=want)
+    finally:
+        RoutingReplay.route = classmethod(orig)
+    assert calls and all(calls) and len(got["log_probs"]) == 4
+
+
+@pytest.mark.parametrize("call", ["compute_log_prob", "compute_topk_log_probs"])
+def test_a_failed_teacher_pass_leaves_nothing_behind(call):
+    actor = _actor(use_routing_replay=True)
+    batch = _batch(actor)
+    RoutingReplay.begin_replay()
+    actor._pack_batch = lambda *a: (_ for _ in ()).throw(RuntimeError("no room"))
+    with pytest.raises(RuntimeError, match="no room"):
+        getattr(actor, call)(batch, "teacher", **({"k": 3} if call != "compute_log_prob" else {}))
+    assert RoutingReplay.mode == "replay" and actor._active_tag == "actor"
