@@ -682,6 +682,7 @@ class TrainActor:
 
     def _dummy_forward(self, backward: bool = False):
         pb = self._pack([[0, 0]], [1])
+        self._cur_ids = []      # (nobody's tokens: nothing to record or to replay)
         if backward:
             if self.role == "critic":
                 (self._forward_values(pb).sum() * 0.0).backward()

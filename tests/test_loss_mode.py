@@ -136,3 +136,17 @@ def test_a_failed_teacher_pass_leaves_nothing_behind(call):
     with pytest.raises(RuntimeError, match="no room"):
         getattr(actor, call)(batch, "teacher", **({"k": 3} if call != "compute_log_prob" else {}))
     assert RoutingReplay.mode == "replay" and actor._active_tag == "actor"
+
+
+@pytest.mark.parametrize("mode", ["record", "replay"])
+def test_a_pass_for_nobody_is_neither_recorded_nor_replayed(mode):
+    """A data-parallel rank with fewer micro-batches runs a filler between and after its own."""
+    actor = _actor(use_routing_replay=True)
+    batch = _batch(actor)
+    RoutingReplay.begin_record()
+    actor.compute_log_prob(batch)
+    kept = dict(RoutingReplay.per_sample)
+    RoutingReplay.mode = mode
+    actor._dummy_forward()
+    actor._dummy_forward(backward=True)
+    assert RoutingReplay.per_sample.keys() == kept.keys() and all(RoutingReplay.per_sample[k] is v for k, v in kept.items())
