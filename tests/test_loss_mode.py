@@ -150,3 +150,57 @@ def test_a_pass_for_nobody_is_neither_recorded_nor_replayed(mode):
     actor._dummy_forward()
     actor._dummy_forward(backward=True)
     assert RoutingReplay.per_sample.keys() == kept.keys() and all(RoutingReplay.per_sample[k] is v for k, v in kept.items())
+
+
+@pytest.mark.parametrize("model,selection", [("tiny", s) for s in SEL] + [("tiny-moe", "union")])
+def test_step_trains_on_the_divergence_of_whole_logits(model, selection):
+    """A step of pure distillation over several micro-batches: every sample's rows carry its own ids and teacher log-probs, the metric is the
+    divergence of whole logits, and parameters get its gradient."""
+    from relax_b200.algo import opd
+
+    actor = _actor(model, micro=3, selection=selection, opd_only_reward=True)
+    batch = _batch(actor)
+    grads, plain = {}, actor.optimizer.step
+
+    def step(**kw):
+        for n, p in actor.model.named_parameters():
+            grads[n] = (p.grad if p.grad is not None else p.main_grad).detach().clone()
+        return plain(**kw)
+
+    made, distill_batch = [], actor._distill_batch
+    actor._distill_batch = lambda b, ids: made.append((list(ids), distill_batch(b, ids))) or made[-1][1]
+    actor.optimizer.step = step
+    m = actor.train(0, batch)
+    assert sorted(i for ids, _ in made for i in ids) == [0, 1, 2, 3] and len(made) > 1
+    # ids and teacher log-probs of every sample, from the teacher's weights alone
+    own = [t for t, _ in _teacher_alone(actor, batch)]
+    whole = _teacher_alone(actor, batch, [torch.arange(actor.mcfg.vocab_size).expand(n, -1) for n in batch["response_lengths"]])
+    total = 0.0
+    model_ = actor.model
+    for p in model_.parameters():      # (gradients of their own, apart from the optimizer's buffer)
+        p.grad = p.main_grad = None
+    for i, (t, r) in enumerate(zip(batch["tokens"], batch["response_lengths"])):
+        h = model_(torch.tensor(t), torch.arange(len(t)), torch.tensor([0, len(t)], dtype=torch.int32), max_seqlen=len(t))
+        lp = torch.log_softmax(model_.logits(h)[len(t) - r - 1:len(t) - 1, : actor.mcfg.vocab_size].double(), -1)
+        student = lp.detach().topk(5, -1).indices
+        ids = {"teacher_topk": own[i], "student_topk": student, "union": torch.cat([student, own[i]], 1)}[selection]
+        for sids, d in made:
+            if i in sids:
+                n0 = sum(batch["response_lengths"][s] for s in sids[: sids.index(i)])
+                rows = (d["ids"][n0:n0 + r], d["teacher"][n0:n0 + r])
+        want_t = whole[i][1]
+        for row in range(r):
+            got = [int(x) for x in rows[0][row] if x >= 0]
+            assert sorted(got) == sorted(set(ids[row].tolist())) and len(got) == len(set(got))
+            there = rows[0][row] >= 0
+            assert torch.allclose(rows[1][row][there].double(), want_t[row, rows[0][row][there]], atol=1e-4, rtol=0)
+        q = rows[0]
+        d = opd.token_kl(lp.gather(-1, q.clamp_min(0)), want_t.gather(-1, q.clamp_min(0)).masked_fill(q < 0, 0.0), "jsd", 0.5, "tail", mask=q >= 0)
+        total = total + d.mean() / 4
+    assert m["opd_loss"] == pytest.approx(float(total), rel=1e-4) and m["pg_loss"] == 0.0
+    total.backward()
+    ref = {n: (p.grad if p.grad is not None else torch.zeros_like(p)) for n, p in actor.model.named_parameters()}
+    norm = math.sqrt(sum(float(g.double().pow(2).sum()) for g in ref.values()))
+    off = math.sqrt(sum(float((grads[n].double() - ref[n].double()).pow(2).sum()) for n in ref))
+    # 32-bit layers on both sides, summed in another order: some thousand roundings of 2^-24
+    assert norm > 0 and off <= 1e-3 * norm
