@@ -224,7 +224,7 @@ int rb_expert_dispatch(const void* x, long long ld, const int* source, const int
 int rb_expert_combine(const void* y, long long ld, const int* dest, const float* weight, void* out, int n, int k, int cols, int dtype, int out_fp32,
                       cudaStream_t st);
 int rb_expert_combine_bwd(const void* d_out, long long ld, const void* y, long long ldy, const int* source, const int* dest, const float* weight, void* d_y,
-                          float* d_w, int cap, int n, int k, int cols, int dtype, cudaStream_t st);
+                          float* d_w, int cap, int n, int k, int cols, int dtype, int out_fp32, cudaStream_t st);
 int rb_embedding(const void* ids, int wide, long long start, const void* table, long long ld, int rows, void* out, int n, int cols, float scale, int dtype,
                  cudaStream_t st);
 int rb_embedding_bwd_bins(int rows);

@@ -146,14 +146,17 @@ struct Combine : Function<Combine> {
     const auto saved = ctx->get_saved_variables();
     const auto &w = saved[1], &dest = saved[2], &source = saved[3];
     const c10::cuda::CUDAGuard guard(g[0].device());
-    const auto d = dense(g[0].to(static_cast<at::ScalarType>(ctx->saved_data["type"].toInt())), "expert_combine");
-    if (!w.defined())
+    if (!w.defined()) {      // (copies: one rounding)
+      const auto d = g[0].to(static_cast<at::ScalarType>(ctx->saved_data["type"].toInt()));
       return once({scatter_rows(d, source, dest, "expert_combine"), torch::Tensor(), torch::Tensor(), torch::Tensor(), torch::Tensor()}, g);
-    const auto y = dense(saved[0], "expert_combine");
+    }
+    const auto d = dense(g[0], "expert_combine"), y = dense(saved[0], "expert_combine");
+    const bool fp32 = d.scalar_type() == at::kFloat;
+    TORCH_CHECK_VALUE(fp32 || d.scalar_type() == y.scalar_type(), "expert_combine: a gradient in ", y.scalar_type(), " or float32, got ", d.scalar_type());
     auto d_y = at::empty({y.size(0), y.size(1)}, y.options()), d_w = at::empty_like(w);
     check(rb_expert_combine_bwd(d.data_ptr(), d.stride(0), y.data_ptr(), y.stride(0), source.data_ptr<int>(), dest.data_ptr<int>(), w.data_ptr<float>(),
                                 d_y.data_ptr(), d_w.data_ptr<float>(), as_int(source.numel(), "expert_combine"), as_int(dest.size(0), "expert_combine"),
-                                as_int(dest.size(1), "expert_combine"), as_int(y.size(1), "expert_combine"), code_of(y, "expert_combine"), cur_stream()),
+                                as_int(dest.size(1), "expert_combine"), as_int(y.size(1), "expert_combine"), code_of(y, "expert_combine"), fp32, cur_stream()),
           "rb_expert_combine_bwd");
     return once({d_y, d_w.to(static_cast<at::ScalarType>(ctx->saved_data["weight_type"].toInt())), torch::Tensor(), torch::Tensor(), torch::Tensor()}, g);
   }

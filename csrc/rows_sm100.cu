@@ -622,10 +622,11 @@ __global__ void __launch_bounds__(N == 1 ? kSingleThreads : 256) sum_kernel(cons
 // buffer rows that a warp looks at for padding: long ones take their time, short ones would be more warps than tokens
 __host__ __device__ inline int padding_rows(int vecs) { return vecs >= 128 ? 8 : 32; }
 
-// Backward of the weighted sum: d_y[dest] = w d_out[t] and d_w = <d_out[t], y[dest]>.  A block per token holds its row of d_out while
-// it walks over the token's rows of y, so that all of them pass once; blocks behind the tokens write the zeros of padding rows.
-template <typename T, int N>
-__global__ void __launch_bounds__(N == 1 ? kSingleThreads : 256) sum_bwd_kernel(const T* __restrict__ d_out, long long ld, const T* __restrict__ y, long long ldy,
+// Backward of the weighted sum: d_y[dest] = w d_out[t] and d_w = <d_out[t], y[dest]>.  A block per token holds its row of d_out (in the
+// type of the sum: fp32 for a sum kept in 32 bits) while it walks over the token's rows of y, so that all of them pass once; blocks behind
+// the tokens write the zeros of padding rows.
+template <typename T, int N, typename G>
+__global__ void __launch_bounds__(N == 1 ? kSingleThreads : 256) sum_bwd_kernel(const G* __restrict__ d_out, long long ld, const T* __restrict__ y, long long ldy,
                                                       const int* __restrict__ source, const int* __restrict__ dest, const float* __restrict__ weight,
                                                       T* __restrict__ d_y, float* __restrict__ d_w, long long cap, long long n, int k, int cols) {
   const int t = threadIdx.x, lane = t & 31, w = t >> 5, warps = blockDim.x >> 5, vecs = cols / N;
@@ -643,7 +644,7 @@ __global__ void __launch_bounds__(N == 1 ? kSingleThreads : 256) sum_bwd_kernel(
   }
   __shared__ float red[8][8];
   constexpr int J = 8;      // rows of y at a time, four of them in flight
-  const Pack<T, N>* a = reinterpret_cast<const Pack<T, N>*>(d_out + row * ld);
+  const Pack<G, N>* a = reinterpret_cast<const Pack<G, N>*>(d_out + row * ld);
   for (int j0 = 0; j0 < k; j0 += J) {
     int d[J];
     float wj[J], dot[J];
@@ -657,7 +658,7 @@ __global__ void __launch_bounds__(N == 1 ? kSingleThreads : 256) sum_bwd_kernel(
       constexpr int S = 4;
       for (int v = t; v < vecs; v += S * kSingleThreads) {
         float f[S];
-        const T* av = d_out + row * ld + v;
+        const G* av = d_out + row * ld + v;
 #pragma unroll
         for (int s = 0; s < S; ++s) f[s] = v + s * kSingleThreads < vecs ? up(av[s * kSingleThreads]) : 0.f;
 #pragma unroll
@@ -964,19 +965,21 @@ int sum_any(const void* in, long long ld, const int* dest, const float* weight, 
              : sum_t<T, 1, OutT>(in, ld, dest, weight, out, n, k, cols, st);
 }
 
-template <typename T>
+template <typename T, typename G>
 int sum_bwd_t(const void* d_out, long long ld, const void* y, long long ldy, const int* source, const int* dest, const float* weight, void* d_y, float* d_w,
               long long cap, long long n, int k, int cols, cudaStream_t st) {
-  const bool wide = wide_rows(d_out, ld, cols, sizeof(T)) && wide_rows(y, ldy, cols, sizeof(T)) && wide_rows(d_y, cols, cols, sizeof(T));
-  const int threads = row_threads(cols / (wide ? 16 / static_cast<int>(sizeof(T)) : 1), !wide);
-  const long long warps = threads / 32, some = padding_rows(cols / (wide ? 16 / static_cast<int>(sizeof(T)) : 1)),
-                  grid = n + ((cap + some - 1) / some + warps - 1) / warps;
+  constexpr int NV = 16 / sizeof(T);
+  const bool wide = wide_rows(y, ldy, cols, sizeof(T)) && wide_rows(d_y, cols, cols, sizeof(T)) && reinterpret_cast<uintptr_t>(d_out) % (NV * sizeof(G)) == 0 &&
+                    ld % NV == 0;      // (so many elements of a row of d_out are one vector, too)
+  const int threads = row_threads(cols / (wide ? NV : 1), !wide);
+  const long long warps = threads / 32, some = padding_rows(cols / (wide ? NV : 1)), grid = n + ((cap + some - 1) / some + warps - 1) / warps;
   if (grid > kMaxGrid) return -3;
-  const T *a = static_cast<const T*>(d_out), *b = static_cast<const T*>(y);
+  const G* a = static_cast<const G*>(d_out);
+  const T* b = static_cast<const T*>(y);
   T* o = static_cast<T*>(d_y);
   const int g = static_cast<int>(grid);
-  if (wide) sum_bwd_kernel<T, 16 / sizeof(T)><<<g, threads, 0, st>>>(a, ld, b, ldy, source, dest, weight, o, d_w, cap, n, k, cols);
-  else sum_bwd_kernel<T, 1><<<g, threads, 0, st>>>(a, ld, b, ldy, source, dest, weight, o, d_w, cap, n, k, cols);
+  if (wide) sum_bwd_kernel<T, NV, G><<<g, threads, 0, st>>>(a, ld, b, ldy, source, dest, weight, o, d_w, cap, n, k, cols);
+  else sum_bwd_kernel<T, 1, G><<<g, threads, 0, st>>>(a, ld, b, ldy, source, dest, weight, o, d_w, cap, n, k, cols);
   rb_note_launch(1);
   return static_cast<int>(cudaGetLastError());
 }
@@ -1070,14 +1073,19 @@ extern "C" int rb_expert_combine(const void* y, long long ld, const int* dest, c
   return -1;
 }
 
+// out_fp32: d_out is in fp32, whatever the type of y
 extern "C" int rb_expert_combine_bwd(const void* d_out, long long ld, const void* y, long long ldy, const int* source, const int* dest, const float* weight,
-                                     void* d_y, float* d_w, int cap, int n, int k, int cols, int dtype, cudaStream_t st) {
+                                     void* d_y, float* d_w, int cap, int n, int k, int cols, int dtype, int out_fp32, cudaStream_t st) {
   if (k < 1 || n < 0 || cap < 0 || cols < 0) return -1;
   if (cap == 0 && n == 0) return 0;
   switch (dtype) {
-    case 0: return sum_bwd_t<__nv_bfloat16>(d_out, ld, y, ldy, source, dest, weight, d_y, d_w, cap, n, k, cols, st);
-    case 1: return sum_bwd_t<__half>(d_out, ld, y, ldy, source, dest, weight, d_y, d_w, cap, n, k, cols, st);
-    case 2: return sum_bwd_t<float>(d_out, ld, y, ldy, source, dest, weight, d_y, d_w, cap, n, k, cols, st);
+    case 0:
+      return out_fp32 ? sum_bwd_t<__nv_bfloat16, float>(d_out, ld, y, ldy, source, dest, weight, d_y, d_w, cap, n, k, cols, st)
+                      : sum_bwd_t<__nv_bfloat16, __nv_bfloat16>(d_out, ld, y, ldy, source, dest, weight, d_y, d_w, cap, n, k, cols, st);
+    case 1:
+      return out_fp32 ? sum_bwd_t<__half, float>(d_out, ld, y, ldy, source, dest, weight, d_y, d_w, cap, n, k, cols, st)
+                      : sum_bwd_t<__half, __half>(d_out, ld, y, ldy, source, dest, weight, d_y, d_w, cap, n, k, cols, st);
+    case 2: return sum_bwd_t<float, float>(d_out, ld, y, ldy, source, dest, weight, d_y, d_w, cap, n, k, cols, st);
   }
   return -1;
 }

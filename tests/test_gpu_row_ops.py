@@ -819,3 +819,30 @@ def test_loss_mode_of_a_routed_student(tmp_path, monkeypatch, selection):
     assert made["ids"].shape[1] == 16 if selection != "union" else 16 < made["ids"].shape[1] <= 32
     assert c.runner.step()["opd_loss"] > 0
     c.runner.close()
+
+
+@pytest.mark.parametrize("H,pitch", [(40, 40), (264, 264), (33, 33), (40, 44), (7, 9)])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_combine_in_fp32_keeps_the_bits_of_its_gradient(dtype, H, pitch):
+    """A sum kept in 32 bits takes a gradient in 32 bits: numbers that 16 bits round (and, in fp16, that they cannot hold)."""
+    g, T, k, E = _gen(41), 90, 3, 5
+    ids = torch.randint(-1, E, (T, k), device="cuda", generator=g)
+    rows = ops.expert_layout(ids, E)
+    cap = rows.source.numel()
+    y = torch.randn(cap, H, device="cuda", generator=g).to(DT[dtype]).requires_grad_()
+    w = (0.001 + 0.01 * torch.rand(T, k, device="cuda", generator=g)).requires_grad_()
+    up = (1e5 * torch.randn(T, pitch, device="cuda", generator=g))[:, :H]
+    d_y, d_w = torch.autograd.grad(ops.expert_combine(y, w, rows, torch.float32), [y, w], up)
+    (plain,) = torch.autograd.grad(ops.expert_combine(y, None, rows, torch.float32), y, up / 1e5)
+    half, dest = _half_step(DT[dtype]), rows.dest.cpu()
+    u, yc, wc = up.double().cpu(), y.detach().double().cpu(), w.detach().double().cpu()
+    want_y, want_p, want_w, size_w = (torch.zeros(*s, dtype=torch.float64) for s in ((cap, H), (cap, H), (T, k), (T, k)))
+    for t in range(T):
+        for j in range(k):
+            d = int(dest[t, j])
+            if d >= 0:
+                want_y[d], want_p[d] = u[t] * wc[t, j], (up[t] / 1e5).double().cpu()
+                want_w[t, j], size_w[t, j] = (u[t] * yc[d]).sum(), (u[t] * yc[d]).abs().sum()
+    _within(d_y, want_y, (half + 2 * F) * want_y.abs() + 2.0 ** -25, "d y")             # a product in 32 bits, one rounding to 16
+    _within(plain, want_p, half * want_p.abs() + 2.0 ** -25, "d y of a plain sum")
+    _within(d_w, want_w, (H + 1) * F * size_w, "d weights")                             # (a rounding per term, in any order)
