@@ -16,14 +16,15 @@ inline cudaStream_t cur_stream() {
 inline void check(int rc, const char* what) {
   TORCH_CHECK(rc == 0, what, " failed with code ", rc, " (", rc > 0 ? cudaGetErrorString(static_cast<cudaError_t>(rc)) : "argument check", ")");
 }
-inline int code_of(const torch::Tensor& t, const char* what) {
-  switch (t.scalar_type()) {
+inline int code_of(at::ScalarType t, const char* what) {
+  switch (t) {
     case at::kBFloat16: return 0;
     case at::kHalf: return 1;
     case at::kFloat: return 2;
-    default: TORCH_CHECK_TYPE(false, what, ": bf16, fp16 or fp32, got ", t.scalar_type());
+    default: TORCH_CHECK_TYPE(false, what, ": bf16, fp16 or fp32, got ", t);
   }
 }
+inline int code_of(const torch::Tensor& t, const char* what) { return code_of(t.scalar_type(), what); }
 inline void same_device(const torch::Tensor& t, const torch::Tensor& as, const char* what) {
   TORCH_CHECK_VALUE(t.device() == as.device(), what, " is on ", t.device(), ", expected ", as.device());
 }
@@ -137,7 +138,9 @@ struct Combine : Function<Combine> {
                                bool fp32) {
     Maybe w;
     if (weight.has_value()) w = weight->to(at::kFloat).contiguous();
-    ctx->save_for_backward({w.has_value() ? y : torch::Tensor(), w.has_value() ? *w : torch::Tensor(), dest, source});
+    // (fixed weights learn nothing from the rows: these are not kept)
+    ctx->save_for_backward({w.has_value() && weight->requires_grad() ? y : torch::Tensor(), w.has_value() ? *w : torch::Tensor(), dest, source});
+    ctx->saved_data["columns"] = y.size(1);
     ctx->saved_data["type"] = static_cast<int64_t>(y.scalar_type());
     ctx->saved_data["weight_type"] = static_cast<int64_t>(weight.has_value() ? weight->scalar_type() : at::kFloat);
     return gather_rows(y, dest, w, fp32, "expert_combine");
@@ -150,15 +153,22 @@ struct Combine : Function<Combine> {
       const auto d = g[0].to(static_cast<at::ScalarType>(ctx->saved_data["type"].toInt()));
       return once({scatter_rows(d, source, dest, "expert_combine"), torch::Tensor(), torch::Tensor(), torch::Tensor(), torch::Tensor()}, g);
     }
-    const auto d = dense(g[0], "expert_combine"), y = dense(saved[0], "expert_combine");
+    const auto type = static_cast<at::ScalarType>(ctx->saved_data["type"].toInt());
+    const auto d = dense(g[0], "expert_combine");
     const bool fp32 = d.scalar_type() == at::kFloat;
-    TORCH_CHECK_VALUE(fp32 || d.scalar_type() == y.scalar_type(), "expert_combine: a gradient in ", y.scalar_type(), " or float32, got ", d.scalar_type());
-    auto d_y = at::empty({y.size(0), y.size(1)}, y.options()), d_w = at::empty_like(w);
-    check(rb_expert_combine_bwd(d.data_ptr(), d.stride(0), y.data_ptr(), y.stride(0), source.data_ptr<int>(), dest.data_ptr<int>(), w.data_ptr<float>(),
-                                d_y.data_ptr(), d_w.data_ptr<float>(), as_int(source.numel(), "expert_combine"), as_int(dest.size(0), "expert_combine"),
-                                as_int(dest.size(1), "expert_combine"), as_int(y.size(1), "expert_combine"), code_of(y, "expert_combine"), fp32, cur_stream()),
+    TORCH_CHECK_VALUE(fp32 || d.scalar_type() == type, "expert_combine: a gradient in ", type, " or float32, got ", d.scalar_type());
+    const int64_t cols = ctx->saved_data["columns"].toInt();
+    torch::Tensor y, d_y, d_w;      // what is asked for
+    if (ctx->needs_input_grad(0)) d_y = at::empty({source.numel(), cols}, d.options().dtype(type));
+    if (saved[0].defined() && ctx->needs_input_grad(1)) y = dense(saved[0], "expert_combine"), d_w = at::empty_like(w);
+    check(rb_expert_combine_bwd(d.data_ptr(), d.stride(0), y.defined() ? y.data_ptr() : nullptr, y.defined() ? y.stride(0) : 0, source.data_ptr<int>(),
+                                dest.data_ptr<int>(), w.data_ptr<float>(), d_y.defined() ? d_y.data_ptr() : nullptr,
+                                d_w.defined() ? d_w.data_ptr<float>() : nullptr, as_int(source.numel(), "expert_combine"),
+                                as_int(dest.size(0), "expert_combine"), as_int(dest.size(1), "expert_combine"), as_int(cols, "expert_combine"),
+                                code_of(type, "expert_combine"), fp32, cur_stream()),
           "rb_expert_combine_bwd");
-    return once({d_y, d_w.to(static_cast<at::ScalarType>(ctx->saved_data["weight_type"].toInt())), torch::Tensor(), torch::Tensor(), torch::Tensor()}, g);
+    if (d_w.defined()) d_w = d_w.to(static_cast<at::ScalarType>(ctx->saved_data["weight_type"].toInt()));
+    return once({d_y, d_w, torch::Tensor(), torch::Tensor(), torch::Tensor()}, g);
   }
 };
 torch::Tensor expert_combine(const torch::Tensor& y, const Maybe& weight, const torch::Tensor& dest, const torch::Tensor& source, bool fp32) {

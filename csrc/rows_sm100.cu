@@ -624,7 +624,8 @@ __host__ __device__ inline int padding_rows(int vecs) { return vecs >= 128 ? 8 :
 
 // Backward of the weighted sum: d_y[dest] = w d_out[t] and d_w = <d_out[t], y[dest]>.  A block per token holds its row of d_out (in the
 // type of the sum: fp32 for a sum kept in 32 bits) while it walks over the token's rows of y, so that all of them pass once; blocks behind
-// the tokens write the zeros of padding rows.
+// the tokens write the zeros of padding rows.  Without d_y (rows that do not learn) nothing is written to the buffer, without d_w (fixed
+// weights) y is not read, and need not be there.
 template <typename T, int N, typename G>
 __global__ void __launch_bounds__(N == 1 ? kSingleThreads : 256) sum_bwd_kernel(const G* __restrict__ d_out, long long ld, const T* __restrict__ y, long long ldy,
                                                       const int* __restrict__ source, const int* __restrict__ dest, const float* __restrict__ weight,
@@ -654,6 +655,7 @@ __global__ void __launch_bounds__(N == 1 ? kSingleThreads : 256) sum_bwd_kernel(
       wj[j] = d[j] >= 0 ? weight[row * k + j0 + j] : 0.f;
       dot[j] = 0.f;
     }
+    const bool read = d_w != nullptr, write = d_y != nullptr;
     if constexpr (N == 1) {      // four elements of a thread at a time, four rows in flight
       constexpr int S = 4;
       for (int v = t; v < vecs; v += S * kSingleThreads) {
@@ -670,7 +672,7 @@ __global__ void __launch_bounds__(N == 1 ? kSingleThreads : 256) sum_bwd_kernel(
             const T* b = y + (d[h + j] < 0 ? 0 : d[h + j]) * ldy + v;
 #pragma unroll
             for (int s = 0; s < S; ++s)
-              if (d[h + j] >= 0 && v + s * kSingleThreads < vecs) q[j][s] = b[s * kSingleThreads];
+              if (read && d[h + j] >= 0 && v + s * kSingleThreads < vecs) q[j][s] = b[s * kSingleThreads];
           }
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
@@ -678,8 +680,8 @@ __global__ void __launch_bounds__(N == 1 ? kSingleThreads : 256) sum_bwd_kernel(
 #pragma unroll
             for (int s = 0; s < S; ++s)
               if (d[h + j] >= 0 && v + s * kSingleThreads < vecs) {
-                dot[h + j] = fmaf(f[s], up(q[j][s]), dot[h + j]);
-                o[s * kSingleThreads] = down<T>(f[s] * wj[h + j]);
+                if (read) dot[h + j] = fmaf(f[s], up(q[j][s]), dot[h + j]);
+                if (write) o[s * kSingleThreads] = down<T>(f[s] * wj[h + j]);
               }
           }
         }
@@ -693,24 +695,28 @@ __global__ void __launch_bounds__(N == 1 ? kSingleThreads : 256) sum_bwd_kernel(
           Pack<T, N> q[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            if (d[h + j] >= 0) q[j] = reinterpret_cast<const Pack<T, N>*>(y + d[h + j] * ldy)[v];
+            if (read && d[h + j] >= 0) q[j] = reinterpret_cast<const Pack<T, N>*>(y + d[h + j] * ldy)[v];
 #pragma unroll
           for (int j = 0; j < 4; ++j)
             if (d[h + j] >= 0) {
               float b[N];
-              q[j].get(b);
+              if (read) {
+                q[j].get(b);
 #pragma unroll
-              for (int i = 0; i < N; ++i) {
-                dot[h + j] = fmaf(f[i], b[i], dot[h + j]);
-                b[i] = f[i] * wj[h + j];
+                for (int i = 0; i < N; ++i) dot[h + j] = fmaf(f[i], b[i], dot[h + j]);
               }
-              Pack<T, N> o;
-              o.set(b);
-              reinterpret_cast<Pack<T, N>*>(d_y + static_cast<long long>(d[h + j]) * cols)[v] = o;
+              if (write) {
+                Pack<T, N> o;
+#pragma unroll
+                for (int i = 0; i < N; ++i) b[i] = f[i] * wj[h + j];
+                o.set(b);
+                reinterpret_cast<Pack<T, N>*>(d_y + static_cast<long long>(d[h + j]) * cols)[v] = o;
+              }
             }
         }
       }
     }
+    if (!read) continue;
 #pragma unroll
     for (int j = 0; j < J; ++j) {
 #pragma unroll
@@ -972,7 +978,7 @@ int sum_bwd_t(const void* d_out, long long ld, const void* y, long long ldy, con
   const bool wide = wide_rows(y, ldy, cols, sizeof(T)) && wide_rows(d_y, cols, cols, sizeof(T)) && reinterpret_cast<uintptr_t>(d_out) % (NV * sizeof(G)) == 0 &&
                     ld % NV == 0;      // (so many elements of a row of d_out are one vector, too)
   const int threads = row_threads(cols / (wide ? NV : 1), !wide);
-  const long long warps = threads / 32, some = padding_rows(cols / (wide ? NV : 1)), grid = n + ((cap + some - 1) / some + warps - 1) / warps;
+  const long long warps = threads / 32, some = padding_rows(cols / (wide ? NV : 1)), grid = n + (d_y ? ((cap + some - 1) / some + warps - 1) / warps : 0);
   if (grid > kMaxGrid) return -3;
   const G* a = static_cast<const G*>(d_out);
   const T* b = static_cast<const T*>(y);
@@ -1073,11 +1079,11 @@ extern "C" int rb_expert_combine(const void* y, long long ld, const int* dest, c
   return -1;
 }
 
-// out_fp32: d_out is in fp32, whatever the type of y
+// out_fp32: d_out is in fp32, whatever the type of y.  d_y and d_w may be null: that gradient is not asked for; y is null where d_w is.
 extern "C" int rb_expert_combine_bwd(const void* d_out, long long ld, const void* y, long long ldy, const int* source, const int* dest, const float* weight,
                                      void* d_y, float* d_w, int cap, int n, int k, int cols, int dtype, int out_fp32, cudaStream_t st) {
   if (k < 1 || n < 0 || cap < 0 || cols < 0) return -1;
-  if (cap == 0 && n == 0) return 0;
+  if ((cap == 0 && n == 0) || (!d_y && (!d_w || n == 0))) return 0;
   switch (dtype) {
     case 0:
       return out_fp32 ? sum_bwd_t<__nv_bfloat16, float>(d_out, ld, y, ldy, source, dest, weight, d_y, d_w, cap, n, k, cols, st)

@@ -846,3 +846,29 @@ def test_combine_in_fp32_keeps_the_bits_of_its_gradient(dtype, H, pitch):
     _within(d_y, want_y, (half + 2 * F) * want_y.abs() + 2.0 ** -25, "d y")             # a product in 32 bits, one rounding to 16
     _within(plain, want_p, half * want_p.abs() + 2.0 ** -25, "d y of a plain sum")
     _within(d_w, want_w, (H + 1) * F * size_w, "d weights")                             # (a rounding per term, in any order)
+
+
+@pytest.mark.parametrize("H,k", [(264, 3), (33, 11)])
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_combine_gives_the_gradients_that_are_asked_for(dtype, H, k):
+    """Rows are neither kept for weights that are fixed nor written for rows that are; what is given is what both together give."""
+    g, T, E = _gen(42), 70, 5
+    rows = ops.expert_layout(torch.randint(-1, E, (T, k), device="cuda", generator=g), E)
+    y = torch.randn(rows.source.numel(), H, device="cuda", generator=g).to(DT[dtype])
+    w, up = torch.rand(T, k, device="cuda", generator=g), torch.randn(T, H, device="cuda", generator=g).to(DT[dtype])
+    yl, wl = y.clone().requires_grad_(), w.clone().requires_grad_()
+    want = torch.autograd.grad(ops.expert_combine(yl, wl, rows), [yl, wl], up)
+    kept = yl * 1.0
+    out = ops.expert_combine(kept, w, rows)
+    with torch.no_grad():
+        kept.zero_()                          # (an error in the backward pass, if it were kept for it)
+    (d_y,) = torch.autograd.grad(out, yl, up)
+    assert torch.equal(d_y, want[0])
+    before = torch.cuda.memory_allocated()
+    out = ops.expert_combine(y, wl, rows)
+    torch.cuda.reset_peak_memory_stats()
+    (d_w,) = torch.autograd.grad(out, wl, up)
+    assert torch.equal(d_w, want[1])
+    assert torch.cuda.max_memory_allocated() - before < y.numel() * y.element_size()
+    (d_w,) = torch.autograd.grad(ops.expert_combine(yl, wl, rows), wl, up)      # only one of two is asked for
+    assert torch.equal(d_w, want[1])
