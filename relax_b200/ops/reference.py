@@ -754,6 +754,11 @@ def expert_layout(expert_of_row, num_experts: int, align: int = 128) -> ExpertRo
     return ExpertRows(dest.view(expert_of_row.shape).int(), source[:cap].int(), tiles, first.int(), num_experts, align)
 
 
+def _sum_type(t):
+    """Sums are held in 32 bits, those of 64-bit rows in 64."""
+    return torch.promote_types(t.dtype, torch.float32)
+
+
 def _with_zero_row(t):
     return torch.cat([t, t.new_zeros(1, t.shape[1])])
 
@@ -767,10 +772,10 @@ def expert_combine(y, weights, rows: ExpertRows, dtype=None):
     d = rows.dest.long()
     here = d >= 0
     yz = _with_zero_row(y)
-    acc = torch.zeros(d.shape[0], y.shape[1], dtype=torch.float32, device=y.device)
+    acc = torch.zeros(d.shape[0], y.shape[1], dtype=_sum_type(y), device=y.device)
     for j in range(d.shape[1]):
-        v = yz[torch.where(here[:, j], d[:, j], y.shape[0])].float()
-        acc = acc + (v if weights is None else v * torch.where(here[:, j], weights[:, j].float(), 0.0)[:, None])
+        v = yz[torch.where(here[:, j], d[:, j], y.shape[0])].to(acc.dtype)
+        acc = acc + (v if weights is None else v * torch.where(here[:, j], weights[:, j].to(acc.dtype), 0.0)[:, None])
     return acc.to(dtype or y.dtype)
 
 
@@ -792,17 +797,17 @@ class _Embedding(torch.autograd.Function):
             return weight.new_zeros(*tokens.shape, weight.shape[1])
         out = weight.detach()[at]
         if scale != 1.0:
-            out = (out.float() * scale).to(weight.dtype)
+            out = (out.to(_sum_type(out)) * scale).to(weight.dtype)
         return torch.where(here[..., None], out, torch.zeros((), dtype=out.dtype, device=out.device))
 
     @staticmethod
     def backward(ctx, dy):
         at, here = ctx.saved_tensors
         w, mg = ctx.weight, main_grad_of(ctx.weight)
-        g = torch.zeros(w.shape, dtype=torch.float32, device=w.device) if mg is None else mg
+        g = torch.zeros(w.shape, dtype=_sum_type(w), device=w.device) if mg is None else mg
         if w.shape[0]:
             # repeated tokens are summed in a fixed order (bit-identical reruns)
-            d = dy[here].float()
+            d = dy[here].to(g.dtype)
             g.index_put_((at[here],), d * ctx.scale if ctx.scale != 1.0 else d, accumulate=True)
         return (g.to(w.dtype) if mg is None else None), None, None, None
 

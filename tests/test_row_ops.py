@@ -286,3 +286,33 @@ def test_extension_uses_the_process_s_cxx_runtime():
         pytest.skip("readelf and a built extension")
     found = subprocess.run(["readelf", "-d", SO_PATH], capture_output=True, text=True, check=True).stdout
     assert "[libstdc++.so" in found
+
+
+def test_rows_of_64_bits_keep_them():
+    """A model in double precision on the CPU: sums, factors and gradients are in 64 bits, off by their own roundings only."""
+    g, D = _gen(5), 2.0 ** -53
+    ids = torch.randint(-1, 4, (30, 3), generator=g)
+    rows = ops.expert_layout(ids, 4, 8)
+    dest = rows.dest.reshape(-1).tolist()
+    y = torch.randn(rows.source.numel(), 6, generator=g, dtype=torch.float64).requires_grad_()
+    w = torch.rand(30, 3, generator=g, dtype=torch.float64).requires_grad_()
+    out = ops.expert_combine(y, w, rows)
+    want, size = O.combine(y.detach(), w.detach(), dest, 3)
+    assert out.dtype == torch.float64 and ((out - want).abs() <= 4 * D * size).all()
+    assert torch.equal(ops.expert_combine(y, w, rows, torch.float32), out.float())
+    up = torch.randn(30, 6, generator=g, dtype=torch.float64)
+    d_y, d_w = torch.autograd.grad(out, [y, w], up)
+    for i, d in enumerate(dest):
+        if d >= 0:
+            assert torch.equal(d_y[d], up[i // 3] * w.detach().reshape(-1)[i])
+            terms = up[i // 3] * y[d].detach()
+            assert abs(float(d_w.reshape(-1)[i] - terms.sum())) <= 12 * D * float(terms.abs().sum())
+    table = torch.randn(9, 5, generator=g, dtype=torch.float64).requires_grad_()
+    tok = torch.randint(-1, 10, (200,), generator=g)
+    got = ops.embedding(tok, table, 1.0 / 3.0)
+    here = (tok >= 0) & (tok < 9)
+    assert torch.equal(got[here], table.detach()[tok[here]] * (1.0 / 3.0)) and not got[~here].any()
+    dy = torch.randn(200, 5, generator=g, dtype=torch.float64)
+    (d,) = torch.autograd.grad(got, table, dy)
+    want, size = O.embedding_grad(tok, dy, 9, 0, 1.0 / 3.0)
+    assert d.dtype == torch.float64 and ((d - want).abs() <= 210 * D * size).all()
