@@ -763,9 +763,20 @@ def _with_zero_row(t):
     return torch.cat([t, t.new_zeros(1, t.shape[1])])
 
 
+class _Dispatch(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, rows):
+        s, k = rows.source.long(), rows.dest.shape[1]
+        ctx.rows = rows
+        return _with_zero_row(x)[torch.where(s < 0, x.shape[0], torch.div(s, k, rounding_mode="floor"))]
+
+    @staticmethod
+    def backward(ctx, dy):
+        return expert_combine(dy, None, ctx.rows), None
+
+
 def expert_dispatch(x, rows: ExpertRows):
-    s, k = rows.source.long(), rows.dest.shape[1]
-    return _with_zero_row(x)[torch.where(s < 0, x.shape[0], torch.div(s, k, rounding_mode="floor"))]
+    return _Dispatch.apply(x, rows)
 
 
 def expert_combine(y, weights, rows: ExpertRows, dtype=None):

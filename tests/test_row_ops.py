@@ -316,3 +316,15 @@ def test_rows_of_64_bits_keep_them():
     (d,) = torch.autograd.grad(got, table, dy)
     want, size = O.embedding_grad(tok, dy, 9, 0, 1.0 / 3.0)
     assert d.dtype == torch.float64 and ((d - want).abs() <= 210 * D * size).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_gradient_of_copied_rows_is_summed_in_32_bits(dtype):
+    g, k = _gen(6), 8
+    rows = ops.expert_layout(torch.randint(-1, 6, (20, k), generator=g), 6, 4)
+    x = torch.randn(20, 5, generator=g).to(dtype).requires_grad_()
+    up = torch.randn(rows.source.numel(), 5, generator=g).to(dtype)
+    (d,) = torch.autograd.grad(ops.expert_dispatch(x, rows), x, up)
+    want, size = O.combine(up, None, rows.dest.reshape(-1).tolist(), k)
+    half = torch.finfo(dtype).eps / 2
+    assert d.dtype == dtype and ((d.double() - want).abs() <= half * want.abs() + (1 + half) * (k + 1) * 2.0 ** -24 * size + 2.0 ** -25).all()
