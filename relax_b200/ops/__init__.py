@@ -394,7 +394,8 @@ def fused_lm_head_topk_distill(hidden, weight, ids, teacher_log_probs, kl_type: 
     if _use_cuda(hidden):
         return _cuda().fused_lm_head_topk_distill(hidden, weight, ids, teacher_log_probs, kl_type, float(alpha), norm_mode, float(temperature),
                                                   log_prob_min_clamp, chunk_size)
-    out = [ref.topk_distill(hidden[s:s + chunk_size] @ weight.t(), ids[s:s + chunk_size], teacher_log_probs[s:s + chunk_size], kl_type, alpha, norm_mode,
+    full = torch.promote_types(hidden.dtype, torch.float32)      # (16-bit products would be rounded before the divergence)
+    out = [ref.topk_distill(hidden[s:s + chunk_size].to(full) @ weight.t().to(full), ids[s:s + chunk_size], teacher_log_probs[s:s + chunk_size], kl_type, alpha, norm_mode,
                             temperature, log_prob_min_clamp, False) for s in range(0, max(1, hidden.shape[0]), chunk_size)]
     return torch.cat(out)
 

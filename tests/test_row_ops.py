@@ -328,3 +328,21 @@ def test_gradient_of_copied_rows_is_summed_in_32_bits(dtype):
     want, size = O.combine(up, None, rows.dest.reshape(-1).tolist(), k)
     half = torch.finfo(dtype).eps / 2
     assert d.dtype == dtype and ((d.double() - want).abs() <= half * want.abs() + (1 + half) * (k + 1) * 2.0 ** -24 * size + 2.0 ** -25).all()
+
+
+def test_fused_head_of_16_bit_weights_has_32_bit_logits():
+    g = _gen(8)
+    _, ids, t, w = _rows(7, 40, 4, 9)
+    h, wt = (3 * torch.randn(7, 64, generator=g)).bfloat16().requires_grad_(), torch.randn(40, 64, generator=g).bfloat16().requires_grad_()
+    loss = ops.fused_lm_head_topk_distill(h, wt, ids, t, chunk_size=3)
+    hd, wd = h.detach().double().requires_grad_(), wt.detach().double().requires_grad_()
+    want, _, size = O.distill(hd.detach() @ wd.detach().t(), ids, t, w)
+    # a logit is off by its 64 products' roundings, the divergence by as much times its terms
+    logit = 65 * 2.0 ** -24 * (hd.detach().abs() @ wd.detach().abs().t()).amax(1)
+    assert loss.dtype == torch.float32 and ((loss.detach().double() - want).abs() <= 2.0 ** -24 * want.abs() + 4 * logit * size).all()
+    d_h, d_w = torch.autograd.grad(loss, [h, wt], w)
+    exact = ops.topk_distill(hd @ wd.t(), ids, t)
+    e_h, e_w = torch.autograd.grad(exact, [hd, wd], w)
+    assert d_h.dtype == d_w.dtype == torch.bfloat16
+    for got, e in ((d_h, e_h), (d_w, e_w)):      # rounded to bf16 once, of a whole row's or (the head's, in pieces) three pieces' sums
+        assert float((got.double() - e).norm() / e.norm()) < 3 * 2.0 ** -8
