@@ -378,7 +378,7 @@ def topk_distill(logits, ids, teacher_log_probs, kl_type: str = "reverse_kl", al
                  log_prob_min_clamp=None, return_log_probs: bool = False):
     """Divergence ``[R]`` of a student, given by whole rows of ``logits [R, V]``, from a teacher known on ``K`` ids per row (``ids [R, K]``, entries
     outside ``0 .. V - 1`` are absent; fp32 ``teacher_log_probs [R, K]``): :func:`relax_b200.algo.opd.token_kl` on the student's log-probs of the
-    ids, differentiable in the logits.  The forward pass reads the logits once, the backward pass once more; rows whose incoming gradient is
+    ids, differentiable in the logits (the teacher gets no gradient).  The forward pass reads the logits once, the backward pass once more; rows whose incoming gradient is
     zero get zeros.  With ``return_log_probs`` also the student's log-probs of the ids (-inf where absent; no gradient)."""
     if logits.dim() != 2 or logits.shape[1] < 1:
         raise ValueError(f"topk_distill: logits [rows, vocabulary], got {tuple(logits.shape)}")

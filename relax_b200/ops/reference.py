@@ -835,7 +835,7 @@ def topk_distill(logits, ids, teacher_log_probs, kl_type, alpha, norm_mode, temp
     z = (logits.double() / temperature).masked_fill(away.all(1, keepdim=True), 0.0)       # (a row without ids has nothing to compare)
     lp = torch.log_softmax(z, -1).gather(1, torch.where(away, 0, ids))
     found = lp.masked_fill(away, float("-inf")).float()
-    t = teacher_log_probs.double()
+    t = teacher_log_probs.detach().double()
     if log_prob_min_clamp is not None:
         lp, t = lp.clamp_min(log_prob_min_clamp), t.clamp_min(log_prob_min_clamp)
     none = torch.zeros((), dtype=torch.float64, device=z.device)

@@ -346,3 +346,12 @@ def test_fused_head_of_16_bit_weights_has_32_bit_logits():
     assert d_h.dtype == d_w.dtype == torch.bfloat16
     for got, e in ((d_h, e_h), (d_w, e_w)):      # rounded to bf16 once, of a whole row's or (the head's, in pieces) three pieces' sums
         assert float((got.double() - e).norm() / e.norm()) < 3 * 2.0 ** -8
+
+
+def test_teacher_gets_no_gradient():
+    z, ids, t, w = _rows(4, 30, 5, 3)
+    t.requires_grad_()
+    assert not ops.topk_distill(z, ids, t, "jsd").requires_grad
+    zl = z.clone().requires_grad_()
+    d_z, d_t = torch.autograd.grad(ops.topk_distill(zl, ids, t, "jsd"), [zl, t], w, allow_unused=True)
+    assert d_t is None and bool(d_z.any())
