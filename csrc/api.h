@@ -218,7 +218,7 @@ int rb_moe_gemm(const void* X, const void* W, void* out, const int* tiles, const
 // ---- rows by key (rows_sm100.cu) and distillation (distill_sm100.cu); dtype 0 = bf16, 1 = fp16, 2 = fp32; ids int64 (wide) or int32
 int rb_sort_counters(long long n, int bins);
 int rb_expert_layout(const void* ids, int wide, int n, int experts, int align, int cap, int* dest, int* source, int* tile_expert, int* bounds, int* hist,
-                     cudaStream_t st);
+                     int* err, cudaStream_t st);
 int rb_expert_dispatch(const void* x, long long ld, const int* source, const int* dest, void* out, int cap, int n, int k, int cols, int dtype,
                        cudaStream_t st);
 int rb_expert_combine(const void* y, long long ld, const int* dest, const float* weight, void* out, int n, int k, int cols, int dtype, int out_fp32,
@@ -226,7 +226,7 @@ int rb_expert_combine(const void* y, long long ld, const int* dest, const float*
 int rb_expert_combine_bwd(const void* d_out, long long ld, const void* y, long long ldy, const int* source, const int* dest, const float* weight, void* d_y,
                           float* d_w, int cap, int n, int k, int cols, int dtype, int out_fp32, cudaStream_t st);
 int rb_embedding(const void* ids, int wide, long long start, const void* table, long long ld, int rows, void* out, int n, int cols, float scale, int dtype,
-                 cudaStream_t st);
+                 int* err, cudaStream_t st);
 int rb_embedding_bwd_bins(int rows);
 int rb_embedding_bwd(const void* ids, int wide, long long start, const void* dy, long long ld, void* out, int add, int2* pairs, int* hist, float* part,
                      int* open, int n, int rows, int cols, float scale, int dtype, cudaStream_t st);

@@ -50,6 +50,13 @@ inline torch::Tensor part_of(const torch::Tensor& all, int64_t offset, at::IntAr
   t.unsafeGetTensorImpl()->set_sizes_contiguous(shape);
   return t;
 }
+// the device's status word, where ids outside a whole table are to be noted
+inline int* status(const c10::optional<torch::Tensor>& err, const torch::Tensor& as) {
+  if (!err.has_value()) return nullptr;
+  same_device(*err, as, "the status word");
+  TORCH_CHECK_VALUE(err->scalar_type() == at::kInt && err->numel() >= 1, "the status word is an int32");
+  return err->data_ptr<int>();
+}
 inline bool recorded(const torch::Tensor& t) { return t.requires_grad() && at::GradMode::is_enabled(); }
 
 using torch::autograd::AutogradContext;
@@ -76,7 +83,7 @@ variable_list once(variable_list grads, const variable_list& incoming) {
 // ----------------------------------------------------------------------------- experts' rows
 
 // (dest [T, k], source [cap], tile_expert [cap / align] or None, bounds [E + 1])
-py::tuple expert_layout(torch::Tensor ids, int64_t experts, int64_t align) {
+py::tuple expert_layout(torch::Tensor ids, int64_t experts, int64_t align, const Maybe& err) {
   const c10::cuda::CUDAGuard guard(ids.device());
   ids = ids.contiguous();
   const int wide = wide_ids(ids, "expert_layout");
@@ -90,7 +97,7 @@ py::tuple expert_layout(torch::Tensor ids, int64_t experts, int64_t align) {
   int* p = all.data_ptr<int>();
   const int64_t at_source = n, at_bounds = at_source + cap, at_tiles = at_bounds + experts + 1, at_hist = at_tiles + (align > 1 ? tiles : 0);
   check(rb_expert_layout(ids.data_ptr(), wide, n, static_cast<int>(experts), static_cast<int>(align), static_cast<int>(cap), p, p + at_source,
-                         align > 1 ? p + at_tiles : nullptr, p + at_bounds, counters > 1 ? p + at_hist : nullptr, cur_stream()),
+                         align > 1 ? p + at_tiles : nullptr, p + at_bounds, counters > 1 ? p + at_hist : nullptr, status(err, ids), cur_stream()),
         "rb_expert_layout");
   return py::make_tuple(part_of(all, 0, ids.sizes()), part_of(all, at_source, {cap}), align > 1 ? py::cast(part_of(all, at_tiles, {tiles})) : py::none(),
                         part_of(all, at_bounds, {experts + 1}));
@@ -179,7 +186,7 @@ torch::Tensor expert_combine(const torch::Tensor& y, const Maybe& weight, const 
 
 // ----------------------------------------------------------------------------- embedding
 
-torch::Tensor look_up(const torch::Tensor& weight, const torch::Tensor& ids, double scale, int64_t start) {
+torch::Tensor look_up(const torch::Tensor& weight, const torch::Tensor& ids, double scale, int64_t start, const Maybe& err) {
   const c10::cuda::CUDAGuard guard(weight.device());
   const auto table = dense(weight, "embedding");
   const int wide = wide_ids(ids, "embedding");
@@ -189,7 +196,7 @@ torch::Tensor look_up(const torch::Tensor& weight, const torch::Tensor& ids, dou
   auto out = at::empty(shape, table.options());
   check(rb_embedding(ids.data_ptr(), wide, start, table.data_ptr(), table.stride(0), as_int(table.size(0), "embedding: table rows"), out.data_ptr(),
                      as_int(ids.numel(), "embedding: tokens"), as_int(table.size(1), "embedding: columns"), static_cast<float>(scale),
-                     code_of(table, "embedding"), cur_stream()),
+                     code_of(table, "embedding"), status(err, table), cur_stream()),
         "rb_embedding");
   return out;
 }
@@ -197,13 +204,13 @@ torch::Tensor look_up(const torch::Tensor& weight, const torch::Tensor& ids, dou
 // The gradient is a new matrix in the rows' type, or is added to `main_grad` (fp32), which then stands for it.
 struct Embedding : Function<Embedding> {
   static torch::Tensor forward(AutogradContext* ctx, const torch::Tensor& weight, const torch::Tensor& ids, double scale, int64_t start,
-                               const Maybe& main_grad) {
+                               const Maybe& main_grad, const Maybe& err) {
     ctx->save_for_backward({ids});
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["start"] = start;
     ctx->saved_data["rows"] = weight.size(0);
     ctx->saved_data["main_grad"] = main_grad;
-    return look_up(weight, ids, scale, start);
+    return look_up(weight, ids, scale, start, err);
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     const auto saved = ctx->get_saved_variables();
@@ -223,17 +230,19 @@ struct Embedding : Function<Embedding> {
                            into.has_value(), reinterpret_cast<int2*>(p), p + at_hist, reinterpret_cast<float*>(p + at_part), p + at_open, n, V, cols,
                            static_cast<float>(ctx->saved_data["scale"].toDouble()), code_of(dy, "embedding"), cur_stream()),
           "rb_embedding_bwd");
-    return once({into.has_value() ? torch::Tensor() : out, torch::Tensor(), torch::Tensor(), torch::Tensor(), torch::Tensor()}, g);
+    variable_list d(6);
+    if (!into.has_value()) d[0] = out;
+    return once(d, g);
   }
 };
-torch::Tensor embedding(const torch::Tensor& weight, const torch::Tensor& tokens, double scale, int64_t start, const Maybe& main_grad) {
+torch::Tensor embedding(const torch::Tensor& weight, const torch::Tensor& tokens, double scale, int64_t start, const Maybe& main_grad, const Maybe& err) {
   if (main_grad.has_value()) {
     same_device(*main_grad, weight, "embedding: main_grad");
     TORCH_CHECK_VALUE(main_grad->scalar_type() == at::kFloat && main_grad->is_contiguous() && main_grad->sizes() == weight.sizes(),
                       "embedding: main_grad is a dense fp32 matrix of the table's shape");
   }
   const auto ids = tokens.contiguous();
-  return recorded(weight) ? Embedding::apply(weight, ids, scale, start, main_grad) : look_up(weight, ids, scale, start);
+  return recorded(weight) ? Embedding::apply(weight, ids, scale, start, main_grad, err) : look_up(weight, ids, scale, start, err);
 }
 
 // ----------------------------------------------------------------------------- distillation from top ids
@@ -321,10 +330,11 @@ py::tuple topk_distill_rows(const torch::Tensor& z, const torch::Tensor& ids, co
 }  // namespace
 
 void register_rows(pybind11::module_& m) {
-  m.def("expert_layout", &expert_layout);
+  m.def("expert_layout", &expert_layout, py::arg("ids"), py::arg("experts"), py::arg("align"), py::arg("err") = py::none());
   m.def("expert_dispatch", &expert_dispatch);
   m.def("expert_combine", &expert_combine);
-  m.def("embedding", &embedding);
+  m.def("embedding", &embedding, py::arg("weight"), py::arg("tokens"), py::arg("scale"), py::arg("start"), py::arg("main_grad"),
+        py::arg("err") = py::none());
   m.def("topk_distill", &topk_distill);
   m.def("topk_distill_rows", &topk_distill_rows);
   m.def("topk_distill_rows_bwd", &distill_rows_bwd);

@@ -88,12 +88,20 @@ __device__ __forceinline__ Pack<T, N> zeros() {
 // moves the counter.  Counters of warps in front, and of blocks in front (count_kernel's), are added then.
 // Up to kOneBlock rows take place_kernel alone.
 
-struct ExpertKeys {      // expert ids; others than 0 .. bins - 1 live elsewhere and take no part
+constexpr int kOutside = 4;      // status word: an id lies outside a table that is whole
+__device__ __noinline__ void note_outside(int* err) {
+  if (err != nullptr) atomicCAS(err, 0, kOutside);
+}
+
+struct ExpertKeys {      // expert ids; others than 0 .. bins - 1 live elsewhere and take no part (where nobody else has experts: noted)
   const void* ids;
   int wide, bins;
+  int* err;
   __device__ __forceinline__ int digit(int i) const {
     const long long e = wide ? static_cast<const long long*>(ids)[i] : static_cast<const int*>(ids)[i];
-    return e >= 0 && e < bins ? static_cast<int>(e) : -1;
+    if (e >= 0 && e < bins) return static_cast<int>(e);
+    note_outside(err);
+    return -1;
   }
 };
 struct TokenKeys {      // first pass over token ids: a row's key is its table row, or `rows` (behind all) for tokens of other shards
@@ -453,9 +461,12 @@ struct TokenRow {      // row r <- table row of its token
   const void* ids;
   int wide, rows;
   long long start;
+  int* err;
   __device__ __forceinline__ long long row(long long r) const {
     const long long a = (wide ? static_cast<const long long*>(ids)[r] : static_cast<const int*>(ids)[r]) - start;
-    return a >= 0 && a < rows ? a : -1;
+    if (a >= 0 && a < rows) return a;
+    note_outside(err);
+    return -1;
   }
 };
 
@@ -1030,12 +1041,13 @@ using namespace rb::rows;
 
 extern "C" int rb_sort_counters(long long n, int bins) { return n > 0 && sort_blocks(n) > 1 ? sort_blocks(n) * bins : 1; }
 
+// err (or null, where other ranks hold experts): a word that becomes 4 where an id is none of 0 .. experts - 1
 extern "C" int rb_expert_layout(const void* ids, int wide, int n, int experts, int align, int cap, int* dest, int* source, int* tile_expert, int* bounds,
-                                int* hist, cudaStream_t st) {
+                                int* hist, int* err, cudaStream_t st) {
   if (n < 0 || n > kMaxSort || experts < 1 || experts > kMaxBins || align < 1 || cap < 0 || cap % align) return -1;
   const int tiles = align > 1 ? cap / align : 0;
   int at = 0;
-  return sort_pass(ExpertKeys{ids, wide, experts}, ExpertOut{dest, source, align > 1 ? tile_expert : nullptr, bounds, cap, tiles}, n, experts, align, hist,
+  return sort_pass(ExpertKeys{ids, wide, experts, err}, ExpertOut{dest, source, align > 1 ? tile_expert : nullptr, bounds, cap, tiles}, n, experts, align, hist,
                    Fill{source, cap, nullptr, 0, 0, nullptr, 0, nullptr}, 1, &at, st);
 }
 
@@ -1096,10 +1108,11 @@ extern "C" int rb_expert_combine_bwd(const void* d_out, long long ld, const void
   return -1;
 }
 
+// err (or null, for a shard): a word that becomes 4 where a token lies outside the table
 extern "C" int rb_embedding(const void* ids, int wide, long long start, const void* table, long long ld, int rows, void* out, int n, int cols, float scale,
-                            int dtype, cudaStream_t st) {
+                            int dtype, int* err, cudaStream_t st) {
   if (n < 0 || cols < 0 || rows < 0) return -1;
-  return move_any(table, ld, TokenRow{ids, wide, rows, start}, out, n, cols, scale, dtype, st);
+  return move_any(table, ld, TokenRow{ids, wide, rows, start, err}, out, n, cols, scale, dtype, st);
 }
 
 extern "C" int rb_embedding_bwd_bins(int rows) {      // counters of one block in every pass

@@ -141,24 +141,24 @@ def padded_expert_layout(expert_of_row: torch.Tensor, num_experts: int, align: i
     return order, dest, cap, tile_expert, expert_rows
 
 
-def experts_mlp(x, expert, weights, w1, w2, dtype=None):
+def experts_mlp(x, expert, weights, w1, w2, dtype=None, whole: bool = False):
     """SwiGLU expert MLPs of ``x [T, H]`` for routed rows with (local) expert ids ``expert [T, k]``: rows are copied into a buffer sorted by
     expert, the two grouped GEMMs (one launch each for all experts) and the activation run on it, and every token's rows come back as
     their sum with ``weights [T, k]`` (None: ones) in ``dtype`` (that of ``x``).  ``w1 [E, 2F, H]``, ``w2 [E, H, F]``.  Ids outside ``[0, E)`` (experts that live on
-    another rank) cost nothing and count nothing."""
+    another rank) cost nothing and count nothing; with ``whole`` there are none (:func:`relax_b200.ops.expert_layout`)."""
     if not x.shape[0]:      # no rows: one that belongs to nobody, so that the graph still reaches the weights
         pad = torch.nn.functional.pad
         return experts_mlp(pad(x, (0, 0, 0, 1)), expert.new_full((1, expert.shape[1]), -1), None if weights is None else pad(weights, (0, 0, 0, 1)),
                            w1, w2, dtype)[:0]
-    rows = ops.expert_layout(expert, w1.shape[0], EXPERT_ROW_ALIGN)
+    rows = ops.expert_layout(expert, w1.shape[0], EXPERT_ROW_ALIGN, whole)
     a = ops.swiglu(ops.grouped_linear(ops.expert_dispatch(x, rows), w1, rows.tile_expert, rows.expert_rows))
     return ops.expert_combine(ops.grouped_linear(a, w2, rows.tile_expert, rows.expert_rows), weights, rows, dtype)
 
 
 def grouped_swiglu_mlp(x, expert_of_row, w1, w2, skip_foreign: bool = False):
     """:func:`experts_mlp` of rows ``x [R, H]`` with one expert each, in the ORIGINAL row order.  With ``skip_foreign`` rows whose id is
-    outside ``[0, E)`` come back as zeros."""
-    return experts_mlp(x, expert_of_row[:, None], None, w1, w2)
+    outside ``[0, E)`` come back as zeros; otherwise such an id is an error."""
+    return experts_mlp(x, expert_of_row[:, None], None, w1, w2, whole=not skip_foreign)
 
 
 def route_tokens(logits, cfg, bias=None):
@@ -260,11 +260,11 @@ class MoEMLP(nn.Module):
             self.last_counts = counts.detach() if self.last_counts is None else self.last_counts + counts.detach()
         if ps.ep.size > 1:
             # copies of the tokens in the order of their experts, so that every rank's rows lie together
-            rows = ops.expert_layout(idx, E, 1)
+            rows = ops.expert_layout(idx, E, 1, whole=True)
             xp = ops.expert_dispatch(x, rows)
             out = ops.expert_combine(self._on_owners(xp, rows.expert_rows.diff().long()), w, rows)
         else:
-            out = experts_mlp(x, idx, w, self.experts.linear_fc1.weight, self.experts.linear_fc2.weight)
+            out = experts_mlp(x, idx, w, self.experts.linear_fc1.weight, self.experts.linear_fc2.weight, whole=True)
         if cfg.moe_shared_expert_ffn > 0:
             out = out + self._shared(x).to(out.dtype)
         return out.to(x.dtype)

@@ -307,11 +307,13 @@ def grouped_linear(x, w, tile_expert, expert_rows):
     return ref.grouped_linear(x, w, tile_expert, expert_rows)
 
 
-def expert_layout(expert_of_row, num_experts: int, align: int = 128):
+def expert_layout(expert_of_row, num_experts: int, align: int = 128, whole: bool = False):
     """Layout of routed rows sorted by expert: ``expert_of_row`` (``[T, k]`` or ``[R]``, int64 or int32) names the expert of every routed row;
     ids outside ``0 .. num_experts - 1`` live elsewhere and get no place.  Rows of an expert keep their order, and every expert begins at a
     multiple of ``align`` (128: the tiles of :func:`grouped_linear`; 1: no padding).  Nothing is read back: the buffer has room for any routing,
-    ``min(R, E) + (R - min(R, E)) // align`` tiles.  Returns :class:`relax_b200.ops.reference.ExpertRows`."""
+    ``min(R, E) + (R - min(R, E)) // align`` tiles.  ``whole``: no expert lives elsewhere, and an id outside the range is an error: raised on the
+    CPU, left in the device's status word on a GPU (:func:`relax_b200.ops.cuda.check_error_flag`).  Returns
+    :class:`relax_b200.ops.reference.ExpertRows`."""
     if expert_of_row.dim() not in (1, 2) or expert_of_row.dtype not in (torch.int64, torch.int32):
         raise ValueError(f"expert_layout: int64 or int32 ids of shape [T, k] or [R], got {expert_of_row.dtype} {tuple(expert_of_row.shape)}")
     if not 1 <= num_experts <= 2048 or not 1 <= align <= 65536:
@@ -319,7 +321,11 @@ def expert_layout(expert_of_row, num_experts: int, align: int = 128):
     ids = expert_of_row if expert_of_row.dim() == 2 else expert_of_row[:, None]
     if ids.shape[1] < 1:
         raise ValueError("expert_layout: at least one expert per row")
-    return (_cuda() if _use_cuda(ids) else ref).expert_layout(ids, int(num_experts), int(align))
+    if _use_cuda(ids):
+        return _cuda().expert_layout(ids, int(num_experts), int(align), whole)
+    if whole and ids.numel() and not 0 <= int(ids.min()) <= int(ids.max()) < num_experts:
+        raise IndexError(f"expert_layout: expert ids {int(ids.min())} .. {int(ids.max())} of {num_experts} experts")
+    return ref.expert_layout(ids, int(num_experts), int(align))
 
 
 def _rows_match(what, t, n):
@@ -350,12 +356,15 @@ def embedding(tokens, weight, scale: float = 1.0, vocab_start: int = 0, whole: b
     """``scale * weight[tokens - vocab_start]``, zeros for tokens outside the table's rows (those of other shards).  The gradient sorts the
     tokens and sums every table row's incoming rows in 32 bits in a fixed order, so reruns give the same bits; it is added to the
     weight's fp32 ``main_grad`` where there is one at the time of the lookup, which touches only rows that were looked up.  ``whole``: the table
-    is the whole vocabulary, and on the CPU a token outside it raises (on a GPU nothing is read back)."""
+    is the whole vocabulary, and a token outside it is an error: raised on the CPU, left in the device's status word on a GPU
+    (:func:`relax_b200.ops.cuda.check_error_flag`; its row is zeros)."""
     if tokens.dtype not in (torch.int64, torch.int32) or weight.dim() != 2:
         raise ValueError(f"embedding: int64 or int32 tokens and a matrix, got {tokens.dtype} and {weight.dim()} dimensions")
-    if whole and not tokens.is_cuda and tokens.numel() and not 0 <= int(tokens.min()) - vocab_start <= int(tokens.max()) - vocab_start < weight.shape[0]:
+    if _use_cuda(weight):
+        return _cuda().embedding(tokens, weight, float(scale), int(vocab_start), whole)
+    if whole and tokens.numel() and not 0 <= int(tokens.min()) - vocab_start <= int(tokens.max()) - vocab_start < weight.shape[0]:
         raise IndexError(f"embedding: token ids {int(tokens.min())} .. {int(tokens.max())} for a table of {weight.shape[0]} rows from {vocab_start}")
-    return (_cuda() if _use_cuda(weight) else ref).embedding(tokens, weight, float(scale), int(vocab_start))
+    return ref.embedding(tokens, weight, float(scale), int(vocab_start))
 
 
 def _distill_args(what, rows, ids, teacher_log_probs, kl_type, alpha, norm_mode, temperature):

@@ -62,7 +62,8 @@ def check_error_flag(device=None):
     v = int(f.item())
     if v != 0:
         f.zero_()
-        raise RuntimeError(f"sm_100a kernel reported error status {v} (1 = barrier wait timed out, 3 = peer wait timed out)")
+        raise RuntimeError(f"sm_100a kernel reported error status {v} (1 = barrier wait timed out, 3 = peer wait timed out, "
+                           f"4 = a token or expert id outside a whole table)")
 
 
 # --------------------------------------------------------------------------- GEMM
@@ -1228,8 +1229,8 @@ def grouped_linear(x, w, tile_expert, expert_rows):
 # --------------------------------------------------------------------------- rows by key
 
 
-def expert_layout(ids, num_experts, align):
-    return ExpertRows(*_load().expert_layout(ids, num_experts, align), num_experts, align)
+def expert_layout(ids, num_experts, align, whole=False):
+    return ExpertRows(*_load().expert_layout(ids, num_experts, align, err_flag(ids.device) if whole else None), num_experts, align)
 
 
 def expert_dispatch(x, rows):
@@ -1240,9 +1241,10 @@ def expert_combine(y, weights, rows, dtype=None):
     return _load().expert_combine(y, weights, rows.dest, rows.source, dtype == torch.float32)
 
 
-def embedding(tokens, weight, scale, vocab_start):
+def embedding(tokens, weight, scale, vocab_start, whole=False):
     mg = main_grad_of(weight)
-    return _load().embedding(weight, tokens, scale, vocab_start, mg if mg is not None and mg.is_contiguous() else None)
+    return _load().embedding(weight, tokens, scale, vocab_start, mg if mg is not None and mg.is_contiguous() else None,
+                             err_flag(weight.device) if whole else None)
 
 
 # --------------------------------------------------------------------------- distillation from top ids

@@ -254,7 +254,8 @@ class RolloutWeights(ComposedForward):
             from ..models.moe import experts_mlp
 
             el = p[pre + "experts_gate_up"].shape[0]
-            out = experts_mlp(x, idx - self.ep_rank * el, w, p[pre + "experts_gate_up"], p[pre + "experts_down"], torch.float32)
+            out = experts_mlp(x, idx - self.ep_rank * el, w, p[pre + "experts_gate_up"], p[pre + "experts_down"], torch.float32,
+                              whole=self.ep_size == 1)
             if pre + "shared_gate_up" in p and self.ep_rank == 0:     # summed over the EP ranks afterwards: one rank adds it
                 sh = ops.linear(ops.swiglu(ops.linear(x, p[pre + "shared_gate_up"])), p[pre + "shared_down"]).float()
                 if pre + "shared_gate" in p:

@@ -1002,6 +1002,10 @@ class TrainActor:
             if dp_cp > 1:
                 dist.all_reduce(tot, group=ps.dp_cp.group)
             gscale = dp_cp / float(tot.clamp_min(1))
+        if self.device.type == "cuda":      # (the step reads the gradient norm back anyway)
+            from ..ops.cuda import check_error_flag
+
+            check_error_flag(self.device)
         norm, skipped = opt.step(grad_scale=gscale)
         if self.mcfg.moe_router_bias:      # auxiliary-loss-free balancing: token counts of this step, all replicas
             for mod in self.model.modules():

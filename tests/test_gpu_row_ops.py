@@ -872,3 +872,70 @@ def test_combine_gives_the_gradients_that_are_asked_for(dtype, H, k):
     assert torch.cuda.max_memory_allocated() - before < y.numel() * y.element_size()
     (d_w,) = torch.autograd.grad(ops.expert_combine(yl, wl, rows), wl, up)      # only one of two is asked for
     assert torch.equal(d_w, want[1])
+
+
+@pytest.fixture
+def status():
+    """The device's status word, clean before and after."""
+    from relax_b200.ops import cuda as C
+
+    C.check_error_flag()
+    yield C.check_error_flag
+    C.err_flag().zero_()
+
+
+@pytest.mark.parametrize("cols,dtype", [(264, "bf16"), (520, "bf16"), (33, "fp32")])
+@pytest.mark.parametrize("bad", [-1, 50, 1 << 40, -(1 << 40)])
+def test_tokens_outside_a_whole_table_are_noted(status, cols, dtype, bad):
+    g = _gen(43)
+    table = torch.randn(50, cols, device="cuda", generator=g).to(DT[dtype]).requires_grad_()
+    tok = torch.randint(0, 50, (700,), device="cuda", generator=g)
+    want = ops.embedding(tok, table, whole=True)
+    assert torch.equal(want, table[tok])
+    status()
+    tok[699] = bad
+    out = ops.embedding(tok, table)                       # a shard's table: others have this token
+    status()
+    assert torch.equal(out[:699], want[:699]) and not out[699].any()
+    out = ops.embedding(tok, table, whole=True)
+    with pytest.raises(RuntimeError, match="status 4"):
+        status()
+    status()
+    assert torch.equal(out[:699], want[:699]) and not out[699].any()
+
+
+@pytest.mark.parametrize("T,k,E", [(5, 2, 4), (1, 8, 128), (30000, 3, 64)])
+def test_expert_ids_outside_a_whole_table_are_noted(status, T, k, E):
+    ids = torch.randint(0, E, (T, k), device="cuda", generator=_gen(44))
+    rows = ops.expert_layout(ids, E, whole=True)
+    status()
+    assert torch.equal(rows.dest, ops.expert_layout(ids, E).dest)
+    for bad in (-1, E):
+        ids[T - 1, k - 1] = bad
+        assert int(ops.expert_layout(ids, E).dest[T - 1, k - 1]) == -1
+        status()
+        ops.expert_layout(ids, E, whole=True)
+        with pytest.raises(RuntimeError, match="status 4"):
+            status()
+        status()
+
+
+def test_training_step_stops_at_a_token_outside_the_vocabulary(status):
+    """Before its weights move, as indexing would have stopped it."""
+    import dataclasses
+
+    from relax_b200.algo.loss import LossConfig
+    from relax_b200.models.config import get_config
+    from relax_b200.train.actor import TrainActor, TrainConfig
+    from relax_b200.train.optimizer import OptimizerConfig
+
+    mcfg = dataclasses.replace(get_config("tiny-moe"), head_dim=128, vocab_size=1024, dtype="bf16")
+    cfg = TrainConfig(advantage_estimator="grpo", global_batch_size=2, n_samples_per_prompt=2, loss=LossConfig(), optim=OptimizerConfig(lr=1e-3))
+    actor = TrainActor(mcfg, cfg, role="actor", device="cuda")
+    batch = lambda first: {"tokens": [[first, 5, 6, 7, 8, 9], [3, 5, 6, 7, 8, 10]], "response_lengths": [3, 3],      # noqa: E731
+                           "loss_masks": [[1.0] * 3] * 2, "rewards": [1.0, 0.0]}
+    before = actor.param_buf.clone()
+    with pytest.raises(RuntimeError, match="status 4"):
+        actor.train(0, batch(1024))
+    assert torch.equal(actor.param_buf, before)
+    assert math.isfinite(actor.train(1, batch(4))["grad_norm"]) and not torch.equal(actor.param_buf, before)

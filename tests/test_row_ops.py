@@ -355,3 +355,25 @@ def test_teacher_gets_no_gradient():
     zl = z.clone().requires_grad_()
     d_z, d_t = torch.autograd.grad(ops.topk_distill(zl, ids, t, "jsd"), [zl, t], w, allow_unused=True)
     assert d_t is None and bool(d_z.any())
+
+
+def test_whole_tables_of_experts_refuse_ids_outside():
+    from relax_b200.models.moe import experts_mlp, grouped_swiglu_mlp
+
+    g = _gen(9)
+    ids = torch.tensor([[0, 3], [2, 1]])
+    assert torch.equal(ops.expert_layout(ids, 4, 8, whole=True).dest, ops.expert_layout(ids, 4, 8).dest)
+    assert ops.expert_layout(ids[:0], 4, whole=True).dest.shape == (0, 2)
+    for bad in (-1, 4):
+        ids[1, 1] = bad
+        with pytest.raises(IndexError, match="of 4 experts"):
+            ops.expert_layout(ids, 4, whole=True)
+        assert int(ops.expert_layout(ids, 4).dest[1, 1]) == -1
+    x, w1, w2 = torch.randn(2, 6, generator=g), torch.randn(4, 10, 6, generator=g), torch.randn(4, 6, 5, generator=g)
+    with pytest.raises(IndexError, match="of 4 experts"):
+        grouped_swiglu_mlp(x, torch.tensor([0, 4]), w1, w2)
+    out = grouped_swiglu_mlp(x, torch.tensor([0, 4]), w1, w2, skip_foreign=True)
+    assert not out[1].any() and torch.equal(out[:1], grouped_swiglu_mlp(x[:1], torch.tensor([0]), w1, w2))
+    with pytest.raises(IndexError, match="of 4 experts"):
+        experts_mlp(x, ids, torch.ones(2, 2), w1, w2, whole=True)
+    assert experts_mlp(x[:0], ids[:0], torch.ones(0, 2), w1, w2, whole=True).shape == (0, 6)
