@@ -326,6 +326,11 @@ class RolloutEngine(SpeculativeMixin, ComposedScheduler):
             # partial rollout: earlier tokens become part of the context, generation continues
             r.output = list(resume_output)
             r.logprobs = list(resume_logprobs or [0.0] * len(r.output))
+        for toks in (r.prompt, r.output):      # (on the device such a token is a row of zeros, or another's)
+            if toks and not 0 <= min(toks) <= max(toks) < self.cfg.vocab_size:
+                bad = [int(t) for t in toks if not 0 <= t < self.cfg.vocab_size and (t < 0 or t != self.cfg.image_token_id)]
+                if bad:
+                    raise ValueError(f"token {bad[0]} is outside the vocabulary of {self.cfg.vocab_size}")
         self._next_rid += 1
         self.waiting.append(r)
         return r.rid

@@ -212,7 +212,13 @@ class EngineServer:
                     t["result"] = {"status": "ok", "aborted": len(done)}
                 t["event"].set()
             for prompt, params, key, t in incoming:
-                rid = eng.add_request(prompt, params, key)
+                try:
+                    rid = eng.add_request(prompt, params, key)
+                except Exception as e:  # noqa: BLE001 - this request's fault: the others go on
+                    t["result"] = {"output_ids": [], "logprobs": [], "finish_reason": f"error: {type(e).__name__}: {e}", "weight_versions": [],
+                                   "cached_tokens": 0}
+                    t["event"].set()
+                    continue
                 self._tickets[rid] = t
             if eng.has_work and not eng.paused:
                 try:

@@ -377,3 +377,26 @@ def test_whole_tables_of_experts_refuse_ids_outside():
     with pytest.raises(IndexError, match="of 4 experts"):
         experts_mlp(x, ids, torch.ones(2, 2), w1, w2, whole=True)
     assert experts_mlp(x[:0], ids[:0], torch.ones(0, 2), w1, w2, whole=True).shape == (0, 6)
+
+
+def test_engine_refuses_prompts_outside_the_vocabulary():
+    """The request alone: before it reaches the device, and without an end to the server or to what others run."""
+    from relax_b200.models.config import get_config
+    from relax_b200.rollout.engine import RolloutEngine, SamplingParams
+    from relax_b200.rollout.http_server import EngineServer
+
+    cfg = get_config("tiny")
+    eng = RolloutEngine(cfg, device="cpu", dtype=torch.float32, num_kv_blocks=64, block_size=8, seed=3)
+    for bad in ([3, cfg.vocab_size], [-1], [1 << 40, 2]):
+        with pytest.raises(ValueError, match="outside the vocabulary of"):
+            eng.add_request(bad, SamplingParams(max_new_tokens=2))
+    with pytest.raises(ValueError, match="outside the vocabulary of"):
+        eng.add_request([3], SamplingParams(max_new_tokens=2), resume_output=[cfg.vocab_size])
+    assert not eng.has_work
+    srv = EngineServer(eng)
+    try:
+        got = srv.generate({"input_ids": [[3, 5], [3, cfg.vocab_size], [0, cfg.vocab_size - 1]], "sampling_params": {"max_new_tokens": 3, "ignore_eos": True}})
+        assert [len(d["output_ids"]) for d in got] == [3, 0, 3]
+        assert "outside the vocabulary" in str(got[1]["finish_reason"])
+    finally:
+        srv.close()
