@@ -502,6 +502,10 @@ def validate_args(a: argparse.Namespace) -> argparse.Namespace:
         if (a.opd_loss_coef or 0.0) != 0.0:
             if max(a.tensor_model_parallel_size, a.context_parallel_size, a.pipeline_model_parallel_size) > 1:
                 raise ValueError("--opd-loss-coef with a top-K selection reads whole rows of logits: trainer tp = cp = pp = 1")
+            if (a.mtp_num_layers or 0) > 0 or a.enable_mtp_training or a.mtp_only_training:
+                raise ValueError("--opd-loss-coef with a top-K selection is a term of the plain decoder's policy loss: no multi-token-prediction blocks")
+            if a.loss_type != "policy_loss" or a.custom_loss_function_path:
+                raise ValueError("--opd-loss-coef with a top-K selection is a term of the policy loss: --loss-type policy_loss")
             most = 512 if a.opd_token_selection == "union" else 1024
             if a.opd_log_prob_top_k > most:
                 raise ValueError(f"--opd-loss-coef with --opd-token-selection {a.opd_token_selection}: --opd-log-prob-top-k up to {most}")

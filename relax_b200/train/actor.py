@@ -128,6 +128,7 @@ class TrainActor:
         self.mcfg, self.cfg, self.role = model_cfg, cfg, role
         self.ps = ps or single_process_state()
         self.device = torch.device(device)
+        self._check_distill_loss()
         self.model = GPTModel(model_cfg, self.ps, device=device, seed=seed, recompute=cfg.recompute)
         if model_cfg.vision is not None:
             # vision-language model: the tower is a sub-module of the language model, so the optimizer, checkpoints
@@ -201,6 +202,17 @@ class TrainActor:
         for mod in self.model.modules():
             if isinstance(mod, MoEMLP):
                 mod.ep_comm = self.ep_comm
+
+    def _check_distill_loss(self):
+        """Top-K distillation as a loss term: what it needs of the model and of the other options is known before anything is generated."""
+        c, m = self.cfg, self.mcfg
+        if self.role != "actor" or c.loss.opd_loss_coef == 0.0 or c.opd_token_selection == "sampled_token":
+            return
+        if max(self.ps.tp.size, self.ps.cp.size, self.ps.pp.size) > 1 or m.mtp_num_layers > 0 or c.loss.custom_loss_function is not None:
+            raise NotImplementedError("top-K distillation as a loss term: the policy loss of the plain decoder, trainer tp = pp = cp = 1")
+        if self.device.type == "cuda" and (m.dtype != "bf16" or m.vocab_size % 8 or m.hidden_size % 8):
+            raise ValueError(f"top-K distillation as a loss term: a bf16 model whose vocabulary and width are multiples of 8, got {m.dtype}, "
+                             f"{m.vocab_size} and {m.hidden_size}")
 
     # ------------------------------------------------------------------ tagged weights
     def _flatten_params(self):
@@ -824,8 +836,7 @@ class TrainActor:
             batch["advantages"] = [torch.zeros_like(a) for a in batch["advantages"]]
             batch["returns"] = [torch.zeros_like(r_) for r_ in batch["returns"]]
         if cfg.loss.opd_loss_coef != 0.0 and cfg.opd_token_selection != "sampled_token":
-            if self.ps.cp.size > 1 or self.ps.pp.size > 1 or self.mcfg.mtp_num_layers > 0 or cfg.loss.custom_loss_function is not None:
-                raise NotImplementedError("top-K distillation as a loss term: the policy loss of the plain decoder, trainer pp = cp = 1")
+            self._check_distill_loss()      # (options may have been set since)
             with self.timer.span("teacher_log_probs"):      # loss mode: the student's side is part of the training forward
                 batch["opd_topk_token_ids"], _, _, batch["opd_teacher_topk_log_probs"] = self._distill_ids(batch)
         elif cfg.loss.opd_loss_coef != 0.0 and batch.get("teacher_log_probs") is None and "teacher" in self.snapshots:

@@ -204,3 +204,41 @@ def test_step_trains_on_the_divergence_of_whole_logits(model, selection):
     off = math.sqrt(sum(float((grads[n].double() - ref[n].double()).pow(2).sum()) for n in ref))
     # 32-bit layers on both sides, summed in another order: some thousand roundings of 2^-24
     assert norm > 0 and off <= 1e-3 * norm
+
+
+def test_what_cannot_be_trained_is_refused_before_anything_is_generated(monkeypatch):
+    """Options when they are read, the model's sizes and type when the trainer is made."""
+    import dataclasses
+
+    from relax_b200.config.arguments import parse_args
+
+    base = ["--model-name", "tiny", "--colocate", "--rollout-batch-size", "2", "--use-opd", "--opd-teacher-load", "somewhere", "--opd-loss-coef", "1.0",
+            "--opd-token-selection", "union", "--opd-log-prob-top-k", "8"]
+    assert parse_args(base).opd_loss_coef == 1.0
+    for extra, match in ((["--mtp-num-layers", "1"], "multi-token-prediction"), (["--enable-mtp-training"], "multi-token-prediction"),
+                         (["--loss-type", "custom_loss", "--custom-loss-function-path", "a.b"], "policy loss"), (["--loss-type", "sft_loss"], "policy loss")):
+        with pytest.raises(ValueError, match=match):
+            parse_args(base + extra)
+        sampled = [x for x in base if x not in ("--opd-token-selection", "union", "--opd-log-prob-top-k", "8")]
+        parse_args(sampled + extra)                                   # (the sampled token's term is as it was)
+    tiny = get_config("tiny")
+    cfg = TrainConfig(opd_token_selection="union", opd_log_prob_top_k=5, loss=LossConfig(opd_loss_coef=1.0))
+
+    class Made(Exception):
+        pass
+
+    def no_model(*a, **kw):
+        raise Made
+
+    monkeypatch.setattr("relax_b200.train.actor.GPTModel", no_model)      # (nothing of the model is made before the refusal)
+    with pytest.raises(NotImplementedError, match="plain decoder"):
+        TrainActor(dataclasses.replace(tiny, mtp_num_layers=1), cfg)
+    bf = dataclasses.replace(tiny, dtype="bf16")
+    for m in (tiny, dataclasses.replace(bf, vocab_size=1020), dataclasses.replace(bf, hidden_size=252)):
+        with pytest.raises(ValueError, match="multiples of 8"):
+            TrainActor(m, cfg, device="cuda")
+        for ok in (dict(device="cuda", role="critic"), dict(device="cpu")):
+            with pytest.raises(Made):
+                TrainActor(m, cfg, **ok)
+    with pytest.raises(Made):
+        TrainActor(bf, cfg, device="cuda")
