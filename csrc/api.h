@@ -230,7 +230,7 @@ int rb_embedding(const void* ids, int wide, long long start, const void* table, 
 int rb_embedding_bwd_bins(int rows);
 int rb_embedding_bwd(const void* ids, int wide, long long start, const void* dy, long long ld, void* out, int add, int2* pairs, int* hist, float* part,
                      int* open, int n, int rows, int cols, float scale, int dtype, cudaStream_t st);
-int rb_topk_distill_parts(long long rows, int vocab, int size);
+int rb_topk_distill_parts(long long rows, int vocab, int k, int size);
 int rb_topk_distill(const void* z, long long ld, const long long* ids, const float* teacher, float* loss, float* coef, float* stats, float* log_probs,
                     double2* sums, long long rows, int vocab, int k, int kl, int norm, double alpha, double clamp, double inv_temp, int dtype, cudaStream_t
                     st);

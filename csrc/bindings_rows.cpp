@@ -250,7 +250,9 @@ torch::Tensor embedding(const torch::Tensor& weight, const torch::Tensor& tokens
 struct Distilled {
   torch::Tensor loss, kept, log_probs;      // kept: statistics [R, 4], sums of parts (a workspace), slopes of the ids [R, K]
 };
-inline int64_t slopes_at(const torch::Tensor& z) { return z.size(0) * (4 + 4 * rb_topk_distill_parts(z.size(0), static_cast<int>(z.size(1)), static_cast<int>(z.element_size()))); }
+inline int64_t slopes_at(const torch::Tensor& z, const torch::Tensor& ids) {
+  return z.size(0) * (4 + 4 * rb_topk_distill_parts(z.size(0), static_cast<int>(z.size(1)), static_cast<int>(ids.size(1)), static_cast<int>(z.element_size())));
+}
 
 Distilled distill_rows(const torch::Tensor& z, const torch::Tensor& ids, const torch::Tensor& teacher, int64_t kl, int64_t norm, double alpha, double clamp,
                        double inv_temp, bool log_probs) {
@@ -263,7 +265,7 @@ Distilled distill_rows(const torch::Tensor& z, const torch::Tensor& ids, const t
   TORCH_CHECK_VALUE(ids.size(1) <= 1024, "topk_distill: up to 1024 ids per row, got ", ids.size(1));
   TORCH_CHECK_VALUE(z.size(1) >= 1 && z.size(1) <= (1 << 24), "topk_distill: 1 to 2^24 tokens in the vocabulary, got ", z.size(1));
   const auto f32 = z.options().dtype(at::kFloat);
-  const int64_t R = z.size(0), K = ids.size(1), slopes = slopes_at(z);
+  const int64_t R = z.size(0), K = ids.size(1), slopes = slopes_at(z, ids);
   const int code = code_of(z, "topk_distill");
   Distilled d{at::empty({R}, f32), at::empty({slopes + R * K}, f32), torch::Tensor()};
   float* kept = d.kept.data_ptr<float>();
@@ -281,7 +283,7 @@ void distill_rows_bwd(const torch::Tensor& z, const torch::Tensor& ids, const to
                       const torch::Tensor& out) {
   const c10::cuda::CUDAGuard guard(z.device());
   TORCH_CHECK_VALUE(out.is_contiguous() && out.sizes() == z.sizes(), "topk_distill: a dense gradient of the logits' shape");
-  const int64_t slopes = slopes_at(z);
+  const int64_t slopes = slopes_at(z, ids);
   TORCH_CHECK_VALUE(g.scalar_type() == at::kFloat && g.is_contiguous() && g.numel() == z.size(0) && ids.is_contiguous() && ids.size(0) == z.size(0) &&
                         kept.scalar_type() == at::kFloat && kept.is_contiguous() && kept.numel() == slopes + ids.numel(),
                     "topk_distill: gradient or kept values of another shape");

@@ -686,7 +686,8 @@ int sums_t(const Params& p, long long rows, cudaStream_t st) {
   return static_cast<int>(cudaGetLastError());
 }
 // Rows that take more than one wave of large blocks but one of blocks half their size: the second wave is mostly empty (777 rows of 32003 in
-// bf16, ids included: 30 us against 39 with large blocks; of 151936 68 against 72; fp32 38 against 41, but 106 against 100, of 65536 57 both).
+// bf16, ids included: 30 us against 39 with large blocks; of 151936 68 against 72; fp32: 777 rows of 4099 17.4 against 19.5, of 32003 39 against
+// 42, of 50000 48.6 against 52, of 65536 57 against 59; 1000 and 1184 rows of 32003 to 65536 within one in a hundred; of 151936 106 against 100).
 inline bool one_wave_of_halves(long long rows, int vocab, int size) {
   return rows > 4ll * num_sms() && rows <= 8ll * num_sms() && vocab <= (size == 2 ? 200000 : 65536);      // (eight bitmaps fit shared memory)
 }
@@ -726,8 +727,11 @@ using namespace rb;
 using namespace rb::distill;
 
 // Blocks per row, and so pairs of doubles per row that rb_topk_distill takes as workspace.  size: bytes of a logit.
-extern "C" int rb_topk_distill_parts(long long rows, int vocab, int size) {
-  if (one_wave_of_halves(rows, vocab, size)) return 1;
+extern "C" int rb_topk_distill_parts(long long rows, int vocab, int k, int size) {
+  // More ids than small blocks hold leave large blocks: parts pay where rows are long (700 rows, 600 ids: of 151936 in bf16 87 us against 91 of
+  // whole rows, of 65536 in fp32 68 against 75), not where every part's own look at the ids costs more (32003 in bf16 52 against 48, in fp32 54
+  // against 53; 65536 in bf16 63 against 60; 100000 in bf16 75 both).
+  if (one_wave_of_halves(rows, vocab, size) && (k <= kMine * kHalfThreads || static_cast<long long>(vocab) * size <= 200000)) return 1;
   const int parts = parts_of(rows, vocab, 4ll * num_sms(), 1000);      // (a fixed 2 us of 4 blocks per SM)
   return vocab / parts > (1 << 20) ? kMaxParts : parts;                 // the bitmap of a part fits shared memory
 }
@@ -738,7 +742,7 @@ extern "C" int rb_topk_distill(const void* z, long long ld, const long long* ids
                                double inv_temp, int dtype, cudaStream_t st) {
   if (rows < 0 || vocab < 1 || vocab > kMaxVocab || k < 0 || k > kMaxIds || kl < 0 || kl > 3 || norm < 0 || norm > 2 || !(inv_temp > 0.0)) return -1;
   if (rows == 0) return 0;
-  const int parts = rb_topk_distill_parts(rows, vocab, dtype == 2 ? 4 : 2);
+  const int parts = rb_topk_distill_parts(rows, vocab, k, dtype == 2 ? 4 : 2);
   if (rows * parts > 2147483647ll) return -3;
   const double scale = inv_temp * kLog2e;
   float c2, c2_low;

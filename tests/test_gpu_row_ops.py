@@ -939,3 +939,22 @@ def test_training_step_stops_at_a_token_outside_the_vocabulary(status):
         actor.train(0, batch(1024))
     assert torch.equal(actor.param_buf, before)
     assert math.isfinite(actor.train(1, batch(4))["grad_norm"]) and not torch.equal(actor.param_buf, before)
+
+
+@pytest.mark.parametrize("V,K,whole", [(151936, 512, True), (151936, 513, False), (151936, 1024, False), (32003, 600, True)])
+def test_distill_rows_of_many_ids_are_shared_out(V, K, whole):
+    """700 rows are two waves of whole rows, the second mostly empty: small blocks take them in one, and where a row is long and has more ids
+    than those hold, several blocks share it."""
+    from relax_b200.ops import cuda as C
+
+    if torch.cuda.get_device_properties(0).multi_processor_count != 148:
+        pytest.skip("waves of 148 multiprocessors")
+    R = 700
+    z = torch.randn(R, V, device="cuda", generator=_gen(45)).bfloat16()
+    ids = torch.arange(K, device="cuda").expand(R, K).contiguous() * 7
+    t = torch.full((R, K), -9.0, device="cuda")
+    loss, kept = C._load().topk_distill_rows(z, ids, t, 0, 0, 0.5, -math.inf, 1.0)
+    parts = (kept.numel() - R * K) // (4 * R) - 1      # (four statistics of a row, two 64-bit numbers of a part)
+    assert (parts == 1) == whole
+    few = ops.topk_distill(z[:3], ids[:3], t[:3])
+    assert torch.allclose(loss[:3], few, rtol=1e-5, atol=1e-6)
