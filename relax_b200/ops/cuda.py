@@ -1270,9 +1270,10 @@ class _FusedHeadDistill(torch.autograd.Function):
         h, w = hidden.contiguous(), weight.contiguous()
         R = ids.shape[0]
         loss, kept = torch.empty(R, dtype=torch.float32, device=h.device), []
+        zs = torch.empty(min(R, chunk), w.shape[0], dtype=torch.float32, device=h.device)      # one piece's logits
         for s in range(0, R, chunk):
             e = min(R, s + chunk)
-            loss[s:e], k = _load().topk_distill_rows(matmul_nt(h[s:e], w, out_dtype=torch.float32), ids[s:e], teacher[s:e], *codes)
+            loss[s:e], k = _load().topk_distill_rows(matmul_nt(h[s:e], w, out=zs[: e - s]), ids[s:e], teacher[s:e], *codes)
             kept.append(k)
         ctx.save_for_backward(h, w, ids, *kept)
         ctx.meta = (codes[-1], chunk, weight)
@@ -1290,10 +1291,12 @@ class _FusedHeadDistill(torch.autograd.Function):
         mg = main_grad_of(weight)
         direct = mg is not None and mg.is_contiguous()
         dw = (mg if direct else torch.zeros(w.shape, dtype=torch.float32, device=h.device)) if learn_w else None
+        # one piece's logits and their gradient (1.9 GB for 2048 rows of 151936), for all pieces
+        zs = torch.empty(min(R, chunk), V, dtype=torch.float32, device=h.device)
+        ds = torch.empty(min(R, chunk), V, dtype=h.dtype, device=h.device)
         for k, s in zip(kept, range(0, R, chunk)):
             e = min(R, s + chunk)
-            z = matmul_nt(h[s:e], w, out_dtype=torch.float32)
-            d = torch.empty(e - s, V, dtype=h.dtype, device=h.device)
+            z, d = matmul_nt(h[s:e], w, out=zs[: e - s]), ds[: e - s]
             _load().topk_distill_rows_bwd(z, ids[s:e], k, g[s:e], inv_temp, d)
             if learn_h:
                 matmul_nn(d, w, out=dh[s:e])

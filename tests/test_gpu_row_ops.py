@@ -958,3 +958,22 @@ def test_distill_rows_of_many_ids_are_shared_out(V, K, whole):
     assert (parts == 1) == whole
     few = ops.topk_distill(z[:3], ids[:3], t[:3])
     assert torch.allclose(loss[:3], few, rtol=1e-5, atol=1e-6)
+
+
+def test_fused_head_holds_one_piece_of_logits():
+    g = _gen(46)
+    R, V, H, K, chunk = 1400, 32768, 64, 6, 512
+    h, wt = torch.randn(R, H, device="cuda", generator=g).bfloat16().requires_grad_(), torch.randn(V, H, device="cuda", generator=g).bfloat16().requires_grad_()
+    wt.main_grad = torch.zeros(V, H, device="cuda")
+    ids, t = torch.arange(K, device="cuda").expand(R, K).contiguous(), torch.full((R, K), -3.0, device="cuda")
+    for _ in range(2):      # (the second time without first calls' workspaces)
+        before = torch.cuda.memory_allocated()
+        torch.cuda.reset_peak_memory_stats()
+        loss = ops.fused_lm_head_topk_distill(h, wt, ids, t, chunk_size=chunk)
+        forward = torch.cuda.max_memory_allocated() - before
+        torch.cuda.reset_peak_memory_stats()
+        loss.sum().backward()
+        backward = torch.cuda.max_memory_allocated() - before
+    piece = chunk * V
+    small = 4 << 20      # (hidden states, their gradient, slopes of the ids)
+    assert forward <= 4 * piece + small and backward <= (4 + 2) * piece + small
