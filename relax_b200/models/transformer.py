@@ -222,7 +222,7 @@ class VocabParallelEmbedding(nn.Module):
         # tokens of other shards give zeros; the gradient goes straight into the optimizer's fp32 buffer of the weight, where it touches
         # only the rows that were looked up
         g = self.ps.tp
-        e = ops.embedding(tokens, self.weight, self.scale, self.start, whole=g.size == 1)
+        e = ops.embedding(tokens.to(self.weight.device), self.weight, self.scale, self.start, whole=g.size == 1)
         if g.size == 1:
             return e
         if sequence_parallel:

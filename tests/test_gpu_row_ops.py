@@ -977,3 +977,19 @@ def test_fused_head_holds_one_piece_of_logits():
     piece = chunk * V
     small = 4 << 20      # (hidden states, their gradient, slopes of the ids)
     assert forward <= 4 * piece + small and backward <= (4 + 2) * piece + small
+
+
+def test_model_takes_tokens_from_the_host():
+    """As indexing a weight did."""
+    import dataclasses
+
+    from relax_b200.models.config import get_config
+    from relax_b200.models.transformer import GPTModel
+
+    m = GPTModel(dataclasses.replace(get_config("tiny"), dtype="bf16"), device="cuda", seed=1)
+    tok = torch.tensor([3, 1023, 0, 3])
+    emb = m.embedding.word_embeddings
+    out = emb(tok, False)
+    assert torch.equal(out, emb.weight[tok.cuda()])
+    up = torch.randn(out.shape, device="cuda").bfloat16()
+    assert torch.equal(*(torch.autograd.grad(emb(t, False), emb.weight, up)[0] for t in (tok, tok.cuda())))
