@@ -316,8 +316,9 @@ def expert_layout(expert_of_row, num_experts: int, align: int = 128, whole: bool
     :class:`relax_b200.ops.reference.ExpertRows`."""
     if expert_of_row.dim() not in (1, 2) or expert_of_row.dtype not in (torch.int64, torch.int32):
         raise ValueError(f"expert_layout: int64 or int32 ids of shape [T, k] or [R], got {expert_of_row.dtype} {tuple(expert_of_row.shape)}")
-    if not 1 <= num_experts <= 2048 or not 1 <= align <= 65536:
-        raise ValueError(f"expert_layout: 1 to 2048 experts and 1 <= align <= 65536, got {num_experts} and {align}")
+    if num_experts < 1 or not 1 <= align <= 65536:
+        raise ValueError(f"expert_layout: one expert or more (the kernels sort up to 2048 experts, torch beyond) and 1 <= align <= 65536, got "
+                         f"{num_experts} and {align}")
     ids = expert_of_row if expert_of_row.dim() == 2 else expert_of_row[:, None]
     if ids.shape[1] < 1:
         raise ValueError("expert_layout: at least one expert per row")

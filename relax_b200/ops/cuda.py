@@ -13,7 +13,7 @@ from typing import Optional
 import torch
 from torch.autograd.function import once_differentiable
 
-from .reference import ExpertRows, main_grad_of
+from .reference import ExpertRows, expert_layout as _layout_by_torch, main_grad_of
 
 _SO = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "_C.so")
 _SO_SERVING = _SO.replace("_C.so", "_C_serving.so")      # serving subset (ops/build.py)
@@ -1230,6 +1230,11 @@ def grouped_linear(x, w, tile_expert, expert_rows):
 
 
 def expert_layout(ids, num_experts, align, whole=False):
+    if num_experts > 2048:      # (more counters than a block's shared memory holds: no model has so many; sorted as before there were kernels)
+        if whole:
+            err = err_flag(ids.device)
+            err.copy_(torch.where((err == 0) & ((ids < 0) | (ids >= num_experts)).any(), 4, err))
+        return _layout_by_torch(ids, num_experts, align)
     return ExpertRows(*_load().expert_layout(ids, num_experts, align, err_flag(ids.device) if whole else None), num_experts, align)
 
 

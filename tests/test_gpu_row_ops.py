@@ -993,3 +993,20 @@ def test_model_takes_tokens_from_the_host():
     assert torch.equal(out, emb.weight[tok.cuda()])
     up = torch.randn(out.shape, device="cuda").bfloat16()
     assert torch.equal(*(torch.autograd.grad(emb(t, False), emb.weight, up)[0] for t in (tok, tok.cuda())))
+
+
+def test_more_experts_than_a_block_counts(status):
+    g = _gen(47)
+    ids = torch.randint(0, 3000, (500, 2), device="cuda", generator=g)
+    x, w = torch.randn(500, 64, device="cuda", generator=g).bfloat16(), torch.rand(500, 2, device="cuda", generator=g)
+    rows = ops.expert_layout(ids.int(), 3000, 16, whole=True)
+    status()
+    dest, source, tiles, bounds = O.layout(ids.cpu(), 3000, 16)
+    assert rows.dest.reshape(-1).tolist() == dest and rows.source.tolist() == source and rows.tile_expert.tolist() == tiles and rows.expert_rows.tolist() == bounds
+    assert torch.equal(ops.expert_combine(ops.expert_dispatch(x, rows), None, rows, torch.float32), 2.0 * x.float())
+    ids[7, 1] = 3000
+    assert int(ops.expert_layout(ids, 3000).dest[7, 1]) == -1
+    status()
+    ops.expert_layout(ids, 3000, whole=True)
+    with pytest.raises(RuntimeError, match="status 4"):
+        status()

@@ -400,3 +400,10 @@ def test_engine_refuses_prompts_outside_the_vocabulary():
         assert "outside the vocabulary" in str(got[1]["finish_reason"])
     finally:
         srv.close()
+
+
+def test_more_experts_than_a_block_counts():
+    ids = torch.randint(-1, 5001, (300, 2), generator=_gen(10))
+    rows = ops.expert_layout(ids, 5000, 8)
+    dest, source, tiles, bounds = O.layout(ids, 5000, 8)
+    assert rows.dest.reshape(-1).tolist() == dest and rows.source.tolist() == source and rows.tile_expert.tolist() == tiles and rows.expert_rows.tolist() == bounds
