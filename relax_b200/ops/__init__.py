@@ -324,7 +324,7 @@ def expert_layout(expert_of_row, num_experts: int, align: int = 128, whole: bool
         raise ValueError("expert_layout: at least one expert per row")
     if _use_cuda(ids):
         return _cuda().expert_layout(ids, int(num_experts), int(align), whole)
-    if whole and ids.numel() and not 0 <= int(ids.min()) <= int(ids.max()) < num_experts:
+    if whole and not ids.is_cuda and ids.numel() and not 0 <= int(ids.min()) <= int(ids.max()) < num_experts:
         raise IndexError(f"expert_layout: expert ids {int(ids.min())} .. {int(ids.max())} of {num_experts} experts")
     return ref.expert_layout(ids, int(num_experts), int(align))
 
@@ -363,7 +363,7 @@ def embedding(tokens, weight, scale: float = 1.0, vocab_start: int = 0, whole: b
         raise ValueError(f"embedding: int64 or int32 tokens and a matrix, got {tokens.dtype} and {weight.dim()} dimensions")
     if _use_cuda(weight):
         return _cuda().embedding(tokens, weight, float(scale), int(vocab_start), whole)
-    if whole and tokens.numel() and not 0 <= int(tokens.min()) - vocab_start <= int(tokens.max()) - vocab_start < weight.shape[0]:
+    if whole and not tokens.is_cuda and tokens.numel() and not 0 <= int(tokens.min()) - vocab_start <= int(tokens.max()) - vocab_start < weight.shape[0]:
         raise IndexError(f"embedding: token ids {int(tokens.min())} .. {int(tokens.max())} for a table of {weight.shape[0]} rows from {vocab_start}")
     return ref.embedding(tokens, weight, float(scale), int(vocab_start))
 
