@@ -1037,6 +1037,7 @@ inline int key_bits(int rows) {      // of the keys 0 .. rows
   return b;
 }
 constexpr int kPassBits = 10;
+static_assert((1 << kPassBits) <= kThreads && (1 << kPassBits) <= kMaxBins, "pack_sort_kernel gives every bin a thread");
 
 }  // namespace rows
 }  // namespace rb

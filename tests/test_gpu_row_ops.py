@@ -1010,3 +1010,22 @@ def test_more_experts_than_a_block_counts(status):
     ops.expert_layout(ids, 3000, whole=True)
     with pytest.raises(RuntimeError, match="status 4"):
         status()
+
+
+def test_serving_forms_in_inference_mode():
+    g = _gen(48)
+    ids, tok = torch.randint(0, 4, (64, 2), device="cuda", generator=g), torch.randint(0, 64, (40,), device="cuda", generator=g)
+    x, w = torch.randn(64, 72, device="cuda", generator=g).bfloat16(), torch.rand(64, 2, device="cuda", generator=g)
+    did, t = torch.randint(0, 72, (64, 3), device="cuda", generator=g), torch.full((64, 3), -2.0, device="cuda")
+    leaf = x.clone().requires_grad_()
+
+    def run():
+        rows = ops.expert_layout(ids, 4)
+        y = ops.expert_dispatch(leaf, rows)
+        return [rows.dest, rows.source, y, ops.expert_combine(y, w, rows), ops.embedding(tok, leaf, 2.0, whole=True),
+                *ops.topk_distill(leaf, did, t, return_log_probs=True)]
+
+    want = [v.detach().clone() for v in run()]
+    with torch.inference_mode():
+        got = run()
+    assert all(v.is_inference() for v in got) and all(torch.equal(a, b) for a, b in zip(want, got))
