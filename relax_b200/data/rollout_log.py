@@ -14,7 +14,7 @@ import torch.distributed as dist
 
 SKIP = {"tokens", "multimodal_train_inputs", "loss_masks", "sample_indices", "sample_index_mask_sums",
         "rollout_routed_experts", "max_seq_lens", "dynamic_global_batch_size", "metadata", "weight_versions", "prompt",
-        "response", "label", "status", "group_index", "index"}
+        "response", "label", "status", "group_index", "index", "opd_teacher_topk_log_probs"}
 
 
 def _flat(val, device=None):

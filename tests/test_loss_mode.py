@@ -242,3 +242,11 @@ def test_what_cannot_be_trained_is_refused_before_anything_is_generated(monkeypa
                 TrainActor(m, cfg, **ok)
     with pytest.raises(Made):
         TrainActor(bf, cfg, device="cuda")
+
+
+@pytest.mark.parametrize("selection", SEL)
+def test_step_reports_finite_numbers(selection):
+    """The teacher's log-probs of padded ids (-inf) are no metric."""
+    actor = _actor("tiny", selection=selection)
+    m = actor.train(0, _batch(actor))
+    assert "rollout/opd_teacher_topk_log_probs" not in m and all(math.isfinite(v) for v in m.values() if isinstance(v, (int, float)))
