@@ -506,6 +506,8 @@ def validate_args(a: argparse.Namespace) -> argparse.Namespace:
                 raise ValueError("--opd-loss-coef with a top-K selection is a term of the plain decoder's policy loss: no multi-token-prediction blocks")
             if a.loss_type != "policy_loss" or a.custom_loss_function_path:
                 raise ValueError("--opd-loss-coef with a top-K selection is a term of the policy loss: --loss-type policy_loss")
+            if not 0.0 <= a.opd_jsd_alpha <= 1.0:
+                raise ValueError(f"--opd-jsd-alpha must lie in [0, 1], got {a.opd_jsd_alpha}")
             most = 512 if a.opd_token_selection == "union" else 1024
             if a.opd_log_prob_top_k > most:
                 raise ValueError(f"--opd-loss-coef with --opd-token-selection {a.opd_token_selection}: --opd-log-prob-top-k up to {most}")

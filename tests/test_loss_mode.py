@@ -250,3 +250,15 @@ def test_step_reports_finite_numbers(selection):
     actor = _actor("tiny", selection=selection)
     m = actor.train(0, _batch(actor))
     assert "rollout/opd_teacher_topk_log_probs" not in m and all(math.isfinite(v) for v in m.values() if isinstance(v, (int, float)))
+
+
+def test_weight_of_the_mixture_is_refused_when_options_are_read():
+    from relax_b200.config.arguments import parse_args
+
+    base = ["--model-name", "tiny", "--colocate", "--rollout-batch-size", "2", "--use-opd", "--opd-teacher-load", "somewhere", "--opd-loss-coef", "1.0",
+            "--opd-token-selection", "union", "--opd-log-prob-top-k", "8", "--opd-kl-type", "jsd", "--opd-jsd-alpha"]
+    for ok in ("0", "0.3", "1"):
+        assert parse_args(base + [ok]).opd_jsd_alpha == float(ok)
+    for bad in ("-0.1", "1.5", "nan"):
+        with pytest.raises(ValueError, match="opd-jsd-alpha"):
+            parse_args(base + [bad])
