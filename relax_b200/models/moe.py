@@ -115,7 +115,8 @@ EXPERT_ROW_ALIGN = 128       # the grouped GEMM walks 128-row tiles; no tile may
 
 
 def padded_expert_layout(expert_of_row: torch.Tensor, num_experts: int, align: int = EXPERT_ROW_ALIGN):
-    """Where every row goes in the expert-sorted buffer whose expert groups are padded to ``align`` rows.
+    """Where every row goes in the expert-sorted buffer whose expert groups are padded to ``align`` rows, in elementary operations
+    (the models use :func:`relax_b200.ops.expert_layout`, whose buffer is smaller; this one is what products on it are compared with).
 
     Everything stays on the device (no count is read back): the buffer is sized for the worst case
     ``rows + num_experts * (align - 1)``, unused tiles are marked in the tile map.  Returns ``(order, dest, cap,

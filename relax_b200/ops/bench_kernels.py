@@ -239,7 +239,6 @@ def bench_moe(args, pk):
     """Grouped expert GEMMs of a Qwen3-30B-A3B layer on one EP rank (16 local experts, hidden 2048, expert FFN 768):
     one launch for all experts against a loop of library GEMMs over the same expert-sorted rows."""
     from .. import ops
-    from ..models.moe import padded_expert_layout
 
     dev, E, H, F = "cuda", 16, 2048, 768
     rows = args.tokens * 8 // 8                      # tokens x top-8 spread over 8 EP ranks
@@ -248,15 +247,15 @@ def bench_moe(args, pk):
     x = torch.randn(rows, H, device=dev, generator=g).bfloat16()
     w1 = (torch.randn(E, 2 * F, H, device=dev, generator=g) * 0.02).bfloat16()
     w2 = (torch.randn(E, H, F, device=dev, generator=g) * 0.02).bfloat16()
-    order, dest, cap, tile_expert, expert_rows = padded_expert_layout(e_of, E)
-    xp = x.new_zeros(cap, H).index_copy(0, dest, x[order])
+    lay = ops.expert_layout(e_of, E)
+    xp = ops.expert_dispatch(x, lay)
     counts = torch.bincount(e_of, minlength=E).tolist()
-    xs = x[order]
+    xs = x[torch.argsort(e_of, stable=True)]
 
     def ours():
         with torch.no_grad():
-            a = ops.swiglu(ops.grouped_linear(xp, w1, tile_expert, expert_rows))
-            return ops.grouped_linear(a, w2, tile_expert, expert_rows)
+            a = ops.swiglu(ops.grouped_linear(xp, w1, lay.tile_expert, lay.expert_rows))
+            return ops.grouped_linear(a, w2, lay.tile_expert, lay.expert_rows)
 
     def lib():
         o, outs = 0, []

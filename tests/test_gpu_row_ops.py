@@ -1029,3 +1029,29 @@ def test_serving_forms_in_inference_mode():
     with torch.inference_mode():
         got = run()
     assert all(v.is_inference() for v in got) and all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+@pytest.mark.parametrize("T,k,E,load", [(1, 8, 16, "even"), (5, 2, 300, "even"), (300, 2, 4, "one"), (257, 3, 7, "steep"), (128, 1, 2, "one"), (700, 8, 64, "even")])
+def test_expert_products_on_their_layout(T, k, E, load):
+    """Both products and all gradients on the buffer that the models use: no room to spare, tiles without rows, experts without rows."""
+    from relax_b200.models.moe import experts_mlp
+
+    g, H, Fh = _gen(49), 128, 64
+    if load == "one":
+        idx = torch.full((T, k), E - 1, device="cuda")
+    elif load == "steep":
+        idx = (torch.rand(T, k, device="cuda", generator=g) ** 4 * E).long()
+    else:
+        idx = torch.rand(T, E, device="cuda", generator=g).topk(k, -1).indices
+    mk = lambda *s, m=1.0: (torch.randn(*s, device="cuda", generator=g) * m).bfloat16().requires_grad_()      # noqa: E731
+    x, w1, w2, gate = mk(T, H), mk(E, 2 * Fh, H, m=0.09), mk(E, H, Fh, m=0.12), torch.rand(T, k, device="cuda", generator=g).requires_grad_()
+    out = experts_mlp(x, idx, gate, w1, w2, whole=True)
+    up = torch.randn(T, H, device="cuda", generator=g).bfloat16()
+    got = [out, *torch.autograd.grad(out, [x, gate, w1, w2], up)]
+    D = [p.detach().double().requires_grad_() for p in (x, gate, w1, w2)]
+    gu = torch.einsum("th,tknh->tkn", D[0], D[2][idx])
+    y = torch.einsum("tkf,tkhf->tkh", torch.nn.functional.silu(gu[..., :Fh]) * gu[..., Fh:], D[3][idx])
+    ref = (y * D[1][..., None]).sum(1)
+    want = [ref, *torch.autograd.grad(ref, D, up.double())]
+    for a, b in zip(got, want):      # five roundings to 16 bits in a row, 2^-8 each
+        assert float((a.double() - b).norm()) <= 5 * 2.0 ** -8 * float(b.norm())
