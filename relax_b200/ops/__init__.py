@@ -356,7 +356,7 @@ def expert_combine(y, weights, rows, dtype=None):
 def embedding(tokens, weight, scale: float = 1.0, vocab_start: int = 0, whole: bool = False):
     """``scale * weight[tokens - vocab_start]``, zeros for tokens outside the table's rows (those of other shards).  The gradient sorts the
     tokens and sums every table row's incoming rows in 32 bits in a fixed order, so reruns give the same bits; it is added to the
-    weight's fp32 ``main_grad`` where there is one at the time of the lookup, which touches only rows that were looked up.  ``whole``: the table
+    weight's fp32 ``main_grad`` where there is one at the time of the lookup (on the CPU: of the backward pass), which touches only rows that were looked up.  ``whole``: the table
     is the whole vocabulary, and a token outside it is an error: raised on the CPU, left in the device's status word on a GPU
     (:func:`relax_b200.ops.cuda.check_error_flag`; its row is zeros)."""
     if tokens.dtype not in (torch.int64, torch.int32) or weight.dim() != 2:
