@@ -636,7 +636,8 @@ __host__ __device__ inline int padding_rows(int vecs) { return vecs >= 128 ? 8 :
 // Backward of the weighted sum: d_y[dest] = w d_out[t] and d_w = <d_out[t], y[dest]>.  A block per token holds its row of d_out (in the
 // type of the sum: fp32 for a sum kept in 32 bits) while it walks over the token's rows of y, so that all of them pass once; blocks behind
 // the tokens write the zeros of padding rows.  Where rows do not learn (kRows false) nothing is written to the buffer, where weights are
-// fixed (kWeights false) y is not read, and need not be there.  (Null pointers asked about in here: 125 us for the case above instead of 104.)
+// fixed (kWeights false) y is not read, and need not be there.  (Null pointers asked about in here, 8192
+// tokens to 8 of 128 experts, width 2048, cold L2: 125 us instead of 104.)
 template <typename T, int N, typename G, bool kRows, bool kWeights>
 __global__ void __launch_bounds__(N == 1 ? kSingleThreads : 256) sum_bwd_kernel(const G* __restrict__ d_out, long long ld, const T* __restrict__ y, long long ldy,
                                                       const int* __restrict__ source, const int* __restrict__ dest, const float* __restrict__ weight,
