@@ -262,3 +262,42 @@ def test_weight_of_the_mixture_is_refused_when_options_are_read():
     for bad in ("-0.1", "1.5", "nan"):
         with pytest.raises(ValueError, match="opd-jsd-alpha"):
             parse_args(base + [bad])
+
+
+def _two_rank_batch(rows):
+    g = torch.Generator().manual_seed(9)
+    lens, rl = (30, 28, 11, 9), [7, 9, 4, 3]
+    toks = [torch.randint(3, 1000, (n,), generator=g).tolist() for n in lens]
+    return {"tokens": [toks[i] for i in rows], "response_lengths": [rl[i] for i in rows], "loss_masks": [[1.0] * rl[i] for i in rows],
+            "rewards": [[1.0, 0.0, 0.0, 1.0][i] for i in rows]}
+
+
+def _two_rank_step(ps, rows, selection):
+    """One step on samples ``rows``; the two long ones do not fit one micro-batch, so a rank with the short ones runs a filler."""
+    cfg = TrainConfig(advantage_estimator="grpo", global_batch_size=4, n_samples_per_prompt=2, use_dynamic_batch_size=True, max_tokens_per_gpu=32,
+                      pad_multiple=1, opd_token_selection=selection, opd_log_prob_top_k=5, opd_kl_type="jsd", opd_only_reward=True, use_routing_replay=True,
+                      loss=LossConfig(opd_loss_coef=1.0, opd_kl_type="jsd"), optim=OptimizerConfig(lr=0.0))
+    actor = TrainActor(get_config("tiny-moe"), cfg, ps, seed=0)
+    teacher = actor.param_buf.clone()
+    for p, o in actor._bound_params():      # (the same change of every weight on every rank, however experts are spread)
+        teacher[o:o + p.numel()] *= 1.3
+    actor.snapshots["teacher"] = teacher
+    m = actor.train(0, _two_rank_batch(rows))
+    return m["opd_loss"], m["grad_norm"], RoutingReplay.mode
+
+
+def _two_rank_worker(rank, world, dims, selection):
+    from relax_b200.parallel.state import ParallelDims, init_parallel_state
+
+    return _two_rank_step(init_parallel_state(ParallelDims(dp=2, **dims)), [0, 1] if rank == 0 else [2, 3], selection)
+
+
+@pytest.mark.parametrize("dims,selection", [({}, "union"), ({"ep": 2}, "teacher_topk")])
+def test_two_replicas_with_uneven_micro_batches(dims, selection):
+    from tests._mp import run_distributed
+
+    got = run_distributed(_two_rank_worker, 2, dims, selection)
+    want = _two_rank_step(None, [0, 1, 2, 3], selection)
+    assert want[2] is None and want[0] > 0 and want[1] > 0
+    for loss, norm, mode in got:      # 32-bit layers, gradients summed in another order
+        assert mode is None and loss == pytest.approx(want[0], rel=1e-4) and norm == pytest.approx(want[1], rel=1e-3)
